@@ -58,6 +58,7 @@ extern "C" {
 /* bits of the device status word */
 #define KD_STATUS_TIMEOUT 0x10000000u  /* | code of the wait that gave up */
 #define KD_STATUS_SPAN_RANGE 0x20000000u /* a span_id does not fit in 24 signed bits */
+#define KD_STATUS_CACHE_RANGE 0x40000000u /* a length or a page number outside a cache's bounds; | 1 length, 2 page */
 
 /* Per-token metadata of one batch, as produced by the reference's collate function
  * (data_builder.py:603-653) and consumed by _flash_attn_fwd (original_kernel.py:332-347,
@@ -272,6 +273,87 @@ int kd_cocktail_index(const int64_t* tokens, int64_t stride_b, int32_t B, int32_
                       int32_t* first_mask, int32_t* counts_host, void* stream);
 int kd_cocktail_scores(const kd_cocktail* p, void* stream);
 int kd_cocktail_grad(const kd_cocktail* p, void* stream);
+
+/* ---- key/value cache in 8 bits: attention over it, appending, reading, eviction -------------------------------------
+ * No counterpart in the reference, whose GPTModel.generate (model.py:316-355) runs the whole sequence again for every token.
+ * The mask is the rule of kd_classify (original_kernel.py:480-517) with the cached tokens as keys.
+ *
+ * A cache is a pool of pages of KD_CACHE_PAGE tokens. k and v hold e4m3 numbers, which stand for their value times the scale of their
+ * page and head: 2^e with -32 <= e <= 31, the smallest e for which the block's largest finite magnitude is at most 448 * 2^e (larger numbers
+ * saturate). Infinities and NaN are stored as NaN. Sequences name their pages through a table. What a table names for blocks at or beyond
+ * the sequence's length is never read. Two sequences may share a page as long as neither appends to it.
+ * Lengths and page numbers live on the device and are checked there: a length is clamped to what the table holds, a page number outside the
+ * pool counts as a block without tokens, and status_mirror is told. Every address is formed from checked numbers. */
+#define KD_CACHE_PAGE 64
+
+typedef struct kd_cache {
+  void *k, *v;              /* e4m3 (pages, H, KD_CACHE_PAGE, D) contiguous, 16-byte aligned */
+  float *k_scale, *v_scale; /* (pages, H) contiguous */
+  uint32_t* desc;           /* NULL: no metadata, or (pages, H, KD_CACHE_PAGE) token descriptors: bit 0 prefix, 1 context, 2 in a span, 3 [MASKQ], 4 same-span
+                               rule armed, 5..7 the key classes (prefix, context, span) that the token sees as a query wherever they are, 8.. the span
+                               id's low 24 bits */
+  int32_t pages, H, D;      /* H key/value heads; D a multiple of 16 from 16 to 128 */
+  uint32_t* status_mirror;  /* NULL, or as in kd_meta */
+} kd_cache;
+
+typedef struct kd_cache_seqs {
+  const int32_t* table;     /* (B, blocks) page numbers, unit stride along blocks */
+  int64_t table_stride;     /* elements between the rows of table */
+  const int32_t* lens;      /* (B) tokens of each sequence */
+  int32_t B, blocks;        /* blocks at most 2^24 */
+} kd_cache_seqs;
+
+/* New keys and values behind the lens[b] tokens that sequence b has. The caller adds n_new to lens. A block that holds tokens already keeps
+ * its scale or gets a larger one; what it holds is then rounded again, which is exact but for subnormal numbers. */
+typedef struct kd_cache_tokens {
+  kd_tensor k, v;           /* (B, H, T, D); pointers and byte strides multiples of 16 */
+  int32_t T, dtype;         /* KD_F16 / KD_BF16 / KD_F32 */
+  const int32_t* n_new;     /* NULL: T, or (B) how many of the T are there */
+  const uint8_t* in_span;   /* (B, T) as in kd_meta, for the T new tokens; NULL: none is. Read only with kd_cache.desc */
+  const int64_t* span_id;
+  const uint8_t* is_prefix;
+  int64_t in_span_stride_b, span_id_stride_b, is_prefix_stride_b;
+} kd_cache_tokens;
+int kd_cache_append(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream);
+
+/* Attention of the newest tokens: query i of sequence b is its token lens[b] - q_lens[b] + i, whose key and value are in the cache already.
+ * Query head h reads key head h / (H / kd_cache.H). With kd_cache.desc the mask is the 4-section rule, else j <= i (causal) or every
+ * cached token. Rows at or beyond q_lens, and rows that see nothing, get O = 0 and LSE = -inf.
+ * weights, if given, has the softmax weights that each cached token receives from all query rows of its head added to it. */
+typedef struct kd_cache_queries {
+  kd_tensor q, o;           /* (B, H, T, D); pointers and byte strides multiples of 16 */
+  int32_t H, T, dtype;      /* KD_F16 / KD_BF16 */
+  int32_t causal;           /* read only without kd_cache.desc */
+  float sm_scale;
+  const int32_t* q_lens;    /* NULL: T, or (B) */
+  float* lse;               /* NULL (not without weights), or (B, H, T) contiguous, base 2 */
+  float* weights;           /* NULL, or (B, kd_cache.H, w_len), unit stride along tokens; tokens at or beyond w_len are left out */
+  int64_t w_stride_b, w_stride_h;
+  int32_t w_len;
+  void* workspace;          /* kd_cache_attention_workspace bytes, 16-byte aligned */
+} kd_cache_queries;
+int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream);
+int kd_cache_attention_workspace(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes);
+
+/* What a sequence keeps of its tokens, for each head: the first `first`, the last `recent` and, of the others, those of the largest weight up to
+ * `keep` in all; of equal weights the lower index, NaN above everything. Kept tokens go in their order to the pages of out_table, which must not
+ * be among the sequences' own, with new scales as if they had been appended. */
+typedef struct kd_cache_eviction {
+  const float* weights;     /* (B, H, w_len) as in kd_cache_queries; tokens at or beyond w_len weigh 0 */
+  int64_t w_stride_b, w_stride_h;
+  int32_t w_len;
+  int32_t keep, recent, first;   /* keep >= 1, first + recent <= keep */
+  const int32_t* out_table; /* (B, ceil(keep / KD_CACHE_PAGE)) */
+  int64_t out_table_stride;
+  int32_t* index;           /* (B, H, keep) contiguous out: the kept tokens' places, ascending, -1 beyond */
+  float* out_weights;       /* (B, H, keep) contiguous out: their weights, 0 beyond */
+  int32_t* out_lens;        /* (B) out: min(lens, keep) */
+} kd_cache_eviction;
+int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream);
+
+/* k, v (B, H, count, D) of the tokens start[b] .. start[b] + count - 1 (start NULL: 0); zeros at and beyond lens[b]. dtype KD_F16 / KD_BF16 / KD_F32. */
+int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k,
+                  const kd_tensor* v, void* stream);
 
 /* Message for the last negative return value on this host thread. */
 const char* kd_last_error(void);

@@ -28,6 +28,7 @@ EXPORTS = (
     "kd_metadata_from_tokens", "kd_span_index", "kd_span_mean",
     "kd_cocktail_index", "kd_cocktail_scores", "kd_cocktail_grad",
     "kd_cast",
+    "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read",
 )
 
 
@@ -62,6 +63,41 @@ class KdAttnParams(Structure):
         ("dq", KdTensor), ("dk", KdTensor), ("dv", KdTensor),
         ("lse", c_void_p), ("delta", c_void_p), ("plan", c_void_p), ("bwd_phases", c_int32), ("bwd_mode", c_int32),
         ("dq_acc", c_void_p), ("heads_per_cta", c_int32), ("plan_ready", c_int32),
+    ]
+
+
+class KdCache(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("desc", c_void_p),
+        ("pages", c_int32), ("H", c_int32), ("D", c_int32), ("status_mirror", c_void_p),
+    ]
+
+
+class KdCacheSeqs(Structure):
+    _fields_ = [("table", c_void_p), ("table_stride", c_int64), ("lens", c_void_p), ("B", c_int32), ("blocks", c_int32)]
+
+
+class KdCacheTokens(Structure):
+    _fields_ = [
+        ("k", KdTensor), ("v", KdTensor), ("T", c_int32), ("dtype", c_int32), ("n_new", c_void_p),
+        ("in_span", c_void_p), ("span_id", c_void_p), ("is_prefix", c_void_p),
+        ("in_span_stride_b", c_int64), ("span_id_stride_b", c_int64), ("is_prefix_stride_b", c_int64),
+    ]
+
+
+class KdCacheQueries(Structure):
+    _fields_ = [
+        ("q", KdTensor), ("o", KdTensor), ("H", c_int32), ("T", c_int32), ("dtype", c_int32), ("causal", c_int32),
+        ("sm_scale", c_float), ("q_lens", c_void_p), ("lse", c_void_p), ("weights", c_void_p),
+        ("w_stride_b", c_int64), ("w_stride_h", c_int64), ("w_len", c_int32), ("workspace", c_void_p),
+    ]
+
+
+class KdCacheEviction(Structure):
+    _fields_ = [
+        ("weights", c_void_p), ("w_stride_b", c_int64), ("w_stride_h", c_int64), ("w_len", c_int32),
+        ("keep", c_int32), ("recent", c_int32), ("first", c_int32), ("out_table", c_void_p), ("out_table_stride", c_int64),
+        ("index", c_void_p), ("out_weights", c_void_p), ("out_lens", c_void_p),
     ]
 
 
@@ -104,8 +140,14 @@ def load() -> ctypes.CDLL:
                                  c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.kd_metadata_from_tokens.argtypes = [c_void_p, c_int64, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64,
                                             c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.kd_cache_append.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheTokens), c_void_p]
+    lib.kd_cache_attention.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheQueries), c_void_p]
+    lib.kd_cache_attention_workspace.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheQueries), POINTER(c_size_t)]
+    lib.kd_cache_evict.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheEviction), c_void_p]
+    lib.kd_cache_read.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), c_void_p, c_int32, c_int32, POINTER(KdTensor), POINTER(KdTensor), c_void_p]
     for name in ("kd_plan_layout_get", "kd_classify", "kd_mask_dense", "kd_attn_fwd", "kd_attn_bwd", "kd_attn_bwd_hadamard", "kd_attn_bwd_static",
-                 "kd_workspace_bytes", "kd_workspace_bytes_fused", "kd_hadamard", "kd_metadata_from_tokens", "kd_span_index", "kd_span_mean"):
+                 "kd_workspace_bytes", "kd_workspace_bytes_fused", "kd_hadamard", "kd_metadata_from_tokens", "kd_span_index", "kd_span_mean",
+                 "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read"):
         getattr(lib, name).restype = c_int32
     _lib = lib
     return lib

@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include "common.cuh"
+#include "kv_cache.cuh"
 
 namespace kd {
 
@@ -376,6 +377,101 @@ int kd_span_mean(int32_t backward, const void* a, int64_t a_sb, int64_t a_st, vo
   if (rc) return rc;
   return launch_span_mean(backward != 0, a, a_sb, a_st, out, o_sb, o_st, B, T, C, S, dtype, starts, ends, n_starts, n_ends,
                           static_cast<cudaStream_t>(stream));
+}
+
+// ---- the 8-bit cache ----
+
+static int check_cache_strides(const kd_tensor& t, int es, const char* name) {
+  if (!t.ptr) return set_error(KD_ERR_ARG, "%s is null", name);
+  if (!aligned16(t, es)) return set_error(KD_ERR_ALIGN, "%s: pointer and byte strides must be multiples of 16", name);
+  return 0;
+}
+
+static int check_cache(const kd_cache* c, const kd_cache_seqs* s) {
+  if (!c || !s) return set_error(KD_ERR_ARG, "cache / sequences is null");
+  if (c->pages < 1 || c->H < 1) return set_error(KD_ERR_ARG, "bad cache shape pages=%d H=%d", c->pages, c->H);
+  if (c->D < 16 || c->D > 128 || c->D % 16 != 0) return set_error(KD_ERR_ARG, "head dim %d not supported (a multiple of 16 from 16 to 128)", c->D);
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(KD_ERR_ARG, "k / v / k_scale / v_scale is null");
+  if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) != 0) return set_error(KD_ERR_ALIGN, "k / v not 16-byte aligned");
+  if (s->B < 0 || s->blocks < 0) return set_error(KD_ERR_ARG, "bad shape B=%d blocks=%d", s->B, s->blocks);
+  if (s->blocks > (1 << 24)) return set_error(KD_ERR_LIMIT, "blocks=%d exceeds 2^24", s->blocks);
+  if (s->B > 0 && !s->lens) return set_error(KD_ERR_ARG, "lens is null");
+  if (s->B > 0 && s->blocks > 0 && !s->table) return set_error(KD_ERR_ARG, "table is null");
+  if (s->B > 1 && s->table_stride < 0) return set_error(KD_ERR_ARG, "table_stride is negative");
+  return 0;
+}
+
+int kd_cache_append(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream) {
+  int rc = check_cache(c, s);
+  if (rc) return rc;
+  if (!t) return set_error(KD_ERR_ARG, "tokens is null");
+  if (t->T < 0 || t->T > (1 << 30)) return set_error(KD_ERR_ARG, "bad token count %d", t->T);
+  if (t->dtype != KD_F16 && t->dtype != KD_BF16 && t->dtype != KD_F32) return set_error(KD_ERR_ARG, "dtype %d not supported", t->dtype);
+  if (s->B == 0 || t->T == 0) return 0;
+  const int es = t->dtype == KD_F32 ? 4 : 2;
+  if ((rc = check_cache_strides(t->k, es, "k")) != 0 || (rc = check_cache_strides(t->v, es, "v")) != 0) return rc;
+  if ((rc = check_device()) != 0) return rc;
+  return launch_cache_append(*c, *s, *t, static_cast<cudaStream_t>(stream));
+}
+
+int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k,
+                  const kd_tensor* v, void* stream) {
+  int rc = check_cache(c, s);
+  if (rc) return rc;
+  if (count < 0) return set_error(KD_ERR_ARG, "bad token count %d", count);
+  if (dtype != KD_F16 && dtype != KD_BF16 && dtype != KD_F32) return set_error(KD_ERR_ARG, "dtype %d not supported", dtype);
+  if (s->B == 0 || count == 0) return 0;
+  if (!k || !v) return set_error(KD_ERR_ARG, "k / v is null");
+  const int es = dtype == KD_F32 ? 4 : 2;
+  if ((rc = check_cache_strides(*k, es, "k")) != 0 || (rc = check_cache_strides(*v, es, "v")) != 0) return rc;
+  if ((rc = check_device()) != 0) return rc;
+  return launch_cache_read(*c, *s, start, count, dtype, *k, *v, static_cast<cudaStream_t>(stream));
+}
+
+int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream) {
+  int rc = check_cache(c, s);
+  if (rc) return rc;
+  if (!e) return set_error(KD_ERR_ARG, "eviction is null");
+  if (e->keep < 1 || e->recent < 0 || e->first < 0 || e->first > e->keep || e->recent > e->keep - e->first)
+    return set_error(KD_ERR_ARG, "bad eviction keep=%d recent=%d first=%d", e->keep, e->recent, e->first);
+  if (e->w_len < 0) return set_error(KD_ERR_ARG, "w_len is negative");
+  if (s->B == 0) return 0;
+  if ((e->w_len > 0 && !e->weights) || !e->out_table || !e->index || !e->out_weights || !e->out_lens)
+    return set_error(KD_ERR_ARG, "weights / out_table / index / out_weights / out_lens is null");
+  if ((rc = check_device()) != 0) return rc;
+  return launch_cache_evict(*c, *s, *e, static_cast<cudaStream_t>(stream));
+}
+
+static int check_queries(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q) {
+  int rc = check_cache(c, s);
+  if (rc) return rc;
+  if (!q) return set_error(KD_ERR_ARG, "queries is null");
+  if (q->T < 0 || q->H < 1 || q->H % c->H != 0) return set_error(KD_ERR_ARG, "bad queries: T=%d, H=%d for %d heads of keys", q->T, q->H, c->H);
+  if (q->dtype != KD_F16 && q->dtype != KD_BF16) return set_error(KD_ERR_ARG, "dtype %d not supported (fp16 / bf16)", q->dtype);
+  if (static_cast<int64_t>(s->B) * q->H > INT32_MAX / (q->T > 0 ? q->T : 1))
+    return set_error(KD_ERR_LIMIT, "%d x %d x %d query rows are too many", s->B, q->H, q->T);
+  return 0;
+}
+
+int kd_cache_attention_workspace(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes) {
+  const int rc = check_queries(c, s, q);
+  if (rc) return rc;
+  if (!bytes) return set_error(KD_ERR_ARG, "bytes is null");
+  *bytes = s->B == 0 || q->T == 0 ? 0 : cache_attention_workspace(*c, *s, *q);
+  return 0;
+}
+
+int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) {
+  int rc = check_queries(c, s, q);
+  if (rc) return rc;
+  if (!(q->sm_scale > 0.f) || q->sm_scale > 3.0e38f) return set_error(KD_ERR_ARG, "sm_scale must be positive and finite");
+  if (s->B == 0 || q->T == 0) return 0;
+  if ((rc = check_cache_strides(q->q, 2, "q")) != 0 || (rc = check_cache_strides(q->o, 2, "o")) != 0) return rc;
+  if (q->weights && (!q->lse || q->w_len < 0)) return set_error(KD_ERR_ARG, "weights need lse and w_len");
+  if (!q->workspace && cache_attention_workspace(*c, *s, *q) > 0) return set_error(KD_ERR_ARG, "workspace is null");
+  if ((reinterpret_cast<uintptr_t>(q->workspace) & 15u) != 0) return set_error(KD_ERR_ALIGN, "workspace not 16-byte aligned");
+  if ((rc = check_device()) != 0) return rc;
+  return launch_cache_attention(*c, *s, *q, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -71,6 +71,11 @@ struct Library {
   decltype(&kd_cocktail_scores) cocktail_scores = nullptr;
   decltype(&kd_cocktail_grad) cocktail_grad = nullptr;
   decltype(&kd_cast) cast = nullptr;
+  decltype(&kd_cache_append) cache_append = nullptr;
+  decltype(&kd_cache_attention) cache_attention = nullptr;
+  decltype(&kd_cache_attention_workspace) cache_attention_workspace = nullptr;
+  decltype(&kd_cache_evict) cache_evict = nullptr;
+  decltype(&kd_cache_read) cache_read = nullptr;
   decltype(&kd_last_error) last_error = nullptr;
 };
 Library lib;
@@ -94,6 +99,11 @@ void bind(const py::dict& a) {
   take(lib.cocktail_scores, a, "kd_cocktail_scores");
   take(lib.cocktail_grad, a, "kd_cocktail_grad");
   take(lib.cast, a, "kd_cast");
+  take(lib.cache_append, a, "kd_cache_append");
+  take(lib.cache_attention, a, "kd_cache_attention");
+  take(lib.cache_attention_workspace, a, "kd_cache_attention_workspace");
+  take(lib.cache_evict, a, "kd_cache_evict");
+  take(lib.cache_read, a, "kd_cache_read");
   take(lib.last_error, a, "kd_last_error");
 }
 
@@ -962,6 +972,10 @@ Tensor cocktail_scores(const Tensor& x_, const Tensor& tokens_, int64_t tok_span
   return scores;
 }
 
+// ---- 8-bit key/value cache -------------------------------------------------------------------------------------
+
+#include "host_cache.hpp"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1005,4 +1019,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention", &attention, NoGil());
   m.def("metadata_from_tokens", &metadata_from_tokens, NoGil());
   m.def("cocktail_scores", &cocktail_scores, NoGil());
+  py::class_<KVCache, KVCachePtr>(m, "KVCache")
+      .def(py::init<const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&>(), NoGil());
+  m.def("cache_append", &cache_append, NoGil());
+  m.def("cache_attention", &cache_attention, NoGil());
+  m.def("cache_evict", &cache_evict, NoGil());
+  m.def("cache_read", &cache_read, NoGil());
 }

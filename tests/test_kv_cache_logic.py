@@ -1,0 +1,114 @@
+"""CPU tests of the 8-bit cache: the entry points' checks of arguments, and the oracle's number format against torch's."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_cache_oracle as ko
+
+
+def _cache():
+    from kerneldev_b200 import _capi
+    c = _capi.KdCache()
+    c.k = c.v = c.k_scale = c.v_scale = 0x10000   # never read: every call here is refused first
+    c.pages, c.H, c.D = 4, 2, 64
+    s = _capi.KdCacheSeqs()
+    s.table = s.lens = 0x10000
+    s.B, s.blocks, s.table_stride = 1, 2, 2
+    return _capi, _capi.load(), c, s
+
+
+def test_entry_points_reject_bad_arguments_before_touching_cuda():
+    m, lib, c, s = _cache()
+    t = m.KdCacheTokens()
+    t.T, t.dtype = 1, m.KD_BF16
+    ref = ctypes.byref
+
+    def refused(rc, code, text):
+        assert rc == code and text in lib.kd_last_error(), lib.kd_last_error()
+
+    refused(lib.kd_cache_append(None, ref(s), ref(t), None), -1, b"null")
+    refused(lib.kd_cache_append(ref(c), ref(s), None, None), -1, b"null")
+    refused(lib.kd_cache_append(ref(c), ref(s), ref(t), None), -1, b"k is null")
+    t.k.ptr = t.v.ptr = 0x10000
+    t.k.stride_t = 3
+    refused(lib.kd_cache_append(ref(c), ref(s), ref(t), None), -2, b"16")
+    t.k.stride_t, t.dtype = 64, 7
+    refused(lib.kd_cache_append(ref(c), ref(s), ref(t), None), -1, b"dtype")
+    t.dtype, t.T = m.KD_F32, -1
+    refused(lib.kd_cache_append(ref(c), ref(s), ref(t), None), -1, b"count")
+    t.T = 0
+    assert lib.kd_cache_append(ref(c), ref(s), ref(t), None) == 0   # nothing to do
+    for field, value, text in (("D", 72, b"head dim"), ("D", 144, b"head dim"), ("pages", 0, b"shape"), ("H", 0, b"shape"), ("k", 0, b"null"), ("v", 0x10008, b"aligned")):
+        old = getattr(c, field)
+        setattr(c, field, value)
+        refused(lib.kd_cache_append(ref(c), ref(s), ref(t), None), -2 if text == b"aligned" else -1, text)
+        setattr(c, field, old)
+    for field, value, code in (("B", -1, -1), ("blocks", -1, -1), ("blocks", (1 << 24) + 1, -4), ("lens", None, -1), ("table", None, -1)):
+        old = getattr(s, field)
+        setattr(s, field, value)
+        assert lib.kd_cache_append(ref(c), ref(s), ref(t), None) == code
+        setattr(s, field, old)
+    q = m.KdCacheQueries()
+    q.H, q.T, q.dtype, q.sm_scale = 3, 1, m.KD_F16, 1.0
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"H=3 for 2 heads")
+    q.H, q.dtype = 4, m.KD_F32
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"dtype")
+    q.dtype, q.sm_scale = m.KD_F16, float("nan")
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"sm_scale")
+    q.sm_scale = 1.0
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"q is null")
+    q.q.ptr = q.o.ptr = 0x10000
+    q.weights = 0x10000
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"lse")
+    q.T = 1 << 30
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -4, b"rows")
+    n = ctypes.c_size_t(1)
+    q.T = 0
+    assert lib.kd_cache_attention_workspace(ref(c), ref(s), ref(q), ref(n)) == 0 and n.value == 0
+    refused(lib.kd_cache_attention_workspace(ref(c), ref(s), ref(q), None), -1, b"null")
+    e = m.KdCacheEviction()
+    for keep, recent, first in ((0, 0, 0), (4, -1, 0), (4, 0, -1), (4, 3, 2), (4, 5, 0)):
+        e.keep, e.recent, e.first = keep, recent, first
+        refused(lib.kd_cache_evict(ref(c), ref(s), ref(e), None), -1, b"eviction")
+    e.keep, e.recent, e.first = 4, 2, 2
+    refused(lib.kd_cache_evict(ref(c), ref(s), ref(e), None), -1, b"null")
+    refused(lib.kd_cache_read(ref(c), ref(s), None, -1, m.KD_F16, None, None, None), -1, b"count")
+    refused(lib.kd_cache_read(ref(c), ref(s), None, 1, 9, None, None, None), -1, b"dtype")
+    refused(lib.kd_cache_read(ref(c), ref(s), None, 1, m.KD_F16, None, None, None), -1, b"null")
+    s.B = 0
+    assert lib.kd_cache_read(ref(c), ref(s), None, 1, m.KD_F16, None, None, None) == 0
+
+
+def test_cache_has_no_cpu_path():
+    from kerneldev_b200 import KVCache
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        KVCache.empty(2, 2, 64, device="cpu")
+    with pytest.raises(ValueError):
+        KVCache.empty(2, 2, 60, device="cpu")
+
+
+def test_oracle_numbers_are_torchs():
+    """Every number of e4m3 and every point halfway between two, with their neighbours in 64 bits."""
+    grid = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    grid = np.unique(grid[np.isfinite(grid)])
+    mid = (grid[1:] + grid[:-1]) / 2
+    x = np.concatenate([grid, mid, np.nextafter(mid, np.inf), np.nextafter(mid, -np.inf)])
+    x32 = x.astype(np.float32).astype(np.float64)
+    assert np.array_equal(ko.e4m3(x32), torch.tensor(x32).float().to(torch.float8_e4m3fn).double().numpy())
+    assert np.isnan(ko.e4m3([np.inf, np.nan])).all() and ko.e4m3([1e9])[0] == 448
+    assert [ko.exponent(np.array([a])) for a in (0.0, 448.0, 448.0001, 1e30, 1e-30, np.inf)] == [-32, 0, 1, 31, -32, -32]
+
+
+def test_oracle_rule_is_the_operators():
+    """The oracle's descriptors and rule give the mask of the attention oracle."""
+    from oracle import attention_oracle as ao
+    rng = np.random.default_rng(0)
+    B, T = 3, 40
+    ins, pre = rng.random((B, T)) < 0.4, rng.random((B, T)) < 0.3
+    sid = rng.integers(-1, 4, (B, T))
+    mask = np.asarray(ao.dense_mask(T, ins, sid, pre, None, B=B)).reshape(B, T, T).astype(bool)
+    d = ko.descriptors(ins, sid, pre)
+    for b in range(B):
+        assert np.array_equal(ko.rule(d[b], np.arange(T), d[b], np.arange(T)), mask[b])
