@@ -204,7 +204,7 @@ def check_attention(c, q, table, lens, q_lens, got, causal=True, scale=None, wei
     l = lse.double().cpu().numpy()
     assert np.array_equal(np.isinf(l), np.isinf(rl)) and (l[np.isinf(l)] < 0).all()
     fin = np.isfinite(rl)
-    assert (np.abs(l - rl)[fin] <= (2 * delta + 2.0 ** -22 * np.abs(np.where(fin, rl, 0)))[fin]).all(), "LSE"
+    assert (np.abs(l[fin] - rl[fin]) <= (2 * delta)[fin] + 2.0 ** -22 * np.abs(rl[fin])).all(), "LSE"
     if weights is not None:
         w = weights.double().cpu().numpy() - (0 if before is None else before.double().cpu().numpy())
         rw = np.pad(rw, ((0, 0), (0, 0), (0, max(0, w.shape[2] - rw.shape[2]))))[..., :w.shape[2]]
@@ -397,7 +397,10 @@ def test_cache_attention_equals_flash_attention_over_the_same_numbers():
     fo, fl = flash_attention(x[2], k, v, lens=i32(lens), return_lse=True, **m)
     # both round probabilities (to a half, to bfloat16) and outputs: 2**-11 + 2**-8 of sum p |v| and two output roundings, |v| < 4 sigma * 30
     a = flash_attention(x[2], k, v.abs(), lens=i32(lens), **m).float()
-    assert ((o.float() - fo.float()).abs() <= a * (2.0 ** -11 + 2.0 ** -8) + (o.float().abs() + fo.float().abs()) * 2.0 ** -8 + a * 2.0 ** -8).all()
+    # a half has no steps below 2**-24, and probabilities are rounded in units of at least 2**-8 of the row's largest: of a token with less than 2**-14 / 2**8
+    # of it up to 2**-25 / 2**8 = 2**-33 is lost, whatever the row's output is (here 3e-10 where the one heavy token's value is 0)
+    floor = 2.0 ** -33 * v.float().abs().sum(2, keepdim=True)
+    assert ((o.float() - fo.float()).abs() <= a * (2.0 ** -11 + 2.0 ** -8) + (o.float().abs() + fo.float().abs()) * 2.0 ** -8 + a * 2.0 ** -8 + floor).all()
     live = torch.isfinite(fl)
     assert torch.equal(live, torch.isfinite(lse)) and ((fl - lse)[live].abs() <= 2e-3).all()
 
