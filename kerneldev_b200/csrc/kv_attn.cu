@@ -19,11 +19,12 @@
 // taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs.
 #include <algorithm>
 
+#include "attn_common.cuh"
 #include "kv_cache.cuh"
 
 namespace kd {
 
-constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_ROWS = 16, KA_UNIT = 32;
+constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_ROWS = 16, KA_UNIT = 32, KA_STAGES = 2, KA_CTAS = 3;   // CTAs of an SM
 constexpr float KA_OFFSET = 8.f, KA_SLACK = 6.f, KA_LOG2E = 1.4426950408889634f;
 constexpr float KA_TINY = 1e-37f;   // in place of factors that a float flushes to 0 (every score is as good as 0 then): masked scores stay -inf, and not 0 * inf
 
@@ -47,23 +48,25 @@ struct AttnWorkspace {
   float2* part_ml;
 };
 
-// ---- loads --------------------------------------------------------------------------------------------------------
+// ---- a unit in shared memory --------------------------------------------------------------------------------------
 
-// N bytes from global memory that nothing writes while the kernel runs
 template <int N>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* w) {
+__device__ __forceinline__ void lds(uint32_t at, uint32_t* w) {
   if constexpr (N == 16) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
   } else if constexpr (N == 8) {
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
   } else if constexpr (N == 4) {
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at));
   } else {
     uint16_t h;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(h) : "l"(p));
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at));
     w[0] = h;
   }
 }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 // How a row of D bytes is spread over lanes. K: the four lanes t of a quad own pieces of KU bytes, 4 KU apart; V: the eight lanes g pieces of VU bytes.
 template <int D>
@@ -77,25 +80,52 @@ struct Spread {
   static __device__ __forceinline__ int v_dim(int m, int n) { return 8 * VU * (m / VU) + VU * n + m % VU; }
 };
 
-// lane (g, t): its pieces of the four 8-token tiles of a unit
+// A warp's copy of a unit: K, V, descriptors, scales. Rows of 128 or 64 bytes would put all rows into the same banks: the 16-byte pieces of a
+// row change places, so that the eight lanes of a part of a load (two g, four t) find theirs in eight different ones: for K by the row's lowest bit,
+// for V by the two above it.
 template <int D>
-__device__ __forceinline__ void load_keys(const uint8_t* unit, int g, int t, uint32_t (&k)[4][Spread<D>::K_WORDS]) {
-  using S = Spread<D>;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < S::K_PIECES; ++i) load_bytes<S::KU>(unit + (8 * j + g) * D + 4 * S::KU * i + S::KU * t, &k[j][i * (S::KU / 4)]);
-}
-// ... its pieces of the tokens 2t, 2t + 1, 2t + 8, 2t + 9 of 16
+struct Stage {
+  static constexpr int V_AT = KA_UNIT * D, DESC_AT = 2 * V_AT, SCALE_AT = DESC_AT + KA_UNIT * 4, BYTES = SCALE_AT + 128;
+  static __device__ __forceinline__ uint32_t k_place(uint32_t o) { return D == 128 ? o ^ ((o >> 1) & 64u) : o; }
+  static __device__ __forceinline__ uint32_t v_place(uint32_t o) { return D == 128 ? o ^ ((o >> 3) & 96u) : D == 64 ? o ^ ((o >> 2) & 96u) : o; }
+};
+// Where a lane finds things in its stage. The places of later steps and tokens are at fixed distances: the bits that a place depends on are the lane's own, but
+// for every second step of V's copy at 128 bytes (bit 9) and V's odd tokens at 64 (bit 6).
 template <int D>
-__device__ __forceinline__ void load_values(const uint8_t* half, int g, int t, uint32_t (&v)[4][Spread<D>::V_WORDS]) {
-  using S = Spread<D>;
+struct Lane {
+  uint32_t copy_k, copy_v[2], k[Spread<D>::K_PIECES], v[2];
+  __device__ __forceinline__ Lane() {
+    using S = Stage<D>;
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    copy_k = S::k_place(lane * 16);
+    copy_v[0] = S::V_AT + S::v_place(lane * 16);
+    copy_v[1] = S::V_AT + S::v_place(lane * 16 + 512);
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int i = 0; i < Spread<D>::K_PIECES; ++i) k[i] = S::k_place(g * D + 4 * Spread<D>::KU * i + Spread<D>::KU * t);
+    v[0] = S::V_AT + S::v_place(2 * t * D + Spread<D>::VU * g);
+    v[1] = S::V_AT + S::v_place((2 * t + 1) * D + Spread<D>::VU * g);
+  }
+  // one operand's bytes, 16 a lane and step
+  template <bool kV>
+  __device__ __forceinline__ void copy(uint32_t stage, const uint8_t* from) const {
 #pragma unroll
-    for (int i = 0; i < S::V_PIECES; ++i)
-      load_bytes<S::VU>(half + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 8 * S::VU * i + S::VU * g, &v[r][i * (S::VU > 4 ? S::VU / 4 : 1)]);
-}
+    for (int i = 0; i < D / 16; ++i) cp_async16(stage + (!kV ? copy_k + 512 * i : copy_v[i & 1] + 512 * (i & ~1)), from + (threadIdx.x & 31) * 16 + 512 * i);
+  }
+  // lane (g, t): its pieces of an 8-token tile of K
+  __device__ __forceinline__ void load_keys(uint32_t stage, int j, uint32_t (&w)[Spread<D>::K_WORDS]) const {
+    using S = Spread<D>;
+#pragma unroll
+    for (int i = 0; i < S::K_PIECES; ++i) lds<S::KU>(stage + k[i] + 8 * D * j, &w[i * (S::KU / 4)]);
+  }
+  // ... its pieces of the tokens 2t, 2t + 1, 2t + 8, 2t + 9 of 16
+  __device__ __forceinline__ void load_values(uint32_t stage, int half, uint32_t (&w)[4][Spread<D>::V_WORDS]) const {
+    using S = Spread<D>;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < S::V_PIECES; ++i) lds<S::VU>(stage + v[r & 1] + (16 * half + 8 * (r >> 1)) * D + 8 * S::VU * i, &w[r][i * (S::VU > 4 ? S::VU / 4 : 1)]);
+  }
+};
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -105,16 +135,23 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t 
 
 // S of a unit: 16 rows against 32 tokens. q: the A operands of every step, [step][lane]
 template <int D>
-__device__ __forceinline__ void scores(const uint4* q, int lane, const uint32_t (&k)[4][Spread<D>::K_WORDS], float (&c)[4][4]) {
+__device__ __forceinline__ void scores(uint32_t stage, const Lane<D>& at, const uint4* q, float (&c)[4][4]) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int x = 0; x < 4; ++x) c[j][x] = 0.f;
+  uint32_t k[4][Spread<D>::K_WORDS];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) at.load_keys(stage, j, k[j]);
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
     const uint4 a = q[s * 32 + lane];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mma_f16(c[j], a, e4m3x2_to_f16x2(k[j][s] & 0xFFFFu), e4m3x2_to_f16x2(k[j][s] >> 16));
+    for (int j = 0; j < 4; ++j) {
+      const HalfPairs b = e4m3x4_to_f16x4(k[j][s]);
+      mma_f16(c[j], a, b.lo, b.hi);
+    }
   }
 }
 
@@ -138,17 +175,19 @@ __device__ __forceinline__ void add_values(float (&o)[D / 8][4], const uint4& p,
         const uint32_t n0 = nan_bytes(b0), n1 = nan_bytes(b1);
         b0 &= ~n0;
         b1 &= ~n1;
+        const HalfPairs one0 = e4m3x4_to_f16x4(n0 & 0x38383838u), one1 = e4m3x4_to_f16x4(n1 & 0x38383838u);   // 0x38: 1 in e4m3
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float hit[4] = {0.f, 0.f, 0.f, 0.f};   // 0x38: 1 in e4m3
-          mma_f16(hit, vis, e4m3x2_to_f16x2((n0 >> (16 * x)) & 0x3838u), e4m3x2_to_f16x2((n1 >> (16 * x)) & 0x3838u));
+          float hit[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16(hit, vis, x == 0 ? one0.lo : one0.hi, x == 0 ? one1.lo : one1.hi);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (hit[i] > 0.f) o[m + x][i] = __uint_as_float(0x7FC00000u);
         }
       }
-      mma_f16(o[m], p, e4m3x2_to_f16x2(b0 & 0xFFFFu), e4m3x2_to_f16x2(b1 & 0xFFFFu));
-      mma_f16(o[m + 1], p, e4m3x2_to_f16x2(b0 >> 16), e4m3x2_to_f16x2(b1 >> 16));
+      const HalfPairs h0 = e4m3x4_to_f16x4(b0), h1 = e4m3x4_to_f16x4(b1);
+      mma_f16(o[m], p, h0.lo, h1.lo);
+      mma_f16(o[m + 1], p, h0.hi, h1.hi);
     }
   }
 }
@@ -186,70 +225,60 @@ template <int D>
 struct QueryTile {
   uint4 frag[D / 16][32];
   RowMask mask[KA_ROWS];
-  int exponent[KA_ROWS];   // of the power of two that a row is multiplied with
   float factor[KA_ROWS];   // what its products are to be multiplied with, sm_scale and log2(e) among it
   int min_limit;           // of the rows that see anything
 };
 
-// Q's tile as A operands in shared memory, all threads of the CTA; ends with a barrier
+// Q's tile as A operands in shared memory, all threads of the CTA; ends with a barrier. bfloat16 rows are multiplied with a power of two that brings the largest
+// finite number to 2^14, so that halves hold them (what falls below a half's subnormals is 2^-38 of the largest).
 template <int D>
 __device__ __forceinline__ void load_queries(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int G, int rows, QueryTile<D>& q) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int PER = KA_ROWS / KA_WARPS;   // rows of a warp, four numbers of each to a lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = 4 * lane;
   const bool bf16 = p.dtype == KD_BF16;
-  auto row_ptr = [&](int r) {
-    const int i = r / G, hq = it.h * G + r - i * G;
-    return static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + i * p.q.stride_t;
-  };
-  if (tid < KA_ROWS) {
-    const RowMask m = row_mask(c, s, p, it, it.tile * KA_ROWS + tid, G, rows, query_count(c, p, it.b));
-    q.mask[tid] = m;
-    const int low = __reduce_min_sync(0xFFFFu, m.limit > 0 ? m.limit : INT_MAX);
-    if (tid == 0) q.min_limit = low;
-  }
-  // bfloat16 rows: times a power of two that brings the largest finite number to 2^14, so that halves hold them (what falls below a half's
-  // subnormals is 2^-38 of the largest)
-  for (int r = warp; r < KA_ROWS; r += KA_WARPS) {
-    int e = 0;
-    const int row = it.tile * KA_ROWS + r;
-    if (bf16 && row < rows) {
-      const uint16_t* x = row_ptr(row);
-      uint32_t top = 0;
-      for (int d = lane; d < D; d += 32) {
-        const uint32_t u = x[d] & 0x7FFFu;
-        top = max(top, u < 0x7F80u ? u : 0u);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
-    }
-    if (lane == 0) {
-      q.exponent[r] = e;
-      q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < D / 16 * 32; i += KA_THREADS) {
-    const int step = i >> 5, l = i & 31, g = l >> 2, t = l & 3, d = Spread<D>::k_dim(step, t);
-    uint32_t w[4];
+  uint2 v[PER];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {   // rows g and g + 8
-      const int row = it.tile * KA_ROWS + g + 8 * x;
-      uint2 v = make_uint2(0u, 0u);
-      if (row < rows) v = *reinterpret_cast<const uint2*>(row_ptr(row) + d);
-      if (bf16) {
-        const float f = exp2i(q.exponent[g + 8 * x]);
-        const float2 a = unpack2<true>(v.x), b = unpack2<true>(v.y);
-        v = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
-      }
-      w[x] = v.x;
-      w[2 + x] = v.y;
+  for (int i = 0; i < PER; ++i) {
+    const int row = it.tile * KA_ROWS + warp * PER + i;
+    v[i] = make_uint2(0u, 0u);
+    if (row < rows && d < D) {
+      const int n = row / G, hq = it.h * G + row - n * G;
+      v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
     }
-    q.frag[step][l] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (threadIdx.x < KA_ROWS) {
+    const RowMask m = row_mask(c, s, p, it, it.tile * KA_ROWS + threadIdx.x, G, rows, query_count(c, p, it.b));
+    q.mask[threadIdx.x] = m;
+    const int low = __reduce_min_sync(0xFFFFu, m.limit > 0 ? m.limit : INT_MAX);
+    if (threadIdx.x == 0) q.min_limit = low;
+  }
+  // the step and quad lane that hold dims d .. d + 3 (see Spread::k_dim)
+  constexpr int KU = Spread<D>::KU;
+  const int step = d / (4 * KU) * (KU / 4) + d % KU / 4, quad = d % (4 * KU) / KU;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = warp * PER + i;
+    int e = 0;
+    if (bf16) {
+      auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
+      const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[i].x), size(v[i].x >> 16)), max(size(v[i].y), size(v[i].y >> 16))));
+      if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
+      const float f = exp2i(e);
+      const float2 a = unpack2<true>(v[i].x), b = unpack2<true>(v[i].y);
+      v[i] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+    }
+    if (lane == 0) q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+    if (d < D) {   // registers 0 and 2 of the operand are those of rows 0 to 7, 1 and 3 of rows 8 to 15
+      uint32_t* w = reinterpret_cast<uint32_t*>(&q.frag[step][(r & 7) * 4 + quad]) + (r >> 3);
+      w[0] = v[i].x;
+      w[2] = v[i].y;
+    }
   }
   __syncthreads();
 }
 
 // masks the scores of a unit: token of c[j][x]: j0 + 8 j + 2 t + (x & 1), row of c[j][x]: lo or hi
-__device__ __forceinline__ void mask_scores(float (&c)[4][4], const kd_cache& cache, const uint32_t* desc, int j0, int t, int end, const RowMask& lo, const RowMask& hi) {
+__device__ __forceinline__ void mask_scores(float (&c)[4][4], const uint32_t* desc, int j0, int t, int end, const RowMask& lo, const RowMask& hi) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int token = j0 + 8 * j + 2 * t;
@@ -268,37 +297,47 @@ __device__ __forceinline__ void mask_scores(float (&c)[4][4], const kd_cache& ca
 
 // ---- the walk -----------------------------------------------------------------------------------------------------
 
-// A warp's share of units first, first + KA_WARPS, ... below `last` of one head of a sequence. The accumulators' rows are lane / 4 and that plus 8.
+// A warp's share of units first, first + KA_WARPS, ... below `last` of one head of a sequence, through a ring of copies of its own: while
+// one unit is worked on, KA_STAGES - 1 are on their way. The accumulators' rows are lane / 4 and that plus 8.
 template <int D>
 struct Walker {
-  using S = Spread<D>;
   float o[D / 8][4];
   float ref[2], sum[2];
 
-  struct Unit {
-    int page;
-    uint32_t k[4][S::K_WORDS];
-    float ks, vs;
-  };
-
-  __device__ __forceinline__ void fetch(const kd_cache& c, int h, int unit, int page, int g, int t, Unit& u) {
-    u.page = page;
-    u.ks = u.vs = 1.f;
-    if (page >= 0) {
-      const size_t at = block_index(c, page, h);
-      load_keys<D>(static_cast<const uint8_t*>(c.k) + (at * KC_PAGE + (unit & 1) * KA_UNIT) * D, g, t, u.k);
-      u.ks = c.k_scale[at];
-      u.vs = c.v_scale[at];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < S::K_WORDS; ++i) u.k[j][i] = 0u;
+  // starts the copies of a unit (nothing at or beyond `last`)
+  static __device__ __forceinline__ void fetch(const kd_cache& c, const Lane<D>& place, int h, int unit, int last, int page, char* stage) {
+    const int lane = threadIdx.x & 31;
+    if (unit < last) {
+      const uint32_t to = smem_u32(stage);
+      page = checked_page(c, page);
+      if (page >= 0) {
+        const size_t at = block_index(c, page, h), token = at * KC_PAGE + (unit & 1) * KA_UNIT;
+        place.template copy<false>(to, static_cast<const uint8_t*>(c.k) + token * D);
+        place.template copy<true>(to, static_cast<const uint8_t*>(c.v) + token * D);
+        if (c.desc != nullptr && lane < 8) cp_async16(to + Stage<D>::DESC_AT + lane * 16, c.desc + token + lane * 4);
+        if (lane < 2) cp_async4(to + Stage<D>::SCALE_AT + lane * 4, (lane == 0 ? c.k_scale : c.v_scale) + at);
+      } else if (lane < 2) {
+        reinterpret_cast<float*>(stage + Stage<D>::SCALE_AT)[lane] = 1.f;   // (any bytes: all of it is masked)
+      }
+      if (lane == 0) *reinterpret_cast<int*>(stage + Stage<D>::SCALE_AT + 8) = page;
     }
+    cp_async_commit();
+  }
+  // the ring's first copies, and the page of the unit behind them
+  static __device__ __forceinline__ int begin(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, int first, int last, char* ring) {
+    const int32_t* table = s.table + it.b * s.table_stride;
+    auto page_at = [&](int i) { return first + i * KA_WARPS < last ? table[(first + i * KA_WARPS) >> 1] : -1; };
+    int pages[KA_STAGES];
+#pragma unroll
+    for (int i = 0; i < KA_STAGES; ++i) pages[i] = page_at(i);
+#pragma unroll
+    for (int i = 0; i + 1 < KA_STAGES; ++i) fetch(c, place, it.h, first + i * KA_WARPS, last, pages[i], ring + i * Stage<D>::BYTES);
+    return pages[KA_STAGES - 1];
   }
 
+  // next_page: what begin returned
   template <bool kSafe>
-  __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Item& it, const QueryTile<D>& q, int first, int last) {
+  __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, const QueryTile<D>& q, int first, int last, int next_page, char* ring) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     ref[0] = ref[1] = -INFINITY;
     sum[0] = sum[1] = 0.f;
@@ -306,28 +345,26 @@ struct Walker {
     for (int m = 0; m < D / 8; ++m)
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[m][x] = 0.f;
-    if (first >= last) return;
     const int32_t* table = s.table + it.b * s.table_stride;
-    const RowMask lo = q.mask[g], hi = q.mask[g + 8];
-    const float f_lo = q.factor[g], f_hi = q.factor[g + 8];
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
-    Unit u;
-    fetch(c, it.h, first, checked_page(c, table[first >> 1]), g, t, u);
+    int slot = 0;
     for (int unit = first; unit < last; unit += KA_WARPS) {
-      const int page = u.page, j0 = unit * KA_UNIT, next = unit + KA_WARPS;
-      const size_t at = block_index(c, max(page, 0), it.h) * KC_PAGE + (unit & 1) * KA_UNIT;
-      int next_page = -1;
-      if (next < last) next_page = table[next >> 1];
-      uint32_t v[2][4][S::V_WORDS];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) load_values<D>(static_cast<const uint8_t*>(c.v) + (at + 16 * i) * D, g, t, v[i]);
+      cp_async_wait<KA_STAGES - 2>();
+      __syncwarp();   // everyone's copies of this unit are there, and everyone is done with the one before it, whose place the next one takes
+      const int ahead = unit + (KA_STAGES - 1) * KA_WARPS;
+      fetch(c, place, it.h, ahead, last, next_page, ring + (slot == 0 ? KA_STAGES - 1 : slot - 1) * Stage<D>::BYTES);
+      if (ahead + KA_WARPS < last) next_page = table[(ahead + KA_WARPS) >> 1];
+      const char* stage = ring + slot * Stage<D>::BYTES;
+      const uint32_t at = smem_u32(stage);
+      slot = slot + 1 == KA_STAGES ? 0 : slot + 1;
+      const float* scale = reinterpret_cast<const float*>(stage + Stage<D>::SCALE_AT);
+      const int page = reinterpret_cast<const int*>(scale)[2], j0 = unit * KA_UNIT;
       float sc[4][4];
-      scores<D>(&q.frag[0][0], lane, u.k, sc);
-      const float k_lo = fmaxf(u.ks * f_lo, KA_TINY), k_hi = fmaxf(u.ks * f_hi, KA_TINY);
-      const int ev = scale_exponent(u.vs);
-      if (next < last) fetch(c, it.h, next, checked_page(c, next_page), g, t, u);
+      scores<D>(at, place, &q.frag[0][0], sc);
+      const float k_lo = fmaxf(scale[0] * q.factor[g], KA_TINY), k_hi = fmaxf(scale[0] * q.factor[g + 8], KA_TINY);
+      const int ev = scale_exponent(scale[1]);
       if (page < 0 || j0 + KA_UNIT > free_end)
-        mask_scores(sc, c, c.desc != nullptr ? c.desc + at : nullptr, j0, t, page < 0 ? 0 : it.len, lo, hi);
+        mask_scores(sc, c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr, j0, t, page < 0 ? 0 : it.len, q.mask[g], q.mask[g + 8]);
       // the rows' maxima over the quad
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -356,7 +393,7 @@ struct Walker {
       }
       const float a_lo = ref[0] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[0];
       const float a_hi = ref[1] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[1];
-      uint4 vis[2];
+      uint4 pr[2], vis[2];
       if constexpr (kSafe) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -376,12 +413,18 @@ struct Walker {
       sum[0] = fmaf(part[0], unscale, sum[0]);
       sum[1] = fmaf(part[1], unscale, sum[1]);
 #pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pr[i] = make_uint4(pack2<false>(sc[2 * i][0], sc[2 * i][1]), pack2<false>(sc[2 * i][2], sc[2 * i][3]), pack2<false>(sc[2 * i + 1][0], sc[2 * i + 1][1]),
+                           pack2<false>(sc[2 * i + 1][2], sc[2 * i + 1][3]));
+#pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint4 pr = make_uint4(pack2<false>(sc[2 * i][0], sc[2 * i][1]), pack2<false>(sc[2 * i][2], sc[2 * i][3]), pack2<false>(sc[2 * i + 1][0], sc[2 * i + 1][1]),
-                                    pack2<false>(sc[2 * i + 1][2], sc[2 * i + 1][3]));
-        add_values<D, kSafe>(o, pr, kSafe ? vis[i] : pr, v[i]);
+        uint32_t v[4][Spread<D>::V_WORDS];
+        place.load_values(at, i, v);
+        add_values<D, kSafe>(o, pr[i], kSafe ? vis[i] : pr[i], v);
       }
     }
+    cp_async_wait<0>();
+    __syncwarp();
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
@@ -405,56 +448,93 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
   if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
 }
 
-// Which (sequence, head and tile) a page of the flat order belongs to, and its place there: sequences in turn, each once for every head and tile. One warp.
+// The flat order of all pages: sequences in turn, each once for every head and tile. A warp holds the page counts of the first 128 sequences, in its lanes.
 struct FlatPlace {
   int b, ht, page, pages;   // page: index within the item
 };
-__device__ __forceinline__ int64_t flat_total(const kd_cache& c, const kd_cache_seqs& s, int HT) {
-  int64_t n = 0;
-  for (int b = threadIdx.x & 31; b < s.B; b += 32) n += (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * HT;
-}
-__device__ __forceinline__ FlatPlace flat_find(const kd_cache& c, const kd_cache_seqs& s, int HT, int64_t at) {
-  const int lane = threadIdx.x & 31;
-  int64_t before = 0;
-  for (int base = 0; base < s.B; base += 32) {
-    const int b = base + lane, pages = b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0;
-    int64_t upto = static_cast<int64_t>(pages) * HT;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += up;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, before + upto > at);
-    if (past != 0u) {
-      const int l = __ffs(past) - 1;
-      const int n = __shfl_sync(0xffffffffu, pages, l);
-      const int64_t rest = at - before - (__shfl_sync(0xffffffffu, upto, l) - static_cast<int64_t>(n) * HT);
-      return FlatPlace{base + l, static_cast<int>(rest / n), static_cast<int>(rest % n), n};
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+struct FlatOrder {
+  static constexpr int HELD = 4;
+  int held[HELD];
+  int64_t total;   // pages
+
+  static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
+  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {   // of sequence 32 i + lane
+    if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
+    return pages_of(c, s, 32 * i + (threadIdx.x & 31));
   }
-  return FlatPlace{-1, 0, 0, 0};
-}
+  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) held[i] = pages_of(c, s, 32 * i + lane);
+    int64_t n = held[0] + held[1] + held[2] + held[3];
+    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    total = n * HT;
+  }
+  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, int64_t at) const {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int i = 0; 32 * i < s.B; ++i) {
+      const int mine = pages(c, s, i);
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * HT > at);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l);
+        const uint64_t rest = static_cast<uint64_t>(at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT);   // less than n * HT
+        const uint64_t ht = rest <= UINT32_MAX ? static_cast<uint32_t>(rest) / static_cast<uint32_t>(n) : rest / static_cast<uint32_t>(n);
+        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n};
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return FlatPlace{-1, 0, 0, 0};
+  }
+  // pages of the sequences before b
+  __device__ __forceinline__ int64_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
+    const int lane = threadIdx.x & 31;
+    int64_t n = 0;
+    for (int i = 0; 32 * i < b; ++i)
+      if (32 * i + lane < b) n += pages(c, s, i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+  }
+};
+
+// Shared memory of the kernel. A warp's rows of O take the place of its ring when it is through.
+template <int D>
+struct AttnShared {
+  union {
+    char ring[KA_STAGES * Stage<D>::BYTES];
+    float o[KA_ROWS][D + 4];
+  } warp[KA_WARPS];
+  QueryTile<D> q;
+  float2 ml[KA_WARPS][KA_ROWS];
+};
 
 // CTAs that share the pages: two pages, a unit for each warp, are the least that one takes. (None takes no page: the join reads a part of every CTA of an item.)
 __device__ __forceinline__ int64_t sharing_ctas(const AttnShape& shape, int64_t total) { return min(static_cast<int64_t>(shape.ctas), (total + 1) / 2); }
 
 template <int D>
-__global__ void __launch_bounds__(KA_THREADS, 2)
+__global__ void __launch_bounds__(KA_THREADS, KA_CTAS)
 cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                        const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
   pdl_wait();
   pdl_launch_dependents();
-  __shared__ QueryTile<D> q;
-  __shared__ float s_o[KA_WARPS][KA_ROWS][D + 4];
-  __shared__ float2 s_ml[KA_WARPS][KA_ROWS];
+  extern __shared__ __align__(1024) char smem[];
+  AttnShared<D>& sh = *reinterpret_cast<AttnShared<D>*>(smem);
+  QueryTile<D>& q = sh.q;
+  const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
   int64_t at = 0, end = 1;
+  const FlatOrder order(c, s, HT);
   if (shape.ctas > 0) {
-    const int64_t total = flat_total(c, s, HT);
+    const int64_t total = order.total;
     const int64_t ctas = sharing_ctas(shape, total);
     if (blockIdx.x >= ctas) return;
     at = total * blockIdx.x / ctas;
@@ -465,7 +545,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
     Item it;
     int page0, pages, here;
     if (shape.ctas > 0) {
-      const FlatPlace f = flat_find(c, s, HT, at);
+      const FlatPlace f = order.find(c, s, HT, at);
       it.b = f.b;
       it.h = f.ht / shape.tiles;
       it.tile = f.ht - it.h * shape.tiles;
@@ -482,30 +562,35 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
       page0 = 0;
       pages = here = (it.len + KC_PAGE - 1) / KC_PAGE;
     }
+    const int first = 2 * page0 + warp, last = min(2 * (page0 + here), (it.len + KA_UNIT - 1) / KA_UNIT);
+    char* ring = sh.warp[warp].ring;
+    int next = Walker<D>::begin(c, s, place, it, first, last, ring);
     load_queries<D>(c, s, p, it, shape.G, shape.rows, q);
-    const int last = min(2 * (page0 + here), (it.len + KA_UNIT - 1) / KA_UNIT);
     Walker<D> w;
-    w.template walk<false>(c, s, it, q, 2 * page0 + warp, last);
-    if (w.any_nan()) w.template walk<true>(c, s, it, q, 2 * page0 + warp, last);
+    w.template walk<false>(c, s, place, it, q, first, last, next, ring);
+    if (w.any_nan()) {
+      next = Walker<D>::begin(c, s, place, it, first, last, ring);
+      w.template walk<true>(c, s, place, it, q, first, last, next, ring);
+    }
     // the warps' parts: maxima and sums first, then everyone's rows on one scale
     if (t == 0) {
-      s_ml[warp][g] = make_float2(w.ref[0], w.sum[0]);
-      s_ml[warp][g + 8] = make_float2(w.ref[1], w.sum[1]);
+      sh.ml[warp][g] = make_float2(w.ref[0], w.sum[0]);
+      sh.ml[warp][g + 8] = make_float2(w.ref[1], w.sum[1]);
     }
 #pragma unroll
     for (int m = 0; m < D / 8; ++m)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s_o[warp][g + 8 * (x >> 1)][Spread<D>::v_dim(m, 2 * t + (x & 1))] = w.o[m][x];
+      for (int x = 0; x < 4; ++x) sh.warp[warp].o[g + 8 * (x >> 1)][Spread<D>::v_dim(m, 2 * t + (x & 1))] = w.o[m][x];
     __syncthreads();
     const int r = tid / 8, row_of_head = it.tile * KA_ROWS + r;
     if (row_of_head < shape.rows) {
       float ref = -INFINITY, sum = 0.f, scale[KA_WARPS];
 #pragma unroll
-      for (int i = 0; i < KA_WARPS; ++i) ref = fmaxf(ref, s_ml[i][r].x);
+      for (int i = 0; i < KA_WARPS; ++i) ref = fmaxf(ref, sh.ml[i][r].x);
 #pragma unroll
       for (int i = 0; i < KA_WARPS; ++i) {
-        scale[i] = s_ml[i][r].x == -INFINITY ? 0.f : fast_exp2(s_ml[i][r].x - ref);
-        sum = fmaf(s_ml[i][r].y, scale[i], sum);
+        scale[i] = sh.ml[i][r].x == -INFINITY ? 0.f : fast_exp2(sh.ml[i][r].x - ref);
+        sum = fmaf(sh.ml[i][r].y, scale[i], sum);
       }
       const int i = row_of_head / shape.G, hq = it.h * shape.G + row_of_head - i * shape.G;
       const bool whole = here == pages, live = q.mask[r].limit > 0;
@@ -517,8 +602,8 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
         float x = 0.f, y = 0.f;
 #pragma unroll
         for (int k = 0; k < KA_WARPS; ++k) {
-          x = fmaf(s_o[k][r][d], scale[k], x);
-          y = fmaf(s_o[k][r][d + 1], scale[k], y);
+          x = fmaf(sh.warp[k].o[r][d], scale[k], x);
+          y = fmaf(sh.warp[k].o[r][d + 1], scale[k], y);
         }
         if (whole) {
           if (inv == 0.f) x = y = 0.f;
@@ -547,13 +632,10 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
   const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5, HT = c.H * shape.tiles;
   const int row_of_head = blockIdx.x % shape.rows, bh = blockIdx.x / shape.rows, b = bh / c.H, h = bh - b * c.H;
   const int tile = row_of_head / KA_ROWS, r = row_of_head - tile * KA_ROWS;
-  const int64_t total = flat_total(c, s, HT), ctas = sharing_ctas(shape, total);
-  int64_t first = 0;   // the item's first page in the flat order
-  for (int i = lane; i < b; i += 32) first += (sequence_length(c, s, i) + KC_PAGE - 1) / KC_PAGE;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+  const FlatOrder order(c, s, HT);
+  const int64_t total = order.total, ctas = sharing_ctas(shape, total);
   const int len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
-  first = first * HT + static_cast<int64_t>(h * shape.tiles + tile) * pages;
+  const int64_t first = order.before(c, s, b) * HT + static_cast<int64_t>(h * shape.tiles + tile) * pages;   // the item's first page in the flat order
   int c0 = 0, c1 = -1;
   if (pages > 0) {
     c0 = static_cast<int>(((first + 1) * ctas - 1) / total);
@@ -599,67 +681,87 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
   if (tid == 0) write_stats(p, ws, shape.stats, (static_cast<size_t>(b) * p.H + hq) * p.T + i, live, ref, sum);
 }
 
-// weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A CTA has one page's 64 tokens for all rows: warps 0, 2 and
-// 1, 3 share a unit and take the tiles of rows in turn, so that nothing is added twice and the order is fixed.
+// weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
+// rows, so that nothing is added twice and the order is fixed; a CTA KW_PAGES pages of one head.
+constexpr int KW_PAGES = 4, KW_UNITS = 2 * KW_PAGES;
 template <int D>
 __global__ void __launch_bounds__(KA_THREADS)
 cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                      const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
   pdl_wait();
   pdl_launch_dependents();
-  __shared__ QueryTile<D> q;
+  constexpr int MINE = KW_UNITS / KA_WARPS;
+  extern __shared__ __align__(1024) char smem[];
+  char* stages = smem + (threadIdx.x >> 5) * MINE * Stage<D>::BYTES;
+  QueryTile<D>& q = *reinterpret_cast<QueryTile<D>*>(smem + KW_UNITS * Stage<D>::BYTES);
   __shared__ float2 s_stat[KA_ROWS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const Lane<D> place;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, groups = (s.blocks + KW_PAGES - 1) / KW_PAGES;
   uint32_t item = blockIdx.x;
-  const int block = static_cast<int>(item % static_cast<uint32_t>(s.blocks));
-  item /= static_cast<uint32_t>(s.blocks);
+  const int first = static_cast<int>(item % static_cast<uint32_t>(groups)) * KW_UNITS + warp;
+  item /= static_cast<uint32_t>(groups);
   Item it;
   it.h = static_cast<int>(item % static_cast<uint32_t>(c.H));
   it.b = static_cast<int>(item / static_cast<uint32_t>(c.H));
   it.len = sequence_length(c, s, it.b);
-  if (block * KC_PAGE >= it.len) return;
-  const int page = page_of(c, s, it.b, block);
-  if (page < 0) return;
-  const int unit = 2 * block + warp, j0 = unit * KA_UNIT;   // warps 0 and 1 work
-  const size_t at = block_index(c, page, it.h);
-  uint32_t k[4][Spread<D>::K_WORDS];
-  if (warp < 2) load_keys<D>(static_cast<const uint8_t*>(c.k) + (at * KC_PAGE + warp * KA_UNIT) * D, g, t, k);
-  const float ks = c.k_scale[at];
-  float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if ((first - warp) * KA_UNIT >= it.len) return;
+  int page[MINE];
+  float ks[MINE], sums[MINE][8];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int unit = first + i * KA_WARPS;
+    page[i] = unit * KA_UNIT < it.len ? page_of(c, s, it.b, unit >> 1) : -1;
+    ks[i] = 1.f;
+    if (page[i] >= 0) {
+      const size_t at = block_index(c, page[i], it.h), token = at * KC_PAGE + (unit & 1) * KA_UNIT;
+      const uint32_t to = smem_u32(stages + i * Stage<D>::BYTES);
+      place.template copy<false>(to, static_cast<const uint8_t*>(c.k) + token * D);
+      if (c.desc != nullptr && lane < 8) cp_async16(to + Stage<D>::DESC_AT + lane * 16, c.desc + token + lane * 4);
+      ks[i] = c.k_scale[at];
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sums[i][x] = 0.f;
+  }
+  cp_async_commit();
   for (it.tile = 0; it.tile < shape.tiles; ++it.tile) {
     load_queries<D>(c, s, p, it, shape.G, shape.rows, q);
     if (tid < KA_ROWS) {
       const int r = it.tile * KA_ROWS + tid, i = r / shape.G;
       s_stat[tid] = r < shape.rows ? ws.stats[(static_cast<size_t>(it.b) * p.H + it.h * shape.G + r - i * shape.G) * p.T + i] : make_float2(0.f, 0.f);
     }
+    cp_async_wait<0>();
     __syncthreads();
-    if (warp < 2) {
+    const float2 st[2] = {s_stat[g], s_stat[g + 8]};
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      if (page[i] < 0) continue;
+      const char* stage = stages + i * Stage<D>::BYTES;
+      const int j0 = (first + i * KA_WARPS) * KA_UNIT;
       float sc[4][4];
-      scores<D>(&q.frag[0][0], lane, k, sc);
+      scores<D>(smem_u32(stage), place, &q.frag[0][0], sc);
       if (c.desc != nullptr || j0 + KA_UNIT > q.min_limit)
-        mask_scores(sc, c, c.desc != nullptr ? c.desc + at * KC_PAGE + warp * KA_UNIT : nullptr, j0, t, it.len, q.mask[g], q.mask[g + 8]);
-      const float2 st[2] = {s_stat[g], s_stat[g + 8]};
-      const float f[2] = {fmaxf(q.factor[g] * ks, KA_TINY), fmaxf(q.factor[g + 8] * ks, KA_TINY)};
+        mask_scores(sc, c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr, j0, t, it.len, q.mask[g], q.mask[g + 8]);
+      const float f[2] = {fmaxf(q.factor[g] * ks[i], KA_TINY), fmaxf(q.factor[g + 8] * ks[i], KA_TINY)};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const float pr = fast_exp2(fmaf(sc[j][x], f[x >> 1], KA_OFFSET - st[x >> 1].x)) * st[x >> 1].y;
-          if (st[x >> 1].y != 0.f && sc[j][x] != -INFINITY) sums[2 * j + (x & 1)] += pr;   // rows that exist, tokens that they see
+          if (st[x >> 1].y != 0.f && sc[j][x] != -INFINITY) sums[i][2 * j + (x & 1)] += pr;   // rows that exist, tokens that they see
         }
     }
     __syncthreads();   // the tile in shared memory is free
   }
-  if (warp < 2) {
+#pragma unroll
+  for (int i = 0; i < MINE; ++i)
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 4);
-      sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 8);
-      sums[x] += __shfl_xor_sync(0xffffffffu, sums[x], 16);
-      const int j = j0 + 8 * (x >> 1) + 2 * t + (x & 1);
-      if (g == 0 && j < it.len && j < p.w_len) p.weights[it.b * p.w_stride_b + it.h * p.w_stride_h + j] += sums[x];
+      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 4);
+      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 8);
+      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 16);
+      const int j = (first + i * KA_WARPS) * KA_UNIT + 8 * (x >> 1) + 2 * t + (x & 1);
+      if (g == 0 && page[i] >= 0 && j < it.len && j < p.w_len) p.weights[it.b * p.w_stride_b + it.h * p.w_stride_h + j] += sums[i][x];
     }
-  }
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
@@ -672,7 +774,7 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   a.stats = p.weights != nullptr;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
   // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined.
-  a.ctas = s.blocks <= 8 || items > 148 * 16 ? 0 : 148 * 2;
+  a.ctas = s.blocks <= 8 || items > 148 * 16 ? 0 : 148 * KA_CTAS;
   return a;
 }
 
@@ -696,11 +798,17 @@ size_t cache_attention_workspace(const kd_cache& c, const kd_cache_seqs& s, cons
 
 template <int D>
 static int launch_for(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
-  const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles, rows = static_cast<int64_t>(s.B) * c.H * a.rows, pages = static_cast<int64_t>(s.B) * c.H * s.blocks;
-  if (items > INT32_MAX || rows > INT32_MAX || (a.stats && pages > INT32_MAX)) return set_error(KD_ERR_LIMIT, "%d sequences of %d blocks are too many for one call", s.B, s.blocks);
-  cudaError_t e = launch(cache_attention_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, 0, stream, c, s, p, a, ws);
+  const int64_t heads = static_cast<int64_t>(s.B) * c.H, items = heads * a.tiles, rows = heads * a.rows, groups = heads * ((s.blocks + KW_PAGES - 1) / KW_PAGES);
+  if (items > INT32_MAX || rows > INT32_MAX || (a.stats && groups > INT32_MAX)) return set_error(KD_ERR_LIMIT, "%d sequences of %d blocks are too many for one call", s.B, s.blocks);
+  constexpr size_t kShared = sizeof(AttnShared<D>), kWeights = KW_UNITS * Stage<D>::BYTES + sizeof(QueryTile<D>);
+  static SmemOptIn opt_in, opt_in_weights;
+  cudaError_t e = opt_in(cache_attention_kernel<D>, kShared);
+  if (e == cudaSuccess) e = launch(cache_attention_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
   if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(rows), 128, 0, stream, c, s, p, a, ws);
-  if (e == cudaSuccess && a.stats && pages > 0) e = launch(cache_weights_kernel<D>, static_cast<unsigned>(pages), KA_THREADS, 0, stream, c, s, p, a, ws);
+  if (e == cudaSuccess && a.stats && groups > 0) {
+    e = opt_in_weights(cache_weights_kernel<D>, kWeights);
+    if (e == cudaSuccess) e = launch(cache_weights_kernel<D>, static_cast<unsigned>(groups), KA_THREADS, kWeights, stream, c, s, p, a, ws);
+  }
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
   return 0;
 }

@@ -54,10 +54,14 @@ __device__ __forceinline__ int exponent_for(uint32_t amax) {
   return amax == 0u ? KC_EXP_MIN : max(KC_EXP_MIN, min(KC_EXP_MAX, e));
 }
 
-// two e4m3 numbers (low byte first) as halves, which hold every e4m3 number exactly
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{\n.reg .b16 lo;\ncvt.u16.u32 lo, %1;\ncvt.rn.f16x2.e4m3x2 %0, lo;\n}\n" : "=r"(r) : "r"(two));
+// Four e4m3 numbers (low byte first) as halves, which hold every e4m3 number exactly: the low two and the high two. (The unpacking is
+// left to the conversion, which can take either half of a register.)
+struct HalfPairs {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ HalfPairs e4m3x4_to_f16x4(uint32_t four) {
+  HalfPairs r;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}\n" : "=r"(r.lo), "=r"(r.hi) : "r"(four));
   return r;
 }
 // two floats to e4m3, nearest even; beyond 448 saturates, NaN stays NaN. lo in the low byte
@@ -68,7 +72,8 @@ __device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t f32x4_to_e4m3x4(const float* f) { return f32x2_to_e4m3x2(f[0], f[1]) | (f32x2_to_e4m3x2(f[2], f[3]) << 16); }
 __device__ __forceinline__ void e4m3x4_to_f32x4(uint32_t w, float* f) {
-  const float2 a = unpack2<false>(e4m3x2_to_f16x2(w & 0xFFFFu)), b = unpack2<false>(e4m3x2_to_f16x2(w >> 16));
+  const HalfPairs h = e4m3x4_to_f16x4(w);
+  const float2 a = unpack2<false>(h.lo), b = unpack2<false>(h.hi);
   f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 
