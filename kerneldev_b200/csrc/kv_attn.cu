@@ -1,14 +1,16 @@
 // Attention of the newest tokens over the 8-bit cache, and the weight that each cached token receives.
 //
 // One key head at a time has few query rows (its group's heads times the new tokens), so what bounds these kernels is reading the cache: 2 D bytes
-// a token. Every warp walks units of 32 tokens on its own, straight from memory to registers, with no shared tile and no barrier:
-//   S = Q K^T   mma m16n8k16, 16 query rows; a lane's 16 bytes of a key row are the B operand of four steps (the order of the head dim
-//               inside a step is free as long as Q's registers have the same)
-//   P = exp2(S) stays in the registers that the second product takes it from (the accumulators of two 8-token tiles are the A operand of one step)
-//   O += P V    a lane's 16 bytes of four value rows are the B operands of 16 column tiles: the columns of tile m are the
-//               m-th bytes of the eight lanes' pieces, so that loads stay 16 bytes wide and no transpose is needed
-// e4m3 numbers become halves by one instruction for two, exactly. Rounded are P (to a half: 2**-11, in place of the output's 2**-8 or 2**-11) and the output;
-// bfloat16 queries become halves exactly, after a power of two for each row.
+// a token. Every warp walks units of 32 tokens on its own, from asynchronous copies of its own, with no tile shared between warps and no barrier:
+//   S^T = K Q^T    mma m16n8k16: the cache's tokens are the wide operand, 8 query rows the narrow one (with the rows in the wide one, half of it would be
+//                  empty for most models). A lane's 16 bytes of a key row are its part of four steps: the order of the head dims inside a step is free as
+//                  long as Q's registers have the same.
+//   P = exp2(S)    each 8 x 8 block transposed between the lanes (movmatrix), as the operand of
+//   O^T += V^T P^T A lane's 16 bytes of four tokens are its parts of all tiles of 16 head dims: the rows g and g + 8 of tile m are the bytes 2 m and 2 m + 1 of the
+//                  eight lanes' pieces, so that loads stay 16 bytes wide.
+// Both on halves: they hold every e4m3 number, and one instruction converts four. Rounded are P (2^-11, beside the output's 2^-8 or 2^-11) and the output; bfloat16
+// queries become halves exactly, after a power of two for each row. (mma on e4m3 itself is made of conversions and products of halves on this
+// chip: with it, and queries in three e4m3 terms, a unit took 740 instructions in place of 510.)
 //
 // Scales. A page's K scale multiplies its scores. Its V scale 2^ev goes into the exponent, p' = 2^(s + ev - ref), where ref is the
 // running maximum of s + ev; then O = sum p' v / sum p' 2^-ev, and no product of its own is spent on it. The exponents differ by at most 63, which
@@ -24,7 +26,9 @@
 
 namespace kd {
 
-constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_ROWS = 16, KA_UNIT = 32, KA_STAGES = 2, KA_CTAS = 3;   // CTAs of an SM
+constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_TILE = 8, KA_UNIT = 32;
+// CTAs of an SM, by tiles of query rows: what registers and shared memory allow
+__host__ __device__ constexpr int ctas_of(int nt) { return nt <= 2 ? 3 : 2; }
 constexpr float KA_OFFSET = 8.f, KA_SLACK = 6.f, KA_LOG2E = 1.4426950408889634f;
 constexpr float KA_TINY = 1e-37f;   // in place of factors that a float flushes to 0 (every score is as good as 0 then): masked scores stay -inf, and not 0 * inf
 
@@ -37,11 +41,11 @@ struct RowMask {
 };
 
 struct AttnShape {
-  int G, rows, tiles;   // heads of a group, query rows of a key head, tiles of KA_ROWS of them
+  int G, rows, tiles;   // heads of a group, query rows of a key head, items that they are cut into: of KA_TILE, 2 or 4 KA_TILE rows
   int ctas;             // 0: a CTA for each (sequence, head, tile); else that many CTAs share all pages evenly
   bool stats;           // leave every row's maximum and sum for the weights
 };
-// Workspace: the rows' statistics (float2 for each, with weights), then for each CTA two parts: KA_ROWS rows of D floats, and their maxima and sums.
+// Workspace: the rows' statistics (float2 for each, with weights), then for each CTA two parts: an item's rows of D floats, and their maxima and sums.
 struct AttnWorkspace {
   float2* stats;
   float* part_o;
@@ -73,11 +77,13 @@ template <int D>
 struct Spread {
   static constexpr int KU = D % 64 == 0 ? 16 : D % 32 == 0 ? 8 : 4, K_PIECES = D / 4 / KU, K_WORDS = D / 16;
   static constexpr int VU = D == 128 ? 16 : D == 64 ? 8 : D % 32 == 0 ? 4 : 2, V_PIECES = D / 8 / VU, V_WORDS = V_PIECES * (VU > 4 ? VU / 4 : 1);
-  static constexpr int TILES = D / 8;   // column tiles of O
-  // the first of the head dims that lane t holds in step s of Q K^T; the step has four of them
-  static __device__ __forceinline__ int k_dim(int s, int t) { return 4 * KU * (s / (KU / 4)) + KU * t + 4 * (s % (KU / 4)); }
-  // the column of O that column n of tile m is
-  static __device__ __forceinline__ int v_dim(int m, int n) { return 8 * VU * (m / VU) + VU * n + m % VU; }
+  // the first of the four head dims that word w of lane t is
+  static __device__ __forceinline__ int k_dim(int w, int t) { return 4 * KU * (w / (KU / 4)) + KU * t + 4 * (w % (KU / 4)); }
+  // ... and the inverse: dims d .. d + 3, d a multiple of 4
+  static __device__ __forceinline__ int k_word(int d) { return d / (4 * KU) * (KU / 4) + d % KU / 4; }
+  static __device__ __forceinline__ int k_lane(int d) { return d % (4 * KU) / KU; }
+  // the head dim that byte m of lane g's pieces of V is
+  static __device__ __forceinline__ int v_dim(int m, int g) { return 8 * VU * (m / VU) + VU * g + m % VU; }
 };
 
 // A warp's copy of a unit: K, V, descriptors, scales. Rows of 128 or 64 bytes would put all rows into the same banks: the 16-byte pieces of a
@@ -112,7 +118,7 @@ struct Lane {
     for (int i = 0; i < D / 16; ++i) cp_async16(stage + (!kV ? copy_k + 512 * i : copy_v[i & 1] + 512 * (i & ~1)), from + (threadIdx.x & 31) * 16 + 512 * i);
   }
   // lane (g, t): its pieces of an 8-token tile of K
-  __device__ __forceinline__ void load_keys(uint32_t stage, int j, uint32_t (&w)[Spread<D>::K_WORDS]) const {
+  __device__ __forceinline__ void load_keys(uint32_t stage, int j, uint32_t* w) const {
     using S = Spread<D>;
 #pragma unroll
     for (int i = 0; i < S::K_PIECES; ++i) lds<S::KU>(stage + k[i] + 8 * D * j, &w[i * (S::KU / 4)]);
@@ -132,62 +138,84 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+// c = a b
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+// an 8 x 8 block of halves, lane (g, t) with row g and columns 2 t, 2 t + 1, transposed
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-// S of a unit: 16 rows against 32 tokens. q: the A operands of every step, [step][lane]
-template <int D>
-__device__ __forceinline__ void scores(uint32_t stage, const Lane<D>& at, const uint4* q, float (&c)[4][4]) {
+// Query rows in shared memory: the operands of every step and what the mask needs. NT tiles of 8 rows.
+template <int D, int NT>
+struct QueryTile {
+  uint2 frag[NT][D / 16][32];
+  RowMask mask[NT * KA_TILE];
+  float factor[NT * KA_TILE];   // what a row's products are to be multiplied with, sm_scale and log2(e) among it
+  int min_limit;                // of the rows that see anything
+};
+
+// S^T of a unit: c[n][i][x] of lane (g, t): token 16 i + g + 8 (x >> 1), row 2 t + (x & 1) of tile n
+template <int D, int NT>
+__device__ __forceinline__ void scores(uint32_t stage, const Lane<D>& at, const QueryTile<D, NT>& q, float (&c)[NT][2][4]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int i = 0; i < 2; ++i) {
+    uint32_t k[2][Spread<D>::K_WORDS];
+    at.load_keys(stage, 2 * i, k[0]);
+    at.load_keys(stage, 2 * i + 1, k[1]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) c[j][x] = 0.f;
-  uint32_t k[4][Spread<D>::K_WORDS];
+    for (int s = 0; s < D / 16; ++s) {
+      const HalfPairs lo = e4m3x4_to_f16x4(k[0][s]), hi = e4m3x4_to_f16x4(k[1][s]);
+      const uint4 a = make_uint4(lo.lo, hi.lo, lo.hi, hi.hi);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) at.load_keys(stage, j, k[j]);
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    const uint4 a = q[s * 32 + lane];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const HalfPairs b = e4m3x4_to_f16x4(k[j][s]);
-      mma_f16(c[j], a, b.lo, b.hi);
+      for (int n = 0; n < NT; ++n) {
+        const uint2 b = q.frag[n][s][lane];
+        if (s == 0) mma_f16_first(c[n][i], a, b.x, b.y);
+        else mma_f16(c[n][i], a, b.x, b.y);
+      }
     }
   }
 }
 
-// bytes 0 and 1 (2 and 3) of two words in turn: for two tokens' values of two columns
+// bytes 0 and 1 (2 and 3) of two words in turn: for two tokens' values of two head dims
 __device__ __forceinline__ uint32_t interleave(uint32_t a, uint32_t b, bool high) { return __byte_perm(a, b, high ? 0x7362 : 0x5140); }
 // the bytes that are NaN, as bytes of ones
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
-// O += P V for 16 tokens. kSafe: see the head of the file; vis: the A operand of indicators
-template <int D, bool kSafe>
-__device__ __forceinline__ void add_values(float (&o)[D / 8][4], const uint4& p, const uint4& vis, const uint32_t (&v)[4][Spread<D>::V_WORDS]) {
+// O^T += V^T P^T for 16 tokens. p: the tiles' operands (two words a tile). kSafe: see the head of the file; vis: the operands of indicators
+template <int D, int NT, bool kSafe>
+__device__ __forceinline__ void add_values(float (&o)[NT][D / 16][4], const uint32_t (&p)[NT][2], const uint32_t (&vis)[NT][2], const uint32_t (&v)[4][Spread<D>::V_WORDS]) {
   using S = Spread<D>;
-  constexpr int PER = S::VU >= 4 ? 4 : 2;   // columns of a word
+  constexpr int PER = S::VU >= 4 ? 2 : 1;   // tiles of a word
 #pragma unroll
   for (int w = 0; w < S::V_WORDS; ++w) {
 #pragma unroll
-    for (int half = 0; half < PER / 2; ++half) {
+    for (int half = 0; half < PER; ++half) {
       uint32_t b0 = interleave(v[0][w], v[1][w], half != 0), b1 = interleave(v[2][w], v[3][w], half != 0);
-      const int m = w * PER + 2 * half;
+      const int m = w * PER + half;
       if constexpr (kSafe) {
         const uint32_t n0 = nan_bytes(b0), n1 = nan_bytes(b1);
         b0 &= ~n0;
         b1 &= ~n1;
         const HalfPairs one0 = e4m3x4_to_f16x4(n0 & 0x38383838u), one1 = e4m3x4_to_f16x4(n1 & 0x38383838u);   // 0x38: 1 in e4m3
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int n = 0; n < NT; ++n) {
           float hit[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(hit, vis, x == 0 ? one0.lo : one0.hi, x == 0 ? one1.lo : one1.hi);
+          mma_f16(hit, make_uint4(one0.lo, one0.hi, one1.lo, one1.hi), vis[n][0], vis[n][1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (hit[i] > 0.f) o[m + x][i] = __uint_as_float(0x7FC00000u);
+            if (hit[i] > 0.f) o[n][m][i] = __uint_as_float(0x7FC00000u);
         }
       }
       const HalfPairs h0 = e4m3x4_to_f16x4(b0), h1 = e4m3x4_to_f16x4(b1);
-      mma_f16(o[m], p, h0.lo, h1.lo);
-      mma_f16(o[m + 1], p, h0.hi, h1.hi);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_f16(o[n][m], make_uint4(h0.lo, h0.hi, h1.lo, h1.hi), p[n][0], p[n][1]);
     }
   }
 }
@@ -221,40 +249,30 @@ __device__ __forceinline__ RowMask row_mask(const kd_cache& c, const kd_cache_se
   return m;
 }
 
-template <int D>
-struct QueryTile {
-  uint4 frag[D / 16][32];
-  RowMask mask[KA_ROWS];
-  float factor[KA_ROWS];   // what its products are to be multiplied with, sm_scale and log2(e) among it
-  int min_limit;           // of the rows that see anything
-};
-
-// Q's tile as A operands in shared memory, all threads of the CTA; ends with a barrier. bfloat16 rows are multiplied with a power of two that brings the largest
-// finite number to 2^14, so that halves hold them (what falls below a half's subnormals is 2^-38 of the largest).
-template <int D>
-__device__ __forceinline__ void load_queries(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int G, int rows, QueryTile<D>& q) {
-  constexpr int PER = KA_ROWS / KA_WARPS;   // rows of a warp, four numbers of each to a lane
+// The query tiles of an item in shared memory, all threads of the CTA; ends with a barrier. bfloat16 rows are multiplied with the power of two that brings their largest
+// finite number to 2^14 (what falls below a half's subnormals is 2^-38 of it).
+template <int D, int NT>
+__device__ __forceinline__ void load_queries(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int G, int rows, QueryTile<D, NT>& q) {
+  using S = Spread<D>;
+  constexpr int ROWS = NT * KA_TILE, PER = ROWS / KA_WARPS;   // rows of a warp, four numbers of each to a lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = 4 * lane;
   const bool bf16 = p.dtype == KD_BF16;
   uint2 v[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int row = it.tile * KA_ROWS + warp * PER + i;
+    const int row = it.tile * ROWS + warp * PER + i;
     v[i] = make_uint2(0u, 0u);
     if (row < rows && d < D) {
       const int n = row / G, hq = it.h * G + row - n * G;
       v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
     }
   }
-  if (threadIdx.x < KA_ROWS) {
-    const RowMask m = row_mask(c, s, p, it, it.tile * KA_ROWS + threadIdx.x, G, rows, query_count(c, p, it.b));
+  if (threadIdx.x < ROWS) {
+    const RowMask m = row_mask(c, s, p, it, it.tile * ROWS + threadIdx.x, G, rows, query_count(c, p, it.b));
     q.mask[threadIdx.x] = m;
-    const int low = __reduce_min_sync(0xFFFFu, m.limit > 0 ? m.limit : INT_MAX);
+    const int low = __reduce_min_sync(ROWS == 32 ? 0xFFFFFFFFu : (1u << ROWS) - 1u, m.limit > 0 ? m.limit : INT_MAX);
     if (threadIdx.x == 0) q.min_limit = low;
   }
-  // the step and quad lane that hold dims d .. d + 3 (see Spread::k_dim)
-  constexpr int KU = Spread<D>::KU;
-  const int step = d / (4 * KU) * (KU / 4) + d % KU / 4, quad = d % (4 * KU) / KU;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int r = warp * PER + i;
@@ -268,41 +286,36 @@ __device__ __forceinline__ void load_queries(const kd_cache& c, const kd_cache_s
       v[i] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
     }
     if (lane == 0) q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
-    if (d < D) {   // registers 0 and 2 of the operand are those of rows 0 to 7, 1 and 3 of rows 8 to 15
-      uint32_t* w = reinterpret_cast<uint32_t*>(&q.frag[step][(r & 7) * 4 + quad]) + (r >> 3);
-      w[0] = v[i].x;
-      w[2] = v[i].y;
-    }
+    if (d < D) q.frag[r / KA_TILE][S::k_word(d)][(r % KA_TILE) * 4 + S::k_lane(d)] = v[i];
   }
   __syncthreads();
 }
 
-// masks the scores of a unit: token of c[j][x]: j0 + 8 j + 2 t + (x & 1), row of c[j][x]: lo or hi
-__device__ __forceinline__ void mask_scores(float (&c)[4][4], const uint32_t* desc, int j0, int t, int end, const RowMask& lo, const RowMask& hi) {
+// masks the scores of a unit (c as above); rows: the masks of a tile's rows
+__device__ __forceinline__ void mask_scores(float (&c)[2][4], const uint32_t* desc, int j0, int g, int t, int end, const RowMask* rows) {
+  const RowMask m[2] = {rows[2 * t], rows[2 * t + 1]};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int token = j0 + 8 * j + 2 * t;
-    uint2 d = make_uint2(TD_CTX, TD_CTX);
-    if (desc != nullptr) d = *reinterpret_cast<const uint2*>(desc + 8 * j + 2 * t);
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const RowMask& m = x < 2 ? lo : hi;
-      const uint32_t kd = (x & 1) != 0 ? d.y : d.x;
-      const int tok = token + (x & 1);
-      const bool see = tok < end && ((kd & (tok < m.limit ? m.sees | m.causal : m.sees)) != 0u || span_match_key(m.span_key, kd) != 0u);
-      if (!see) c[j][x] = -INFINITY;
+    for (int y = 0; y < 2; ++y) {
+      const int at = 16 * i + 8 * y + g, token = j0 + at;
+      const uint32_t kd = desc != nullptr ? desc[at] : TD_CTX;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const bool see = token < end && ((kd & (token < m[x].limit ? m[x].sees | m[x].causal : m[x].sees)) != 0u || span_match_key(m[x].span_key, kd) != 0u);
+        if (!see) c[i][2 * y + x] = -INFINITY;
+      }
     }
-  }
 }
 
 // ---- the walk -----------------------------------------------------------------------------------------------------
 
-// A warp's share of units first, first + KA_WARPS, ... below `last` of one head of a sequence, through a ring of copies of its own: while
-// one unit is worked on, KA_STAGES - 1 are on their way. The accumulators' rows are lane / 4 and that plus 8.
-template <int D>
+// A warp's share of units first, first + KA_WARPS, ... below `last` of one head of a sequence, through two copies of its own: while
+// one unit is worked on, the next is on its way. Accumulators: rows 2 t + {0, 1} of a tile (registers x & 1), head dims v_dim(2 m + (x >> 1), g); maxima and sums: rows 2 t and 2 t + 1.
+template <int D, int NT>
 struct Walker {
-  float o[D / 8][4];
-  float ref[2], sum[2];
+  float o[NT][D / 16][4];
+  float ref[NT][2], sum[NT][2];
 
   // starts the copies of a unit (nothing at or beyond `last`)
   static __device__ __forceinline__ void fetch(const kd_cache& c, const Lane<D>& place, int h, int unit, int last, int page, char* stage) {
@@ -323,121 +336,122 @@ struct Walker {
     }
     cp_async_commit();
   }
-  // the ring's first copies, and the page of the unit behind them
+  // the first copy, and the page of the unit behind it
   static __device__ __forceinline__ int begin(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, int first, int last, char* ring) {
     const int32_t* table = s.table + it.b * s.table_stride;
-    auto page_at = [&](int i) { return first + i * KA_WARPS < last ? table[(first + i * KA_WARPS) >> 1] : -1; };
-    int pages[KA_STAGES];
-#pragma unroll
-    for (int i = 0; i < KA_STAGES; ++i) pages[i] = page_at(i);
-#pragma unroll
-    for (int i = 0; i + 1 < KA_STAGES; ++i) fetch(c, place, it.h, first + i * KA_WARPS, last, pages[i], ring + i * Stage<D>::BYTES);
-    return pages[KA_STAGES - 1];
+    const int page = first < last ? table[first >> 1] : -1, next = first + KA_WARPS < last ? table[(first + KA_WARPS) >> 1] : -1;
+    fetch(c, place, it.h, first, last, page, ring);
+    return next;
   }
 
   // next_page: what begin returned
   template <bool kSafe>
-  __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, const QueryTile<D>& q, int first, int last, int next_page, char* ring) {
+  __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, const QueryTile<D, NT>& q, int first, int last, int next_page,
+                                       char* ring) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    ref[0] = ref[1] = -INFINITY;
-    sum[0] = sum[1] = 0.f;
 #pragma unroll
-    for (int m = 0; m < D / 8; ++m)
+    for (int n = 0; n < NT; ++n) {
+      ref[n][0] = ref[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) o[m][x] = 0.f;
+      for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[n][m][x] = 0.f;
+    }
     const int32_t* table = s.table + it.b * s.table_stride;
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
-    int slot = 0;
+    char* stage = ring;
     for (int unit = first; unit < last; unit += KA_WARPS) {
-      cp_async_wait<KA_STAGES - 2>();
+      cp_async_wait<0>();
       __syncwarp();   // everyone's copies of this unit are there, and everyone is done with the one before it, whose place the next one takes
-      const int ahead = unit + (KA_STAGES - 1) * KA_WARPS;
-      fetch(c, place, it.h, ahead, last, next_page, ring + (slot == 0 ? KA_STAGES - 1 : slot - 1) * Stage<D>::BYTES);
+      char* other = stage == ring ? ring + Stage<D>::BYTES : ring;
+      const int ahead = unit + KA_WARPS;
+      fetch(c, place, it.h, ahead, last, next_page, other);
       if (ahead + KA_WARPS < last) next_page = table[(ahead + KA_WARPS) >> 1];
-      const char* stage = ring + slot * Stage<D>::BYTES;
       const uint32_t at = smem_u32(stage);
-      slot = slot + 1 == KA_STAGES ? 0 : slot + 1;
       const float* scale = reinterpret_cast<const float*>(stage + Stage<D>::SCALE_AT);
+      const uint32_t* desc = c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr;
       const int page = reinterpret_cast<const int*>(scale)[2], j0 = unit * KA_UNIT;
-      float sc[4][4];
-      scores<D>(at, place, &q.frag[0][0], sc);
-      const float k_lo = fmaxf(scale[0] * q.factor[g], KA_TINY), k_hi = fmaxf(scale[0] * q.factor[g + 8], KA_TINY);
+      const float ks = scale[0];
       const int ev = scale_exponent(scale[1]);
-      if (page < 0 || j0 + KA_UNIT > free_end)
-        mask_scores(sc, c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr, j0, t, page < 0 ? 0 : it.len, q.mask[g], q.mask[g + 8]);
-      // the rows' maxima over the quad
-      float top[2] = {-INFINITY, -INFINITY};
+      float sc[NT][2][4];
+      scores<D, NT>(at, place, q, sc);
+      uint32_t p[2][NT][2], vis[2][NT][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        top[0] = fmaxf(top[0], fmaxf(sc[j][0], sc[j][1]));
-        top[1] = fmaxf(top[1], fmaxf(sc[j][2], sc[j][3]));
-      }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        top[x] = fmaf(top[x], x == 0 ? k_lo : k_hi, static_cast<float>(ev));
-      }
-      if (__any_sync(0xffffffffu, top[0] > ref[0] + KA_SLACK || top[1] > ref[1] + KA_SLACK)) {
+      for (int n = 0; n < NT; ++n) {
+        if (page < 0 || j0 + KA_UNIT > free_end) mask_scores(sc[n], desc, j0, g, t, page < 0 ? 0 : it.len, &q.mask[n * KA_TILE]);
+        float k[2], add[2], shrink[2];
+        bool grown = false;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const float to = top[x] > ref[x] + KA_SLACK ? top[x] : ref[x], shrink = to == ref[x] ? 1.f : fast_exp2(ref[x] - to);
-          ref[x] = to;
-          sum[x] *= shrink;
+          k[x] = fmaxf(ks * q.factor[n * KA_TILE + 2 * t + x], KA_TINY);
+          // the row's maximum, over the lanes of its tokens
+          float top = fmaxf(fmaxf(sc[n][0][x], sc[n][0][2 + x]), fmaxf(sc[n][1][x], sc[n][1][2 + x]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaf(top, k[x], static_cast<float>(ev));
+          const bool up = top > ref[n][x] + KA_SLACK;
+          shrink[x] = up ? fast_exp2(ref[n][x] - top) : 1.f;
+          ref[n][x] = up ? top : ref[n][x];
+          grown = grown || up;
+          add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x];
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+          sum[n][0] *= shrink[0];
+          sum[n][1] *= shrink[1];
 #pragma unroll
-          for (int m = 0; m < D / 8; ++m) {
-            o[m][2 * x] *= shrink;
-            o[m][2 * x + 1] *= shrink;
+          for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[n][m][x] *= shrink[x & 1];
+        }
+        if constexpr (kSafe) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              vis[i][n][y] = transpose8x8((sc[n][i][2 * y] == -INFINITY ? 0u : 0x3C00u) | (sc[n][i][2 * y + 1] == -INFINITY ? 0u : 0x3C000000u));
+        }
+        float part[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float a = fast_exp2(fmaf(sc[n][i][2 * y], k[0], add[0])), b = fast_exp2(fmaf(sc[n][i][2 * y + 1], k[1], add[1]));
+            part[0] += a;
+            part[1] += b;
+            p[i][n][y] = transpose8x8(pack2<false>(a, b));
           }
-        }
+        const float unscale = exp2i(-ev);
+        sum[n][0] = fmaf(part[0], unscale, sum[n][0]);
+        sum[n][1] = fmaf(part[1], unscale, sum[n][1]);
       }
-      const float a_lo = ref[0] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[0];
-      const float a_hi = ref[1] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[1];
-      uint4 pr[2], vis[2];
-      if constexpr (kSafe) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          auto seen = [&](float a, float b) { return (a == -INFINITY ? 0u : 0x3C00u) | (b == -INFINITY ? 0u : 0x3C000000u); };
-          vis[i] = make_uint4(seen(sc[2 * i][0], sc[2 * i][1]), seen(sc[2 * i][2], sc[2 * i][3]), seen(sc[2 * i + 1][0], sc[2 * i + 1][1]), seen(sc[2 * i + 1][2], sc[2 * i + 1][3]));
-        }
-      }
-      float part[2] = {0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          sc[j][x] = fast_exp2(fmaf(sc[j][x], x < 2 ? k_lo : k_hi, x < 2 ? a_lo : a_hi));
-          part[x >> 1] += sc[j][x];
-        }
-      const float unscale = exp2i(-ev);
-      sum[0] = fmaf(part[0], unscale, sum[0]);
-      sum[1] = fmaf(part[1], unscale, sum[1]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        pr[i] = make_uint4(pack2<false>(sc[2 * i][0], sc[2 * i][1]), pack2<false>(sc[2 * i][2], sc[2 * i][3]), pack2<false>(sc[2 * i + 1][0], sc[2 * i + 1][1]),
-                           pack2<false>(sc[2 * i + 1][2], sc[2 * i + 1][3]));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t v[4][Spread<D>::V_WORDS];
         place.load_values(at, i, v);
-        add_values<D, kSafe>(o, pr[i], kSafe ? vis[i] : pr[i], v);
+        add_values<D, NT, kSafe>(o, p[i], kSafe ? vis[i] : p[i], v);
       }
+      stage = other;
     }
     cp_async_wait<0>();
     __syncwarp();
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
-      sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) sum[n][x] += __shfl_xor_sync(0xffffffffu, sum[n][x], o);
   }
 
   __device__ __forceinline__ bool any_nan() const {
     bool bad = false;
 #pragma unroll
-    for (int m = 0; m < D / 8; ++m)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) bad = bad || is_nan(o[m][x]);
+      for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) bad = bad || is_nan(o[n][m][x]);
     return __any_sync(0xffffffffu, bad);
   }
 };
@@ -448,46 +462,54 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
   if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
 }
 
-// The flat order of all pages: sequences in turn, each once for every head and tile. A warp holds the page counts of the first 128 sequences, in its lanes.
+// The flat order of all pages: sequences in turn, each once for every head and tile, cut into even ranges for the CTAs. 32 bits are enough: the host sees to
+// it that there are fewer than 2^30 pages. A warp holds the page counts of the first 128 sequences, in its lanes.
 struct FlatPlace {
   int b, ht, page, pages;   // page: index within the item
 };
 struct FlatOrder {
   static constexpr int HELD = 4;
   int held[HELD];
-  int64_t total;   // pages
+  uint32_t total;             // pages
+  uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
 
   static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
   __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {   // of sequence 32 i + lane
     if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
     return pages_of(c, s, 32 * i + (threadIdx.x & 31));
   }
-  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT) {
+  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT, int most_ctas) {
     const int lane = threadIdx.x & 31;
+    uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) held[i] = pages_of(c, s, 32 * i + lane);
-    int64_t n = held[0] + held[1] + held[2] + held[3];
+    for (int i = 0; i < HELD; ++i) n += held[i] = pages_of(c, s, 32 * i + lane);
     for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total = n * HT;
+    total = __reduce_add_sync(0xffffffffu, n) * HT;
+    // Two pages, a unit for each warp, are the least that a CTA takes. (None takes no page: the join reads a part of every CTA of an item.)
+    ctas = max(min(static_cast<uint32_t>(most_ctas), (total + 1) / 2), 1u);
+    each = total / ctas;
+    more = total - each * ctas;
   }
-  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, int64_t at) const {
+  __device__ __forceinline__ uint32_t start(uint32_t cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ uint32_t cta_of(uint32_t page) const {
+    const uint32_t longer = more * (each + 1);
+    return page < longer ? page / (each + 1) : more + (page - longer) / each;
+  }
+  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, uint32_t at) const {
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;
+    uint32_t before = 0;
     for (int i = 0; 32 * i < s.B; ++i) {
       const int mine = pages(c, s, i);
-      int64_t upto = mine;
+      uint32_t upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += up;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * HT > at);
       if (past != 0u) {
         const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l);
-        const uint64_t rest = static_cast<uint64_t>(at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT);   // less than n * HT
-        const uint64_t ht = rest <= UINT32_MAX ? static_cast<uint32_t>(rest) / static_cast<uint32_t>(n) : rest / static_cast<uint32_t>(n);
+        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT, ht = rest / static_cast<uint32_t>(n);
         return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n};
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -495,206 +517,244 @@ struct FlatOrder {
     return FlatPlace{-1, 0, 0, 0};
   }
   // pages of the sequences before b
-  __device__ __forceinline__ int64_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
+  __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
     const int lane = threadIdx.x & 31;
-    int64_t n = 0;
+    uint32_t n = 0;
     for (int i = 0; 32 * i < b; ++i)
       if (32 * i + lane < b) n += pages(c, s, i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
+    return __reduce_add_sync(0xffffffffu, n);
   }
 };
 
-// Shared memory of the kernel. A warp's rows of O take the place of its ring when it is through.
-template <int D>
+// Shared memory of the kernel. A warp's rows of O take the place of its second copy (and more, with many rows) when it is through; the first one belongs to the next item by then.
+template <int D, int NT>
 struct AttnShared {
-  union {
-    char ring[KA_STAGES * Stage<D>::BYTES];
-    float o[KA_ROWS][D + 4];
+  static constexpr int ROWS = NT * KA_TILE, O_BYTES = ROWS * (D + 4) * 4;
+  struct Warp {
+    char stage[2 * Stage<D>::BYTES + (O_BYTES > Stage<D>::BYTES ? O_BYTES - Stage<D>::BYTES + 127 & ~127 : 0)];
+    __device__ __forceinline__ float* o(int row) { return reinterpret_cast<float*>(stage + Stage<D>::BYTES) + row * (D + 4); }
   } warp[KA_WARPS];
-  QueryTile<D> q;
-  float2 ml[KA_WARPS][KA_ROWS];
+  QueryTile<D, NT> q;
+  float2 ml[KA_WARPS][ROWS];      // the warps' maxima and sums
+  float scale[KA_WARPS][ROWS];    // what a warp's rows are multiplied with: all on one maximum, and divided by the sum where the item is whole
 };
 
-// CTAs that share the pages: two pages, a unit for each warp, are the least that one takes. (None takes no page: the join reads a part of every CTA of an item.)
-__device__ __forceinline__ int64_t sharing_ctas(const AttnShape& shape, int64_t total) { return min(static_cast<int64_t>(shape.ctas), (total + 1) / 2); }
-
-template <int D>
-__global__ void __launch_bounds__(KA_THREADS, KA_CTAS)
+template <int D, int NT>
+__global__ void __launch_bounds__(KA_THREADS, ctas_of(NT))
 cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                        const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
   pdl_wait();
   pdl_launch_dependents();
+  constexpr int ROWS = NT * KA_TILE;
   extern __shared__ __align__(1024) char smem[];
-  AttnShared<D>& sh = *reinterpret_cast<AttnShared<D>*>(smem);
-  QueryTile<D>& q = sh.q;
+  AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
-  int64_t at = 0, end = 1;
-  const FlatOrder order(c, s, HT);
+  const FlatOrder order(c, s, HT, shape.ctas);
+  uint32_t at = 0, end = 1;
   if (shape.ctas > 0) {
-    const int64_t total = order.total;
-    const int64_t ctas = sharing_ctas(shape, total);
-    if (blockIdx.x >= ctas) return;
-    at = total * blockIdx.x / ctas;
-    end = total * (blockIdx.x + 1) / ctas;
+    if (blockIdx.x >= order.ctas || order.total == 0) return;
+    at = order.start(blockIdx.x);
+    end = order.start(blockIdx.x + 1);
   }
-  const int64_t begin = at;
-  while (at < end) {
+  const uint32_t begin = at;
+  struct Share {   // of an item: pages page0 .. page0 + here - 1 of `pages`, the warp's units
     Item it;
-    int page0, pages, here;
+    int pages, here, first, last, next_page;
+  };
+  auto share_at = [&](uint32_t place_of) {
+    Share r;
+    int page0 = 0;
     if (shape.ctas > 0) {
-      const FlatPlace f = order.find(c, s, HT, at);
-      it.b = f.b;
-      it.h = f.ht / shape.tiles;
-      it.tile = f.ht - it.h * shape.tiles;
-      it.len = sequence_length(c, s, it.b);
+      const FlatPlace f = order.find(c, s, HT, place_of);
+      r.it.b = f.b;
+      r.it.h = f.ht / shape.tiles;
+      r.it.tile = f.ht - r.it.h * shape.tiles;
+      r.it.len = sequence_length(c, s, r.it.b);
       page0 = f.page;
-      pages = f.pages;
-      here = static_cast<int>(min(end - at, static_cast<int64_t>(pages - page0)));
+      r.pages = f.pages;
+      r.here = min(static_cast<int>(end - place_of), r.pages - page0);
     } else {
       const int item = blockIdx.x;
-      it.b = item / HT;
-      it.h = (item - it.b * HT) / shape.tiles;
-      it.tile = item - it.b * HT - it.h * shape.tiles;
-      it.len = sequence_length(c, s, it.b);
-      page0 = 0;
-      pages = here = (it.len + KC_PAGE - 1) / KC_PAGE;
+      r.it.b = item / HT;
+      r.it.h = (item - r.it.b * HT) / shape.tiles;
+      r.it.tile = item - r.it.b * HT - r.it.h * shape.tiles;
+      r.it.len = sequence_length(c, s, r.it.b);
+      r.pages = r.here = (r.it.len + KC_PAGE - 1) / KC_PAGE;
     }
-    const int first = 2 * page0 + warp, last = min(2 * (page0 + here), (it.len + KA_UNIT - 1) / KA_UNIT);
-    char* ring = sh.warp[warp].ring;
-    int next = Walker<D>::begin(c, s, place, it, first, last, ring);
-    load_queries<D>(c, s, p, it, shape.G, shape.rows, q);
-    Walker<D> w;
-    w.template walk<false>(c, s, place, it, q, first, last, next, ring);
+    r.first = 2 * page0 + warp;
+    r.last = min(2 * (page0 + r.here), (r.it.len + KA_UNIT - 1) / KA_UNIT);
+    return r;
+  };
+  char* ring = sh.warp[warp].stage;
+  Share now = share_at(at);
+  now.next_page = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
+  while (at < end) {
+    load_queries<D, NT>(c, s, p, now.it, shape.G, shape.rows, sh.q);
+    Walker<D, NT> w;
+    w.template walk<false>(c, s, place, now.it, sh.q, now.first, now.last, now.next_page, ring);
     if (w.any_nan()) {
-      next = Walker<D>::begin(c, s, place, it, first, last, ring);
-      w.template walk<true>(c, s, place, it, q, first, last, next, ring);
+      const int next = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
+      w.template walk<true>(c, s, place, now.it, sh.q, now.first, now.last, next, ring);
     }
-    // the warps' parts: maxima and sums first, then everyone's rows on one scale
-    if (t == 0) {
-      sh.ml[warp][g] = make_float2(w.ref[0], w.sum[0]);
-      sh.ml[warp][g + 8] = make_float2(w.ref[1], w.sum[1]);
+    const uint32_t after = at + (shape.ctas > 0 ? now.here : 1);
+    const Item it = now.it;
+    const bool whole = now.here == now.pages, first_of_cta = at == begin;
+    if (after < end) {   // the next item's first copies run while this one's rows are joined
+      now = share_at(after);
+      now.next_page = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
     }
+    if (g == 0)
 #pragma unroll
-    for (int m = 0; m < D / 8; ++m)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) sh.warp[warp].o[g + 8 * (x >> 1)][Spread<D>::v_dim(m, 2 * t + (x & 1))] = w.o[m][x];
+        for (int x = 0; x < 2; ++x) sh.ml[warp][n * KA_TILE + 2 * t + x] = make_float2(w.ref[n][x], w.sum[n][x]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sh.warp[warp].o(n * KA_TILE + 2 * t + (x & 1))[Spread<D>::v_dim(2 * m + (x >> 1), g)] = w.o[n][m][x];
     __syncthreads();
-    const int r = tid / 8, row_of_head = it.tile * KA_ROWS + r;
-    if (row_of_head < shape.rows) {
+    const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (first_of_cta ? 0 : 1);
+    auto place_of_row = [&](int row, int& hq, int& i) {   // of the key head
+      i = row / shape.G;
+      hq = it.h * shape.G + row - i * shape.G;
+    };
+    if (tid < ROWS && it.tile * ROWS + tid < shape.rows) {
       float ref = -INFINITY, sum = 0.f, scale[KA_WARPS];
 #pragma unroll
-      for (int i = 0; i < KA_WARPS; ++i) ref = fmaxf(ref, sh.ml[i][r].x);
+      for (int k = 0; k < KA_WARPS; ++k) ref = fmaxf(ref, sh.ml[k][tid].x);
 #pragma unroll
-      for (int i = 0; i < KA_WARPS; ++i) {
-        scale[i] = sh.ml[i][r].x == -INFINITY ? 0.f : fast_exp2(sh.ml[i][r].x - ref);
-        sum = fmaf(sh.ml[i][r].y, scale[i], sum);
+      for (int k = 0; k < KA_WARPS; ++k) {
+        scale[k] = sh.ml[k][tid].x == -INFINITY ? 0.f : fast_exp2(sh.ml[k][tid].x - ref);
+        sum = fmaf(sh.ml[k][tid].y, scale[k], sum);
       }
-      const int i = row_of_head / shape.G, hq = it.h * shape.G + row_of_head - i * shape.G;
-      const bool whole = here == pages, live = q.mask[r].limit > 0;
-      const float inv = whole ? (live && sum != 0.f ? 1.f / sum : 0.f) : 1.f;
-      const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (at > begin ? 1 : 0);
-      uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + it.b * p.o.stride_b + hq * p.o.stride_h + i * p.o.stride_t;
-      float* part_o = ws.part_o + (part * KA_ROWS + r) * D;
-      for (int d = (tid & 7) * 2; d < D; d += 16) {
-        float x = 0.f, y = 0.f;
+      const bool live = sh.q.mask[tid].limit > 0;
+      const float inv = whole ? (live && sum != 0.f ? 1.f / sum : -1.f) : 1.f;   // -1: nothing is seen
+#pragma unroll
+      for (int k = 0; k < KA_WARPS; ++k) sh.scale[k][tid] = inv < 0.f ? -1.f : scale[k] * inv;
+      if (whole) {
+        int hq, i;
+        place_of_row(it.tile * ROWS + tid, hq, i);
+        write_stats(p, ws, shape.stats, (static_cast<size_t>(it.b) * p.H + hq) * p.T + i, live, ref, sum);
+      } else {
+        ws.part_ml[part * ROWS + tid] = make_float2(ref, sum);
+      }
+    }
+    __syncthreads();
+    const int rows = min(ROWS, shape.rows - it.tile * ROWS);
+    for (int x = tid; x < rows * (D / 4); x += KA_THREADS) {
+      const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (sh.scale[0][r] >= 0.f || is_nan(sh.scale[0][r])) {
 #pragma unroll
         for (int k = 0; k < KA_WARPS; ++k) {
-          x = fmaf(sh.warp[k].o[r][d], scale[k], x);
-          y = fmaf(sh.warp[k].o[r][d + 1], scale[k], y);
-        }
-        if (whole) {
-          if (inv == 0.f) x = y = 0.f;
-          *reinterpret_cast<uint32_t*>(out + d) = p.dtype == KD_BF16 ? pack2<true>(x * inv, y * inv) : pack2<false>(x * inv, y * inv);
-        } else {
-          *reinterpret_cast<float2*>(part_o + d) = make_float2(x, y);
+          const float f = sh.scale[k][r];
+          const float4 y = *reinterpret_cast<const float4*>(sh.warp[k].o(r) + d);
+          v.x = fmaf(y.x, f, v.x);
+          v.y = fmaf(y.y, f, v.y);
+          v.z = fmaf(y.z, f, v.z);
+          v.w = fmaf(y.w, f, v.w);
         }
       }
-      if ((tid & 7) == 0) {
-        if (whole) write_stats(p, ws, shape.stats, (static_cast<size_t>(it.b) * p.H + hq) * p.T + i, live, ref, sum);
-        else ws.part_ml[part * KA_ROWS + r] = make_float2(ref, sum);
+      if (whole) {
+        int hq, i;
+        place_of_row(it.tile * ROWS + r, hq, i);
+        uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + it.b * p.o.stride_b + hq * p.o.stride_h + i * p.o.stride_t + d;
+        *reinterpret_cast<uint2*>(out) = p.dtype == KD_BF16 ? make_uint2(pack2<true>(v.x, v.y), pack2<true>(v.z, v.w)) : make_uint2(pack2<false>(v.x, v.y), pack2<false>(v.z, v.w));
+      } else {
+        *reinterpret_cast<float4*>(ws.part_o + (part * ROWS + r) * D + d) = v;
       }
     }
     __syncthreads();   // shared memory is free for the next item
-    at += shape.ctas > 0 ? here : 1;
+    at = after;
   }
 }
 
-// One query row whose pages several CTAs shared: their parts on one scale. Four groups of 32 threads take parts in turn.
-__global__ void __launch_bounds__(128)
+// One query row whose pages several CTAs shared: their parts on one scale. Eight groups of 32 threads take parts in turn. What it needs to know of the lengths
+// was there before the kernel ahead of it, so it is looked up while that one runs.
+constexpr int KJ_GROUPS = 8;
+__global__ void __launch_bounds__(KJ_GROUPS * 32)
 cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
-                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
-  pdl_wait();
-  pdl_launch_dependents();
-  __shared__ float s_o[4][128], s_sum[4];
+                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws, int rows_of_item) {
+  __shared__ float4 s_o[KJ_GROUPS][32];
+  __shared__ float2 s_ml[KJ_GROUPS];
   const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5, HT = c.H * shape.tiles;
   const int row_of_head = blockIdx.x % shape.rows, bh = blockIdx.x / shape.rows, b = bh / c.H, h = bh - b * c.H;
-  const int tile = row_of_head / KA_ROWS, r = row_of_head - tile * KA_ROWS;
-  const FlatOrder order(c, s, HT);
-  const int64_t total = order.total, ctas = sharing_ctas(shape, total);
+  const int tile = row_of_head / rows_of_item, r = row_of_head - tile * rows_of_item;
+  const FlatOrder order(c, s, HT, shape.ctas);
   const int len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
-  const int64_t first = order.before(c, s, b) * HT + static_cast<int64_t>(h * shape.tiles + tile) * pages;   // the item's first page in the flat order
+  const uint32_t first = order.before(c, s, b) * HT + (h * shape.tiles + tile) * pages;   // the item's first page in the flat order
+  const int n = query_count(c, p, b);
   int c0 = 0, c1 = -1;
   if (pages > 0) {
-    c0 = static_cast<int>(((first + 1) * ctas - 1) / total);
-    c1 = static_cast<int>(((first + pages) * ctas - 1) / total);
-    if (c0 == c1) return;   // the one CTA has written the row
+    c0 = static_cast<int>(order.cta_of(first));
+    c1 = static_cast<int>(order.cta_of(first + pages - 1));
   }
-  auto part_of = [&](int k) { return (2 * static_cast<size_t>(k) + (total * k / ctas >= first ? 0 : 1)) * KA_ROWS + r; };
-  float ref = -INFINITY;
-  for (int k = c0 + lane; k <= c1; k += 32) ref = fmaxf(ref, ws.part_ml[part_of(k)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  const size_t first_part = (2 * static_cast<size_t>(c0) + (order.start(c0) >= first ? 0 : 1)) * rows_of_item + r;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (c0 == c1) return;   // the one CTA has written the row
   const int d = lane * 4;
+  float ref = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = c0 + grp; k <= c1; k += 4) {
-    const size_t part = part_of(k);
+  for (int k = c0 + grp; k <= c1; k += KJ_GROUPS) {
+    const size_t part = k == c0 ? first_part : 2 * static_cast<size_t>(k) * rows_of_item + r;
     const float2 ml = ws.part_ml[part];
+    const float4 v = d < c.D ? *reinterpret_cast<const float4*>(ws.part_o + part * c.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     if (ml.x == -INFINITY) continue;
-    const float scale = fast_exp2(ml.x - ref);
-    sum = fmaf(ml.y, scale, sum);
-    if (d < c.D) {
-      const float4 v = *reinterpret_cast<const float4*>(ws.part_o + part * c.D + d);
-      acc[0] = fmaf(v.x, scale, acc[0]);
-      acc[1] = fmaf(v.y, scale, acc[1]);
-      acc[2] = fmaf(v.z, scale, acc[2]);
-      acc[3] = fmaf(v.w, scale, acc[3]);
-    }
+    const float to = fmaxf(ref, ml.x), keep = ref == to ? 1.f : fast_exp2(ref - to), scale = ml.x == to ? 1.f : fast_exp2(ml.x - to);
+    ref = to;
+    sum = fmaf(ml.y, scale, sum * keep);
+    acc = make_float4(fmaf(v.x, scale, acc.x * keep), fmaf(v.y, scale, acc.y * keep), fmaf(v.z, scale, acc.z * keep), fmaf(v.w, scale, acc.w * keep));
   }
-  if (d < c.D)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) s_o[grp][d + x] = acc[x];
-  if (lane == 0) s_sum[grp] = sum;
+  s_o[grp][lane] = acc;
+  if (lane == 0) s_ml[grp] = make_float2(ref, sum);
   __syncthreads();
-  const int i = row_of_head / shape.G, hq = h * shape.G + row_of_head - i * shape.G, n = query_count(c, p, b);
-  const bool live = i < n && len - n + i >= 0;
-  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const float inv = live && sum != 0.f ? 1.f / sum : 0.f;
-  if (tid < c.D) {
-    const float x = inv == 0.f ? 0.f : (s_o[0][tid] + s_o[1][tid] + s_o[2][tid] + s_o[3][tid]) * inv;
-    uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + b * p.o.stride_b + hq * p.o.stride_h + i * p.o.stride_t;
-    out[tid] = static_cast<uint16_t>(p.dtype == KD_BF16 ? pack2<true>(x, 0.f) : pack2<false>(x, 0.f));
+  if (grp > 0) return;
+  ref = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < KJ_GROUPS; ++k) ref = fmaxf(ref, s_ml[k].x);
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < KJ_GROUPS; ++k) {
+    if (s_ml[k].x == -INFINITY) continue;
+    const float scale = fast_exp2(s_ml[k].x - ref);
+    const float4 v = s_o[k][lane];
+    sum = fmaf(s_ml[k].y, scale, sum);
+    acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
   }
-  if (tid == 0) write_stats(p, ws, shape.stats, (static_cast<size_t>(b) * p.H + hq) * p.T + i, live, ref, sum);
+  const int i = row_of_head / shape.G, hq = h * shape.G + row_of_head - i * shape.G;
+  const bool live = i < n && len - n + i >= 0;
+  const float inv = 1.f / sum;
+  if (!live || sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if (d < c.D) {
+    uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + b * p.o.stride_b + hq * p.o.stride_h + i * p.o.stride_t + d;
+    *reinterpret_cast<uint2*>(out) = p.dtype == KD_BF16 ? make_uint2(pack2<true>(acc.x, acc.y), pack2<true>(acc.z, acc.w)) : make_uint2(pack2<false>(acc.x, acc.y), pack2<false>(acc.z, acc.w));
+  }
+  if (lane == 0) write_stats(p, ws, shape.stats, (static_cast<size_t>(b) * p.H + hq) * p.T + i, live, ref, sum);
 }
 
 // weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
 // rows, so that nothing is added twice and the order is fixed; a CTA KW_PAGES pages of one head.
-constexpr int KW_PAGES = 4, KW_UNITS = 2 * KW_PAGES;
+constexpr int KW_PAGES = 8, KW_UNITS = 2 * KW_PAGES;
 template <int D>
+constexpr int KW_STAGE = Stage<D>::V_AT + KA_UNIT * 4;   // K and descriptors
+template <int D, int NT>
 __global__ void __launch_bounds__(KA_THREADS)
 cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                      const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int MINE = KW_UNITS / KA_WARPS;
+  constexpr int MINE = KW_UNITS / KA_WARPS, ROWS = NT * KA_TILE;
   extern __shared__ __align__(1024) char smem[];
-  char* stages = smem + (threadIdx.x >> 5) * MINE * Stage<D>::BYTES;
-  QueryTile<D>& q = *reinterpret_cast<QueryTile<D>*>(smem + KW_UNITS * Stage<D>::BYTES);
-  __shared__ float2 s_stat[KA_ROWS];
+  char* stages = smem + (threadIdx.x >> 5) * MINE * KW_STAGE<D>;
+  QueryTile<D, NT>& q = *reinterpret_cast<QueryTile<D, NT>*>(smem + KW_UNITS * KW_STAGE<D>);
+  __shared__ float2 s_stat[ROWS];
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, groups = (s.blocks + KW_PAGES - 1) / KW_PAGES;
   uint32_t item = blockIdx.x;
@@ -706,7 +766,7 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
   it.len = sequence_length(c, s, it.b);
   if ((first - warp) * KA_UNIT >= it.len) return;
   int page[MINE];
-  float ks[MINE], sums[MINE][8];
+  float ks[MINE], sums[MINE][4];
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
     const int unit = first + i * KA_WARPS;
@@ -714,67 +774,75 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
     ks[i] = 1.f;
     if (page[i] >= 0) {
       const size_t at = block_index(c, page[i], it.h), token = at * KC_PAGE + (unit & 1) * KA_UNIT;
-      const uint32_t to = smem_u32(stages + i * Stage<D>::BYTES);
+      const uint32_t to = smem_u32(stages + i * KW_STAGE<D>);
       place.template copy<false>(to, static_cast<const uint8_t*>(c.k) + token * D);
-      if (c.desc != nullptr && lane < 8) cp_async16(to + Stage<D>::DESC_AT + lane * 16, c.desc + token + lane * 4);
+      if (c.desc != nullptr && lane < 8) cp_async16(to + Stage<D>::V_AT + lane * 16, c.desc + token + lane * 4);
       ks[i] = c.k_scale[at];
     }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) sums[i][x] = 0.f;
+    for (int x = 0; x < 4; ++x) sums[i][x] = 0.f;
   }
   cp_async_commit();
   for (it.tile = 0; it.tile < shape.tiles; ++it.tile) {
-    load_queries<D>(c, s, p, it, shape.G, shape.rows, q);
-    if (tid < KA_ROWS) {
-      const int r = it.tile * KA_ROWS + tid, i = r / shape.G;
+    load_queries<D, NT>(c, s, p, it, shape.G, shape.rows, q);
+    if (tid < ROWS) {
+      const int r = it.tile * ROWS + tid, i = r / shape.G;
       s_stat[tid] = r < shape.rows ? ws.stats[(static_cast<size_t>(it.b) * p.H + it.h * shape.G + r - i * shape.G) * p.T + i] : make_float2(0.f, 0.f);
     }
     cp_async_wait<0>();
     __syncthreads();
-    const float2 st[2] = {s_stat[g], s_stat[g + 8]};
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       if (page[i] < 0) continue;
-      const char* stage = stages + i * Stage<D>::BYTES;
+      const char* stage = stages + i * KW_STAGE<D>;
       const int j0 = (first + i * KA_WARPS) * KA_UNIT;
-      float sc[4][4];
-      scores<D>(smem_u32(stage), place, &q.frag[0][0], sc);
-      if (c.desc != nullptr || j0 + KA_UNIT > q.min_limit)
-        mask_scores(sc, c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr, j0, t, it.len, q.mask[g], q.mask[g + 8]);
-      const float f[2] = {fmaxf(q.factor[g] * ks[i], KA_TINY), fmaxf(q.factor[g + 8] * ks[i], KA_TINY)};
+      float sc[NT][2][4];
+      scores<D, NT>(smem_u32(stage), place, q, sc);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int n = 0; n < NT; ++n) {
+        if (c.desc != nullptr || j0 + KA_UNIT > q.min_limit)
+          mask_scores(sc[n], c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::V_AT) : nullptr, j0, g, t, it.len, &q.mask[n * KA_TILE]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float pr = fast_exp2(fmaf(sc[j][x], f[x >> 1], KA_OFFSET - st[x >> 1].x)) * st[x >> 1].y;
-          if (st[x >> 1].y != 0.f && sc[j][x] != -INFINITY) sums[i][2 * j + (x & 1)] += pr;   // rows that exist, tokens that they see
+        for (int x = 0; x < 2; ++x) {
+          const int r = n * KA_TILE + 2 * t + x;
+          const float2 st = s_stat[r];
+          const float f = fmaxf(q.factor[r] * ks[i], KA_TINY);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float v = sc[n][y >> 1][2 * (y & 1) + x], pr = fast_exp2(fmaf(v, f, KA_OFFSET - st.x)) * st.y;
+            if (st.y != 0.f && v != -INFINITY) sums[i][y] += pr;   // rows that exist, tokens that they see
+          }
         }
+      }
     }
     __syncthreads();   // the tile in shared memory is free
   }
 #pragma unroll
   for (int i = 0; i < MINE; ++i)
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 4);
-      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 8);
-      sums[i][x] += __shfl_xor_sync(0xffffffffu, sums[i][x], 16);
-      const int j = (first + i * KA_WARPS) * KA_UNIT + 8 * (x >> 1) + 2 * t + (x & 1);
-      if (g == 0 && page[i] >= 0 && j < it.len && j < p.w_len) p.weights[it.b * p.w_stride_b + it.h * p.w_stride_h + j] += sums[i][x];
+    for (int y = 0; y < 4; ++y) {
+      sums[i][y] += __shfl_xor_sync(0xffffffffu, sums[i][y], 1);
+      sums[i][y] += __shfl_xor_sync(0xffffffffu, sums[i][y], 2);
+      const int j = (first + i * KA_WARPS) * KA_UNIT + 8 * y + g;
+      if (t == 0 && page[i] >= 0 && j < it.len && j < p.w_len) p.weights[it.b * p.w_stride_b + it.h * p.w_stride_h + j] += sums[i][y];
     }
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
+// Query tiles of an item: as many as the rows fill, up to four.
+static int tiles_of_item(int rows) { return rows <= KA_TILE ? 1 : rows <= 2 * KA_TILE ? 2 : 4; }
+
 static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p) {
   AttnShape a;
   a.G = p.H / c.H;
   a.rows = a.G * p.T;
-  a.tiles = (a.rows + KA_ROWS - 1) / KA_ROWS;
+  const int nt = tiles_of_item(a.rows), rows = nt * KA_TILE;
+  a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
-  // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined.
-  a.ctas = s.blocks <= 8 || items > 148 * 16 ? 0 : 148 * KA_CTAS;
+  // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
+  a.ctas = s.blocks <= 8 || items > 148 * 16 || items * s.blocks >= (1 << 30) ? 0 : 148 * ctas_of(nt);
   return a;
 }
 
@@ -785,9 +853,10 @@ static size_t workspace_of(const kd_cache& c, const kd_cache_seqs& s, const kd_c
     n += (bytes + 255) & ~size_t(255);
     return at;
   };
+  const size_t part_rows = size_t(2) * a.ctas * tiles_of_item(a.rows) * KA_TILE;
   ws->stats = reinterpret_cast<float2*>(take(a.stats ? static_cast<size_t>(s.B) * p.H * p.T * sizeof(float2) : 0));
-  ws->part_o = reinterpret_cast<float*>(take(size_t(2) * a.ctas * KA_ROWS * c.D * sizeof(float)));
-  ws->part_ml = reinterpret_cast<float2*>(take(size_t(2) * a.ctas * KA_ROWS * sizeof(float2)));
+  ws->part_o = reinterpret_cast<float*>(take(part_rows * c.D * sizeof(float)));
+  ws->part_ml = reinterpret_cast<float2*>(take(part_rows * sizeof(float2)));
   return n;
 }
 
@@ -796,36 +865,45 @@ size_t cache_attention_workspace(const kd_cache& c, const kd_cache_seqs& s, cons
   return workspace_of(c, s, p, shape_of(c, s, p), nullptr, &ws);
 }
 
-template <int D>
+template <int D, int NT>
 static int launch_for(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
   const int64_t heads = static_cast<int64_t>(s.B) * c.H, items = heads * a.tiles, rows = heads * a.rows, groups = heads * ((s.blocks + KW_PAGES - 1) / KW_PAGES);
   if (items > INT32_MAX || rows > INT32_MAX || (a.stats && groups > INT32_MAX)) return set_error(KD_ERR_LIMIT, "%d sequences of %d blocks are too many for one call", s.B, s.blocks);
-  constexpr size_t kShared = sizeof(AttnShared<D>), kWeights = KW_UNITS * Stage<D>::BYTES + sizeof(QueryTile<D>);
+  constexpr size_t kShared = sizeof(AttnShared<D, NT>), kWeights = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
   static SmemOptIn opt_in, opt_in_weights;
-  cudaError_t e = opt_in(cache_attention_kernel<D>, kShared);
-  if (e == cudaSuccess) e = launch(cache_attention_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
-  if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(rows), 128, 0, stream, c, s, p, a, ws);
+  cudaError_t e = opt_in(cache_attention_kernel<D, NT>, kShared);
+  if (e == cudaSuccess) e = launch(cache_attention_kernel<D, NT>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
+  if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(rows), KJ_GROUPS * 32, 0, stream, c, s, p, a, ws, NT * KA_TILE);
   if (e == cudaSuccess && a.stats && groups > 0) {
-    e = opt_in_weights(cache_weights_kernel<D>, kWeights);
-    if (e == cudaSuccess) e = launch(cache_weights_kernel<D>, static_cast<unsigned>(groups), KA_THREADS, kWeights, stream, c, s, p, a, ws);
+    e = opt_in_weights(cache_weights_kernel<D, NT>, kWeights);
+    if (e == cudaSuccess) e = launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kWeights, stream, c, s, p, a, ws);
   }
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
   return 0;
 }
 
-int launch_cache_attention(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, cudaStream_t stream) {
+template <int D>
+static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, cudaStream_t stream) {
   const AttnShape a = shape_of(c, s, p);
   AttnWorkspace ws;
   workspace_of(c, s, p, a, static_cast<char*>(p.workspace), &ws);
+  switch (tiles_of_item(a.rows)) {
+    case 1: return launch_for<D, 1>(c, s, p, a, ws, stream);
+    case 2: return launch_for<D, 2>(c, s, p, a, ws, stream);
+    default: return launch_for<D, 4>(c, s, p, a, ws, stream);
+  }
+}
+
+int launch_cache_attention(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, cudaStream_t stream) {
   switch (c.D) {
-    case 16: return launch_for<16>(c, s, p, a, ws, stream);
-    case 32: return launch_for<32>(c, s, p, a, ws, stream);
-    case 48: return launch_for<48>(c, s, p, a, ws, stream);
-    case 64: return launch_for<64>(c, s, p, a, ws, stream);
-    case 80: return launch_for<80>(c, s, p, a, ws, stream);
-    case 96: return launch_for<96>(c, s, p, a, ws, stream);
-    case 112: return launch_for<112>(c, s, p, a, ws, stream);
-    default: return launch_for<128>(c, s, p, a, ws, stream);
+    case 16: return launch_dim<16>(c, s, p, stream);
+    case 32: return launch_dim<32>(c, s, p, stream);
+    case 48: return launch_dim<48>(c, s, p, stream);
+    case 64: return launch_dim<64>(c, s, p, stream);
+    case 80: return launch_dim<80>(c, s, p, stream);
+    case 96: return launch_dim<96>(c, s, p, stream);
+    case 112: return launch_dim<112>(c, s, p, stream);
+    default: return launch_dim<128>(c, s, p, stream);
   }
 }
 
