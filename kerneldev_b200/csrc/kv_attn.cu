@@ -22,35 +22,13 @@
 #include <algorithm>
 
 #include "attn_common.cuh"
-#include "kv_cache.cuh"
+#include "kv_attn.cuh"
 
 namespace kd {
 
 constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_TILE = 8, KA_UNIT = 32;
 // CTAs of an SM, by tiles of query rows: what registers and shared memory allow
 __host__ __device__ constexpr int ctas_of(int nt) { return nt <= 2 ? 3 : 2; }
-constexpr float KA_OFFSET = 8.f, KA_SLACK = 6.f, KA_LOG2E = 1.4426950408889634f;
-constexpr float KA_TINY = 1e-37f;   // in place of factors that a float flushes to 0 (every score is as good as 0 then): masked scores stay -inf, and not 0 * inf
-
-// What the mask needs of a query row. A row that does not exist, or sees nothing, has limit 0, sees 0 and a key that no descriptor matches.
-struct RowMask {
-  int limit;          // keys j < limit are no later than the row's own token (or all, without causality)
-  uint32_t sees;      // classes seen wherever they are
-  uint32_t causal;    // classes seen up to limit
-  uint32_t span_key;  // see span_key_of_query
-};
-
-struct AttnShape {
-  int G, rows, tiles;   // heads of a group, query rows of a key head, items that they are cut into: of KA_TILE, 2 or 4 KA_TILE rows
-  int ctas;             // 0: a CTA for each (sequence, head, tile); else that many CTAs share all pages evenly
-  bool stats;           // leave every row's maximum and sum for the weights
-};
-// Workspace: the rows' statistics (float2 for each, with weights), then for each CTA two parts: an item's rows of D floats, and their maxima and sums.
-struct AttnWorkspace {
-  float2* stats;
-  float* part_o;
-  float2* part_ml;
-};
 
 // ---- a unit in shared memory --------------------------------------------------------------------------------------
 
@@ -220,34 +198,7 @@ __device__ __forceinline__ void add_values(float (&o)[NT][D / 16][4], const uint
   }
 }
 
-__device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) > 0x7F800000u; }
-
 // ---- query rows ---------------------------------------------------------------------------------------------------
-
-struct Item {
-  int b, h, tile, len;
-};
-
-__device__ __forceinline__ int query_count(const kd_cache& c, const kd_cache_queries& p, int b) {
-  return p.q_lens != nullptr ? checked_count(c, p.q_lens[b], p.T) : p.T;
-}
-
-// one row's mask; r: row of the key head (query r / G of head r % G of the group)
-__device__ __forceinline__ RowMask row_mask(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int r, int G, int rows, int n_queries) {
-  const int i = r / G, at = it.len - n_queries + i;
-  RowMask m{0, 0u, 0u, 1u};
-  if (r >= rows || i >= n_queries || at < 0) return m;
-  uint32_t d = pack_plain(true);
-  m.limit = p.causal != 0 || c.desc != nullptr ? at + 1 : it.len;
-  if (c.desc != nullptr) {
-    const int page = page_of(c, s, it.b, at / KC_PAGE);
-    d = page >= 0 ? c.desc[block_index(c, page, it.h) * KC_PAGE + at % KC_PAGE] : 0u;
-    m.span_key = span_key_of_query(d);
-  }
-  m.sees = (d >> TD_SEES_SHIFT) & 7u;
-  m.causal = d & TD_CTX;
-  return m;
-}
 
 // The query tiles of an item in shared memory, all threads of the CTA; ends with a barrier. bfloat16 rows are multiplied with the power of two that brings their largest
 // finite number to 2^14 (what falls below a half's subnormals is 2^-38 of it).
@@ -456,76 +407,6 @@ struct Walker {
   }
 };
 
-// A row's output from its sum and accumulated values (scaled by 1 / sum): 16 bits, and its log-sum-exp and statistics.
-__device__ __forceinline__ void write_stats(const kd_cache_queries& p, const AttnWorkspace& ws, bool stats, size_t row, bool live, float ref, float sum) {
-  if (p.lse != nullptr) p.lse[row] = live && sum != 0.f ? ref - KA_OFFSET + log2f(sum) : -INFINITY;
-  if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
-}
-
-// The flat order of all pages: sequences in turn, each once for every head and tile, cut into even ranges for the CTAs. 32 bits are enough: the host sees to
-// it that there are fewer than 2^30 pages. A warp holds the page counts of the first 128 sequences, in its lanes.
-struct FlatPlace {
-  int b, ht, page, pages;   // page: index within the item
-};
-struct FlatOrder {
-  static constexpr int HELD = 4;
-  int held[HELD];
-  uint32_t total;             // pages
-  uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
-
-  static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
-  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {   // of sequence 32 i + lane
-    if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
-    return pages_of(c, s, 32 * i + (threadIdx.x & 31));
-  }
-  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT, int most_ctas) {
-    const int lane = threadIdx.x & 31;
-    uint32_t n = 0;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) n += held[i] = pages_of(c, s, 32 * i + lane);
-    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b);
-    total = __reduce_add_sync(0xffffffffu, n) * HT;
-    // Two pages, a unit for each warp, are the least that a CTA takes. (None takes no page: the join reads a part of every CTA of an item.)
-    ctas = max(min(static_cast<uint32_t>(most_ctas), (total + 1) / 2), 1u);
-    each = total / ctas;
-    more = total - each * ctas;
-  }
-  __device__ __forceinline__ uint32_t start(uint32_t cta) const { return cta * each + min(cta, more); }
-  __device__ __forceinline__ uint32_t cta_of(uint32_t page) const {
-    const uint32_t longer = more * (each + 1);
-    return page < longer ? page / (each + 1) : more + (page - longer) / each;
-  }
-  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, uint32_t at) const {
-    const int lane = threadIdx.x & 31;
-    uint32_t before = 0;
-    for (int i = 0; 32 * i < s.B; ++i) {
-      const int mine = pages(c, s, i);
-      uint32_t upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += up;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * HT > at);
-      if (past != 0u) {
-        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l);
-        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT, ht = rest / static_cast<uint32_t>(n);
-        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n};
-      }
-      before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return FlatPlace{-1, 0, 0, 0};
-  }
-  // pages of the sequences before b
-  __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
-    const int lane = threadIdx.x & 31;
-    uint32_t n = 0;
-    for (int i = 0; 32 * i < b; ++i)
-      if (32 * i + lane < b) n += pages(c, s, i);
-    return __reduce_add_sync(0xffffffffu, n);
-  }
-};
-
 // Shared memory of the kernel. A warp's rows of O take the place of its second copy (and more, with many rows) when it is through; the first one belongs to the next item by then.
 template <int D, int NT>
 struct AttnShared {
@@ -550,7 +431,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
-  const FlatOrder order(c, s, HT, shape.ctas);
+  const FlatOrder order(c, s, HT, shape);
   uint32_t at = 0, end = 1;
   if (shape.ctas > 0) {
     if (blockIdx.x >= order.ctas || order.total == 0) return;
@@ -683,7 +564,7 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
   const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5, HT = c.H * shape.tiles;
   const int row_of_head = blockIdx.x % shape.rows, bh = blockIdx.x / shape.rows, b = bh / c.H, h = bh - b * c.H;
   const int tile = row_of_head / rows_of_item, r = row_of_head - tile * rows_of_item;
-  const FlatOrder order(c, s, HT, shape.ctas);
+  const FlatOrder order(c, s, HT, shape);
   const int len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
   const uint32_t first = order.before(c, s, b) * HT + (h * shape.tiles + tile) * pages;   // the item's first page in the flat order
   const int n = query_count(c, p, b);
@@ -830,19 +711,21 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
-// Query tiles of an item: as many as the rows fill, up to four.
-static int tiles_of_item(int rows) { return rows <= KA_TILE ? 1 : rows <= 2 * KA_TILE ? 2 : 4; }
+// Rows of an item: as many tiles of eight as the rows fill, up to four; beyond CHUNK_FROM rows the items are those of the kernel for many rows.
+constexpr int CHUNK_FROM = 32;
+static int rows_of_item(int rows) { return rows > CHUNK_FROM ? KC_ROWS : rows <= KA_TILE ? KA_TILE : rows <= 2 * KA_TILE ? 2 * KA_TILE : 4 * KA_TILE; }
 
 static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p) {
   AttnShape a;
   a.G = p.H / c.H;
   a.rows = a.G * p.T;
-  const int nt = tiles_of_item(a.rows), rows = nt * KA_TILE;
+  const int rows = rows_of_item(a.rows);
   a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
   // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
-  a.ctas = s.blocks <= 8 || items > 148 * 16 || items * s.blocks >= (1 << 30) ? 0 : 148 * ctas_of(nt);
+  a.ctas = s.blocks <= 8 || items > 148 * 16 || items * s.blocks >= (1 << 30) ? 0 : 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
+  a.least = rows == KC_ROWS ? 8 : 2;   // four tiles of 128 tokens; a unit for each warp
   return a;
 }
 
@@ -853,7 +736,7 @@ static size_t workspace_of(const kd_cache& c, const kd_cache_seqs& s, const kd_c
     n += (bytes + 255) & ~size_t(255);
     return at;
   };
-  const size_t part_rows = size_t(2) * a.ctas * tiles_of_item(a.rows) * KA_TILE;
+  const size_t part_rows = size_t(2) * a.ctas * rows_of_item(a.rows);
   ws->stats = reinterpret_cast<float2*>(take(a.stats ? static_cast<size_t>(s.B) * p.H * p.T * sizeof(float2) : 0));
   ws->part_o = reinterpret_cast<float*>(take(part_rows * c.D * sizeof(float)));
   ws->part_ml = reinterpret_cast<float2*>(take(part_rows * sizeof(float2)));
@@ -865,33 +748,46 @@ size_t cache_attention_workspace(const kd_cache& c, const kd_cache_seqs& s, cons
   return workspace_of(c, s, p, shape_of(c, s, p), nullptr, &ws);
 }
 
+// the weights from the rows' statistics
 template <int D, int NT>
-static int launch_for(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
-  const int64_t heads = static_cast<int64_t>(s.B) * c.H, items = heads * a.tiles, rows = heads * a.rows, groups = heads * ((s.blocks + KW_PAGES - 1) / KW_PAGES);
-  if (items > INT32_MAX || rows > INT32_MAX || (a.stats && groups > INT32_MAX)) return set_error(KD_ERR_LIMIT, "%d sequences of %d blocks are too many for one call", s.B, s.blocks);
-  constexpr size_t kShared = sizeof(AttnShared<D, NT>), kWeights = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
-  static SmemOptIn opt_in, opt_in_weights;
-  cudaError_t e = opt_in(cache_attention_kernel<D, NT>, kShared);
-  if (e == cudaSuccess) e = launch(cache_attention_kernel<D, NT>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
-  if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(rows), KJ_GROUPS * 32, 0, stream, c, s, p, a, ws, NT * KA_TILE);
-  if (e == cudaSuccess && a.stats && groups > 0) {
-    e = opt_in_weights(cache_weights_kernel<D, NT>, kWeights);
-    if (e == cudaSuccess) e = launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kWeights, stream, c, s, p, a, ws);
-  }
-  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
-  return 0;
+static cudaError_t launch_weights(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, AttnShape a, const AttnWorkspace& ws, cudaStream_t stream) {
+  const int64_t groups = static_cast<int64_t>(s.B) * c.H * ((s.blocks + KW_PAGES - 1) / KW_PAGES);
+  if (!a.stats || groups == 0) return cudaSuccess;
+  constexpr size_t kShared = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
+  static SmemOptIn opt_in;
+  a.tiles = (a.rows + NT * KA_TILE - 1) / (NT * KA_TILE);
+  const cudaError_t e = opt_in(cache_weights_kernel<D, NT>, kShared);
+  return e != cudaSuccess ? e : launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kShared, stream, c, s, p, a, ws);
+}
+
+template <int D, int NT>
+static cudaError_t launch_rows(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
+  constexpr size_t kShared = sizeof(AttnShared<D, NT>);
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(cache_attention_kernel<D, NT>, kShared);
+  const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
+  return e != cudaSuccess ? e : launch(cache_attention_kernel<D, NT>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
 }
 
 template <int D>
 static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, cudaStream_t stream) {
   const AttnShape a = shape_of(c, s, p);
+  const int64_t heads = static_cast<int64_t>(s.B) * c.H;
+  if (heads * a.rows > INT32_MAX || (a.stats && heads * s.blocks > INT32_MAX)) return set_error(KD_ERR_LIMIT, "%d sequences of %d blocks are too many for one call", s.B, s.blocks);
   AttnWorkspace ws;
   workspace_of(c, s, p, a, static_cast<char*>(p.workspace), &ws);
-  switch (tiles_of_item(a.rows)) {
-    case 1: return launch_for<D, 1>(c, s, p, a, ws, stream);
-    case 2: return launch_for<D, 2>(c, s, p, a, ws, stream);
-    default: return launch_for<D, 4>(c, s, p, a, ws, stream);
+  const int rows = rows_of_item(a.rows);
+  cudaError_t e = cudaSuccess;
+  if (rows == KC_ROWS) {
+    const int rc = launch_attention_chunk(c, s, p, a, ws, stream);
+    if (rc) return rc;
+  } else {
+    e = rows == KA_TILE ? launch_rows<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_rows<D, 2>(c, s, p, a, ws, stream) : launch_rows<D, 4>(c, s, p, a, ws, stream);
   }
+  if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(heads * a.rows), KJ_GROUPS * 32, 0, stream, c, s, p, a, ws, rows);
+  if (e == cudaSuccess) e = rows == KA_TILE ? launch_weights<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);
+  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
+  return 0;
 }
 
 int launch_cache_attention(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, cudaStream_t stream) {

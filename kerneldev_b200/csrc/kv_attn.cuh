@@ -1,0 +1,133 @@
+// What the two kernels of the cache's attention share (kv_attn.cu: few query rows, kv_attn_chunk.cu: many): rows and their masks, how the pages
+// are shared out, the parts that a join puts together.
+#pragma once
+#include "kv_cache.cuh"
+
+namespace kd {
+
+constexpr float KA_OFFSET = 8.f, KA_SLACK = 6.f, KA_LOG2E = 1.4426950408889634f;
+constexpr float KA_TINY = 1e-37f;   // in place of factors that a float flushes to 0 (every score is as good as 0 then): masked scores stay -inf, and not 0 * inf
+
+// What the mask needs of a query row. A row that does not exist, or sees nothing, has limit 0, sees 0 and a key that no descriptor matches.
+struct RowMask {
+  int limit;          // keys j < limit are no later than the row's own token (or all, without causality)
+  uint32_t sees;      // classes seen wherever they are
+  uint32_t causal;    // classes seen up to limit
+  uint32_t span_key;  // see span_key_of_query
+};
+
+struct AttnShape {
+  int G, rows, tiles;   // heads of a group, query rows of a key head, items that they are cut into
+  int ctas;             // 0: a CTA for each (sequence, head, tile); else at most that many CTAs share all pages evenly
+  int least;            // pages that such a CTA has at least
+  bool stats;           // leave every row's maximum and sum for the weights
+};
+// Workspace: the rows' statistics (float2 for each, with weights), then for each CTA two parts: an item's rows of D floats, and their maxima and sums.
+struct AttnWorkspace {
+  float2* stats;
+  float* part_o;
+  float2* part_ml;
+};
+
+__device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) > 0x7F800000u; }
+
+struct Item {
+  int b, h, tile, len;
+};
+
+__device__ __forceinline__ int query_count(const kd_cache& c, const kd_cache_queries& p, int b) {
+  return p.q_lens != nullptr ? checked_count(c, p.q_lens[b], p.T) : p.T;
+}
+
+// one row's mask; r: row of the key head (query r / G of head r % G of the group)
+__device__ __forceinline__ RowMask row_mask(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int r, int G, int rows, int n_queries) {
+  const int i = r / G, at = it.len - n_queries + i;
+  RowMask m{0, 0u, 0u, 1u};
+  if (r >= rows || i >= n_queries || at < 0) return m;
+  uint32_t d = pack_plain(true);
+  m.limit = p.causal != 0 || c.desc != nullptr ? at + 1 : it.len;
+  if (c.desc != nullptr) {
+    const int page = page_of(c, s, it.b, at / KC_PAGE);
+    d = page >= 0 ? c.desc[block_index(c, page, it.h) * KC_PAGE + at % KC_PAGE] : 0u;
+    m.span_key = span_key_of_query(d);
+  }
+  m.sees = (d >> TD_SEES_SHIFT) & 7u;
+  m.causal = d & TD_CTX;
+  return m;
+}
+
+// A row's output from its sum and accumulated values (scaled by 1 / sum): 16 bits, and its log-sum-exp and statistics.
+__device__ __forceinline__ void write_stats(const kd_cache_queries& p, const AttnWorkspace& ws, bool stats, size_t row, bool live, float ref, float sum) {
+  if (p.lse != nullptr) p.lse[row] = live && sum != 0.f ? ref - KA_OFFSET + log2f(sum) : -INFINITY;
+  if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
+}
+
+// The flat order of all pages: sequences in turn, each once for every head and tile, cut into even ranges for the CTAs. 32 bits are enough: the host sees to
+// it that there are fewer than 2^30 pages. A warp holds the page counts of the first 128 sequences, in its lanes.
+struct FlatPlace {
+  int b, ht, page, pages;   // page: index within the item
+};
+struct FlatOrder {
+  static constexpr int HELD = 4;
+  int held[HELD];
+  uint32_t total;             // pages
+  uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
+
+  static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
+  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {   // of sequence 32 i + lane
+    if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
+    return pages_of(c, s, 32 * i + (threadIdx.x & 31));
+  }
+  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT, const AttnShape& shape) {
+    const int lane = threadIdx.x & 31;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) n += held[i] = pages_of(c, s, 32 * i + lane);
+    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b);
+    total = __reduce_add_sync(0xffffffffu, n) * HT;
+    // (None of them has no page: the join reads a part of every CTA of an item.)
+    ctas = max(min(static_cast<uint32_t>(shape.ctas), (total + shape.least - 1) / shape.least), 1u);
+    each = total / ctas;
+    more = total - each * ctas;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t cta) const { return cta * each + min(cta, more); }
+  __device__ __forceinline__ uint32_t cta_of(uint32_t page) const {
+    const uint32_t longer = more * (each + 1);
+    return page < longer ? page / (each + 1) : more + (page - longer) / each;
+  }
+  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, uint32_t at) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t before = 0;
+    for (int i = 0; 32 * i < s.B; ++i) {
+      const int mine = pages(c, s, i);
+      uint32_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * HT > at);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l);
+        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT, ht = rest / static_cast<uint32_t>(n);
+        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n};
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return FlatPlace{-1, 0, 0, 0};
+  }
+  // pages of the sequences before b
+  __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t n = 0;
+    for (int i = 0; 32 * i < b; ++i)
+      if (32 * i + lane < b) n += pages(c, s, i);
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+};
+
+// kv_attn_chunk.cu
+constexpr int KC_ROWS = 128, KC_CTAS = 2;   // query rows of an item, CTAs of an SM
+int launch_attention_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+
+}  // namespace kd

@@ -1,0 +1,538 @@
+// Attention over the 8-bit cache for many query rows of a key head (a chunk of a prompt): 128 rows of a CTA on tcgen05, two CTAs an SM.
+//
+// The products are GEMMs here, so the cache's tiles are converted once for 128 rows: e4m3 to halves (exact) into swizzled shared memory, and both
+// products run on halves with S, P and O in TMEM. Roles (256 threads, so that each has 128 registers):
+//   warps 0-3  softmax, a thread to a row: masks, running maximum, P over the scores it was made from. Warp 0 issues the products: P V when all four
+//              warps' P is there, directly behind it the next scores
+//   warps 4-7  converters: 128 tokens (two pages) at a time from global memory through registers, one tile ahead. They decide which tiles are worked on:
+//              one that no row of the CTA sees is left out (spans of a hierarchical mask, tokens behind the chunk)
+// Q, one K tile and one V tile are 96 KB at head dim 128 and S and O 256 columns, so that two CTAs share an SM: the exponentials of one run under
+// the products of the other. Scales, the offset of the probabilities and the slack of the maximum are as in kv_attn.cu.
+//
+// A tile's chain is: K converted -> S -> softmax -> P V, and the next S directly behind P V. Barriers, each used once a tile:
+//   K   converters: K and the tile's record are there     S   S is complete (K is free)
+//   V   converters: V is there                            P   softmax: P is there         PV  P V is complete (V, P's columns and O are free)
+// Every wait is bounded. One that runs out is reported through status_mirror, and all roles end their item.
+//
+// NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
+// token gets NaN there.
+#include <algorithm>
+
+#include "attn_common.cuh"
+#include "kv_attn.cuh"
+
+namespace kd {
+
+constexpr int CH_THREADS = 256, CH_TOKENS = 128, CH_RECORDS = 3;
+constexpr uint32_t CH_SITE = 0x900u;   // wait sites 0x900 .. : role << 4 | barrier
+
+// One tile of the walk, written by the converters for the others. Three slots in turn: the words of the tile ahead are written while the tile in hand is worked on, and the
+// one before it may be.
+struct ChunkRecord {
+  int j0;                // first token
+  int end;               // there is no tile: the item is done
+  float ks[2];           // the pages' K scales and V exponents
+  int ev[2];
+  uint32_t words[3][4];  // tokens that are prefix, context, in a span (without metadata: all that exist, as context)
+  uint32_t desc[CH_TOKENS];
+};
+
+// What no row of the CTA sees can be left out: what its rows see, put together.
+struct ChunkRows {
+  uint32_t sees, causal;   // classes
+  int max_limit;
+  int spans;               // some row looks for its own span
+};
+
+template <int D>
+struct ChunkShared {
+  static constexpr int BLOCKS = D > 64 ? 2 : 1, BLOCK = 128 * 128, TILE = BLOCKS * BLOCK;   // 64 head dims of 128 rows
+  uint8_t q[TILE], k[TILE], v[TILE];
+  ChunkRecord record[CH_RECORDS];
+  uint16_t nan_bits[CH_TOKENS][8];   // second pass alone: which of a token's head dims are NaN, 16 to a word
+  float factor[KC_ROWS];
+  RowMask mask[KC_ROWS];
+  ChunkRows rows;
+  uint64_t bar[5];
+  uint32_t tmem, any_nan;
+  int tiles;                         // of the pass
+  AbortFlag abort;
+};
+enum { CB_K, CB_S, CB_V, CB_P, CB_PV };
+
+// byte of element (row, d) in a tile: 64 head dims of a row are 128 bytes, swizzled
+__device__ __forceinline__ uint32_t chunk_place(int row, int d) { return (d >> 6) * (128 * 128) + sw128_offset(row, (d & 63) >> 3) + (d & 7) * 2; }
+
+// words of what a row sees of a tile
+__device__ __forceinline__ void row_words(const RowMask& m, const ChunkRecord& r, bool metadata, int lane, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t upto = low_bits(m.limit - r.j0 - 32 * i);
+    w[i] = r.words[1][i] & (((m.sees & TD_CTX) != 0u ? 0xFFFFFFFFu : 0u) | ((m.causal & TD_CTX) != 0u ? upto : 0u));
+    if (metadata) {
+      if ((m.sees & TD_PRE) != 0u) w[i] |= r.words[0][i];
+      if ((m.sees & TD_INS) != 0u) w[i] |= r.words[2][i];
+    }
+  }
+  if (!metadata || (r.words[2][0] | r.words[2][1] | r.words[2][2] | r.words[2][3]) == 0u) return;
+  uint32_t todo = __ballot_sync(0xffffffffu, m.span_key != 1u);   // one round for each span among the rows
+  while (todo != 0u) {
+    const uint32_t key = __shfl_sync(0xffffffffu, m.span_key, __ffs(todo) - 1);
+    const bool mine = m.span_key == key;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, span_match_key(key, r.desc[32 * i + lane]) != 0u);
+      if (mine) w[i] |= hit;
+    }
+    todo &= ~__ballot_sync(0xffffffffu, mine);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(CH_THREADS, KC_CTAS)
+cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
+                             const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  using Sh = ChunkShared<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Sh& sh = *reinterpret_cast<Sh*>(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), HT = c.H * shape.tiles;
+  const bool metadata = c.desc != nullptr;
+  auto bar = [&](int i) { return smem_u32(&sh.bar[i]); };
+  if (tid == 0) {
+    sh.abort.v = 0;
+    mbar_init(bar(CB_K), 4);
+    mbar_init(bar(CB_S), 1);
+    mbar_init(bar(CB_V), 4);
+    mbar_init(bar(CB_P), 4);
+    mbar_init(bar(CB_PV), 1);
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(&sh.tmem), 256);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tS = sh.tmem, tO = tS + CH_TOKENS;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const FlatOrder order(c, s, HT, shape);
+  uint32_t at = 0, end = 1;
+  if (shape.ctas > 0) {
+    const bool mine = blockIdx.x < order.ctas && order.total > 0;
+    at = mine ? order.start(blockIdx.x) : 0;
+    end = mine ? order.start(blockIdx.x + 1) : 0;
+  }
+  const uint32_t begin = at;
+  int n_k = 0, n_t = 0;   // uses of barrier K (one more than tiles for each pass over an item) and of the others
+  auto wait = [&](int i, int use, int role) {
+    return __all_sync(0xffffffffu, mbar_wait(bar(i), use & 1, &sh.abort, CH_SITE | role << 4 | i));
+  };
+  while (at < end) {
+    Item it;
+    int page0 = 0, pages, here;
+    if (shape.ctas > 0) {
+      const FlatPlace f = order.find(c, s, HT, at);
+      it.b = f.b;
+      it.h = f.ht / shape.tiles;
+      it.tile = f.ht - it.h * shape.tiles;
+      it.len = sequence_length(c, s, it.b);
+      page0 = f.page;
+      pages = f.pages;
+      here = min(static_cast<int>(end - at), pages - page0);
+    } else {
+      const int item = blockIdx.x;
+      it.b = item / HT;
+      it.h = (item - it.b * HT) / shape.tiles;
+      it.tile = item - it.b * HT - it.h * shape.tiles;
+      it.len = sequence_length(c, s, it.b);
+      pages = here = (it.len + KC_PAGE - 1) / KC_PAGE;
+    }
+    const int page_end = page0 + here;
+
+    // ---- Q as halves (bfloat16 times a power of two, see kv_attn.cu), masks and what the rows see together ----
+    if (tid == 0) {
+      sh.rows = ChunkRows{0u, 0u, 0, 0};
+      sh.any_nan = 0u;
+    }
+    __syncthreads();
+    for (int r = warp; r < KC_ROWS; r += CH_THREADS / 32) {
+      const int row = it.tile * KC_ROWS + r, d = 4 * lane;
+      uint2 v = make_uint2(0u, 0u);
+      if (row < shape.rows && d < D) {
+        const int n = row / shape.G, hq = it.h * shape.G + row - n * shape.G;
+        v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
+      }
+      int e = 0;
+      if (p.dtype == KD_BF16) {
+        auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
+        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v.x), size(v.x >> 16)), max(size(v.y), size(v.y >> 16))));
+        if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
+        const float f = exp2i(e);
+        const float2 a = unpack2<true>(v.x), b = unpack2<true>(v.y);
+        v = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+      }
+      if (lane == 0) sh.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+      if (d < D) *reinterpret_cast<uint2*>(sh.q + chunk_place(r, d)) = v;
+    }
+    if (tid < KC_ROWS) {
+      const RowMask m = row_mask(c, s, p, it, it.tile * KC_ROWS + tid, shape.G, shape.rows, query_count(c, p, it.b));
+      sh.mask[tid] = m;
+      const uint32_t sees = __reduce_or_sync(0xffffffffu, m.sees), causal = __reduce_or_sync(0xffffffffu, m.causal);
+      const int limit = __reduce_max_sync(0xffffffffu, m.limit);
+      const bool spans = __any_sync(0xffffffffu, m.span_key != 1u);
+      if (lane == 0) {
+        atomicOr(&sh.rows.sees, sees);
+        atomicOr(&sh.rows.causal, causal);
+        atomicMax(&sh.rows.max_limit, limit);
+        if (spans) sh.rows.spans = 1;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+
+    const bool whole = here == pages;
+    const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (at == begin ? 0 : 1);
+    for (int pass = 0; pass < 2; ++pass) {   // the second one where the first one's output has NaN
+      const bool safe = pass == 1;
+      if (warp >= 4) {
+        // ---------------------------------------- converters ----------------------------------------
+        const int r = tid - 128;   // this thread's token of the tile for the descriptors
+        const ChunkRows rows = sh.rows;
+        // thread: 16 head dims of tokens; a quarter of a warp has two tokens' 64 head dims of a block, so that its stores take all banks
+        const int col = (r & 3) * 16, row0 = r >> 2;
+        constexpr int ROUNDS = 4 * Sh::BLOCKS;   // 32 tokens and one block of 64 head dims each
+        struct Tile {
+          int page[2], j0;
+          uint32_t desc;
+        } cur;
+        uint4 kreg[ROUNDS], vreg[ROUNDS];
+        int next = page0;
+        bool ok = true;
+        // The next tile that some row sees, from `next` on. All four warps come to the same answer: the words are exchanged through the record that is to have them.
+        auto find = [&](int slot) {
+          ChunkRecord& rec = sh.record[slot];
+          for (; next < page_end; next += 2) {
+            cur.j0 = next * KC_PAGE;
+            cur.page[0] = page_of(c, s, it.b, next);
+            cur.page[1] = next + 1 < page_end ? page_of(c, s, it.b, next + 1) : -1;
+            const int page = r < KC_PAGE ? cur.page[0] : cur.page[1];
+            const bool alive = cur.j0 + r < it.len && page >= 0;
+            cur.desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
+            const uint32_t pre = __ballot_sync(0xffffffffu, (cur.desc & TD_PRE) != 0u), ctx = __ballot_sync(0xffffffffu, (cur.desc & TD_CTX) != 0u),
+                           ins = __ballot_sync(0xffffffffu, (cur.desc & TD_INS) != 0u);
+            if (!metadata) {
+              if (cur.j0 >= rows.max_limit) continue;   // (the limits are no more than the length)
+              if (lane == 0) rec.words[1][r >> 5] = ctx;
+              next += 2;
+              return true;
+            }
+            named_bar_sync(1, 128);   // everyone has looked at the words of the tile before
+            if (lane == 0) {
+              rec.words[0][r >> 5] = pre;
+              rec.words[1][r >> 5] = ctx;
+              rec.words[2][r >> 5] = ins;
+            }
+            named_bar_sync(1, 128);
+            uint32_t any[3];
+#pragma unroll
+            for (int x = 0; x < 3; ++x) any[x] = rec.words[x][0] | rec.words[x][1] | rec.words[x][2] | rec.words[x][3];
+            const bool seen = ((rows.sees & TD_PRE) != 0u && any[0] != 0u) || ((rows.sees & TD_CTX) != 0u && any[1] != 0u) || (((rows.sees & TD_INS) != 0u || rows.spans != 0) && any[2] != 0u) ||
+                              ((rows.causal & TD_CTX) != 0u && any[1] != 0u && cur.j0 < rows.max_limit);
+            if (seen) {
+              next += 2;
+              return true;
+            }
+          }
+          return false;
+        };
+        auto fetch = [&](const void* from, uint4 (&reg)[ROUNDS]) {
+#pragma unroll
+          for (int i = 0; i < ROUNDS; ++i) {
+            const int token = (i & 3) * 32 + row0, d = (i >> 2) * 64 + col, page = cur.page[token / KC_PAGE];
+            reg[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (page >= 0 && d < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(from) + (block_index(c, page, it.h) * KC_PAGE + token % KC_PAGE) * D + d));
+          }
+        };
+        auto store = [&](uint8_t* to, const uint4 (&reg)[ROUNDS], bool without_nan) {
+#pragma unroll
+          for (int i = 0; i < ROUNDS; ++i) {
+            const int token = (i & 3) * 32 + row0, d = (i >> 2) * 64 + col;
+            uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+            if (without_nan) {
+              uint32_t bits = 0;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const uint32_t n = __vcmpeq4(w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+                w[x] &= ~n;
+                bits |= ((n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u)) << (4 * x);
+              }
+              if (d < D) sh.nan_bits[token][d / 16] = static_cast<uint16_t>(bits);
+            }
+            uint4 out[2];
+            uint32_t* o = reinterpret_cast<uint32_t*>(out);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const HalfPairs h = e4m3x4_to_f16x4(w[x]);
+              o[2 * x] = h.lo;
+              o[2 * x + 1] = h.hi;
+            }
+            *reinterpret_cast<uint4*>(to + chunk_place(token, d)) = out[0];
+            *reinterpret_cast<uint4*>(to + chunk_place(token, d + 8)) = out[1];
+          }
+        };
+        int u = 0;   // tiles of this pass
+        bool have = find(n_k % CH_RECORDS);
+        if (have) fetch(c.k, kreg);
+        if (have) fetch(c.v, vreg);
+        for (;; ++u) {
+          // (K's place and the record's slot are free when the scores of the tile before are complete; the slot of two tiles before by then, too)
+          if (u > 0 && !(ok = wait(CB_S, n_t + u - 1, 1))) break;
+          ChunkRecord& rec = sh.record[(n_k + u) % CH_RECORDS];
+          if (r < 2) {
+            const int page = cur.page[r];
+            const size_t place = have && page >= 0 ? block_index(c, page, it.h) : 0;
+            rec.ks[r] = have && page >= 0 ? c.k_scale[place] : 1.f;
+            rec.ev[r] = have && page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
+          }
+          if (r == 0) {
+            rec.j0 = cur.j0;
+            rec.end = have ? 0 : 1;
+          }
+          if (have) {
+            if (metadata) rec.desc[r] = cur.desc;
+            store(sh.k, kreg, false);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(CB_K));
+          if (!have) break;
+          const bool more = find((n_k + u + 1) % CH_RECORDS);
+          if (more) fetch(c.k, kreg);
+          if (u > 0 && !(ok = wait(CB_PV, n_t + u - 1, 1))) break;
+          store(sh.v, vreg, safe);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(CB_V));
+          have = more;
+          if (more) fetch(c.v, vreg);
+        }
+      } else {
+        // ---------------------------------------- softmax ----------------------------------------
+        const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, mS = tS + lanes, mO = tO + lanes;
+        const RowMask mask = sh.mask[tid];
+        const float factor = sh.factor[tid];
+        const uint32_t idesc_s = make_idesc_f16(0, 0, 0, KC_ROWS, CH_TOKENS), idesc_o = make_idesc_f16(0, 0, 1, KC_ROWS, 64 * Sh::BLOCKS);
+        auto issue_scores = [&]() {   // of a tile whose K is there
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint32_t q = smem_u32(sh.q), k = smem_u32(sh.k);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+              mma_ss(tS, desc_kmajor_sw128(q + (i / 4) * Sh::BLOCK, i & 3), desc_kmajor_sw128(k + (i / 4) * Sh::BLOCK, i & 3), idesc_s, i > 0 ? 1u : 0u);
+            mma_commit(bar(CB_S));
+          }
+          __syncwarp();
+        };
+        auto issue_values = [&](bool first) {   // with P and V there
+          tc_fence_after_sync();
+          if (elect_one()) {
+            const uint32_t v = smem_u32(sh.v);
+#pragma unroll
+            for (int i = 0; i < CH_TOKENS / 16; ++i) mma_ts(tO, tS + 8 * i, desc_mnmajor_sw128(v, i, Sh::BLOCK), idesc_o, !first || i > 0 ? 1u : 0u);
+            mma_commit(bar(CB_PV));
+          }
+          __syncwarp();
+        };
+        float ref = -INFINITY, sum = 0.f;
+        uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
+        bool ok = true;
+        int u = 0;
+        for (;; ++u) {
+          if (!(ok = wait(CB_K, n_k + u, 0))) break;
+          const ChunkRecord& rec = sh.record[(n_k + u) % CH_RECORDS];
+          if (*const_cast<const volatile int*>(&rec.end) != 0) break;
+          if (warp == 0) issue_scores();
+          uint32_t w[4];
+          row_words(mask, rec, metadata, lane, w);
+          const float kf[2] = {fmaxf(rec.ks[0] * factor, KA_TINY), fmaxf(rec.ks[1] * factor, KA_TINY)};
+          const int ev[2] = {rec.ev[0], rec.ev[1]};
+          if (safe) {
+            if (!(ok = wait(CB_V, n_t + u, 0))) break;
+            for (int j = 0; j < CH_TOKENS; ++j) {
+              if ((w[j >> 5] >> (j & 31) & 1u) == 0u) continue;
+              const uint4 n = *reinterpret_cast<const uint4*>(sh.nan_bits[j]);
+              nan_cols[0] |= n.x;
+              nan_cols[1] |= n.y;
+              nan_cols[2] |= n.z;
+              nan_cols[3] |= n.w;
+            }
+          }
+          if (!(ok = wait(CB_S, n_t + u, 0))) break;
+          tc_fence_after_sync();
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (__all_sync(0xffffffffu, w[i] == 0u)) continue;
+            uint32_t x[32];
+            tmem_ld32(mS + 32 * i, x);
+            tmem_wait_ld();
+            if (!__all_sync(0xffffffffu, w[i] == 0xFFFFFFFFu)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if ((w[i] & (1u << j)) == 0u) x[j] = 0xFF800000u;
+            }
+            float m4[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m4[j] = __uint_as_float(x[j]);
+#pragma unroll
+            for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(x[j]));
+            top[i >> 1] = fmaxf(top[i >> 1], fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+          }
+          const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
+          const bool up = high > ref + KA_SLACK;
+          if (__any_sync(0xffffffffu, up)) {
+            const float to = up ? high : ref, shrink = up ? fast_exp2(ref - to) : 1.f;
+            if (u > 0 && __any_sync(0xffffffffu, up && ref != -INFINITY)) {   // O is complete: its last product came before these scores
+#pragma unroll 1
+              for (int i = 0; i < D; i += 16) {
+                uint32_t x[16];
+                tmem_ld16(mO + i, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * shrink);
+                tmem_st16(mO + i, x);
+              }
+            }
+            sum *= shrink;
+            ref = to;
+          }
+          const float base = ref == -INFINITY ? 0.f : KA_OFFSET - ref;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t pk[16];
+            if (__all_sync(0xffffffffu, w[i] == 0u)) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) pk[j] = 0u;
+            } else {
+              uint32_t x[32];
+              tmem_ld32(mS + 32 * i, x);
+              tmem_wait_ld();
+              if (!__all_sync(0xffffffffu, w[i] == 0xFFFFFFFFu)) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if ((w[i] & (1u << j)) == 0u) x[j] = 0xFF800000u;
+              }
+              const float k = kf[i >> 1], add = base + static_cast<float>(ev[i >> 1]);
+              float part[2] = {0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float a = fast_exp2(fmaf(__uint_as_float(x[2 * j]), k, add)), b = fast_exp2(fmaf(__uint_as_float(x[2 * j + 1]), k, add));
+                part[0] += a;
+                part[1] += b;
+                pk[j] = pack2<false>(a, b);
+              }
+              sum = fmaf(part[0] + part[1], exp2i(-ev[i >> 1]), sum);
+            }
+            tmem_st16(mS + 16 * i, pk);   // over scores that have been read
+          }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(CB_P));
+          if (warp == 0) {
+            if (!(ok = wait(CB_V, n_t + u, 0) && wait(CB_P, n_t + u, 0))) break;
+            issue_values(u == 0);
+          }
+        }
+        if (ok && u > 0) ok = wait(CB_PV, n_t + u - 1, 0);
+        tc_fence_after_sync();
+        // ---- this row's output ----
+        const int row = it.tile * KC_ROWS + tid;
+        const bool live = mask.limit > 0, exists = row < shape.rows;
+        const int i = row / shape.G, hq = it.h * shape.G + row - i * shape.G;
+        const float inv = !whole ? 1.f : live && sum != 0.f ? 1.f / sum : 0.f;
+        bool bad = false;
+        if (ok) {
+          if (exists && whole) write_stats(p, ws, shape.stats, (static_cast<size_t>(it.b) * p.H + hq) * p.T + i, live, ref, sum);
+          if (exists && !whole) ws.part_ml[part * KC_ROWS + tid] = make_float2(ref, sum);
+          uint16_t* out = static_cast<uint16_t*>(p.o.ptr) + it.b * p.o.stride_b + hq * p.o.stride_h + i * p.o.stride_t;
+          float* part_o = ws.part_o + (part * KC_ROWS + tid) * D;
+#pragma unroll
+          for (int d = 0; d < D; d += 16) {
+            uint32_t x[16];
+            if (u > 0) {
+              tmem_ld16(mO + d, x);
+              tmem_wait_ld();
+            }
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              f[j] = u > 0 && inv != 0.f ? __uint_as_float(x[j]) * inv : 0.f;
+              if (safe && inv != 0.f && (nan_cols[d >> 5] >> ((d & 16) + j) & 1u) != 0u) f[j] = __uint_as_float(0x7FC00000u);
+              bad = bad || is_nan(f[j]);
+            }
+            if (exists && whole) {
+              if (p.dtype == KD_BF16) store16<KD_BF16>(out + d, f);
+              else store16<KD_F16>(out + d, f);
+            } else if (exists) {
+              store16<KD_F32>(part_o + d, f);
+            }
+          }
+          tc_fence_before_sync();
+        }
+        if (bad) sh.any_nan = 1u;
+        if (tid == 0) sh.tiles = u;   // (the converters' count is the same)
+        if (!ok && warp == 0) {   // what has been issued ends before TMEM is given back
+          if (u > 0) drain_wait(bar(CB_PV), (n_t + u - 1) & 1);
+          drain_wait(bar(CB_S), (n_t + u) & 1);
+        }
+      }
+      __syncthreads();
+      const int tiles = sh.tiles;
+      n_k += tiles + 1;
+      n_t += tiles;
+      const bool again = pass == 0 && sh.any_nan != 0u;
+      if (sh.abort.v != 0u || !again) break;
+      __syncthreads();
+    }
+    __syncthreads();   // the next item's rows may take this one's place
+    if (sh.abort.v != 0u) break;
+    at += shape.ctas > 0 ? here : 1;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (tid == 0 && sh.abort.v != 0u) cache_report(c, sh.abort.v);
+  if (warp == 4) tmem_dealloc(tS, 256);
+}
+
+template <int D>
+static cudaError_t launch_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
+  constexpr size_t kShared = sizeof(ChunkShared<D>);
+  static_assert(kShared <= 113 * 1024, "two CTAs share an SM");
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(cache_attention_chunk_kernel<D>, kShared);
+  const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
+  return e != cudaSuccess ? e : launch(cache_attention_chunk_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), CH_THREADS, kShared, stream, c, s, p, a, ws);
+}
+
+int launch_attention_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
+  cudaError_t e;
+  switch (c.D) {
+    case 16: e = launch_chunk<16>(c, s, p, a, ws, stream); break;
+    case 32: e = launch_chunk<32>(c, s, p, a, ws, stream); break;
+    case 48: e = launch_chunk<48>(c, s, p, a, ws, stream); break;
+    case 64: e = launch_chunk<64>(c, s, p, a, ws, stream); break;
+    case 80: e = launch_chunk<80>(c, s, p, a, ws, stream); break;
+    case 96: e = launch_chunk<96>(c, s, p, a, ws, stream); break;
+    case 112: e = launch_chunk<112>(c, s, p, a, ws, stream); break;
+    default: e = launch_chunk<128>(c, s, p, a, ws, stream);
+  }
+  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention_chunk launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+}  // namespace kd
