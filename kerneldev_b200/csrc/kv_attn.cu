@@ -431,7 +431,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
-  const FlatOrder order(c, s, HT, shape);
+  const FlatOrder order(c, s, p, shape);
   uint32_t at = 0, end = 1;
   if (shape.ctas > 0) {
     if (blockIdx.x >= order.ctas || order.total == 0) return;
@@ -447,10 +447,10 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
     Share r;
     int page0 = 0;
     if (shape.ctas > 0) {
-      const FlatPlace f = order.find(c, s, HT, place_of);
+      const FlatPlace f = order.find(c, s, p, shape, place_of);
       r.it.b = f.b;
-      r.it.h = f.ht / shape.tiles;
-      r.it.tile = f.ht - r.it.h * shape.tiles;
+      r.it.h = f.ht / f.tiles;
+      r.it.tile = f.ht - r.it.h * f.tiles;
       r.it.len = sequence_length(c, s, r.it.b);
       page0 = f.page;
       r.pages = f.pages;
@@ -553,36 +553,40 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   }
 }
 
-// One query row whose pages several CTAs shared: their parts on one scale. Eight groups of 32 threads take parts in turn. What it needs to know of the lengths
-// was there before the kernel ahead of it, so it is looked up while that one runs.
-constexpr int KJ_GROUPS = 8;
-__global__ void __launch_bounds__(KJ_GROUPS * 32)
+// Query rows whose pages several CTAs shared: their parts on one scale. kGroups warps of a CTA take a row's parts in turn, 8 / kGroups rows a CTA: eight warps for a row where
+// there are few rows (a long context has dozens of parts), one where there are many. Rows without a query, and those of sequences without a token, get their zeros here.
+// What it needs to know of the lengths was there before the kernel ahead of it, so it is looked up while that one runs.
+constexpr int KJ_WARPS = 8;
+template <int kGroups>
+__global__ void __launch_bounds__(KJ_WARPS * 32)
 cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
-                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws, int rows_of_item) {
-  __shared__ float4 s_o[KJ_GROUPS][32];
-  __shared__ float2 s_ml[KJ_GROUPS];
-  const int tid = threadIdx.x, lane = tid & 31, grp = tid >> 5, HT = c.H * shape.tiles;
-  const int row_of_head = blockIdx.x % shape.rows, bh = blockIdx.x / shape.rows, b = bh / c.H, h = bh - b * c.H;
-  const int tile = row_of_head / rows_of_item, r = row_of_head - tile * rows_of_item;
-  const FlatOrder order(c, s, HT, shape);
-  const int len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
-  const uint32_t first = order.before(c, s, b) * HT + (h * shape.tiles + tile) * pages;   // the item's first page in the flat order
-  const int n = query_count(c, p, b);
+                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  constexpr int ROWS = KJ_WARPS / kGroups;
+  __shared__ float4 s_o[kGroups > 1 ? KJ_WARPS : 1][32];
+  __shared__ float2 s_ml[KJ_WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, grp = (tid >> 5) % kGroups;
+  const int per_head = (shape.rows + ROWS - 1) / ROWS;
+  const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + (tid >> 5) / kGroups;
+  const int tile = row_of_head / shape.item_rows, r = row_of_head - tile * shape.item_rows;
+  const FlatOrder order(c, s, p, shape);
+  const int len = sequence_length(c, s, b), n = query_count(c, p, b), tiles = (n * shape.G + shape.item_rows - 1) / shape.item_rows;
+  const int pages = tile < tiles ? (len + KC_PAGE - 1) / KC_PAGE : 0;   // of the item
+  const uint32_t first = order.before(c, s, p, shape, b) + (h * tiles + tile) * pages;   // the item's first page in the flat order
   int c0 = 0, c1 = -1;
   if (pages > 0) {
     c0 = static_cast<int>(order.cta_of(first));
     c1 = static_cast<int>(order.cta_of(first + pages - 1));
   }
-  const size_t first_part = (2 * static_cast<size_t>(c0) + (order.start(c0) >= first ? 0 : 1)) * rows_of_item + r;
+  const size_t first_part = (2 * static_cast<size_t>(c0) + (order.start(c0) >= first ? 0 : 1)) * shape.item_rows + r;
   pdl_wait();
   pdl_launch_dependents();
-  if (c0 == c1) return;   // the one CTA has written the row
+  if (c0 == c1 || row_of_head >= shape.rows) return;   // the one CTA has written the row (with kGroups > 1 there is one row, so that all warps leave)
   const int d = lane * 4;
   float ref = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = c0 + grp; k <= c1; k += KJ_GROUPS) {
-    const size_t part = k == c0 ? first_part : 2 * static_cast<size_t>(k) * rows_of_item + r;
+  for (int k = c0 + grp; k <= c1; k += kGroups) {
+    const size_t part = k == c0 ? first_part : 2 * static_cast<size_t>(k) * shape.item_rows + r;
     const float2 ml = ws.part_ml[part];
     const float4 v = d < c.D ? *reinterpret_cast<const float4*>(ws.part_o + part * c.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     if (ml.x == -INFINITY) continue;
@@ -591,22 +595,25 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
     sum = fmaf(ml.y, scale, sum * keep);
     acc = make_float4(fmaf(v.x, scale, acc.x * keep), fmaf(v.y, scale, acc.y * keep), fmaf(v.z, scale, acc.z * keep), fmaf(v.w, scale, acc.w * keep));
   }
-  s_o[grp][lane] = acc;
-  if (lane == 0) s_ml[grp] = make_float2(ref, sum);
-  __syncthreads();
-  if (grp > 0) return;
-  ref = -INFINITY;
+  if constexpr (kGroups > 1) {
+    static_assert(ROWS == 1, "the barrier below is the whole CTA's");
+    s_o[grp][lane] = acc;
+    if (lane == 0) s_ml[grp] = make_float2(ref, sum);
+    __syncthreads();
+    if (grp > 0) return;
+    ref = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < KJ_GROUPS; ++k) ref = fmaxf(ref, s_ml[k].x);
-  sum = 0.f;
-  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < kGroups; ++k) ref = fmaxf(ref, s_ml[k].x);
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int k = 0; k < KJ_GROUPS; ++k) {
-    if (s_ml[k].x == -INFINITY) continue;
-    const float scale = fast_exp2(s_ml[k].x - ref);
-    const float4 v = s_o[k][lane];
-    sum = fmaf(s_ml[k].y, scale, sum);
-    acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
+    for (int k = 0; k < kGroups; ++k) {
+      if (s_ml[k].x == -INFINITY) continue;
+      const float scale = fast_exp2(s_ml[k].x - ref);
+      const float4 v = s_o[k][lane];
+      sum = fmaf(s_ml[k].y, scale, sum);
+      acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
+    }
   }
   const int i = row_of_head / shape.G, hq = h * shape.G + row_of_head - i * shape.G;
   const bool live = i < n && len - n + i >= 0;
@@ -719,7 +726,7 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   AttnShape a;
   a.G = p.H / c.H;
   a.rows = a.G * p.T;
-  const int rows = rows_of_item(a.rows);
+  const int rows = a.item_rows = rows_of_item(a.rows);
   a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
@@ -755,7 +762,8 @@ static cudaError_t launch_weights(const kd_cache& c, const kd_cache_seqs& s, con
   if (!a.stats || groups == 0) return cudaSuccess;
   constexpr size_t kShared = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
   static SmemOptIn opt_in;
-  a.tiles = (a.rows + NT * KA_TILE - 1) / (NT * KA_TILE);
+  a.item_rows = NT * KA_TILE;
+  a.tiles = (a.rows + a.item_rows - 1) / a.item_rows;
   const cudaError_t e = opt_in(cache_weights_kernel<D, NT>, kShared);
   return e != cudaSuccess ? e : launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kShared, stream, c, s, p, a, ws);
 }
@@ -784,7 +792,12 @@ static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_
   } else {
     e = rows == KA_TILE ? launch_rows<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_rows<D, 2>(c, s, p, a, ws, stream) : launch_rows<D, 4>(c, s, p, a, ws, stream);
   }
-  if (e == cudaSuccess && a.ctas > 0) e = launch(cache_join_kernel, static_cast<unsigned>(heads * a.rows), KJ_GROUPS * 32, 0, stream, c, s, p, a, ws, rows);
+  if (e == cudaSuccess && a.ctas > 0) {
+    // up to one row for each warp that fits on the device
+    const bool few = heads * a.rows <= 148 * 16;
+    e = few ? launch(cache_join_kernel<KJ_WARPS>, static_cast<unsigned>(heads * a.rows), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
+            : launch(cache_join_kernel<1>, static_cast<unsigned>(heads * ((a.rows + KJ_WARPS - 1) / KJ_WARPS)), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
+  }
   if (e == cudaSuccess) e = rows == KA_TILE ? launch_weights<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
   return 0;

@@ -19,6 +19,7 @@ struct RowMask {
 struct AttnShape {
   int G, rows, tiles;   // heads of a group, query rows of a key head, items that they are cut into
   int ctas;             // 0: a CTA for each (sequence, head, tile); else at most that many CTAs share all pages evenly
+  int item_rows;        // query rows of an item
   int least;            // pages that such a CTA has at least
   bool stats;           // leave every row's maximum and sum for the weights
 };
@@ -62,29 +63,42 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
   if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
 }
 
-// The flat order of all pages: sequences in turn, each once for every head and tile, cut into even ranges for the CTAs. 32 bits are enough: the host sees to
-// it that there are fewer than 2^30 pages. A warp holds the page counts of the first 128 sequences, in its lanes.
+// The flat order of all pages: sequences in turn, each once for every head and tile of rows that has a query, cut into even ranges for the CTAs. 32 bits are
+// enough: the host sees to it that there are fewer than 2^30 pages. A warp holds the counts of the first 128 sequences, in its lanes.
 struct FlatPlace {
-  int b, ht, page, pages;   // page: index within the item
+  int b, ht, page, pages, tiles;   // ht: head * tiles + tile, tiles: of the sequence; page: index within the item
 };
 struct FlatOrder {
   static constexpr int HELD = 4;
-  int held[HELD];
+  int held[HELD], held_tiles[HELD];
   uint32_t total;             // pages
   uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
 
   static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
-  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {   // of sequence 32 i + lane
+  static __device__ __forceinline__ int tiles_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) {
+    return b < s.B ? (query_count(c, p, b) * shape.G + shape.item_rows - 1) / shape.item_rows : 0;
+  }
+  // of sequence 32 i + lane
+  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {
     if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
     return pages_of(c, s, 32 * i + (threadIdx.x & 31));
   }
-  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, int HT, const AttnShape& shape) {
+  __device__ __forceinline__ int tiles(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int i) const {
+    if (i < HELD) return i == 0 ? held_tiles[0] : i == 1 ? held_tiles[1] : i == 2 ? held_tiles[2] : held_tiles[3];
+    return tiles_of(c, s, p, shape, 32 * i + (threadIdx.x & 31));
+  }
+  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape) {
     const int lane = threadIdx.x & 31;
     uint32_t n = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) n += held[i] = pages_of(c, s, 32 * i + lane);
-    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b);
-    total = __reduce_add_sync(0xffffffffu, n) * HT;
+    for (int i = 0; i < HELD; ++i) {
+      held[i] = pages_of(c, s, 32 * i + lane);
+      held_tiles[i] = tiles_of(c, s, p, shape, 32 * i + lane);
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) n += held[i] * held_tiles[i];
+    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b) * tiles_of(c, s, p, shape, b);
+    total = __reduce_add_sync(0xffffffffu, n) * c.H;
     // (None of them has no page: the join reads a part of every CTA of an item.)
     ctas = max(min(static_cast<uint32_t>(shape.ctas), (total + shape.least - 1) / shape.least), 1u);
     each = total / ctas;
@@ -95,34 +109,34 @@ struct FlatOrder {
     const uint32_t longer = more * (each + 1);
     return page < longer ? page / (each + 1) : more + (page - longer) / each;
   }
-  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, int HT, uint32_t at) const {
+  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, uint32_t at) const {
     const int lane = threadIdx.x & 31;
     uint32_t before = 0;
     for (int i = 0; 32 * i < s.B; ++i) {
-      const int mine = pages(c, s, i);
-      uint32_t upto = mine;
+      const int mine = pages(c, s, i), my_tiles = tiles(c, s, p, shape, i);
+      uint32_t upto = mine * my_tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += up;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * HT > at);
+      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * c.H > at);
       if (past != 0u) {
-        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l);
-        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n) * HT, ht = rest / static_cast<uint32_t>(n);
-        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n};
+        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l), tiles_b = __shfl_sync(0xffffffffu, my_tiles, l);
+        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n * tiles_b) * c.H, ht = rest / static_cast<uint32_t>(n);
+        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n, tiles_b};
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    return FlatPlace{-1, 0, 0, 0};
+    return FlatPlace{-1, 0, 0, 0, 0};
   }
   // pages of the sequences before b
-  __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, int b) const {
+  __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) const {
     const int lane = threadIdx.x & 31;
     uint32_t n = 0;
     for (int i = 0; 32 * i < b; ++i)
-      if (32 * i + lane < b) n += pages(c, s, i);
-    return __reduce_add_sync(0xffffffffu, n);
+      if (32 * i + lane < b) n += pages(c, s, i) * tiles(c, s, p, shape, i);
+    return __reduce_add_sync(0xffffffffu, n) * c.H;
   }
 };
 

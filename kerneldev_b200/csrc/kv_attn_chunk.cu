@@ -118,7 +118,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   pdl_wait();
   pdl_launch_dependents();
 
-  const FlatOrder order(c, s, HT, shape);
+  const FlatOrder order(c, s, p, shape);
   uint32_t at = 0, end = 1;
   if (shape.ctas > 0) {
     const bool mine = blockIdx.x < order.ctas && order.total > 0;
@@ -134,10 +134,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
     Item it;
     int page0 = 0, pages, here;
     if (shape.ctas > 0) {
-      const FlatPlace f = order.find(c, s, HT, at);
+      const FlatPlace f = order.find(c, s, p, shape, at);
       it.b = f.b;
-      it.h = f.ht / shape.tiles;
-      it.tile = f.ht - it.h * shape.tiles;
+      it.h = f.ht / f.tiles;
+      it.tile = f.ht - it.h * f.tiles;
       it.len = sequence_length(c, s, it.b);
       page0 = f.page;
       pages = f.pages;
@@ -248,18 +248,21 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           return false;
         };
+        const uint32_t place[2] = {chunk_place(row0, col), chunk_place(row0, col + 8)};   // of later rounds at fixed distances: 32 tokens 4 KB, a block 16 KB
         auto fetch = [&](const void* from, uint4 (&reg)[ROUNDS]) {
+          const uint8_t* base[2];
 #pragma unroll
-          for (int i = 0; i < ROUNDS; ++i) {
-            const int token = (i & 3) * 32 + row0, d = (i >> 2) * 64 + col, page = cur.page[token / KC_PAGE];
+          for (int x = 0; x < 2; ++x) base[x] = static_cast<const uint8_t*>(from) + (block_index(c, max(cur.page[x], 0), it.h) * KC_PAGE + row0) * D + col;
+#pragma unroll
+          for (int i = 0; i < ROUNDS; ++i) {   // tokens 32 (i & 3) + row0, head dims 64 (i >> 2) + col
+            const int x = (i & 3) >> 1;
             reg[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (page >= 0 && d < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(from) + (block_index(c, page, it.h) * KC_PAGE + token % KC_PAGE) * D + d));
+            if (cur.page[x] >= 0 && (i >> 2) * 64 + col < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(base[x] + (i & 1) * 32 * D + (i >> 2) * 64));
           }
         };
         auto store = [&](uint8_t* to, const uint4 (&reg)[ROUNDS], bool without_nan) {
 #pragma unroll
           for (int i = 0; i < ROUNDS; ++i) {
-            const int token = (i & 3) * 32 + row0, d = (i >> 2) * 64 + col;
             uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
             if (without_nan) {
               uint32_t bits = 0;
@@ -269,18 +272,13 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
                 w[x] &= ~n;
                 bits |= ((n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u)) << (4 * x);
               }
-              if (d < D) sh.nan_bits[token][d / 16] = static_cast<uint16_t>(bits);
+              const int d = (i >> 2) * 64 + col;
+              if (d < D) sh.nan_bits[32 * (i & 3) + row0][d / 16] = static_cast<uint16_t>(bits);
             }
-            uint4 out[2];
-            uint32_t* o = reinterpret_cast<uint32_t*>(out);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const HalfPairs h = e4m3x4_to_f16x4(w[x]);
-              o[2 * x] = h.lo;
-              o[2 * x + 1] = h.hi;
-            }
-            *reinterpret_cast<uint4*>(to + chunk_place(token, d)) = out[0];
-            *reinterpret_cast<uint4*>(to + chunk_place(token, d + 8)) = out[1];
+            const HalfPairs h0 = e4m3x4_to_f16x4(w[0]), h1 = e4m3x4_to_f16x4(w[1]), h2 = e4m3x4_to_f16x4(w[2]), h3 = e4m3x4_to_f16x4(w[3]);
+            uint8_t* at = to + (i & 3) * 4096 + (i >> 2) * Sh::BLOCK;
+            *reinterpret_cast<uint4*>(at + place[0]) = make_uint4(h0.lo, h0.hi, h1.lo, h1.hi);
+            *reinterpret_cast<uint4*>(at + place[1]) = make_uint4(h2.lo, h2.hi, h3.lo, h3.hi);
           }
         };
         int u = 0;   // tiles of this pass
@@ -341,7 +339,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (elect_one()) {
             const uint32_t v = smem_u32(sh.v);
 #pragma unroll
-            for (int i = 0; i < CH_TOKENS / 16; ++i) mma_ts(tO, tS + 8 * i, desc_mnmajor_sw128(v, i, Sh::BLOCK), idesc_o, !first || i > 0 ? 1u : 0u);
+            for (int i = 0; i < CH_TOKENS / 16; ++i) mma_ts(tO, tS + (i / 4) * 64 + (i & 3) * 8, desc_mnmajor_sw128(v, i, Sh::BLOCK), idesc_o, !first || i > 0 ? 1u : 0u);
             mma_commit(bar(CB_PV));
           }
           __syncwarp();
@@ -372,24 +370,34 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           if (!(ok = wait(CB_S, n_t + u, 0))) break;
           tc_fence_after_sync();
-          float top[2] = {-INFINITY, -INFINITY};
+          // Scores of 64 tokens (a page) in registers at a time: page 0's for its maximum alone, then page 1's, which stay there; after the exponentials of a half page its
+          // registers take page 0's scores again.
+          uint32_t x[2][32];
+          auto masked = [&](uint32_t (&y)[32], uint32_t bits) {
+            if (__all_sync(0xffffffffu, bits == 0xFFFFFFFFu)) return;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (__all_sync(0xffffffffu, w[i] == 0u)) continue;
-            uint32_t x[32];
-            tmem_ld32(mS + 32 * i, x);
+            for (int j = 0; j < 32; ++j)
+              if ((bits & (1u << j)) == 0u) y[j] = 0xFF800000u;
+          };
+          auto highest = [&](const uint32_t (&y)[32]) {
+            float m4[4] = {__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]), __uint_as_float(y[3])};
+#pragma unroll
+            for (int j = 4; j + 8 <= 32; j += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) m4[k] = fmax3(m4[k], __uint_as_float(y[j + k]), __uint_as_float(y[j + 4 + k]));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], __uint_as_float(y[28 + k]));
+            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          };
+          float top[2];
+#pragma unroll
+          for (int page = 0; page < 2; ++page) {
+            tmem_ld32(mS + 64 * page, x[0]);
+            tmem_ld32(mS + 64 * page + 32, x[1]);
             tmem_wait_ld();
-            if (!__all_sync(0xffffffffu, w[i] == 0xFFFFFFFFu)) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if ((w[i] & (1u << j)) == 0u) x[j] = 0xFF800000u;
-            }
-            float m4[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m4[j] = __uint_as_float(x[j]);
-#pragma unroll
-            for (int j = 4; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(x[j]));
-            top[i >> 1] = fmaxf(top[i >> 1], fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            masked(x[0], w[2 * page]);
+            masked(x[1], w[2 * page + 1]);
+            top[page] = fmaxf(highest(x[0]), highest(x[1]));
           }
           const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
           const bool up = high > ref + KA_SLACK;
@@ -398,12 +406,12 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             if (u > 0 && __any_sync(0xffffffffu, up && ref != -INFINITY)) {   // O is complete: its last product came before these scores
 #pragma unroll 1
               for (int i = 0; i < D; i += 16) {
-                uint32_t x[16];
-                tmem_ld16(mO + i, x);
+                uint32_t y[16];
+                tmem_ld16(mO + i, y);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * shrink);
-                tmem_st16(mO + i, x);
+                for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink);
+                tmem_st16(mO + i, y);
               }
             }
             sum *= shrink;
@@ -411,32 +419,27 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           const float base = ref == -INFINITY ? 0.f : KA_OFFSET - ref;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t pk[16];
-            if (__all_sync(0xffffffffu, w[i] == 0u)) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) pk[j] = 0u;
-            } else {
-              uint32_t x[32];
-              tmem_ld32(mS + 32 * i, x);
-              tmem_wait_ld();
-              if (!__all_sync(0xffffffffu, w[i] == 0xFFFFFFFFu)) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if ((w[i] & (1u << j)) == 0u) x[j] = 0xFF800000u;
-              }
-              const float k = kf[i >> 1], add = base + static_cast<float>(ev[i >> 1]);
-              float part[2] = {0.f, 0.f};
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float a = fast_exp2(fmaf(__uint_as_float(x[2 * j]), k, add)), b = fast_exp2(fmaf(__uint_as_float(x[2 * j + 1]), k, add));
-                part[0] += a;
-                part[1] += b;
-                pk[j] = pack2<false>(a, b);
-              }
-              sum = fmaf(part[0] + part[1], exp2i(-ev[i >> 1]), sum);
+          for (int half = 0; half < 4; ++half) {   // page 1's halves, then page 0's; P of a page over its first 32 columns
+            const int page = half < 2 ? 1 : 0, part = half & 1;
+            if (half >= 2) {
+              tmem_wait_ld();   // (both halves' loads, at the first of them)
+              masked(x[part], w[part]);
             }
-            tmem_st16(mS + 16 * i, pk);   // over scores that have been read
+            const float k = kf[page], add = base + static_cast<float>(ev[page]);
+            const uint64_t k2 = pack_f32x2(k, k), add2 = pack_f32x2(add, add);
+            uint64_t sums[2] = {0u, 0u};
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t y = fma_f32x2(pack_u32x2(x[part][2 * j], x[part][2 * j + 1]), k2, add2);
+              const float a = fast_exp2(lo_f32x2(y)), b = fast_exp2(hi_f32x2(y));
+              sums[j & 1] = add_f32x2(sums[j & 1], pack_f32x2(a, b));
+              pk[j] = pack2<false>(a, b);
+            }
+            const uint64_t both = add_f32x2(sums[0], sums[1]);
+            sum = fmaf(lo_f32x2(both) + hi_f32x2(both), exp2i(-ev[page]), sum);
+            if (half < 2) tmem_ld32(mS + 32 * part, x[part]);
+            tmem_st16(mS + 64 * page + 16 * part, pk);
           }
           tmem_wait_st();
           tc_fence_before_sync();
