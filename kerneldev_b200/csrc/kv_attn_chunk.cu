@@ -24,6 +24,9 @@
 namespace kd {
 
 constexpr int CH_THREADS = 256, CH_TOKENS = 128, CH_RECORDS = 3;
+// registers: 128 a thread at launch; the converters release what the softmax warps take
+constexpr uint32_t CH_REGS_LIGHT = 96, CH_REGS_COMPUTE = 160;
+static_assert(CH_REGS_LIGHT + CH_REGS_COMPUTE <= 2 * 128, "register pool");
 constexpr uint32_t CH_SITE = 0x900u;   // wait sites 0x900 .. : role << 4 | barrier
 
 // One tile of the walk, written by the converters for the others. Three slots in turn: the words of the tile ahead are written while the tile in hand is worked on, and the
@@ -44,15 +47,24 @@ struct ChunkRows {
   int spans;               // some row looks for its own span
 };
 
+// The item in hand: pages page0 .. page0 + here - 1 of the `pages` that it has. In shared memory, as what finds it is: the roles need their registers (with 30 of them
+// taken here, the converters' loads were spilled, which waits for them).
+struct ChunkItem {
+  Item it;
+  int page0, pages, here;   // here < 0: there is none
+  int second;               // the CTA's second part (see AttnWorkspace)
+};
+
 template <int D>
 struct ChunkShared {
-  static constexpr int BLOCKS = D > 64 ? 2 : 1, BLOCK = 128 * 128, TILE = BLOCKS * BLOCK;   // 64 head dims of 128 rows
+  static constexpr int BLOCKS = D > 64 ? 2 : 1, BLOCK = 128 * 128, TILE = BLOCKS * BLOCK;   // blocks of 64 head dims of 128 rows (16 KB: see koff_kmajor and desc_lo_mnmajor)
   uint8_t q[TILE], k[TILE], v[TILE];
   ChunkRecord record[CH_RECORDS];
   uint16_t nan_bits[CH_TOKENS][8];   // second pass alone: which of a token's head dims are NaN, 16 to a word
   float factor[KC_ROWS];
   RowMask mask[KC_ROWS];
   ChunkRows rows;
+  ChunkItem item;
   uint64_t bar[5];
   uint32_t tmem, any_nan;
   int tiles;                         // of the pass
@@ -88,6 +100,31 @@ __device__ __forceinline__ void row_words(const RowMask& m, const ChunkRecord& r
   }
 }
 
+// A converter thread's bytes of a tile as halves: rounds of 32 tokens and a block of 64 head dims, at fixed distances from the first one's two places.
+// kWithoutNan: NaN as zeros, and a bit for each in nan_bits (of the first round's token and head dims).
+template <int D, bool kWithoutNan>
+__device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[2], const uint4 (&reg)[4 * ChunkShared<D>::BLOCKS], uint16_t (*nan_bits)[8], int col) {
+#pragma unroll
+  for (int i = 0; i < 4 * ChunkShared<D>::BLOCKS; ++i) {
+    uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+    if constexpr (kWithoutNan) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t n = __vcmpeq4(w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+        w[x] &= ~n;
+        bits |= ((n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u)) << (4 * x);
+      }
+      const int d = (i >> 2) * 64 + col;
+      if (d < D) nan_bits[32 * (i & 3)][d / 16] = static_cast<uint16_t>(bits);
+    }
+    const HalfPairs h0 = e4m3x4_to_f16x4(w[0]), h1 = e4m3x4_to_f16x4(w[1]), h2 = e4m3x4_to_f16x4(w[2]), h3 = e4m3x4_to_f16x4(w[3]);
+    uint8_t* at = to + (i & 3) * 4096 + (i >> 2) * ChunkShared<D>::BLOCK;
+    *reinterpret_cast<uint4*>(at + place[0]) = make_uint4(h0.lo, h0.hi, h1.lo, h1.hi);
+    *reinterpret_cast<uint4*>(at + place[1]) = make_uint4(h2.lo, h2.hi, h3.lo, h3.hi);
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(CH_THREADS, KC_CTAS)
 cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
@@ -95,7 +132,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   using Sh = ChunkShared<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Sh& sh = *reinterpret_cast<Sh*>(smem);
-  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), HT = c.H * shape.tiles;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const bool metadata = c.desc != nullptr;
   auto bar = [&](int i) { return smem_u32(&sh.bar[i]); };
   if (tid == 0) {
@@ -114,68 +151,77 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tS = sh.tmem, tO = tS + CH_TOKENS;
+  const uint32_t tS = __reduce_max_sync(0xffffffffu, sh.tmem), tO = tS + CH_TOKENS;   // warp-uniform for the compiler
   pdl_wait();
   pdl_launch_dependents();
 
-  const FlatOrder order(c, s, p, shape);
-  uint32_t at = 0, end = 1;
-  if (shape.ctas > 0) {
-    const bool mine = blockIdx.x < order.ctas && order.total > 0;
-    at = mine ? order.start(blockIdx.x) : 0;
-    end = mine ? order.start(blockIdx.x + 1) : 0;
-  }
-  const uint32_t begin = at;
   int n_k = 0, n_t = 0;   // uses of barrier K (one more than tiles for each pass over an item) and of the others
   auto wait = [&](int i, int use, int role) {
     return __all_sync(0xffffffffu, mbar_wait(bar(i), use & 1, &sh.abort, CH_SITE | role << 4 | i));
   };
-  while (at < end) {
-    Item it;
-    int page0 = 0, pages, here;
-    if (shape.ctas > 0) {
-      const FlatPlace f = order.find(c, s, p, shape, at);
-      it.b = f.b;
-      it.h = f.ht / f.tiles;
-      it.tile = f.ht - it.h * f.tiles;
-      it.len = sequence_length(c, s, it.b);
-      page0 = f.page;
-      pages = f.pages;
-      here = min(static_cast<int>(end - at), pages - page0);
-    } else {
-      const int item = blockIdx.x;
-      it.b = item / HT;
-      it.h = (item - it.b * HT) / shape.tiles;
-      it.tile = item - it.b * HT - it.h * shape.tiles;
-      it.len = sequence_length(c, s, it.b);
-      pages = here = (it.len + KC_PAGE - 1) / KC_PAGE;
+  auto all_sync = [&]() { named_bar_sync(2, CH_THREADS); };   // (from the roles' own code)
+  uint32_t done = 0;   // pages that this CTA has worked on
+  // The next item, its rows in shared memory; false: there is none. All threads.
+  auto open_item = [&]() -> bool {
+    if (warp == 0) {
+      ChunkItem n;
+      n.here = -1;
+      n.second = done > 0 ? 1 : 0;
+      if (shape.ctas > 0) {
+        const FlatOrder order(c, s, p, shape);
+        if (blockIdx.x < order.ctas) {
+          const uint32_t at = order.start(blockIdx.x) + done, end = order.start(blockIdx.x + 1);
+          if (at < end) {
+            const FlatPlace f = order.find(c, s, p, shape, at);
+            const int h = f.ht / f.tiles;
+            n = ChunkItem{Item{f.b, h, f.ht - h * f.tiles, sequence_length(c, s, f.b)}, f.page, f.pages, min(static_cast<int>(end - at), f.pages - f.page), n.second};
+          }
+        }
+      } else if (done == 0) {
+        const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles, len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
+        n = ChunkItem{Item{b, h, ht - h * shape.tiles, len}, 0, pages, pages, 0};
+      }
+      if (lane == 0) sh.item = n;
     }
-    const int page_end = page0 + here;
+    all_sync();
+    if (sh.item.here < 0) return false;
+    const Item it = sh.item.it;
 
     // ---- Q as halves (bfloat16 times a power of two, see kv_attn.cu), masks and what the rows see together ----
     if (tid == 0) {
       sh.rows = ChunkRows{0u, 0u, 0, 0};
       sh.any_nan = 0u;
     }
-    __syncthreads();
-    for (int r = warp; r < KC_ROWS; r += CH_THREADS / 32) {
-      const int row = it.tile * KC_ROWS + r, d = 4 * lane;
-      uint2 v = make_uint2(0u, 0u);
-      if (row < shape.rows && d < D) {
-        const int n = row / shape.G, hq = it.h * shape.G + row - n * shape.G;
-        v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
+    all_sync();
+    constexpr int BATCH = 8, WARPS = CH_THREADS / 32;   // rows that a warp has on their way at once
+#pragma unroll 1
+    for (int r0 = warp; r0 < KC_ROWS; r0 += WARPS * BATCH) {
+      const int d = 4 * lane;
+      uint2 v[BATCH];
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int row = it.tile * KC_ROWS + r0 + x * WARPS;
+        v[x] = make_uint2(0u, 0u);
+        if (row < shape.rows && d < D) {
+          const int n = row / shape.G, hq = it.h * shape.G + row - n * shape.G;
+          v[x] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
+        }
       }
-      int e = 0;
-      if (p.dtype == KD_BF16) {
-        auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
-        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v.x), size(v.x >> 16)), max(size(v.y), size(v.y >> 16))));
-        if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
-        const float f = exp2i(e);
-        const float2 a = unpack2<true>(v.x), b = unpack2<true>(v.y);
-        v = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+#pragma unroll
+      for (int x = 0; x < BATCH; ++x) {
+        const int r = r0 + x * WARPS;
+        int e = 0;
+        if (p.dtype == KD_BF16) {
+          auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
+          const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[x].x), size(v[x].x >> 16)), max(size(v[x].y), size(v[x].y >> 16))));
+          if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
+          const float f = exp2i(e);
+          const float2 a = unpack2<true>(v[x].x), b = unpack2<true>(v[x].y);
+          v[x] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+        }
+        if (lane == 0) sh.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+        if (d < D) *reinterpret_cast<uint2*>(sh.q + chunk_place(r, d)) = v[x];
       }
-      if (lane == 0) sh.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
-      if (d < D) *reinterpret_cast<uint2*>(sh.q + chunk_place(r, d)) = v;
     }
     if (tid < KC_ROWS) {
       const RowMask m = row_mask(c, s, p, it, it.tile * KC_ROWS + tid, shape.G, shape.rows, query_count(c, p, it.b));
@@ -191,13 +237,27 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
       }
     }
     fence_proxy_async_smem();
-    __syncthreads();
-
-    const bool whole = here == pages;
-    const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (at == begin ? 0 : 1);
-    for (int pass = 0; pass < 2; ++pass) {   // the second one where the first one's output has NaN
-      const bool safe = pass == 1;
-      if (warp >= 4) {
+    all_sync();
+    return true;
+  };
+  // After a pass over an item: whether there is to be another one. All threads.
+  auto again = [&](int pass) -> bool {
+    all_sync();
+    const int tiles = sh.tiles;
+    n_k += tiles + 1;
+    n_t += tiles;
+    const bool more = pass == 0 && sh.any_nan != 0u && sh.abort.v == 0u;   // NaN: once more, with care
+    if (!more) done += max(sh.item.here, 1);
+    all_sync();
+    return more;
+  };
+  if (warp >= 4) {
+    reg_dealloc<CH_REGS_LIGHT>();
+    while (open_item()) {
+      const Item it = sh.item.it;
+      int pass = 0;
+      do {
+        const bool safe = pass == 1;
         // ---------------------------------------- converters ----------------------------------------
         const int r = tid - 128;   // this thread's token of the tile for the descriptors
         const ChunkRows rows = sh.rows;
@@ -205,30 +265,59 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         const int col = (r & 3) * 16, row0 = r >> 2;
         constexpr int ROUNDS = 4 * Sh::BLOCKS;   // 32 tokens and one block of 64 head dims each
         struct Tile {
-          int page[2], j0;
+          int page[2], j0, ev[2];
+          float ks[2];
           uint32_t desc;
         } cur;
-        uint4 kreg[ROUNDS], vreg[ROUNDS];
-        int next = page0;
+        uint4 reg[ROUNDS];   // K of a tile, then its V: each is asked for when the other has been stored, and awaited when its place is free
         bool ok = true;
+        // Page numbers and scales of 32 blocks in the lanes of each warp, the page numbers of the 32 behind them already asked for: with a look-up for each tile, its
+        // chain of loads (page, scale) stood between two tiles.
+        const int32_t* table = s.table + it.b * s.table_stride;
+        const int page0 = sh.item.page0, page_end = page0 + sh.item.here;
+        int next = page0, batch = page0, batch_page, raw_ahead = 0, batch_ev;
+        float batch_ks;
+        auto ask = [&](int from) { return from + lane < page_end ? table[from + lane] : -1; };
+        auto open_batch = [&](int from, int raw) {
+          batch = from;
+          batch_page = from + lane < page_end ? checked_page(c, raw) : -1;
+          const size_t place = block_index(c, max(batch_page, 0), it.h);
+          batch_ks = batch_page >= 0 ? c.k_scale[place] : 1.f;
+          batch_ev = batch_page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
+          raw_ahead = ask(from + 32);
+        };
+        open_batch(page0, ask(page0));
+        // the descriptor of this thread's token of the tile at `next`, asked for when the tile before it was found
+        uint32_t ahead_desc = 0u;
+        auto peek = [&]() {
+          if (next - batch >= 32) open_batch(next, raw_ahead);
+          const int p0 = __shfl_sync(0xffffffffu, batch_page, next - batch), p1 = __shfl_sync(0xffffffffu, batch_page, next - batch + 1), page = r < KC_PAGE ? p0 : p1;
+          const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0;
+          ahead_desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
+        };
+        peek();
         // The next tile that some row sees, from `next` on. All four warps come to the same answer: the words are exchanged through the record that is to have them.
         auto find = [&](int slot) {
           ChunkRecord& rec = sh.record[slot];
-          for (; next < page_end; next += 2) {
+          while (next < page_end) {
             cur.j0 = next * KC_PAGE;
-            cur.page[0] = page_of(c, s, it.b, next);
-            cur.page[1] = next + 1 < page_end ? page_of(c, s, it.b, next + 1) : -1;
-            const int page = r < KC_PAGE ? cur.page[0] : cur.page[1];
-            const bool alive = cur.j0 + r < it.len && page >= 0;
-            cur.desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
-            const uint32_t pre = __ballot_sync(0xffffffffu, (cur.desc & TD_PRE) != 0u), ctx = __ballot_sync(0xffffffffu, (cur.desc & TD_CTX) != 0u),
-                           ins = __ballot_sync(0xffffffffu, (cur.desc & TD_INS) != 0u);
+            cur.desc = ahead_desc;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              cur.page[x] = __shfl_sync(0xffffffffu, batch_page, next - batch + x);
+              cur.ks[x] = __shfl_sync(0xffffffffu, batch_ks, next - batch + x);
+              cur.ev[x] = __shfl_sync(0xffffffffu, batch_ev, next - batch + x);
+            }
+            const uint32_t ctx = __ballot_sync(0xffffffffu, (cur.desc & TD_CTX) != 0u);
+            next += 2;
             if (!metadata) {
-              if (cur.j0 >= rows.max_limit) continue;   // (the limits are no more than the length)
+              if (cur.j0 >= rows.max_limit) return false;   // (the limits are no more than the length)
+              peek();
               if (lane == 0) rec.words[1][r >> 5] = ctx;
-              next += 2;
               return true;
             }
+            const uint32_t pre = __ballot_sync(0xffffffffu, (cur.desc & TD_PRE) != 0u), ins = __ballot_sync(0xffffffffu, (cur.desc & TD_INS) != 0u);
+            peek();
             named_bar_sync(1, 128);   // everyone has looked at the words of the tile before
             if (lane == 0) {
               rec.words[0][r >> 5] = pre;
@@ -239,17 +328,14 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             uint32_t any[3];
 #pragma unroll
             for (int x = 0; x < 3; ++x) any[x] = rec.words[x][0] | rec.words[x][1] | rec.words[x][2] | rec.words[x][3];
-            const bool seen = ((rows.sees & TD_PRE) != 0u && any[0] != 0u) || ((rows.sees & TD_CTX) != 0u && any[1] != 0u) || (((rows.sees & TD_INS) != 0u || rows.spans != 0) && any[2] != 0u) ||
-                              ((rows.causal & TD_CTX) != 0u && any[1] != 0u && cur.j0 < rows.max_limit);
-            if (seen) {
-              next += 2;
+            if (((rows.sees & TD_PRE) != 0u && any[0] != 0u) || ((rows.sees & TD_CTX) != 0u && any[1] != 0u) || (((rows.sees & TD_INS) != 0u || rows.spans != 0) && any[2] != 0u) ||
+                ((rows.causal & TD_CTX) != 0u && any[1] != 0u && cur.j0 < rows.max_limit))
               return true;
-            }
           }
           return false;
         };
         const uint32_t place[2] = {chunk_place(row0, col), chunk_place(row0, col + 8)};   // of later rounds at fixed distances: 32 tokens 4 KB, a block 16 KB
-        auto fetch = [&](const void* from, uint4 (&reg)[ROUNDS]) {
+        auto fetch = [&](const void* from) {
           const uint8_t* base[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) base[x] = static_cast<const uint8_t*>(from) + (block_index(c, max(cur.page[x], 0), it.h) * KC_PAGE + row0) * D + col;
@@ -260,89 +346,68 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             if (cur.page[x] >= 0 && (i >> 2) * 64 + col < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(base[x] + (i & 1) * 32 * D + (i >> 2) * 64));
           }
         };
-        auto store = [&](uint8_t* to, const uint4 (&reg)[ROUNDS], bool without_nan) {
-#pragma unroll
-          for (int i = 0; i < ROUNDS; ++i) {
-            uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
-            if (without_nan) {
-              uint32_t bits = 0;
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const uint32_t n = __vcmpeq4(w[x] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-                w[x] &= ~n;
-                bits |= ((n & 1u) | (n >> 7 & 2u) | (n >> 14 & 4u) | (n >> 21 & 8u)) << (4 * x);
-              }
-              const int d = (i >> 2) * 64 + col;
-              if (d < D) sh.nan_bits[32 * (i & 3) + row0][d / 16] = static_cast<uint16_t>(bits);
-            }
-            const HalfPairs h0 = e4m3x4_to_f16x4(w[0]), h1 = e4m3x4_to_f16x4(w[1]), h2 = e4m3x4_to_f16x4(w[2]), h3 = e4m3x4_to_f16x4(w[3]);
-            uint8_t* at = to + (i & 3) * 4096 + (i >> 2) * Sh::BLOCK;
-            *reinterpret_cast<uint4*>(at + place[0]) = make_uint4(h0.lo, h0.hi, h1.lo, h1.hi);
-            *reinterpret_cast<uint4*>(at + place[1]) = make_uint4(h2.lo, h2.hi, h3.lo, h3.hi);
-          }
-        };
         int u = 0;   // tiles of this pass
         bool have = find(n_k % CH_RECORDS);
-        if (have) fetch(c.k, kreg);
-        if (have) fetch(c.v, vreg);
+        if (have) fetch(c.k);
         for (;; ++u) {
           // (K's place and the record's slot are free when the scores of the tile before are complete; the slot of two tiles before by then, too)
           if (u > 0 && !(ok = wait(CB_S, n_t + u - 1, 1))) break;
           ChunkRecord& rec = sh.record[(n_k + u) % CH_RECORDS];
-          if (r < 2) {
-            const int page = cur.page[r];
-            const size_t place = have && page >= 0 ? block_index(c, page, it.h) : 0;
-            rec.ks[r] = have && page >= 0 ? c.k_scale[place] : 1.f;
-            rec.ev[r] = have && page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
-          }
           if (r == 0) {
+            rec.ks[0] = cur.ks[0];
+            rec.ks[1] = cur.ks[1];
+            rec.ev[0] = cur.ev[0];
+            rec.ev[1] = cur.ev[1];
             rec.j0 = cur.j0;
             rec.end = have ? 0 : 1;
           }
           if (have) {
             if (metadata) rec.desc[r] = cur.desc;
-            store(sh.k, kreg, false);
+            store_tile<D, false>(sh.k, place, reg, nullptr, col);
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(CB_K));
           if (!have) break;
-          const bool more = find((n_k + u + 1) % CH_RECORDS);
-          if (more) fetch(c.k, kreg);
+          fetch(c.v);
+          have = find((n_k + u + 1) % CH_RECORDS);
           if (u > 0 && !(ok = wait(CB_PV, n_t + u - 1, 1))) break;
-          store(sh.v, vreg, safe);
+          if (safe) store_tile<D, true>(sh.v, place, reg, sh.nan_bits + row0, col);
+          else store_tile<D, false>(sh.v, place, reg, nullptr, col);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(CB_V));
-          have = more;
-          if (more) fetch(c.v, vreg);
+          if (have) fetch(c.k);
         }
-      } else {
+      } while (again(pass++));
+      if (sh.abort.v != 0u) break;
+    }
+  } else {
+    reg_alloc<CH_REGS_COMPUTE>();
+    while (open_item()) {
+      const Item it = sh.item.it;
+      int pass = 0;
+      do {
+        const bool safe = pass == 1;
         // ---------------------------------------- softmax ----------------------------------------
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, mS = tS + lanes, mO = tO + lanes;
         const RowMask mask = sh.mask[tid];
         const float factor = sh.factor[tid];
         const uint32_t idesc_s = make_idesc_f16(0, 0, 0, KC_ROWS, CH_TOKENS), idesc_o = make_idesc_f16(0, 0, 1, KC_ROWS, 64 * Sh::BLOCKS);
+        const uint32_t hi = desc_hi_sw128();
         auto issue_scores = [&]() {   // of a tile whose K is there
           tc_fence_after_sync();
-          if (elect_one()) {
-            const uint32_t q = smem_u32(sh.q), k = smem_u32(sh.k);
+          const uint32_t q = desc_lo_kmajor(smem_u32(sh.q)), k = desc_lo_kmajor(smem_u32(sh.k));
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-              mma_ss(tS, desc_kmajor_sw128(q + (i / 4) * Sh::BLOCK, i & 3), desc_kmajor_sw128(k + (i / 4) * Sh::BLOCK, i & 3), idesc_s, i > 0 ? 1u : 0u);
-            mma_commit(bar(CB_S));
-          }
-          __syncwarp();
+          for (int i = 0; i < D / 16; ++i) mma_ss_uniform(tS, q + koff_kmajor(i), k + koff_kmajor(i), hi, idesc_s, i > 0 ? 1u : 0u);
+          commit_uniform(bar(CB_S));
         };
         auto issue_values = [&](bool first) {   // with P and V there
           tc_fence_after_sync();
-          if (elect_one()) {
-            const uint32_t v = smem_u32(sh.v);
+          const uint32_t v = desc_lo_mnmajor(smem_u32(sh.v));
 #pragma unroll
-            for (int i = 0; i < CH_TOKENS / 16; ++i) mma_ts(tO, tS + (i / 4) * 64 + (i & 3) * 8, desc_mnmajor_sw128(v, i, Sh::BLOCK), idesc_o, !first || i > 0 ? 1u : 0u);
-            mma_commit(bar(CB_PV));
-          }
-          __syncwarp();
+          for (int i = 0; i < CH_TOKENS / 16; ++i) mma_ts_uniform(tO, tS + (i / 4) * 64 + (i & 3) * 8, v + koff_mnmajor(i), hi, idesc_o, !first || i > 0 ? 1u : 0u);
+          commit_uniform(bar(CB_PV));
         };
         float ref = -INFINITY, sum = 0.f;
         uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
@@ -454,7 +519,8 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         tc_fence_after_sync();
         // ---- this row's output ----
         const int row = it.tile * KC_ROWS + tid;
-        const bool live = mask.limit > 0, exists = row < shape.rows;
+        const bool live = mask.limit > 0, exists = row < shape.rows, whole = sh.item.here == sh.item.pages;
+        const size_t part = 2 * static_cast<size_t>(blockIdx.x) + sh.item.second;
         const int i = row / shape.G, hq = it.h * shape.G + row - i * shape.G;
         const float inv = !whole ? 1.f : live && sum != 0.f ? 1.f / sum : 0.f;
         bool bad = false;
@@ -492,18 +558,9 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (u > 0) drain_wait(bar(CB_PV), (n_t + u - 1) & 1);
           drain_wait(bar(CB_S), (n_t + u) & 1);
         }
-      }
-      __syncthreads();
-      const int tiles = sh.tiles;
-      n_k += tiles + 1;
-      n_t += tiles;
-      const bool again = pass == 0 && sh.any_nan != 0u;
-      if (sh.abort.v != 0u || !again) break;
-      __syncthreads();
+      } while (again(pass++));
+      if (sh.abort.v != 0u) break;
     }
-    __syncthreads();   // the next item's rows may take this one's place
-    if (sh.abort.v != 0u) break;
-    at += shape.ctas > 0 ? here : 1;
   }
   tc_fence_before_sync();
   __syncthreads();
