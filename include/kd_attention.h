@@ -326,7 +326,7 @@ typedef struct kd_cache_queries {
   int32_t causal;           /* read only without kd_cache.desc */
   float sm_scale;
   const int32_t* q_lens;    /* NULL: T, or (B) */
-  float* lse;               /* NULL (not without weights), or (B, H, T) contiguous, base 2 */
+  float* lse;               /* NULL, or (B, H, T) contiguous, base 2 */
   float* weights;           /* NULL, or (B, kd_cache.H, w_len), unit stride along tokens; tokens at or beyond w_len are left out */
   int64_t w_stride_b, w_stride_h;
   int32_t w_len;

@@ -467,7 +467,7 @@ int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache
   if (!(q->sm_scale > 0.f) || q->sm_scale > 3.0e38f) return set_error(KD_ERR_ARG, "sm_scale must be positive and finite");
   if (s->B == 0 || q->T == 0) return 0;
   if ((rc = check_cache_strides(q->q, 2, "q")) != 0 || (rc = check_cache_strides(q->o, 2, "o")) != 0) return rc;
-  if (q->weights && (!q->lse || q->w_len < 0)) return set_error(KD_ERR_ARG, "weights need lse and w_len");
+  if (q->weights && q->w_len < 0) return set_error(KD_ERR_ARG, "w_len is negative");
   if (!q->workspace && cache_attention_workspace(*c, *s, *q) > 0) return set_error(KD_ERR_ARG, "workspace is null");
   if ((reinterpret_cast<uintptr_t>(q->workspace) & 15u) != 0) return set_error(KD_ERR_ALIGN, "workspace not 16-byte aligned");
   if ((rc = check_device()) != 0) return rc;

@@ -182,7 +182,7 @@ std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const T
     p.w_stride_h = w.stride(1);
     p.w_len = static_cast<int32_t>(w.size(2));
   }
-  if (return_lse || weights.has_value()) {
+  if (return_lse) {
     lse = empty_on({B, H, T}, at::kFloat, q.device());
     p.lse = lse.data_ptr<float>();
   }

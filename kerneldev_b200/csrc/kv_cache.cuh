@@ -77,29 +77,7 @@ __device__ __forceinline__ void e4m3x4_to_f32x4(uint32_t w, float* f) {
   f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
 }
 
-// 16 numbers of a row: 16 bytes of e4m3, 32 of a 16-bit type, 64 of float
-template <int kType>
-__device__ __forceinline__ void load16(const void* p, float (&f)[16]) {
-  if constexpr (kType == KD_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(p)[i];
-      f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack2<kType == KD_BF16>(w[j]);
-        f[8 * i + 2 * j] = x.x;
-        f[8 * i + 2 * j + 1] = x.y;
-      }
-    }
-  }
-}
+// 16 numbers of a row, 32 bytes of a 16-bit type, 64 of float
 template <int kType>
 __device__ __forceinline__ void store16(void* p, const float (&f)[16]) {
   if constexpr (kType == KD_F32) {
@@ -128,25 +106,15 @@ __device__ __forceinline__ void dequantise16(const uint4& v, int e, float (&f)[1
   for (int i = 0; i < 16; ++i) f[i] *= s;
 }
 // floats to e4m3 in units of 2^e: one rounding, since the division by a power of two is exact (what it flushes is far below the smallest e4m3
-// number). An infinity becomes NaN, which is what e4m3 has in its place.
+// number). kSpecial: there may be an infinity, which becomes NaN, what e4m3 has in its place.
+template <bool kSpecial>
 __device__ __forceinline__ uint4 quantise16(const float (&f)[16], int e) {
   const float s = exp2i(-e);
   float x[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = (__float_as_uint(f[i]) & 0x7F800000u) == 0x7F800000u ? __uint_as_float(0x7FC00000u) : f[i] * s;
+  for (int i = 0; i < 16; ++i) x[i] = kSpecial && (__float_as_uint(f[i]) & 0x7F800000u) == 0x7F800000u ? __uint_as_float(0x7FC00000u) : f[i] * s;
   return make_uint4(f32x4_to_e4m3x4(x), f32x4_to_e4m3x4(x + 4), f32x4_to_e4m3x4(x + 8), f32x4_to_e4m3x4(x + 12));
 }
-// the largest finite magnitude, as the bits of a float
-__device__ __forceinline__ uint32_t amax16(const float (&f)[16]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t u = __float_as_uint(f[i]) & 0x7FFFFFFFu;
-    m = max(m, u < 0x7F800000u ? u : 0u);
-  }
-  return m;
-}
-
 int launch_cache_append(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_tokens& t, cudaStream_t stream);
 int launch_cache_read(const kd_cache& c, const kd_cache_seqs& s, const int32_t* start, int count, int dtype, const kd_tensor& k,
                       const kd_tensor& v, cudaStream_t stream);

@@ -60,8 +60,8 @@ def test_entry_points_reject_bad_arguments_before_touching_cuda():
     q.sm_scale = 1.0
     refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"q is null")
     q.q.ptr = q.o.ptr = 0x10000
-    q.weights = 0x10000
-    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"lse")
+    q.weights, q.w_len = 0x10000, -1
+    refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -1, b"w_len")
     q.T = 1 << 30
     refused(lib.kd_cache_attention(ref(c), ref(s), ref(q), None), -4, b"rows")
     n = ctypes.c_size_t(1)
