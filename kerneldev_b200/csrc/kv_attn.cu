@@ -424,6 +424,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(KA_THREADS, ctas_of(NT))
 cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                        const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  touch_parameters(c, s, p, shape, ws);
   pdl_wait();
   pdl_launch_dependents();
   constexpr int ROWS = NT * KA_TILE;
@@ -431,9 +432,10 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
-  const FlatOrder order(c, s, p, shape);
+  FlatOrder order;
   uint32_t at = 0, end = 1;
   if (shape.ctas > 0) {
+    order.look_up(c, s, p, shape);
     if (blockIdx.x >= order.ctas || order.total == 0) return;
     at = order.start(blockIdx.x);
     end = order.start(blockIdx.x + 1);
@@ -451,9 +453,9 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
       r.it.b = f.b;
       r.it.h = f.ht / f.tiles;
       r.it.tile = f.ht - r.it.h * f.tiles;
-      r.it.len = sequence_length(c, s, r.it.b);
+      r.it.len = f.len;
       page0 = f.page;
-      r.pages = f.pages;
+      r.pages = pages_of_length(f.len);
       r.here = min(static_cast<int>(end - place_of), r.pages - page0);
     } else {
       const int item = blockIdx.x;
@@ -461,7 +463,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
       r.it.h = (item - r.it.b * HT) / shape.tiles;
       r.it.tile = item - r.it.b * HT - r.it.h * shape.tiles;
       r.it.len = sequence_length(c, s, r.it.b);
-      r.pages = r.here = (r.it.len + KC_PAGE - 1) / KC_PAGE;
+      r.pages = r.here = pages_of_length(r.it.len);
     }
     r.first = 2 * page0 + warp;
     r.last = min(2 * (page0 + r.here), (r.it.len + KA_UNIT - 1) / KA_UNIT);
@@ -568,9 +570,10 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
   const int per_head = (shape.rows + ROWS - 1) / ROWS;
   const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + (tid >> 5) / kGroups;
   const int tile = row_of_head / shape.item_rows, r = row_of_head - tile * shape.item_rows;
-  const FlatOrder order(c, s, p, shape);
+  FlatOrder order;
+  order.look_up(c, s, p, shape);
   const int len = sequence_length(c, s, b), n = query_count(c, p, b), tiles = (n * shape.G + shape.item_rows - 1) / shape.item_rows;
-  const int pages = tile < tiles ? (len + KC_PAGE - 1) / KC_PAGE : 0;   // of the item
+  const int pages = tile < tiles ? pages_of_length(len) : 0;   // of the item
   const uint32_t first = order.before(c, s, p, shape, b) + (h * tiles + tile) * pages;   // the item's first page in the flat order
   int c0 = 0, c1 = -1;
   if (pages > 0) {
@@ -636,6 +639,7 @@ template <int D, int NT>
 __global__ void __launch_bounds__(KA_THREADS)
 cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                      const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  touch_parameters(c, s, p, shape, ws);
   pdl_wait();
   pdl_launch_dependents();
   constexpr int MINE = KW_UNITS / KA_WARPS, ROWS = NT * KA_TILE;

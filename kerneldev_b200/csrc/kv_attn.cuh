@@ -66,38 +66,39 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
 // The flat order of all pages: sequences in turn, each once for every head and tile of rows that has a query, cut into even ranges for the CTAs. 32 bits are
 // enough: the host sees to it that there are fewer than 2^30 pages. A warp holds the counts of the first 128 sequences, in its lanes.
 struct FlatPlace {
-  int b, ht, page, pages, tiles;   // ht: head * tiles + tile, tiles: of the sequence; page: index within the item
+  int b, ht, page, len, tiles;   // ht: head * tiles + tile; len and tiles: of the sequence; page: index within the item
 };
+__device__ __forceinline__ int pages_of_length(int len) { return (len + KC_PAGE - 1) / KC_PAGE; }
 struct FlatOrder {
   static constexpr int HELD = 4;
-  int held[HELD], held_tiles[HELD];
+  int held[HELD], held_tiles[HELD];   // lengths, tiles
   uint32_t total;             // pages
   uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
 
-  static __device__ __forceinline__ int pages_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? (sequence_length(c, s, b) + KC_PAGE - 1) / KC_PAGE : 0; }
+  static __device__ __forceinline__ int length_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? sequence_length(c, s, b) : 0; }
   static __device__ __forceinline__ int tiles_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) {
     return b < s.B ? (query_count(c, p, b) * shape.G + shape.item_rows - 1) / shape.item_rows : 0;
   }
   // of sequence 32 i + lane
-  __device__ __forceinline__ int pages(const kd_cache& c, const kd_cache_seqs& s, int i) const {
+  __device__ __forceinline__ int length(const kd_cache& c, const kd_cache_seqs& s, int i) const {
     if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
-    return pages_of(c, s, 32 * i + (threadIdx.x & 31));
+    return length_of(c, s, 32 * i + (threadIdx.x & 31));
   }
   __device__ __forceinline__ int tiles(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int i) const {
     if (i < HELD) return i == 0 ? held_tiles[0] : i == 1 ? held_tiles[1] : i == 2 ? held_tiles[2] : held_tiles[3];
     return tiles_of(c, s, p, shape, 32 * i + (threadIdx.x & 31));
   }
-  __device__ __forceinline__ FlatOrder(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape) {
+  __device__ __forceinline__ void look_up(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape) {
     const int lane = threadIdx.x & 31;
     uint32_t n = 0;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-      held[i] = pages_of(c, s, 32 * i + lane);
+      held[i] = length_of(c, s, 32 * i + lane);
       held_tiles[i] = tiles_of(c, s, p, shape, 32 * i + lane);
     }
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) n += held[i] * held_tiles[i];
-    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of(c, s, b) * tiles_of(c, s, p, shape, b);
+    for (int i = 0; i < HELD; ++i) n += pages_of_length(held[i]) * held_tiles[i];
+    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of_length(length_of(c, s, b)) * tiles_of(c, s, p, shape, b);
     total = __reduce_add_sync(0xffffffffu, n) * c.H;
     // (None of them has no page: the join reads a part of every CTA of an item.)
     ctas = max(min(static_cast<uint32_t>(shape.ctas), (total + shape.least - 1) / shape.least), 1u);
@@ -113,8 +114,8 @@ struct FlatOrder {
     const int lane = threadIdx.x & 31;
     uint32_t before = 0;
     for (int i = 0; 32 * i < s.B; ++i) {
-      const int mine = pages(c, s, i), my_tiles = tiles(c, s, p, shape, i);
-      uint32_t upto = mine * my_tiles;
+      const int my_len = length(c, s, i), my_tiles = tiles(c, s, p, shape, i);
+      uint32_t upto = pages_of_length(my_len) * my_tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
@@ -122,9 +123,9 @@ struct FlatOrder {
       }
       const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * c.H > at);
       if (past != 0u) {
-        const int l = __ffs(past) - 1, n = __shfl_sync(0xffffffffu, mine, l), tiles_b = __shfl_sync(0xffffffffu, my_tiles, l);
+        const int l = __ffs(past) - 1, len = __shfl_sync(0xffffffffu, my_len, l), n = pages_of_length(len), tiles_b = __shfl_sync(0xffffffffu, my_tiles, l);
         const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n * tiles_b) * c.H, ht = rest / static_cast<uint32_t>(n);
-        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), n, tiles_b};
+        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), len, tiles_b};
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
@@ -135,10 +136,27 @@ struct FlatOrder {
     const int lane = threadIdx.x & 31;
     uint32_t n = 0;
     for (int i = 0; 32 * i < b; ++i)
-      if (32 * i + lane < b) n += pages(c, s, i) * tiles(c, s, p, shape, i);
+      if (32 * i + lane < b) n += pages_of_length(length(c, s, i)) * tiles(c, s, p, shape, i);
     return __reduce_add_sync(0xffffffffu, n) * c.H;
   }
 };
+
+// Reads a line of the kernel's parameters here and now. A first read takes as long as one of global memory, and longer once the loads of all CTAs are on
+// their way: ahead of the wait for the kernel before, it costs nothing.
+__device__ __forceinline__ void touch(uint32_t x) { asm volatile("" ::"r"(x)); }
+__device__ __forceinline__ void touch_parameters(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, const AttnWorkspace& ws) {
+  touch(c.pages);
+  touch(s.blocks);
+  touch(p.H);
+  touch(static_cast<uint32_t>(p.q.stride_t));
+  touch(static_cast<uint32_t>(p.o.stride_t));
+  touch(p.causal);
+  touch(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p.lse)));
+  touch(static_cast<uint32_t>(p.w_len));
+  touch(shape.G);
+  touch(shape.least);
+  touch(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ws.part_ml)));
+}
 
 // kv_attn_chunk.cu
 constexpr int KC_ROWS = 128, KC_CTAS = 2;   // query rows of an item, CTAs of an SM

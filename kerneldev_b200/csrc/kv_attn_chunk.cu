@@ -152,6 +152,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tS = __reduce_max_sync(0xffffffffu, sh.tmem), tO = tS + CH_TOKENS;   // warp-uniform for the compiler
+  touch_parameters(c, s, p, shape, ws);
   pdl_wait();
   pdl_launch_dependents();
 
@@ -168,17 +169,19 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
       n.here = -1;
       n.second = done > 0 ? 1 : 0;
       if (shape.ctas > 0) {
-        const FlatOrder order(c, s, p, shape);
+        FlatOrder order;
+        order.look_up(c, s, p, shape);
         if (blockIdx.x < order.ctas) {
           const uint32_t at = order.start(blockIdx.x) + done, end = order.start(blockIdx.x + 1);
           if (at < end) {
             const FlatPlace f = order.find(c, s, p, shape, at);
             const int h = f.ht / f.tiles;
-            n = ChunkItem{Item{f.b, h, f.ht - h * f.tiles, sequence_length(c, s, f.b)}, f.page, f.pages, min(static_cast<int>(end - at), f.pages - f.page), n.second};
+            const int pages = pages_of_length(f.len);
+            n = ChunkItem{Item{f.b, h, f.ht - h * f.tiles, f.len}, f.page, pages, min(static_cast<int>(end - at), pages - f.page), n.second};
           }
         }
       } else if (done == 0) {
-        const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles, len = sequence_length(c, s, b), pages = (len + KC_PAGE - 1) / KC_PAGE;
+        const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles, len = sequence_length(c, s, b), pages = pages_of_length(len);
         n = ChunkItem{Item{b, h, ht - h * shape.tiles, len}, 0, pages, pages, 0};
       }
       if (lane == 0) sh.item = n;
