@@ -200,47 +200,55 @@ __device__ __forceinline__ void add_values(float (&o)[NT][D / 16][4], const uint
 
 // ---- query rows ---------------------------------------------------------------------------------------------------
 
-// The query tiles of an item in shared memory, all threads of the CTA; ends with a barrier. bfloat16 rows are multiplied with the power of two that brings their largest
-// finite number to 2^14 (what falls below a half's subnormals is 2^-38 of it).
+// The query tiles of an item. fetch: loads, ahead of the item's first copies of the cache (behind them, with the copies of all CTAs on their way, they took
+// 2 us); store: into shared memory, all threads of the CTA, ends with a barrier. bfloat16 rows are multiplied with the power of two that brings their largest finite number to 2^14
+// (what falls below a half's subnormals is 2^-38 of it).
 template <int D, int NT>
-__device__ __forceinline__ void load_queries(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int G, int rows, QueryTile<D, NT>& q) {
-  using S = Spread<D>;
-  constexpr int ROWS = NT * KA_TILE, PER = ROWS / KA_WARPS;   // rows of a warp, four numbers of each to a lane
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = 4 * lane;
-  const bool bf16 = p.dtype == KD_BF16;
+struct QueryLoad {
+  static constexpr int ROWS = NT * KA_TILE, PER = ROWS / KA_WARPS;   // rows of a warp, four numbers of each to a lane
   uint2 v[PER];
+  RowMask mask;   // of thread r < ROWS: row r
+
+  __device__ __forceinline__ void fetch(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const Item& it, int G, int rows) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = 4 * lane;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = it.tile * ROWS + warp * PER + i;
-    v[i] = make_uint2(0u, 0u);
-    if (row < rows && d < D) {
-      const int n = row / G, hq = it.h * G + row - n * G;
-      v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
+    for (int i = 0; i < PER; ++i) {
+      const int row = it.tile * ROWS + warp * PER + i;
+      v[i] = make_uint2(0u, 0u);
+      if (row < rows && d < D) {
+        const int n = row / G, hq = it.h * G + row - n * G;
+        v[i] = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q.ptr) + it.b * p.q.stride_b + hq * p.q.stride_h + n * p.q.stride_t + d);
+      }
     }
+    if (threadIdx.x < ROWS) mask = row_mask(c, s, p, it, it.tile * ROWS + threadIdx.x, G, rows, query_count(c, p, it.b));
   }
-  if (threadIdx.x < ROWS) {
-    const RowMask m = row_mask(c, s, p, it, it.tile * ROWS + threadIdx.x, G, rows, query_count(c, p, it.b));
-    q.mask[threadIdx.x] = m;
-    const int low = __reduce_min_sync(ROWS == 32 ? 0xFFFFFFFFu : (1u << ROWS) - 1u, m.limit > 0 ? m.limit : INT_MAX);
-    if (threadIdx.x == 0) q.min_limit = low;
-  }
+  __device__ __forceinline__ void store(const kd_cache_queries& p, QueryTile<D, NT>& q) {
+    using S = Spread<D>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = 4 * lane;
+    const bool bf16 = p.dtype == KD_BF16;
+    if (threadIdx.x < ROWS) {
+      q.mask[threadIdx.x] = mask;
+      const int low = __reduce_min_sync(ROWS == 32 ? 0xFFFFFFFFu : (1u << ROWS) - 1u, mask.limit > 0 ? mask.limit : INT_MAX);
+      if (threadIdx.x == 0) q.min_limit = low;
+    }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int r = warp * PER + i;
-    int e = 0;
-    if (bf16) {
-      auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
-      const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[i].x), size(v[i].x >> 16)), max(size(v[i].y), size(v[i].y >> 16))));
-      if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
-      const float f = exp2i(e);
-      const float2 a = unpack2<true>(v[i].x), b = unpack2<true>(v[i].y);
-      v[i] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+    for (int i = 0; i < PER; ++i) {
+      const int r = warp * PER + i;
+      int e = 0;
+      if (bf16) {
+        auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
+        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[i].x), size(v[i].x >> 16)), max(size(v[i].y), size(v[i].y >> 16))));
+        if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
+        const float f = exp2i(e);
+        const float2 a = unpack2<true>(v[i].x), b = unpack2<true>(v[i].y);
+        v[i] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+      }
+      if (lane == 0) q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+      if (d < D) q.frag[r / KA_TILE][S::k_word(d)][(r % KA_TILE) * 4 + S::k_lane(d)] = v[i];
     }
-    if (lane == 0) q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
-    if (d < D) q.frag[r / KA_TILE][S::k_word(d)][(r % KA_TILE) * 4 + S::k_lane(d)] = v[i];
+    __syncthreads();
   }
-  __syncthreads();
-}
+};
 
 // masks the scores of a unit (c as above); rows: the masks of a tile's rows
 __device__ __forceinline__ void mask_scores(float (&c)[2][4], const uint32_t* desc, int j0, int g, int t, int end, const RowMask* rows) {
@@ -296,9 +304,10 @@ struct Walker {
   }
 
   // next_page: what begin returned
+  // scores: of the item's first token, or null: they are not wanted
   template <bool kSafe>
   __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, const QueryTile<D, NT>& q, int first, int last, int next_page,
-                                       char* ring) {
+                                       char* ring, float* all_scores, int score_rows) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -333,6 +342,12 @@ struct Walker {
         if (page < 0 || j0 + KA_UNIT > free_end) mask_scores(sc[n], desc, j0, g, t, page < 0 ? 0 : it.len, &q.mask[n * KA_TILE]);
         float k[2], add[2], shrink[2];
         bool grown = false;
+        if (NT == 1 && all_scores != nullptr && 2 * t < score_rows) {
+          const float k0 = fmaxf(ks * q.factor[2 * t], KA_TINY), k1 = fmaxf(ks * q.factor[2 * t + 1], KA_TINY);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            *reinterpret_cast<float2*>(all_scores + static_cast<size_t>(j0 + 8 * y + g) * score_rows + 2 * t) = make_float2(sc[n][y >> 1][2 * (y & 1)] * k0, sc[n][y >> 1][2 * (y & 1) + 1] * k1);
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           k[x] = fmaxf(ks * q.factor[n * KA_TILE + 2 * t + x], KA_TINY);
@@ -431,61 +446,25 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   extern __shared__ __align__(1024) char smem[];
   AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, HT = c.H * shape.tiles;
-  FlatOrder order;
-  uint32_t at = 0, end = 1;
-  if (shape.ctas > 0) {
-    order.look_up(c, s, p, shape);
-    if (blockIdx.x >= order.ctas || order.total == 0) return;
-    at = order.start(blockIdx.x);
-    end = order.start(blockIdx.x + 1);
-  }
-  const uint32_t begin = at;
-  struct Share {   // of an item: pages page0 .. page0 + here - 1 of `pages`, the warp's units
-    Item it;
-    int pages, here, first, last, next_page;
-  };
-  auto share_at = [&](uint32_t place_of) {
-    Share r;
-    int page0 = 0;
-    if (shape.ctas > 0) {
-      const FlatPlace f = order.find(c, s, p, shape, place_of);
-      r.it.b = f.b;
-      r.it.h = f.ht / f.tiles;
-      r.it.tile = f.ht - r.it.h * f.tiles;
-      r.it.len = f.len;
-      page0 = f.page;
-      r.pages = pages_of_length(f.len);
-      r.here = min(static_cast<int>(end - place_of), r.pages - page0);
-    } else {
-      const int item = blockIdx.x;
-      r.it.b = item / HT;
-      r.it.h = (item - r.it.b * HT) / shape.tiles;
-      r.it.tile = item - r.it.b * HT - r.it.h * shape.tiles;
-      r.it.len = sequence_length(c, s, r.it.b);
-      r.pages = r.here = pages_of_length(r.it.len);
-    }
-    r.first = 2 * page0 + warp;
-    r.last = min(2 * (page0 + r.here), (r.it.len + KA_UNIT - 1) / KA_UNIT);
-    return r;
-  };
-  char* ring = sh.warp[warp].stage;
-  Share now = share_at(at);
-  now.next_page = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
-  while (at < end) {
-    load_queries<D, NT>(c, s, p, now.it, shape.G, shape.rows, sh.q);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+#pragma unroll 1
+  for (uint32_t done = 0;;) {
+    const ItemShare share = share_of_cta(c, s, p, shape, done);
+    if (share.here < 0) return;
+    const Item it = share.it;
+    const int first = 2 * share.page0 + warp, last = min(2 * (share.page0 + share.here), (it.len + KA_UNIT - 1) / KA_UNIT);
+    const bool whole = share.here == share.pages;
+    char* ring = sh.warp[warp].stage;
+    QueryLoad<D, NT> queries;
+    queries.fetch(c, s, p, it, shape.G, shape.rows);
+    int next_page = Walker<D, NT>::begin(c, s, place, it, first, last, ring);
+    queries.store(p, sh.q);
     Walker<D, NT> w;
-    w.template walk<false>(c, s, place, now.it, sh.q, now.first, now.last, now.next_page, ring);
+    float* scores = shape.score_rows > 0 ? ws.scores + (static_cast<size_t>(it.b) * c.H + it.h) * s.blocks * KC_PAGE * shape.score_rows : nullptr;
+    w.template walk<false>(c, s, place, it, sh.q, first, last, next_page, ring, scores, shape.score_rows);
     if (w.any_nan()) {
-      const int next = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
-      w.template walk<true>(c, s, place, now.it, sh.q, now.first, now.last, next, ring);
-    }
-    const uint32_t after = at + (shape.ctas > 0 ? now.here : 1);
-    const Item it = now.it;
-    const bool whole = now.here == now.pages, first_of_cta = at == begin;
-    if (after < end) {   // the next item's first copies run while this one's rows are joined
-      now = share_at(after);
-      now.next_page = Walker<D, NT>::begin(c, s, place, now.it, now.first, now.last, ring);
+      next_page = Walker<D, NT>::begin(c, s, place, it, first, last, ring);
+      w.template walk<true>(c, s, place, it, sh.q, first, last, next_page, ring, nullptr, 0);
     }
     if (g == 0)
 #pragma unroll
@@ -499,7 +478,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
 #pragma unroll
         for (int x = 0; x < 4; ++x) sh.warp[warp].o(n * KA_TILE + 2 * t + (x & 1))[Spread<D>::v_dim(2 * m + (x >> 1), g)] = w.o[n][m][x];
     __syncthreads();
-    const size_t part = 2 * static_cast<size_t>(blockIdx.x) + (first_of_cta ? 0 : 1);
+    const size_t part = share.part;
     auto place_of_row = [&](int row, int& hq, int& i) {   // of the key head
       i = row / shape.G;
       hq = it.h * shape.G + row - i * shape.G;
@@ -550,46 +529,28 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
         *reinterpret_cast<float4*>(ws.part_o + (part * ROWS + r) * D + d) = v;
       }
     }
+    if (!shape.even) return;
+    done += share.here;
     __syncthreads();   // shared memory is free for the next item
-    at = after;
   }
 }
 
-// Query rows whose pages several CTAs shared: their parts on one scale. kGroups warps of a CTA take a row's parts in turn, 8 / kGroups rows a CTA: eight warps for a row where
-// there are few rows (a long context has dozens of parts), one where there are many. Rows without a query, and those of sequences without a token, get their zeros here.
-// What it needs to know of the lengths was there before the kernel ahead of it, so it is looked up while that one runs.
+// One query row whose pages several CTAs shared: their parts on one scale, and its output. kGroups warps take the parts in turn (grp: this warp's number; with more than
+// one they are the whole CTA, and meet at barriers).
 constexpr int KJ_WARPS = 8;
+struct JoinShared {
+  float4 o[KJ_WARPS][32];
+  float2 ml[KJ_WARPS];
+};
 template <int kGroups>
-__global__ void __launch_bounds__(KJ_WARPS * 32)
-cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
-                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
-  constexpr int ROWS = KJ_WARPS / kGroups;
-  __shared__ float4 s_o[kGroups > 1 ? KJ_WARPS : 1][32];
-  __shared__ float2 s_ml[KJ_WARPS];
-  const int tid = threadIdx.x, lane = tid & 31, grp = (tid >> 5) % kGroups;
-  const int per_head = (shape.rows + ROWS - 1) / ROWS;
-  const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + (tid >> 5) / kGroups;
-  const int tile = row_of_head / shape.item_rows, r = row_of_head - tile * shape.item_rows;
-  FlatOrder order;
-  order.look_up(c, s, p, shape);
-  const int len = sequence_length(c, s, b), n = query_count(c, p, b), tiles = (n * shape.G + shape.item_rows - 1) / shape.item_rows;
-  const int pages = tile < tiles ? pages_of_length(len) : 0;   // of the item
-  const uint32_t first = order.before(c, s, p, shape, b) + (h * tiles + tile) * pages;   // the item's first page in the flat order
-  int c0 = 0, c1 = -1;
-  if (pages > 0) {
-    c0 = static_cast<int>(order.cta_of(first));
-    c1 = static_cast<int>(order.cta_of(first + pages - 1));
-  }
-  const size_t first_part = (2 * static_cast<size_t>(c0) + (order.start(c0) >= first ? 0 : 1)) * shape.item_rows + r;
-  pdl_wait();
-  pdl_launch_dependents();
-  if (c0 == c1 || row_of_head >= shape.rows) return;   // the one CTA has written the row (with kGroups > 1 there is one row, so that all warps leave)
-  const int d = lane * 4;
+__device__ __forceinline__ void join_row(const kd_cache& c, const kd_cache_queries& p, const AttnShape& shape, const AttnWorkspace& ws, const ItemParts& parts, int b, int h,
+                                         int row_of_head, int len, int n, int grp, JoinShared* sh) {
+  const int lane = threadIdx.x & 31, d = lane * 4, r = row_of_head % shape.item_rows;
   float ref = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int k = c0 + grp; k <= c1; k += kGroups) {
-    const size_t part = k == c0 ? first_part : 2 * static_cast<size_t>(k) * shape.item_rows + r;
+  for (int k = grp; k < parts.count; k += kGroups) {
+    const size_t part = static_cast<size_t>(parts.at(k)) * shape.item_rows + r;
     const float2 ml = ws.part_ml[part];
     const float4 v = d < c.D ? *reinterpret_cast<const float4*>(ws.part_o + part * c.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     if (ml.x == -INFINITY) continue;
@@ -599,24 +560,26 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
     acc = make_float4(fmaf(v.x, scale, acc.x * keep), fmaf(v.y, scale, acc.y * keep), fmaf(v.z, scale, acc.z * keep), fmaf(v.w, scale, acc.w * keep));
   }
   if constexpr (kGroups > 1) {
-    static_assert(ROWS == 1, "the barrier below is the whole CTA's");
-    s_o[grp][lane] = acc;
-    if (lane == 0) s_ml[grp] = make_float2(ref, sum);
+    sh->o[grp][lane] = acc;
+    if (lane == 0) sh->ml[grp] = make_float2(ref, sum);
     __syncthreads();
-    if (grp > 0) return;
-    ref = -INFINITY;
+    if (grp == 0) {
+      ref = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) ref = fmaxf(ref, s_ml[k].x);
-    sum = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < kGroups; ++k) ref = fmaxf(ref, sh->ml[k].x);
+      sum = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      if (s_ml[k].x == -INFINITY) continue;
-      const float scale = fast_exp2(s_ml[k].x - ref);
-      const float4 v = s_o[k][lane];
-      sum = fmaf(s_ml[k].y, scale, sum);
-      acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
+      for (int k = 0; k < kGroups; ++k) {
+        if (sh->ml[k].x == -INFINITY) continue;
+        const float scale = fast_exp2(sh->ml[k].x - ref);
+        const float4 v = sh->o[k][lane];
+        sum = fmaf(sh->ml[k].y, scale, sum);
+        acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
+      }
     }
+    __syncthreads();   // (for the next row)
+    if (grp > 0) return;
   }
   const int i = row_of_head / shape.G, hq = h * shape.G + row_of_head - i * shape.G;
   const bool live = i < n && len - n + i >= 0;
@@ -628,6 +591,90 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
     *reinterpret_cast<uint2*>(out) = p.dtype == KD_BF16 ? make_uint2(pack2<true>(acc.x, acc.y), pack2<true>(acc.z, acc.w)) : make_uint2(pack2<false>(acc.x, acc.y), pack2<false>(acc.z, acc.w));
   }
   if (lane == 0) write_stats(p, ws, shape.stats, (static_cast<size_t>(b) * p.H + hq) * p.T + i, live, ref, sum);
+}
+
+// The rows of all items: eight warps for a row where there are few rows (a long context has dozens of parts), one where there are many. Rows without a query, and those of
+// sequences without a token, get their zeros here. What it needs to know of the lengths was there before the kernel ahead of it, so it is looked up while that one runs.
+template <int kGroups>
+__global__ void __launch_bounds__(KJ_WARPS * 32)
+cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
+                  const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  constexpr int ROWS = KJ_WARPS / kGroups;
+  static_assert(kGroups == 1 || ROWS == 1, "join_row's barriers are the whole CTA's");
+  __shared__ JoinShared sh;
+  const int warp = threadIdx.x >> 5, per_head = (shape.rows + ROWS - 1) / ROWS;
+  const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + warp / kGroups;
+  const int len = sequence_length(c, s, b), n = query_count(c, p, b);
+  const ItemParts parts = parts_of(c, s, p, shape, b, h, row_of_head / shape.item_rows, len, n);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (parts.count == 1 || row_of_head >= shape.rows) return;   // the one CTA has written the row
+  join_row<kGroups>(c, p, shape, ws, parts, b, h, row_of_head, len, n, warp % kGroups, &sh);
+}
+
+// The weights of few rows, from the scores that the kernel ahead has left, and the join: a CTA has KS_TOKENS tokens of a head, the first ones of a head its rows too. (One launch
+// less, and K is not read again: with cache_weights_kernel behind cache_join_kernel 8 x 4096 tokens of 8 heads of 128 took 31 us, so NNN.)
+constexpr int KS_TOKENS = 1024;
+__global__ void __launch_bounds__(KJ_WARPS * 32)
+cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
+                          const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
+  __shared__ JoinShared sh;
+  __shared__ float2 s_stat[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, groups = (s.blocks * KC_PAGE + KS_TOKENS - 1) / KS_TOKENS;
+  const int bh = blockIdx.x / groups, group = blockIdx.x - bh * groups, b = bh / c.H, h = bh - b * c.H;
+  const int len = sequence_length(c, s, b), n = query_count(c, p, b);
+  if (group * KS_TOKENS >= len && group > 0) return;
+  ItemParts parts{0, 0, 0, 1};
+  if (shape.ctas > 0) parts = parts_of(c, s, p, shape, b, h, 0, len, n);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (parts.count != 1)
+    for (int r = group; r < shape.rows; r += max((len + KS_TOKENS - 1) / KS_TOKENS, 1)) join_row<KJ_WARPS>(c, p, shape, ws, parts, b, h, r, len, n, warp, &sh);
+  // the rows' maxima and sums, a warp for each (what join_row leaves in the workspace may be another CTA's work)
+  if (warp < shape.rows) {
+    const int i = warp / shape.G, hq = h * shape.G + warp - i * shape.G;
+    float2 st;
+    if (parts.count == 1) {
+      st = ws.stats[(static_cast<size_t>(b) * p.H + hq) * p.T + i];
+    } else {
+      float ref = -INFINITY, sum = 0.f;
+      for (int k = lane; k < parts.count; k += 32) {
+        const float2 ml = ws.part_ml[static_cast<size_t>(parts.at(k)) * shape.item_rows + warp];
+        const float to = fmaxf(ref, ml.x);
+        if (to == -INFINITY) continue;
+        sum = sum * fast_exp2(ref - to) + ml.y * fast_exp2(ml.x - to);
+        ref = to;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, ref, o), other_sum = __shfl_xor_sync(0xffffffffu, sum, o), to = fmaxf(ref, other);
+        if (to != -INFINITY) sum = sum * fast_exp2(ref - to) + other_sum * fast_exp2(other - to);
+        ref = to;
+      }
+      const bool live = i < n && len - n + i >= 0;
+      st = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
+    }
+    if (lane == 0) s_stat[warp] = st;
+  }
+  __syncthreads();
+  const float* scores = ws.scores + static_cast<size_t>(bh) * s.blocks * KC_PAGE * shape.score_rows;
+  float* weights = p.weights + b * p.w_stride_b + h * p.w_stride_h;
+#pragma unroll
+  for (int x = 0; x < KS_TOKENS; x += KJ_WARPS * 32) {
+    const int j = group * KS_TOKENS + x + tid;
+    if (j >= len || j >= p.w_len) continue;
+    float add = 0.f;
+    for (int r = 0; r < shape.score_rows; r += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(scores + static_cast<size_t>(j) * shape.score_rows + r);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float score = y == 0 ? v.x : v.y;
+        const float2 st = r + y < shape.rows ? s_stat[r + y] : make_float2(0.f, 0.f);
+        if (st.y != 0.f && score != -INFINITY) add += fast_exp2(score + (KA_OFFSET - st.x)) * st.y;   // rows that exist, tokens that they see
+      }
+    }
+    weights[j] += add;
+  }
 }
 
 // weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
@@ -676,7 +723,9 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
   }
   cp_async_commit();
   for (it.tile = 0; it.tile < shape.tiles; ++it.tile) {
-    load_queries<D, NT>(c, s, p, it, shape.G, shape.rows, q);
+    QueryLoad<D, NT> queries;
+    queries.fetch(c, s, p, it, shape.G, shape.rows);
+    queries.store(p, q);
     if (tid < ROWS) {
       const int r = it.tile * ROWS + tid, i = r / shape.G;
       s_stat[tid] = r < shape.rows ? ws.stats[(static_cast<size_t>(it.b) * p.H + it.h * shape.G + r - i * shape.G) * p.T + i] : make_float2(0.f, 0.f);
@@ -733,9 +782,13 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   const int rows = a.item_rows = rows_of_item(a.rows);
   a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
-  const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
+  a.score_rows = !a.stats || a.rows > KA_TILE ? 0 : a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : 8;
+  const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles, pages = items * s.blocks;
   // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
-  a.ctas = s.blocks <= 8 || items > 148 * 16 || items * s.blocks >= (1 << 30) ? 0 : 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
+  const int slots = 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
+  a.ctas = s.blocks <= 8 || items > 148 * 16 || pages >= (1 << 30) ? 0 : slots;
+  a.even = items > slots / 2;   // see FlatOrder
+  a.spread = a.even ? 1 : slots - static_cast<int>(items);
   a.least = rows == KC_ROWS ? 8 : 2;   // four tiles of 128 tokens; a unit for each warp
   return a;
 }
@@ -747,7 +800,8 @@ static size_t workspace_of(const kd_cache& c, const kd_cache_seqs& s, const kd_c
     n += (bytes + 255) & ~size_t(255);
     return at;
   };
-  const size_t part_rows = size_t(2) * a.ctas * rows_of_item(a.rows);
+  const size_t part_rows = (a.even ? size_t(2) : size_t(1)) * a.ctas * rows_of_item(a.rows);
+  ws->scores = reinterpret_cast<float*>(take(static_cast<size_t>(s.B) * c.H * s.blocks * KC_PAGE * a.score_rows * sizeof(float)));
   ws->stats = reinterpret_cast<float2*>(take(a.stats ? static_cast<size_t>(s.B) * p.H * p.T * sizeof(float2) : 0));
   ws->part_o = reinterpret_cast<float*>(take(part_rows * c.D * sizeof(float)));
   ws->part_ml = reinterpret_cast<float2*>(take(part_rows * sizeof(float2)));
@@ -796,13 +850,19 @@ static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_
   } else {
     e = rows == KA_TILE ? launch_rows<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_rows<D, 2>(c, s, p, a, ws, stream) : launch_rows<D, 4>(c, s, p, a, ws, stream);
   }
+  if (a.score_rows > 0 && s.blocks > 0) {
+    const int64_t groups = heads * ((static_cast<int64_t>(s.blocks) * KC_PAGE + KS_TOKENS - 1) / KS_TOKENS);
+    if (e == cudaSuccess) e = launch(cache_join_weights_kernel, static_cast<unsigned>(groups), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
+    if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
+    return 0;
+  }
   if (e == cudaSuccess && a.ctas > 0) {
-    // up to one row for each warp that fits on the device
-    const bool few = heads * a.rows <= 148 * 16;
+    // (1024 CTAs for as many rows of two or three parts were two waves)
+    const bool few = heads * a.rows <= 148 * 2;
     e = few ? launch(cache_join_kernel<KJ_WARPS>, static_cast<unsigned>(heads * a.rows), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
             : launch(cache_join_kernel<1>, static_cast<unsigned>(heads * ((a.rows + KJ_WARPS - 1) / KJ_WARPS)), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
   }
-  if (e == cudaSuccess) e = rows == KA_TILE ? launch_weights<D, 1>(c, s, p, a, ws, stream) : rows == 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);
+  if (e == cudaSuccess) e = rows == 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);   // (one tile of rows: above)
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
   return 0;
 }

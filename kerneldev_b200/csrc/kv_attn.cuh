@@ -18,13 +18,18 @@ struct RowMask {
 
 struct AttnShape {
   int G, rows, tiles;   // heads of a group, query rows of a key head, items that they are cut into
-  int ctas;             // 0: a CTA for each (sequence, head, tile); else at most that many CTAs share all pages evenly
+  int ctas;             // 0: a CTA for each (sequence, head, tile); else that many share the pages (FlatOrder)
+  int spread;           // ... those beyond one for each item
+  bool even;            // see FlatOrder
   int item_rows;        // query rows of an item
   int least;            // pages that such a CTA has at least
   bool stats;           // leave every row's maximum and sum for the weights
+  int score_rows;       // 0, or the rows of a key head rounded up to 2, 4 or 8: leave the scores too
 };
-// Workspace: the rows' statistics (float2 for each, with weights), then for each CTA two parts: an item's rows of D floats, and their maxima and sums.
+// Workspace: the rows' statistics (float2 for each, with weights), then the parts (see FlatOrder): an item's rows of D floats, and their maxima and sums. With weights and
+// few rows, every score (times log2(e)) as well: for each token of each key head of the table, score_rows of them.
 struct AttnWorkspace {
+  float* scores;
   float2* stats;
   float* part_o;
   float2* part_ml;
@@ -63,83 +68,152 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
   if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
 }
 
-// The flat order of all pages: sequences in turn, each once for every head and tile of rows that has a query, cut into even ranges for the CTAs. 32 bits are
-// enough: the host sees to it that there are fewer than 2^30 pages. A warp holds the counts of the first 128 sequences, in its lanes.
+// How the pages are shared out. An item is a sequence, a head and a tile of rows that has a query; `Units` of it are counted by a flat order: sequences in turn, each once for
+// every head and tile. Two ways:
+//   shares  an item of n pages goes to ceil(n / most) CTAs, evenly, and `most` is such that there are CTAs enough for all. A CTA has one item's pages alone.
+//           The way of few items in one wave of CTAs: their time is mostly latency, and a CTA with two items has it twice (16 x 1357 tokens of 4 heads, 5 queries: 15 us, 20 with even pages).
+//   even    every CTA of one wave has the same number of pages, wherever that begins and ends. The way of many items: 32 x 4096 tokens of 8 heads 42 us, 46 to 49 with
+//           one to three waves of shares.
+// The units of the flat order are CTAs or pages. 32 bits are enough: the host sees to it that there are fewer than 2^30 pages. A warp holds what it needs of the first 32
+// sequences in its lanes; a loop over the ones behind reads them again, from L1: the code is what a CTA that starts waits for.
 struct FlatPlace {
-  int b, ht, page, len, tiles;   // ht: head * tiles + tile; len and tiles: of the sequence; page: index within the item
+  int b, ht, at, units, len, tiles;   // ht: head * tiles + tile; unit `at` of `units` of the item; len and tiles: of the sequence
 };
 __device__ __forceinline__ int pages_of_length(int len) { return (len + KC_PAGE - 1) / KC_PAGE; }
 struct FlatOrder {
-  static constexpr int HELD = 4;
-  int held[HELD], held_tiles[HELD];   // lengths, tiles
-  uint32_t total;             // pages
-  uint32_t ctas, each, more;  // that share them: `each` pages, and one more for the first `more` CTAs
+  int held, held_tiles;       // length and tiles of sequence `lane`
+  uint32_t most;              // pages of a unit
+  uint32_t total;             // even: pages ...
+  uint32_t ctas, each, more;  // ... and the CTAs that have them: `each`, and one more for the first `more`
 
   static __device__ __forceinline__ int length_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? sequence_length(c, s, b) : 0; }
   static __device__ __forceinline__ int tiles_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) {
+    if (p.q_lens == nullptr) return shape.tiles;
     return b < s.B ? (query_count(c, p, b) * shape.G + shape.item_rows - 1) / shape.item_rows : 0;
   }
-  // of sequence 32 i + lane
-  __device__ __forceinline__ int length(const kd_cache& c, const kd_cache_seqs& s, int i) const {
-    if (i < HELD) return i == 0 ? held[0] : i == 1 ? held[1] : i == 2 ? held[2] : held[3];
-    return length_of(c, s, 32 * i + (threadIdx.x & 31));
-  }
-  __device__ __forceinline__ int tiles(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int i) const {
-    if (i < HELD) return i == 0 ? held_tiles[0] : i == 1 ? held_tiles[1] : i == 2 ? held_tiles[2] : held_tiles[3];
-    return tiles_of(c, s, p, shape, 32 * i + (threadIdx.x & 31));
-  }
+  __device__ __forceinline__ uint32_t units_of(int len) const { return (pages_of_length(len) + most - 1) / most; }
   __device__ __forceinline__ void look_up(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape) {
     const int lane = threadIdx.x & 31;
-    uint32_t n = 0;
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      held[i] = length_of(c, s, 32 * i + lane);
-      held_tiles[i] = tiles_of(c, s, p, shape, 32 * i + lane);
-    }
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) n += pages_of_length(held[i]) * held_tiles[i];
-    for (int b = 32 * HELD + lane; b < s.B; b += 32) n += pages_of_length(length_of(c, s, b)) * tiles_of(c, s, p, shape, b);
+    held = length_of(c, s, lane);
+    held_tiles = tiles_of(c, s, p, shape, lane);
+    uint32_t n = pages_of_length(held) * held_tiles;
+#pragma unroll 1
+    for (int b = 32 + lane; b < s.B; b += 32) n += pages_of_length(length_of(c, s, b)) * tiles_of(c, s, p, shape, b);
     total = __reduce_add_sync(0xffffffffu, n) * c.H;
-    // (None of them has no page: the join reads a part of every CTA of an item.)
-    ctas = max(min(static_cast<uint32_t>(shape.ctas), (total + shape.least - 1) / shape.least), 1u);
-    each = total / ctas;
-    more = total - each * ctas;
+    if (shape.even) {
+      most = 1;
+      // (None of them has no page: the join reads a part of every CTA of an item.)
+      ctas = max(min(static_cast<uint32_t>(shape.ctas), (total + shape.least - 1) / shape.least), 1u);
+      each = total / ctas;
+      more = total - each * ctas;
+    } else {
+      // sum of ceil(n / most) <= total / most + items <= CTAs
+      most = max((total + shape.spread - 1) / shape.spread, static_cast<uint32_t>(shape.least));
+    }
   }
+  // even: a CTA's first page, and a page's CTA
   __device__ __forceinline__ uint32_t start(uint32_t cta) const { return cta * each + min(cta, more); }
   __device__ __forceinline__ uint32_t cta_of(uint32_t page) const {
     const uint32_t longer = more * (each + 1);
     return page < longer ? page / (each + 1) : more + (page - longer) / each;
   }
-  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, uint32_t at) const {
+  // whose a unit is; b < 0: nobody's
+  __device__ __forceinline__ FlatPlace find(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, uint32_t unit) const {
     const int lane = threadIdx.x & 31;
     uint32_t before = 0;
-    for (int i = 0; 32 * i < s.B; ++i) {
-      const int my_len = length(c, s, i), my_tiles = tiles(c, s, p, shape, i);
-      uint32_t upto = pages_of_length(my_len) * my_tiles;
+#pragma unroll 1
+    for (int base = 0; base < s.B; base += 32) {
+      const int my_len = base == 0 ? held : length_of(c, s, base + lane), my_tiles = base == 0 ? held_tiles : tiles_of(c, s, p, shape, base + lane);
+      const uint32_t mine = units_of(my_len);
+      uint32_t upto = mine * my_tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += up;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * c.H > at);
+      const uint32_t past = __ballot_sync(0xffffffffu, (before + upto) * c.H > unit);
       if (past != 0u) {
-        const int l = __ffs(past) - 1, len = __shfl_sync(0xffffffffu, my_len, l), n = pages_of_length(len), tiles_b = __shfl_sync(0xffffffffu, my_tiles, l);
-        const uint32_t rest = at - (before + __shfl_sync(0xffffffffu, upto, l) - n * tiles_b) * c.H, ht = rest / static_cast<uint32_t>(n);
-        return FlatPlace{32 * i + l, static_cast<int>(ht), static_cast<int>(rest - ht * n), len, tiles_b};
+        const int l = __ffs(past) - 1, len = __shfl_sync(0xffffffffu, my_len, l), tiles_b = __shfl_sync(0xffffffffu, my_tiles, l);
+        const uint32_t units = __shfl_sync(0xffffffffu, mine, l), rest = unit - (before + __shfl_sync(0xffffffffu, upto, l) - units * tiles_b) * c.H, ht = rest / units;
+        return FlatPlace{base + l, static_cast<int>(ht), static_cast<int>(rest - ht * units), static_cast<int>(units), len, tiles_b};
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    return FlatPlace{-1, 0, 0, 0, 0};
+    return FlatPlace{-1, 0, 0, 0, 0, 0};
   }
-  // pages of the sequences before b
+  // units of the sequences before b
   __device__ __forceinline__ uint32_t before(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) const {
     const int lane = threadIdx.x & 31;
-    uint32_t n = 0;
-    for (int i = 0; 32 * i < b; ++i)
-      if (32 * i + lane < b) n += pages_of_length(length(c, s, i)) * tiles(c, s, p, shape, i);
+    uint32_t n = lane < b ? units_of(held) * held_tiles : 0u;
+#pragma unroll 1
+    for (int i = 32 + lane; i < b; i += 32) n += units_of(length_of(c, s, i)) * tiles_of(c, s, p, shape, i);
     return __reduce_add_sync(0xffffffffu, n) * c.H;
   }
 };
+
+// What a CTA works on next: pages page0 .. page0 + here - 1 of the `pages` of an item. here < 0: nothing.
+struct ItemShare {
+  Item it;
+  int page0, here, pages;
+  uint32_t part;   // where its rows go if that is not all of the item
+};
+// done: pages that the CTA has worked on
+__device__ __forceinline__ ItemShare share_of_cta(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, uint32_t done) {
+  ItemShare r;
+  r.here = -1;
+  if (shape.ctas == 0) {
+    if (done > 0) return r;
+    const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles;
+    r.it = Item{b, h, ht - h * shape.tiles, sequence_length(c, s, b)};
+    r.page0 = 0;
+    r.pages = r.here = pages_of_length(r.it.len);
+    return r;
+  }
+  FlatOrder order;
+  order.look_up(c, s, p, shape);
+  uint32_t unit = blockIdx.x, left = 0;
+  if (shape.even) {
+    if (blockIdx.x >= order.ctas) return r;
+    unit = order.start(blockIdx.x) + done;
+    left = order.start(blockIdx.x + 1) - unit;
+    if (left == 0) return r;
+  } else if (done > 0) {
+    return r;
+  }
+  const FlatPlace f = order.find(c, s, p, shape, unit);
+  if (f.b < 0) return r;
+  const int h = f.ht / f.tiles;
+  r.it = Item{f.b, h, f.ht - h * f.tiles, f.len};
+  r.pages = pages_of_length(f.len);
+  if (shape.even) {
+    r.page0 = f.at;
+    r.here = min(static_cast<int>(left), r.pages - f.at);
+    r.part = 2 * blockIdx.x + (done > 0 ? 1 : 0);   // (what lies between its first and its last item is whole)
+  } else {
+    const int each = r.pages / f.units, more = r.pages - each * f.units;   // the first `more` shares have one page more
+    r.page0 = f.at * each + min(f.at, more);
+    r.here = each + (f.at < more ? 1 : 0);
+    r.part = blockIdx.x;
+  }
+  return r;
+}
+
+// The parts of an item, `count` of them: `first`, then one every `step` from `next` on. One part alone is no part: its CTA has written the rows.
+struct ItemParts {
+  uint32_t first, next, step;
+  int count;
+  __device__ __forceinline__ uint32_t at(int k) const { return k == 0 ? first : next + (k - 1) * step; }
+};
+__device__ __forceinline__ ItemParts parts_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b, int h, int tile, int len, int n_queries) {
+  FlatOrder order;
+  order.look_up(c, s, p, shape);
+  const int tiles = (n_queries * shape.G + shape.item_rows - 1) / shape.item_rows;
+  const uint32_t units = tile < tiles ? order.units_of(len) : 0, first = order.before(c, s, p, shape, b) + (h * tiles + tile) * units;
+  if (units == 0) return ItemParts{0, 0, 0, 0};
+  if (!shape.even) return ItemParts{first, first + 1, 1, static_cast<int>(units)};
+  const uint32_t c0 = order.cta_of(first), c1 = order.cta_of(first + units - 1);
+  return ItemParts{2 * c0 + (order.start(c0) >= first ? 0 : 1), 2 * c0 + 2, 2, static_cast<int>(c1 - c0 + 1)};
+}
 
 // Reads a line of the kernel's parameters here and now. A first read takes as long as one of global memory, and longer once the loads of all CTAs are on
 // their way: ahead of the wait for the kernel before, it costs nothing.

@@ -12,7 +12,7 @@
 // A tile's chain is: K converted -> S -> softmax -> P V, and the next S directly behind P V. Barriers, each used once a tile:
 //   K   converters: K and the tile's record are there     S   S is complete (K is free)
 //   V   converters: V is there                            P   softmax: P is there         PV  P V is complete (V, P's columns and O are free)
-// Every wait is bounded. One that runs out is reported through status_mirror, and all roles end their item.
+// Every wait is bounded. One that runs out is reported through status_mirror, and all roles end.
 //
 // NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
 // token gets NaN there.
@@ -47,14 +47,6 @@ struct ChunkRows {
   int spans;               // some row looks for its own span
 };
 
-// The item in hand: pages page0 .. page0 + here - 1 of the `pages` that it has. In shared memory, as what finds it is: the roles need their registers (with 30 of them
-// taken here, the converters' loads were spilled, which waits for them).
-struct ChunkItem {
-  Item it;
-  int page0, pages, here;   // here < 0: there is none
-  int second;               // the CTA's second part (see AttnWorkspace)
-};
-
 template <int D>
 struct ChunkShared {
   static constexpr int BLOCKS = D > 64 ? 2 : 1, BLOCK = 128 * 128, TILE = BLOCKS * BLOCK;   // blocks of 64 head dims of 128 rows (16 KB: see koff_kmajor and desc_lo_mnmajor)
@@ -64,7 +56,7 @@ struct ChunkShared {
   float factor[KC_ROWS];
   RowMask mask[KC_ROWS];
   ChunkRows rows;
-  ChunkItem item;
+  ItemShare item;                    // in shared memory: the roles need their registers (with 30 of them taken, the converters' loads were spilled, which waits for them)
   uint64_t bar[5];
   uint32_t tmem, any_nan;
   int tiles;                         // of the pass
@@ -162,28 +154,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   };
   auto all_sync = [&]() { named_bar_sync(2, CH_THREADS); };   // (from the roles' own code)
   uint32_t done = 0;   // pages that this CTA has worked on
-  // The next item, its rows in shared memory; false: there is none. All threads.
+  // The CTA's next item, its rows in shared memory; false: it has none. All threads.
   auto open_item = [&]() -> bool {
     if (warp == 0) {
-      ChunkItem n;
-      n.here = -1;
-      n.second = done > 0 ? 1 : 0;
-      if (shape.ctas > 0) {
-        FlatOrder order;
-        order.look_up(c, s, p, shape);
-        if (blockIdx.x < order.ctas) {
-          const uint32_t at = order.start(blockIdx.x) + done, end = order.start(blockIdx.x + 1);
-          if (at < end) {
-            const FlatPlace f = order.find(c, s, p, shape, at);
-            const int h = f.ht / f.tiles;
-            const int pages = pages_of_length(f.len);
-            n = ChunkItem{Item{f.b, h, f.ht - h * f.tiles, f.len}, f.page, pages, min(static_cast<int>(end - at), pages - f.page), n.second};
-          }
-        }
-      } else if (done == 0) {
-        const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles, len = sequence_length(c, s, b), pages = pages_of_length(len);
-        n = ChunkItem{Item{b, h, ht - h * shape.tiles, len}, 0, pages, pages, 0};
-      }
+      const ItemShare n = share_of_cta(c, s, p, shape, done);
       if (lane == 0) sh.item = n;
     }
     all_sync();
@@ -383,7 +357,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (have) fetch(c.k);
         }
       } while (again(pass++));
-      if (sh.abort.v != 0u) break;
+      if (sh.abort.v != 0u || !shape.even) break;
     }
   } else {
     reg_alloc<CH_REGS_COMPUTE>();
@@ -523,7 +497,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         // ---- this row's output ----
         const int row = it.tile * KC_ROWS + tid;
         const bool live = mask.limit > 0, exists = row < shape.rows, whole = sh.item.here == sh.item.pages;
-        const size_t part = 2 * static_cast<size_t>(blockIdx.x) + sh.item.second;
+        const size_t part = sh.item.part;
         const int i = row / shape.G, hq = it.h * shape.G + row - i * shape.G;
         const float inv = !whole ? 1.f : live && sum != 0.f ? 1.f / sum : 0.f;
         bool bad = false;
@@ -562,7 +536,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           drain_wait(bar(CB_S), (n_t + u) & 1);
         }
       } while (again(pass++));
-      if (sh.abort.v != 0u) break;
+      if (sh.abort.v != 0u || !shape.even) break;
     }
   }
   tc_fence_before_sync();

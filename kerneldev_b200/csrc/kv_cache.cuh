@@ -13,12 +13,14 @@ constexpr int KC_PAGE = KD_CACHE_PAGE;
 constexpr int KC_EXP_MIN = -32, KC_EXP_MAX = 31;
 constexpr uint32_t KC_BAD_LENGTH = KD_STATUS_CACHE_RANGE | 1u, KC_BAD_PAGE = KD_STATUS_CACHE_RANGE | 2u;
 
-__device__ __forceinline__ void cache_report(const kd_cache& c, uint32_t code) {
-  if (c.status_mirror != nullptr) {
-    *const_cast<volatile uint32_t*>(c.status_mirror) = code;
+// (no part of the callers' code: they have it at every look-up)
+static __device__ __noinline__ void cache_report_to(uint32_t* mirror, uint32_t code) {
+  if (mirror != nullptr) {
+    *const_cast<volatile uint32_t*>(mirror) = code;
     __threadfence_system();
   }
 }
+__device__ __forceinline__ void cache_report(const kd_cache& c, uint32_t code) { cache_report_to(c.status_mirror, code); }
 
 // a count from device memory, clamped to 0 .. most
 __device__ __forceinline__ int checked_count(const kd_cache& c, int n, int most) {
