@@ -431,6 +431,7 @@ struct AttnShared {
     __device__ __forceinline__ float* o(int row) { return reinterpret_cast<float*>(stage + Stage<D>::BYTES) + row * (D + 4); }
   } warp[KA_WARPS];
   QueryTile<D, NT> q;
+  ItemShare next;
   float2 ml[KA_WARPS][ROWS];      // the warps' maxima and sums
   float scale[KA_WARPS][ROWS];    // what a warp's rows are multiplied with: all on one maximum, and divided by the sum where the item is whole
 };
@@ -447,18 +448,27 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   AttnShared<D, NT>& sh = *reinterpret_cast<AttnShared<D, NT>*>(smem);
   const Lane<D> place;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  ItemShare share = share_of_cta(c, s, p, shape, 0);
+  if (share.here < 0) return;
+  char* ring = sh.warp[warp].stage;
+  QueryLoad<D, NT> queries;
+  int first, last, next_page;
+  auto begin = [&]() {   // an item's first loads
+    first = 2 * share.page0 + warp;
+    last = min(2 * (share.page0 + share.here), (share.it.len + KA_UNIT - 1) / KA_UNIT);
+    queries.fetch(c, s, p, share.it, shape.G, shape.rows);
+    next_page = Walker<D, NT>::begin(c, s, place, share.it, first, last, ring);
+  };
+  begin();
 #pragma unroll 1
-  for (uint32_t done = 0;;) {
-    const ItemShare share = share_of_cta(c, s, p, shape, done);
-    if (share.here < 0) return;
+  for (uint32_t done = share.here;;) {
     const Item it = share.it;
-    const int first = 2 * share.page0 + warp, last = min(2 * (share.page0 + share.here), (it.len + KA_UNIT - 1) / KA_UNIT);
     const bool whole = share.here == share.pages;
-    char* ring = sh.warp[warp].stage;
-    QueryLoad<D, NT> queries;
-    queries.fetch(c, s, p, it, shape.G, shape.rows);
-    int next_page = Walker<D, NT>::begin(c, s, place, it, first, last, ring);
     queries.store(p, sh.q);
+    if (shape.even && warp == 0) {   // what comes next is looked up while this item's copies are on their way
+      const ItemShare next = share_of_cta(c, s, p, shape, done);
+      if (lane == 0) sh.next = next;
+    }
     Walker<D, NT> w;
     float* scores = shape.score_rows > 0 ? ws.scores + (static_cast<size_t>(it.b) * c.H + it.h) * s.blocks * KC_PAGE * shape.score_rows : nullptr;
     w.template walk<false>(c, s, place, it, sh.q, first, last, next_page, ring, scores, shape.score_rows);
@@ -477,8 +487,12 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int x = 0; x < 4; ++x) sh.warp[warp].o(n * KA_TILE + 2 * t + (x & 1))[Spread<D>::v_dim(2 * m + (x >> 1), g)] = w.o[n][m][x];
-    __syncthreads();
     const size_t part = share.part;
+    __syncthreads();
+    if (shape.even) {   // its first copies run while this one's rows are put together
+      share = sh.next;
+      if (share.here >= 0) begin();
+    }
     auto place_of_row = [&](int row, int& hq, int& i) {   // of the key head
       i = row / shape.G;
       hq = it.h * shape.G + row - i * shape.G;
@@ -529,7 +543,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
         *reinterpret_cast<float4*>(ws.part_o + (part * ROWS + r) * D + d) = v;
       }
     }
-    if (!shape.even) return;
+    if (!shape.even || share.here < 0) return;
     done += share.here;
     __syncthreads();   // shared memory is free for the next item
   }
@@ -820,9 +834,11 @@ static cudaError_t launch_weights(const kd_cache& c, const kd_cache_seqs& s, con
   if (!a.stats || groups == 0) return cudaSuccess;
   constexpr size_t kShared = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
   static SmemOptIn opt_in;
+  static SharedFirst shared_first;
   a.item_rows = NT * KA_TILE;
   a.tiles = (a.rows + a.item_rows - 1) / a.item_rows;
-  const cudaError_t e = opt_in(cache_weights_kernel<D, NT>, kShared);
+  cudaError_t e = opt_in(cache_weights_kernel<D, NT>, kShared);
+  if (e == cudaSuccess) e = shared_first(cache_weights_kernel<D, NT>);
   return e != cudaSuccess ? e : launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kShared, stream, c, s, p, a, ws);
 }
 
@@ -830,9 +846,11 @@ template <int D, int NT>
 static cudaError_t launch_rows(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
   constexpr size_t kShared = sizeof(AttnShared<D, NT>);
   static SmemOptIn opt_in;
-  const cudaError_t e = opt_in(cache_attention_kernel<D, NT>, kShared);
+  static SharedFirst shared_first;
+  cudaError_t e = opt_in(cache_attention_kernel<D, NT>, kShared);
+  if (e == cudaSuccess) e = shared_first(cache_attention_kernel<D, NT>);
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
-  return e != cudaSuccess ? e : launch(cache_attention_kernel<D, NT>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
+  return e != cudaSuccess ? e : launch_shares(a.ctas > 0 && a.even, cache_attention_kernel<D, NT>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), KA_THREADS, kShared, stream, c, s, p, a, ws);
 }
 
 template <int D>
@@ -852,6 +870,8 @@ static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_
   }
   if (a.score_rows > 0 && s.blocks > 0) {
     const int64_t groups = heads * ((static_cast<int64_t>(s.blocks) * KC_PAGE + KS_TOKENS - 1) / KS_TOKENS);
+    static SharedFirst shared_first;
+    if (e == cudaSuccess) e = shared_first(cache_join_weights_kernel);
     if (e == cudaSuccess) e = launch(cache_join_weights_kernel, static_cast<unsigned>(groups), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
     if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
     return 0;
@@ -859,6 +879,9 @@ static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_
   if (e == cudaSuccess && a.ctas > 0) {
     // (1024 CTAs for as many rows of two or three parts were two waves)
     const bool few = heads * a.rows <= 148 * 2;
+    static SharedFirst first_few, first_many;
+    e = few ? first_few(cache_join_kernel<KJ_WARPS>) : first_many(cache_join_kernel<1>);
+    if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_join_kernel attribute: %s", cudaGetErrorString(e));
     e = few ? launch(cache_join_kernel<KJ_WARPS>, static_cast<unsigned>(heads * a.rows), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
             : launch(cache_join_kernel<1>, static_cast<unsigned>(heads * ((a.rows + KJ_WARPS - 1) / KJ_WARPS)), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
   }

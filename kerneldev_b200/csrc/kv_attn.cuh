@@ -1,6 +1,9 @@
 // What the two kernels of the cache's attention share (kv_attn.cu: few query rows, kv_attn_chunk.cu: many): rows and their masks, how the pages
 // are shared out, the parts that a join puts together.
 #pragma once
+#include <atomic>
+#include <utility>
+
 #include "kv_cache.cuh"
 
 namespace kd {
@@ -230,6 +233,36 @@ __device__ __forceinline__ void touch_parameters(const kd_cache& c, const kd_cac
   touch(shape.G);
   touch(shape.least);
   touch(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ws.part_ml)));
+}
+
+// An SM divides its memory between L1 and shared memory anew only while it is idle, and beside the kernels before and behind it never is. So all kernels of a call
+// ask for the division that the large ones need, and one that counts on a place for every CTA (even pages) starts when the kernel before has left: on an SM that
+// never gets idle one CTA of 444 found no room until others ended, again and again, and 32 x 4096 tokens took 48 us in place of NNN.
+struct SharedFirst {
+  std::atomic<uint64_t> done{0};   // bit d: asked on device d
+  template <typename Kernel>
+  cudaError_t operator()(Kernel kernel) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
+
+// launch, without the early start where pages are shared evenly
+template <typename... P, typename... A>
+inline cudaError_t launch_shares(bool even, void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+  if (!even) return launch(kernel, grid, block, smem, stream, std::forward<A>(args)...);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
 // kv_attn_chunk.cu

@@ -551,9 +551,11 @@ static cudaError_t launch_chunk(const kd_cache& c, const kd_cache_seqs& s, const
   constexpr size_t kShared = sizeof(ChunkShared<D>);
   static_assert(kShared <= 113 * 1024, "two CTAs share an SM");
   static SmemOptIn opt_in;
-  const cudaError_t e = opt_in(cache_attention_chunk_kernel<D>, kShared);
+  static SharedFirst shared_first;
+  cudaError_t e = opt_in(cache_attention_chunk_kernel<D>, kShared);
+  if (e == cudaSuccess) e = shared_first(cache_attention_chunk_kernel<D>);
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
-  return e != cudaSuccess ? e : launch(cache_attention_chunk_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), CH_THREADS, kShared, stream, c, s, p, a, ws);
+  return e != cudaSuccess ? e : launch_shares(a.ctas > 0 && a.even, cache_attention_chunk_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), CH_THREADS, kShared, stream, c, s, p, a, ws);
 }
 
 int launch_attention_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
