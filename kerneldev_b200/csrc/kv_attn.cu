@@ -19,6 +19,8 @@
 //
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
 // taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs.
+#include <stdlib.h>
+
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -461,7 +463,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
   };
   begin();
 #pragma unroll 1
-  for (uint32_t done = share.here;;) {
+  for (uint32_t done = share.here;;) {   // (with even pages an item has at least one: `done` grows)
     const Item it = share.it;
     const bool whole = share.here == share.pages;
     queries.store(p, sh.q);
@@ -793,6 +795,10 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   AttnShape a;
   a.G = p.H / c.H;
   a.rows = a.G * p.T;
+#ifdef KD_TEST_DROP_LOAD
+  const char* drop = getenv("KD_TEST_DROP_LOAD");
+  a.test_drop = drop != nullptr ? atoi(drop) : 0;
+#endif
   const int rows = a.item_rows = rows_of_item(a.rows);
   a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
@@ -801,7 +807,7 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
   const int slots = 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
   a.ctas = s.blocks <= 8 || items > 148 * 16 || pages >= (1 << 30) ? 0 : slots;
-  a.even = items > slots / 2;   // see FlatOrder
+  a.even = a.ctas > 0 && items > slots / 2;   // see FlatOrder
   a.spread = a.even ? 1 : slots - static_cast<int>(items);
   a.least = rows == KC_ROWS ? 8 : 2;   // four tiles of 128 tokens; a unit for each warp
   return a;

@@ -27,6 +27,9 @@ struct AttnShape {
   int item_rows;        // query rows of an item
   int least;            // pages that such a CTA has at least
   bool stats;           // leave every row's maximum and sum for the weights
+#ifdef KD_TEST_DROP_LOAD
+  int test_drop;        // wait time-out test build: the converters of CTA 0 do not announce the first K (5) or V (6) tile
+#endif
   int score_rows;       // 0, or the rows of a key head rounded up to 2, 4 or 8: leave the scores too
 };
 // Workspace: the rows' statistics (float2 for each, with weights), then the parts (see FlatOrder): an item's rows of D floats, and their maxima and sums. With weights and

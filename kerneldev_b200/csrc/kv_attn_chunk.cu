@@ -344,6 +344,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           fence_proxy_async_smem();
           __syncwarp();
+#ifdef KD_TEST_DROP_LOAD
+          if (shape.test_drop == 5 && blockIdx.x == 0 && u == 0) {
+          } else
+#endif
           if (lane == 0) mbar_arrive(bar(CB_K));
           if (!have) break;
           fetch(c.v);
@@ -353,6 +357,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           else store_tile<D, false>(sh.v, place, reg, nullptr, col);
           fence_proxy_async_smem();
           __syncwarp();
+#ifdef KD_TEST_DROP_LOAD
+          if (shape.test_drop == 6 && blockIdx.x == 0 && u == 0) {
+          } else
+#endif
           if (lane == 0) mbar_arrive(bar(CB_V));
           if (have) fetch(c.k);
         }

@@ -288,6 +288,22 @@ def test_attention_does_not_read_what_is_masked(T, G):
     assert torch.isnan(o[0, ..., 3]).all() and torch.isfinite(o[0, ..., :3]).all() and torch.isfinite(o[0, ..., 4:]).all()
 
 
+@pytest.mark.parametrize("B,Hkv,G,T,D,meta", [(70, 2, 2, 1, 64, True), (300, 1, 8, 1, 32, False), (140, 4, 1, 3, 48, True), (300, 8, 1, 1, 16, False), (40, 8, 5, 8, 64, False),
+                                              (7, 1, 12, 3, 128, True)])
+def test_attention_many_sequences(B, Hkv, G, T, D, meta):
+    """More sequences than lanes, shares of few and of many heads, CTAs with several items, empty sequences and sequences without a query among them."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, 140, B)
+    lens[rng.integers(0, B, 3)] = [700, 641, 0]
+    q_lens = rng.integers(0, T + 1, B) if T > 1 else None
+    c, table = filled(rng, B, Hkv, D, lens, torch.float16, meta)
+    q = rand_kv(rng, (B, Hkv * G, T, D), torch.float16, False).to(DEV)
+    w = torch.zeros((B, Hkv, int(lens.max())), device=DEV)
+    got = cache_attention(q, c, i32(table), i32(lens), None if q_lens is None else i32(q_lens), return_lse=True, weights=w)
+    check_attention(c, q, table, lens, [T] * B if q_lens is None else q_lens, got, weights=w)
+
+
 def test_attention_scales_far_apart():
     """Blocks whose scales lie 2**40 apart, keys that make scores of hundreds, a block of zeros."""
     from kerneldev_b200 import cache_append, cache_attention
@@ -331,6 +347,9 @@ EVICTIONS = [
     (1, 48, [700], 64, 10, 20, "zeros"),
     (2, 96, [900, 901], 200, 0, 3, "odd"),
     (1, 32, [300], 100, 0, 0, "short"),
+    (2, 16, [4096, 4097, 9000], 1000, 100, 1, "ties"),       # one CTA of 256 threads, and clusters
+    (1, 16, [40000, 3], 30000, 5, 0, "spread"),              # clusters of larger CTAs
+    (1, 16, [131072 + 700], 70000, 64, 64, "ties"),          # keys beyond what stays in registers
 ]
 
 

@@ -164,3 +164,45 @@ def test_waits_do_not_run_while_the_kernel_ahead_does():
     env.pop("KD_CHECK_STATUS", None)
     r = subprocess.run([sys.executable, "-c", CHILD_EARLY_START % {"root": ROOT}], env=env, capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "no time-out" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+CHILD_CACHE = r"""
+import os, sys
+sys.path.insert(0, %(root)r)
+import torch
+from kerneldev_b200 import KVCache, _capi, cache_append, cache_attention, cache_read
+assert "waittest" in str(_capi.LIB_PATH)
+dev = "cuda:0"
+D, n, T = %(D)d, 700, 40
+g = torch.Generator().manual_seed(5)
+k, v, q = (torch.randn((1, 2, t, D), generator=g).to(torch.bfloat16).to(dev) for t in (n, n, T))
+c = KVCache.empty(12, 2, D, device=dev)
+table, lens = torch.arange(11, dtype=torch.int32, device=dev).view(1, 11), torch.tensor([n], dtype=torch.int32, device=dev)
+cache_append(c, k, v, table, torch.zeros_like(lens))
+os.environ["KD_TEST_DROP_LOAD"] = "0"
+good = cache_attention(q, c, table, lens)
+torch.cuda.synchronize()
+os.environ["KD_TEST_DROP_LOAD"] = "%(drop)d"
+cache_attention(q, c, table, lens)                     # returns: the failure is on the device
+torch.cuda.synchronize()                               # the kernel ended by itself
+os.environ["KD_TEST_DROP_LOAD"] = "0"
+try:
+    cache_read(c, table, lens, 1)                      # the next call with the cache raises, without a sync of its own
+    raise SystemExit("no exception")
+except RuntimeError as e:
+    assert "timed out" in str(e) and "0x9" in str(e), str(e)
+assert torch.equal(cache_attention(q, c, table, lens), good)   # reported once; the device is usable and correct
+print("unwound and recovered")
+"""
+
+
+@pytest.mark.parametrize("drop", [5, 6], ids=["K", "V"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_wait_timeout_in_the_cache_attention_of_many_rows(D, drop):
+    """The converters of one CTA do not announce their first K or V tile: the chain behind it times out, every role ends."""
+    from kerneldev_b200.build import build
+    lib = build(name="waittest", extra_flags=WAITTEST_FLAGS)
+    env = dict(os.environ, KD_LIB_PATH=str(lib))
+    env.pop("KD_CHECK_STATUS", None)
+    r = subprocess.run([sys.executable, "-c", CHILD_CACHE % {"root": ROOT, "D": D, "drop": drop}], env=env, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "unwound and recovered" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
