@@ -464,7 +464,7 @@ int kd_cache_attention_workspace(const kd_cache* c, const kd_cache_seqs* s, cons
 int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) {
   int rc = check_queries(c, s, q);
   if (rc) return rc;
-  if (!(q->sm_scale > 0.f) || q->sm_scale > 3.0e38f) return set_error(KD_ERR_ARG, "sm_scale must be positive and finite");
+  if (!(q->sm_scale > 0.f) || !(q->sm_scale < 1e30f)) return set_error(KD_ERR_ARG, "sm_scale must be positive and finite");
   if (s->B == 0 || q->T == 0) return 0;
   if ((rc = check_cache_strides(q->q, 2, "q")) != 0 || (rc = check_cache_strides(q->o, 2, "o")) != 0) return rc;
   if (q->weights && q->w_len < 0) return set_error(KD_ERR_ARG, "w_len is negative");

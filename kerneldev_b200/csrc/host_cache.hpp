@@ -41,7 +41,11 @@ struct KVCache {
   KVCache(const KVCache&) = delete;
   ~KVCache() { status_words().give_back(std::move(word)); }
 
+  // before a call's launch: what earlier ones reported, and whether the addresses still are the tensors' (storages can be resized or replaced)
   void poll() {
+    KD_VALUE(k.const_data_ptr() == abi.k && v.const_data_ptr() == abi.v && k_scale.const_data_ptr() == abi.k_scale && v_scale.const_data_ptr() == abi.v_scale &&
+                 (abi.desc == nullptr || desc->const_data_ptr() == abi.desc),
+             "the tensors of the cache have been given other memory: make a new KVCache of them");
     const uint32_t s = *status;
     if (s == 0) return;
     *status = 0;
@@ -176,7 +180,11 @@ std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const T
              "weights must be float32 (batch, cache heads, tokens) with unit stride along tokens");
     KD_VALUE(w.device() == c.k.device(), "weights must live on ", c.k.device());
     KD_VALUE(w.size(2) <= INT32_MAX, "weights has too many tokens");
-    KD_VALUE((B <= 1 || w.stride(0) > 0) && (c.abi.H <= 1 || w.stride(1) > 0), "weights must have memory of its own for every head");
+    // each head's tokens behind those of the one before, in either order of the two outer dimensions
+    const bool batch_first = B <= 1 || (c.abi.H > 1 && w.stride(0) >= w.stride(1));
+    const int64_t inner = batch_first ? c.abi.H : B, inner_stride = w.stride(batch_first ? 1 : 0), outer = batch_first ? B : c.abi.H, outer_stride = w.stride(batch_first ? 0 : 1);
+    KD_VALUE(w.numel() == 0 || ((inner <= 1 || inner_stride >= w.size(2)) && (outer <= 1 || outer_stride >= (inner <= 1 ? 0 : (inner - 1) * inner_stride) + w.size(2))),
+             "weights must have memory of its own for every head");
     TORCH_CHECK(!w.requires_grad() || !at::GradMode::is_enabled(), "weights is written in place and holds no history");
     p.weights = w.data_ptr<float>();
     p.w_stride_b = w.stride(0);

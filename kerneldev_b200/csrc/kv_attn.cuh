@@ -74,7 +74,7 @@ __device__ __forceinline__ void write_stats(const kd_cache_queries& p, const Att
   if (stats) ws.stats[row] = live && sum != 0.f ? make_float2(ref, __frcp_rn(sum)) : make_float2(0.f, 0.f);
 }
 
-// How the pages are shared out. An item is a sequence, a head and a tile of rows that has a query; `Units` of it are counted by a flat order: sequences in turn, each once for
+// How the pages are shared out. An item is a sequence, a head and a tile of rows that has a query. A flat order counts the units of all items: sequences in turn, each once for
 // every head and tile. Two ways:
 //   shares  an item of n pages goes to ceil(n / most) CTAs, evenly, and `most` is such that there are CTAs enough for all. A CTA has one item's pages alone.
 //           The way of few items in one wave of CTAs: their time is mostly latency, and a CTA with two items has it twice (16 x 1357 tokens of 4 heads, 5 queries: 15 us, 20 with even pages).
@@ -172,7 +172,7 @@ __device__ __forceinline__ ItemShare share_of_cta(const kd_cache& c, const kd_ca
     const int HT = c.H * shape.tiles, b = blockIdx.x / HT, ht = blockIdx.x - b * HT, h = ht / shape.tiles;
     r.it = Item{b, h, ht - h * shape.tiles, sequence_length(c, s, b)};
     r.page0 = 0;
-    r.pages = r.here = pages_of_length(r.it.len);
+    r.pages = r.here = p.q_lens != nullptr && r.it.tile * shape.item_rows >= query_count(c, p, b) * shape.G ? 0 : pages_of_length(r.it.len);   // (rows without a query: zeros)
     return r;
   }
   FlatOrder order;
@@ -240,7 +240,7 @@ __device__ __forceinline__ void touch_parameters(const kd_cache& c, const kd_cac
 
 // An SM divides its memory between L1 and shared memory anew only while it is idle, and beside the kernels before and behind it never is. So all kernels of a call
 // ask for the division that the large ones need, and one that counts on a place for every CTA (even pages) starts when the kernel before has left: on an SM that
-// never gets idle one CTA of 444 found no room until others ended, again and again, and 32 x 4096 tokens took 48 us in place of NNN.
+// never gets idle one CTA of 444 found no room until others ended, again and again, and 32 x 4096 tokens took 48 us in place of 42.
 struct SharedFirst {
   std::atomic<uint64_t> done{0};   // bit d: asked on device d
   template <typename Kernel>

@@ -386,6 +386,7 @@ cache_select_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ 
   }
   uint32_t all_stay = total[0];
   if (cluster > 1) {
+    if (wanted == 0u) cluster_sync();   // all have begun (the search has had its barriers)
     if (tid < cluster)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {   // into every CTA's table

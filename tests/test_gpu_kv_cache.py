@@ -350,6 +350,7 @@ EVICTIONS = [
     (2, 16, [4096, 4097, 9000], 1000, 100, 1, "ties"),       # one CTA of 256 threads, and clusters
     (1, 16, [40000, 3], 30000, 5, 0, "spread"),              # clusters of larger CTAs
     (1, 16, [131072 + 700], 70000, 64, 64, "ties"),          # keys beyond what stays in registers
+    (2, 16, [9000, 100, 5000], 5000, 3000, 2000, "spread"),  # clusters that have nothing to search for
 ]
 
 
@@ -657,6 +658,78 @@ def test_on_another_stream_and_host_thread():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not errors, errors
+
+
+@pytest.mark.parametrize("T,G", [(1, 3), (20, 4)])
+def test_sequences_that_share_pages_and_padding_that_is_nan(T, G):
+    """One table for all (a batch stride of zero) whose last page comes twice, queries of one head for all heads, rows without a query full of NaN, sequences
+    without any among them."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(40 + T)
+    c, table = filled(rng, 1, 2, 64, [200], torch.bfloat16, False)
+    B, rows = 3, np.array([table[0].tolist()[:3] + [table[0, 2]]] * 3)
+    shared = i32(rows[:1]).expand(B, 4)
+    q_lens = [T, 0, max(T // 2, 1)]
+    lens = [256, 192, 70]
+    one = rand_kv(rng, (B, 1, T, 64), torch.bfloat16, False).to(DEV)
+    for b in range(B):
+        one[b, :, q_lens[b]:] = float("nan")
+    q = one.expand(B, 2 * G, T, 64)
+    w = torch.zeros((2, B, 256), device=DEV).transpose(0, 1)
+    got = cache_attention(q, c, shared, i32(lens), i32(q_lens), return_lse=True, weights=w)
+    check_attention(c, q, rows, lens, q_lens, got, weights=w)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_two_graphs_of_one_cache_replayed_on_two_streams(T):
+    """Each has a workspace of its own, though both run at once."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(50 + T)
+    lens = [3000, 900]
+    c, table = filled(rng, 2, 2, 128, lens, torch.float16, False)
+    t, n = i32(table), i32(lens)
+    streams, graphs, qs, outs = [torch.cuda.Stream() for _ in range(2)], [], [], []
+    for i in range(2):
+        q = rand_kv(rng, (2, 8, T, 128), torch.float16, False).to(DEV)
+        cache_attention(q, c, t, n)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        w = torch.zeros((2, 2, 3000), device=DEV)
+        with torch.cuda.graph(g, stream=streams[i]):
+            w.zero_()
+            outs.append((cache_attention(q, c, t, n, return_lse=True, weights=w), w))
+        graphs.append(g)
+        qs.append(q)
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for q, (got, w) in zip(qs, outs):
+        check_attention(c, q, table, lens, [T, T], got, weights=w)
+
+
+def test_memory_that_is_not_the_calls_own_is_refused():
+    from kerneldev_b200 import KVCache, cache_append, cache_attention, cache_evict, cache_read
+    c = KVCache.empty(4, 2, 64, device=DEV)
+    q, k = torch.zeros((2, 4, 1, 64), dtype=torch.bfloat16, device=DEV), torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16, device=DEV)
+    t, n, wide = i32([[0], [1]]), i32([5, 6]), torch.zeros(1000, device=DEV)
+    for strides in ((0, 64, 1), (64, 0, 1), (100, 63, 1), (64, 100, 1), (128, 127, 1), (63, 128, 1)):   # heads or sequences over one another
+        with pytest.raises(ValueError, match="weights"):
+            cache_attention(q, c, t, n, weights=wide.as_strided((2, 2, 64), strides))
+    for strides in ((128, 64, 1), (64, 128, 1), (300, 70, 1)):
+        w = wide.zero_().as_strided((2, 2, 64), strides)
+        cache_attention(q, c, t, n, weights=w)
+        assert torch.allclose(w.sum(2), torch.full((2, 2), 2.0, device=DEV)) and float(wide.sum()) == pytest.approx(8.0)
+    w = torch.zeros((2, 2, 64), device=DEV)
+    old = c.k_scale.data
+    c.k_scale.data = old.clone()   # the cache would go on with the storage that this leaves
+    for f in (lambda: cache_attention(q, c, t, n), lambda: cache_append(c, k, k, t, n), lambda: cache_evict(c, t, n, w, t, 2), lambda: cache_read(c, t, n, 2)):
+        with pytest.raises(ValueError, match="other memory"):
+            f()
+    KVCache(c.k, c.v, c.k_scale, c.v_scale)
+    c.k_scale.data = old
+    cache_attention(q, c, t, n)
 
 
 def test_status_is_checked_after_every_call():
