@@ -694,26 +694,26 @@ cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_const
 }
 
 // weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
-// rows, so that nothing is added twice and the order is fixed; a CTA KW_PAGES pages of one head.
-constexpr int KW_PAGES = 8, KW_UNITS = 2 * KW_PAGES;
+// rows, so that nothing is added twice and the order is fixed; a CTA kPages pages of one head: 8, and 2 where those would be CTAs for less than half
+// of the SMs (8 x 2000 tokens of one head, 1024 rows: 203 us with 2, 301 with 8; 2 x 8192 tokens of 8 heads, 512 rows: 284 and 223: each CTA goes through all query rows). The queries of the next tile of rows are asked for before the tile in hand is worked on.
 template <int D>
 constexpr int KW_STAGE = Stage<D>::V_AT + KA_UNIT * 4;   // K and descriptors
-template <int D, int NT>
+template <int D, int NT, int kPages>
 __global__ void __launch_bounds__(KA_THREADS)
 cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                      const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
   touch_parameters(c, s, p, shape, ws);
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int MINE = KW_UNITS / KA_WARPS, ROWS = NT * KA_TILE;
+  constexpr int UNITS = 2 * kPages, MINE = UNITS / KA_WARPS, ROWS = NT * KA_TILE;
   extern __shared__ __align__(1024) char smem[];
   char* stages = smem + (threadIdx.x >> 5) * MINE * KW_STAGE<D>;
-  QueryTile<D, NT>& q = *reinterpret_cast<QueryTile<D, NT>*>(smem + KW_UNITS * KW_STAGE<D>);
+  QueryTile<D, NT>& q = *reinterpret_cast<QueryTile<D, NT>*>(smem + UNITS * KW_STAGE<D>);
   __shared__ float2 s_stat[ROWS];
   const Lane<D> place;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, groups = (s.blocks + KW_PAGES - 1) / KW_PAGES;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, groups = (s.blocks + kPages - 1) / kPages;
   uint32_t item = blockIdx.x;
-  const int first = static_cast<int>(item % static_cast<uint32_t>(groups)) * KW_UNITS + warp;
+  const int first = static_cast<int>(item % static_cast<uint32_t>(groups)) * UNITS + warp;
   item /= static_cast<uint32_t>(groups);
   Item it;
   it.h = static_cast<int>(item % static_cast<uint32_t>(c.H));
@@ -738,12 +738,15 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
     for (int x = 0; x < 4; ++x) sums[i][x] = 0.f;
   }
   cp_async_commit();
-  for (it.tile = 0; it.tile < shape.tiles; ++it.tile) {
-    QueryLoad<D, NT> queries;
-    queries.fetch(c, s, p, it, shape.G, shape.rows);
+  QueryLoad<D, NT> queries;
+  it.tile = 0;
+  queries.fetch(c, s, p, it, shape.G, shape.rows);
+  for (int tile = 0; tile < shape.tiles; ++tile) {
     queries.store(p, q);
+    it.tile = tile + 1;
+    if (it.tile < shape.tiles) queries.fetch(c, s, p, it, shape.G, shape.rows);
     if (tid < ROWS) {
-      const int r = it.tile * ROWS + tid, i = r / shape.G;
+      const int r = tile * ROWS + tid, i = r / shape.G;
       s_stat[tid] = r < shape.rows ? ws.stats[(static_cast<size_t>(it.b) * p.H + it.h * shape.G + r - i * shape.G) * p.T + i] : make_float2(0.f, 0.f);
     }
     cp_async_wait<0>();
@@ -787,7 +790,8 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
-// Rows of an item: as many tiles of eight as the rows fill, up to four; beyond CHUNK_FROM rows the items are those of the kernel for many rows.
+// Rows of an item: as many tiles of eight as the rows fill, up to four; beyond CHUNK_FROM rows the items are those of the kernel for many rows
+// (8 x 4096 tokens of 8 heads of 128: 32 rows take 35 us here and 71 there, 36 rows 45 there; here they would be two items that read the cache twice).
 constexpr int CHUNK_FROM = 32;
 static int rows_of_item(int rows) { return rows > CHUNK_FROM ? KC_ROWS : rows <= KA_TILE ? KA_TILE : rows <= 2 * KA_TILE ? 2 * KA_TILE : 4 * KA_TILE; }
 
@@ -834,18 +838,24 @@ size_t cache_attention_workspace(const kd_cache& c, const kd_cache_seqs& s, cons
 }
 
 // the weights from the rows' statistics
-template <int D, int NT>
-static cudaError_t launch_weights(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, AttnShape a, const AttnWorkspace& ws, cudaStream_t stream) {
-  const int64_t groups = static_cast<int64_t>(s.B) * c.H * ((s.blocks + KW_PAGES - 1) / KW_PAGES);
-  if (!a.stats || groups == 0) return cudaSuccess;
-  constexpr size_t kShared = KW_UNITS * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
+template <int D, int NT, int kPages>
+static cudaError_t launch_weights_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, AttnShape a, const AttnWorkspace& ws, cudaStream_t stream) {
+  const int64_t groups = static_cast<int64_t>(s.B) * c.H * ((s.blocks + kPages - 1) / kPages);
+  constexpr size_t kShared = 2 * kPages * KW_STAGE<D> + sizeof(QueryTile<D, NT>);
   static SmemOptIn opt_in;
   static SharedFirst shared_first;
   a.item_rows = NT * KA_TILE;
   a.tiles = (a.rows + a.item_rows - 1) / a.item_rows;
-  cudaError_t e = opt_in(cache_weights_kernel<D, NT>, kShared);
-  if (e == cudaSuccess) e = shared_first(cache_weights_kernel<D, NT>);
-  return e != cudaSuccess ? e : launch(cache_weights_kernel<D, NT>, static_cast<unsigned>(groups), KA_THREADS, kShared, stream, c, s, p, a, ws);
+  cudaError_t e = opt_in(cache_weights_kernel<D, NT, kPages>, kShared);
+  if (e == cudaSuccess) e = shared_first(cache_weights_kernel<D, NT, kPages>);
+  return e != cudaSuccess ? e : launch(cache_weights_kernel<D, NT, kPages>, static_cast<unsigned>(groups), KA_THREADS, kShared, stream, c, s, p, a, ws);
+}
+
+template <int D, int NT>
+static cudaError_t launch_weights(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
+  if (!a.stats || s.blocks == 0) return cudaSuccess;
+  const bool few = static_cast<int64_t>(s.B) * c.H * s.blocks < 148 / 2 * 8;
+  return few ? launch_weights_of<D, NT, 2>(c, s, p, a, ws, stream) : launch_weights_of<D, NT, 8>(c, s, p, a, ws, stream);
 }
 
 template <int D, int NT>
