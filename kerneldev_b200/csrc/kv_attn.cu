@@ -554,6 +554,8 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
 // One query row whose pages several CTAs shared: their parts on one scale, and its output. kGroups warps take the parts in turn (grp: this warp's number; with more than
 // one they are the whole CTA, and meet at barriers).
 constexpr int KJ_WARPS = 8;
+// A part whose row has seen nothing. NaN scores leave the maximum at -inf as well (no comparison with them holds), but make the sum NaN: such a part makes the row NaN.
+__device__ __forceinline__ bool empty_part(const float2& ml) { return ml.x == -INFINITY && ml.y == 0.f; }
 struct JoinShared {
   float4 o[KJ_WARPS][32];
   float2 ml[KJ_WARPS];
@@ -569,7 +571,7 @@ __device__ __forceinline__ void join_row(const kd_cache& c, const kd_cache_queri
     const size_t part = static_cast<size_t>(parts.at(k)) * shape.item_rows + r;
     const float2 ml = ws.part_ml[part];
     const float4 v = d < c.D ? *reinterpret_cast<const float4*>(ws.part_o + part * c.D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ml.x == -INFINITY) continue;
+    if (empty_part(ml)) continue;
     const float to = fmaxf(ref, ml.x), keep = ref == to ? 1.f : fast_exp2(ref - to), scale = ml.x == to ? 1.f : fast_exp2(ml.x - to);
     ref = to;
     sum = fmaf(ml.y, scale, sum * keep);
@@ -587,8 +589,8 @@ __device__ __forceinline__ void join_row(const kd_cache& c, const kd_cache_queri
       acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
-        if (sh->ml[k].x == -INFINITY) continue;
-        const float scale = fast_exp2(sh->ml[k].x - ref);
+        if (empty_part(sh->ml[k])) continue;
+        const float scale = fast_exp2(sh->ml[k].x - ref);   // (all maxima -inf: NaN, as the sums are then)
         const float4 v = sh->o[k][lane];
         sum = fmaf(sh->ml[k].y, scale, sum);
         acc = make_float4(fmaf(v.x, scale, acc.x), fmaf(v.y, scale, acc.y), fmaf(v.z, scale, acc.z), fmaf(v.w, scale, acc.w));
@@ -656,15 +658,15 @@ cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_const
       float ref = -INFINITY, sum = 0.f;
       for (int k = lane; k < parts.count; k += 32) {
         const float2 ml = ws.part_ml[static_cast<size_t>(parts.at(k)) * shape.item_rows + warp];
+        if (empty_part(ml)) continue;
         const float to = fmaxf(ref, ml.x);
-        if (to == -INFINITY) continue;
-        sum = sum * fast_exp2(ref - to) + ml.y * fast_exp2(ml.x - to);
+        sum = sum * fast_exp2(ref - to) + ml.y * fast_exp2(ml.x - to);   // (both maxima -inf: NaN, as the part's sum is then)
         ref = to;
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const float other = __shfl_xor_sync(0xffffffffu, ref, o), other_sum = __shfl_xor_sync(0xffffffffu, sum, o), to = fmaxf(ref, other);
-        if (to != -INFINITY) sum = sum * fast_exp2(ref - to) + other_sum * fast_exp2(other - to);
+        sum = to != -INFINITY ? sum * fast_exp2(ref - to) + other_sum * fast_exp2(other - to) : sum + other_sum;
         ref = to;
       }
       const bool live = i < n && len - n + i >= 0;
