@@ -12,10 +12,12 @@
 // queries become halves exactly, after a power of two for each row. (mma on e4m3 itself is made of conversions and products of halves on this
 // chip: with it, and queries in three e4m3 terms, a unit took 740 instructions in place of 510.)
 //
-// Scales. A page's K scale multiplies its scores. Its V scale 2^ev goes into the exponent, p' = 2^(s + ev - ref), where ref is the
-// running maximum of s + ev; then O = sum p' v / sum p' 2^-ev, and no product of its own is spent on it. The exponents differ by at most 63, which
-// leaves p' far from the bottom of a float. p' is kept below 2^(8 + 6): the maximum is followed only in steps of 6 or more (the accumulators are rescaled then), and the offset
-// of 8 keeps probabilities down to 2^-22 of the largest out of the half's subnormals: long tails keep their weight.
+// Scales. A page's K scale multiplies its scores. Its V scale 2^ev goes into the exponent, p' = 2^(s + ev - ref + 8), and no product of its own is spent on it:
+// O = sum p' v / sum p' 2^-ev. A half has 30 exponents for p', the scales of two pages may lie 63 apart, and what a page of small values brings must not
+// get lost beside a page that has one large number: its other channels may be all zeros. So ref follows the maximum of s + ev, in steps of 6 or more; the offset of 8 keeps
+// probabilities down to 2^-22 of the largest out of the half's subnormals, so that long tails keep their weight. And where a unit's scale is more than 2^4 below one that came before it, ref follows
+// the unit's own maximum down (below_reference): its largest p' is 2^-4 at least. What has been added up is rescaled by powers of two, exactly. A half is off by 2^-25 at most below 2^-14: in
+// probabilities that is 2^-28 of the row's largest, or 2^-20 of the unit's.
 //
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
 // taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs.
@@ -322,6 +324,7 @@ struct Walker {
     }
     const int32_t* table = s.table + it.b * s.table_stride;
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
+    int ev_top = KC_EXP_MIN;   // the largest so far
     char* stage = ring;
     for (int unit = first; unit < last; unit += KA_WARPS) {
       cp_async_wait<0>();
@@ -336,20 +339,22 @@ struct Walker {
       const int page = reinterpret_cast<const int*>(scale)[2], j0 = unit * KA_UNIT;
       const float ks = scale[0];
       const int ev = scale_exponent(scale[1]);
+      const bool apart = scales_apart(ev, ev, ev_top);
       float sc[NT][2][4];
       scores<D, NT>(at, place, q, sc);
       uint32_t p[2][NT][2], vis[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (page < 0 || j0 + KA_UNIT > free_end) mask_scores(sc[n], desc, j0, g, t, page < 0 ? 0 : it.len, &q.mask[n * KA_TILE]);
-        float k[2], add[2], shrink[2];
-        bool grown = false;
+        float k[2], add[2], high[2], old[2];
+        bool moves = false;
         if (NT == 1 && all_scores != nullptr && 2 * t < score_rows) {
           const float k0 = fmaxf(ks * q.factor[2 * t], KA_TINY), k1 = fmaxf(ks * q.factor[2 * t + 1], KA_TINY);
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             *reinterpret_cast<float2*>(all_scores + static_cast<size_t>(j0 + 8 * y + g) * score_rows + 2 * t) = make_float2(sc[n][y >> 1][2 * (y & 1)] * k0, sc[n][y >> 1][2 * (y & 1) + 1] * k1);
         }
+        auto set_add = [&](int x) { add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x]; };
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           k[x] = fmaxf(ks * q.factor[n * KA_TILE + 2 * t + x], KA_TINY);
@@ -358,16 +363,28 @@ struct Walker {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          top = fmaf(top, k[x], static_cast<float>(ev));
-          const bool up = top > ref[n][x] + KA_SLACK;
-          shrink[x] = up ? fast_exp2(ref[n][x] - top) : 1.f;
-          ref[n][x] = up ? top : ref[n][x];
-          grown = grown || up;
-          add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x];
+          high[x] = fmaf(top, k[x], static_cast<float>(ev));
+          old[x] = ref[n][x];
+          const bool up = above_reference(high[x], old[x]);
+          moves = moves || up;
+          ref[n][x] = up ? rintf(high[x]) : old[x];   // (ahead of the vote: the exponentials wait for it)
+          set_add(x);
         }
-        if (__any_sync(0xffffffffu, grown)) {
-          sum[n][0] *= shrink[0];
-          sum[n][1] *= shrink[1];
+        if (apart) moves = moves || below_reference(high[0], old[0]) || below_reference(high[1], old[1]);
+        if (__any_sync(0xffffffffu, moves)) {
+          float shrink[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float total = sum[n][x];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            if (apart && below_reference(high[x], old[x])) {
+              ref[n][x] = reference_below(high[x], old[x], total);
+              set_add(x);
+            }
+            shrink[x] = exp2_whole(old[x] - ref[n][x]);
+            sum[n][x] *= shrink[x];
+          }
 #pragma unroll
           for (int m = 0; m < D / 16; ++m)
 #pragma unroll

@@ -252,7 +252,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         // chain of loads (page, scale) stood between two tiles.
         const int32_t* table = s.table + it.b * s.table_stride;
         const int page0 = sh.item.page0, page_end = page0 + sh.item.here;
-        int next = page0, batch = page0, batch_page, raw_ahead = 0, batch_ev;
+        int next = page0, step = 2, batch = page0, batch_page, raw_ahead = 0, batch_ev;
         float batch_ks;
         auto ask = [&](int from) { return from + lane < page_end ? table[from + lane] : -1; };
         auto open_batch = [&](int from, int raw) {
@@ -264,12 +264,15 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           raw_ahead = ask(from + 32);
         };
         open_batch(page0, ask(page0));
-        // the descriptor of this thread's token of the tile at `next`, asked for when the tile before it was found
+        // The descriptor of this thread's token of the tile at `next`, asked for when the tile before it was found, and the tile's pages: two, or one where the V scales of
+        // two are too far apart for one reference of the exponents.
         uint32_t ahead_desc = 0u;
         auto peek = [&]() {
-          if (next - batch >= 32) open_batch(next, raw_ahead);
+          if (next - batch > 30) open_batch(next, next - batch == 32 ? raw_ahead : ask(next));
           const int p0 = __shfl_sync(0xffffffffu, batch_page, next - batch), p1 = __shfl_sync(0xffffffffu, batch_page, next - batch + 1), page = r < KC_PAGE ? p0 : p1;
-          const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0;
+          const int apart = __shfl_sync(0xffffffffu, batch_ev, next - batch) - __shfl_sync(0xffffffffu, batch_ev, next - batch + 1);
+          step = p0 >= 0 && p1 >= 0 && (apart < -KA_APART || apart > KA_APART) ? 1 : 2;
+          const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0 && r < KC_PAGE * step;
           ahead_desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
         };
         peek();
@@ -285,8 +288,11 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
               cur.ks[x] = __shfl_sync(0xffffffffu, batch_ks, next - batch + x);
               cur.ev[x] = __shfl_sync(0xffffffffu, batch_ev, next - batch + x);
             }
+            if (step == 1) cur.page[1] = -1;
+            if (cur.page[1] < 0) cur.ev[1] = cur.ev[0];   // (a page that is not there says nothing about scales)
+            if (cur.page[0] < 0) cur.ev[0] = cur.ev[1];
             const uint32_t ctx = __ballot_sync(0xffffffffu, (cur.desc & TD_CTX) != 0u);
-            next += 2;
+            next += step;
             if (!metadata) {
               if (cur.j0 >= rows.max_limit) return false;   // (the limits are no more than the length)
               peek();
@@ -395,6 +401,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           commit_uniform(bar(CB_PV));
         };
         float ref = -INFINITY, sum = 0.f;
+        int ev_top = KC_EXP_MIN;
         uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
         bool ok = true;
         int u = 0;
@@ -450,10 +457,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             top[page] = fmaxf(highest(x[0]), highest(x[1]));
           }
           const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
-          const bool up = high > ref + KA_SLACK;
-          if (__any_sync(0xffffffffu, up)) {
-            const float to = up ? high : ref, shrink = up ? fast_exp2(ref - to) : 1.f;
-            if (u > 0 && __any_sync(0xffffffffu, up && ref != -INFINITY)) {   // O is complete: its last product came before these scores
+          const bool up = above_reference(high, ref), down = scales_apart(min(ev[0], ev[1]), max(ev[0], ev[1]), ev_top) && below_reference(high, ref);
+          if (__any_sync(0xffffffffu, up || down)) {
+            const float to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref, shrink = exp2_whole(ref - to);
+            if (u > 0 && __any_sync(0xffffffffu, to != ref && ref != -INFINITY)) {   // O is complete: its last product came before these scores
 #pragma unroll 1
               for (int i = 0; i < D; i += 16) {
                 uint32_t y[16];

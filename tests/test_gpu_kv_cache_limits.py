@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_kv_cache import DEV, filled, i32, rand_kv
+from oracle import kv_cache_oracle as ko
+from tests.test_gpu_kv_cache import DEV, as_oracle, filled, i32, make_cache, rand_kv, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,93 @@ def test_share_whose_visible_keys_are_all_nan(B, Hkv, G, T, weigh):
         assert torch.equal(o[~hit], clean[0][~hit]) and torch.equal(lse[~hit], clean[1][~hit])
         if weigh:
             assert torch.isnan(w[b, Hkv - 1, :int(lens[b]) - T + 1]).all() and torch.isfinite(w[b, :Hkv - 1]).all() and torch.isfinite(w[:b]).all()
+
+
+def values_of(rng, B, Hkv, n, D, kind):
+    """Keys and values of which a page holds numbers of 2**38 and the next one of 2**-20; the large ones are few, so that in their page all other channels become zeros."""
+    x = rand_kv(rng, (2, B, Hkv, n, D), torch.float32, False)
+    if kind == "alternate":   # every second page has one large number, each in another channel
+        for page in range(1, n // 64, 2):
+            x[1, :, :, 64 * page + int(rng.integers(64)), int(rng.integers(D))] = 2.0 ** int(rng.integers(20, 38))
+        return x
+    for b in range(B):
+        for h in range(Hkv):
+            for at in rng.integers(0, 1100, 2 if kind == "two" else 1):
+                x[1, b, h, at, int(rng.integers(D))] = 2.0 ** int(rng.integers(10, 39))
+                if kind == "unlikely":   # a token of 2**-40 of the others' probability and a value that makes up for it
+                    x[0, b, h, at] = -80 * np.log(2.0) / D ** 0.5
+    if kind == "two":
+        x[1, :, :, 640:768] *= 2.0 ** -20
+    return x
+
+
+def check_causal(c, q, table, lens, o, lse, weights):
+    """Against the definition in 64 bits, without metadata. Tolerances as derived in test_gpu_kv_cache.py, and one term more: probabilities are rounded to halves, whose steps end at
+    2**-24. With M the row's largest p 2**ev (ev: the exponent of the page's V scale), P its largest p and m the largest p 2**ev of a page, the kernels bring a token's p 2**ev to a half after a
+    factor of at least 2**8 / (sqrt(2) M), and of 2**8 / (sqrt(2) 2**4 P 2**ev) or 2**-4 / (sqrt(2) m) (their reference is a whole number, hence the root): it is off by 2**-25 / factor, which is
+    sqrt(2) 2**-33 min(M, max(2**4 P 2**ev, 2**12 m)), times the stored number. A tile of many rows has two pages whose exponents are at most 4 apart: m of a page and its neighbours. Taken as 2**-32."""
+    want = as_oracle(c)
+    B, H, T, D = q.shape
+    Hkv = want["k"].shape[1]
+    G = H // Hkv
+    o, lse = o.double().cpu().numpy(), lse.double().cpu().numpy()
+    qs = q.double().cpu().numpy()
+    assert np.isfinite(o).all() and np.isfinite(lse).all()
+    for b in range(B):
+        n, pages = int(lens[b]), table[b, :-(-int(lens[b]) // 64)]
+        blocks = len(pages)
+        for h in range(Hkv):
+            k, v = ko.values(want, table[b], n, h, "k"), ko.values(want, table[b], n, h, "v")
+            scale = np.repeat(want["v_scale"][pages, h], 64)[:n]
+            total = np.zeros(n)
+            deltas = []
+            for g in range(G):
+                x = qs[b, h * G + g]
+                see = np.arange(n)[None] <= (n - T + np.arange(T))[:, None]
+                s = np.where(see, x @ k.T * D ** -0.5, -np.inf)
+                top = s.max(1, keepdims=True)
+                p = np.exp(s - top)
+                l = p.sum(1, keepdims=True)
+                p /= l
+                ref = p @ v
+                a = p @ np.abs(v)
+                mag = np.where(see, np.abs(x) @ np.abs(k).T, 0).max(1) * D ** -0.5
+                delta = 2.0 ** -21 * (mag * 1.5 + 2) + n * 2.0 ** -24
+                m = np.pad(p * scale, ((0, 0), (0, 64 * blocks - n))).reshape(T, blocks, 64).max(2)
+                near = np.abs(np.diff(np.log2(want["v_scale"][pages, h]))) <= 4   # page and next one
+                m = np.maximum(m, np.maximum(np.pad(np.where(near, m[:, :-1], 0), ((0, 0), (1, 0))), np.pad(np.where(near, m[:, 1:], 0), ((0, 0), (0, 1)))))
+                step = 2.0 ** -32 * np.minimum(m.max(1, keepdims=True), np.maximum(2.0 ** 12 * np.repeat(m, 64, axis=1)[:, :n], 2.0 ** 4 * p.max(1, keepdims=True) * scale))
+                floor = np.where(see, step, 0) @ np.abs(v / scale[:, None])
+                got = o[b, h * G + g]
+                tol = torch.finfo(q.dtype).eps / 2 * (np.abs(ref) + 0.01 * a) + a * (2.0 ** -11 + 2 * delta[:, None]) + floor + 2.0 ** -25
+                err = np.abs(got - ref)
+                assert (err <= tol).all(), f"O: {(err / tol).max()} of the tolerance at {b, h, g, np.unravel_index((err / tol).argmax(), err.shape)}"
+                rl = (top + np.log(l))[:, 0] / np.log(2.0)
+                assert (np.abs(lse[b, h * G + g] - rl) <= 2 * delta + 2.0 ** -22 * np.abs(rl)).all(), "LSE"
+                total += p.sum(0)
+                deltas.append(delta.max())
+            w = weights[b, h].double().cpu().numpy()
+            assert (np.abs(w[:n] - total) <= total * (3 * max(deltas) + G * T * 2.0 ** -24) + 1e-30).all() and not w[n:].any(), "weights"
+
+
+@pytest.mark.parametrize("B,Hkv,G,T", [(1, 1, 1, 1), *SHARED])
+@pytest.mark.parametrize("kind", ["one", "two", "unlikely", "alternate"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_far_apart(B, Hkv, G, T, kind, D):
+    """A page's large number takes nothing from the other channels, which the other pages alone have, whatever their scales. (bfloat16, whose range the outputs need.)"""
+    from kerneldev_b200 import cache_append, cache_attention
+    rng = np.random.default_rng(B + T)
+    n = 1300 if B > 1 else 500   # (one sequence: a short table, whose pages are not shared)
+    lens = rng.integers(n - 200, n, B)
+    pages = B * (-(-n // 64))
+    c = make_cache(pages, Hkv, D)
+    table = tables(rng, B, pages // B, pages)
+    x = values_of(rng, B, Hkv, max(n, 1100), D, kind)[:, :, :, :n]
+    cache_append(c, x[0].to(DEV), x[1].to(DEV), i32(table), i32(np.zeros(B)), i32(lens))
+    q = rand_kv(rng, (B, Hkv * G, T, D), torch.float32, False)
+    if kind == "unlikely":
+        q = 0.5 + 0.1 * q.clamp(-1, 1)   # about -40 bits with the key above
+    q = q.to(torch.bfloat16).to(DEV)
+    w = torch.zeros((B, Hkv, n), device=DEV)
+    o, lse = cache_attention(q, c, i32(table), i32(lens), return_lse=True, weights=w)
+    check_causal(c, q, table, lens, o, lse, w)
