@@ -29,7 +29,7 @@ struct AttnShape {
   int least;            // pages that such a CTA has at least
   bool stats;           // leave every row's maximum and sum for the weights
 #ifdef KD_TEST_DROP_LOAD
-  int test_drop;        // wait time-out test build: the converters of CTA 0 do not announce the first K (5) or V (6) tile
+  int test_drop;        // wait time-out test build: the converters of CTA 0 do not announce the first K (5) or V (6) tile, or one of their warps takes its second wait for S (7) or PV (8) as run out
 #endif
   int score_rows;       // 0, or the rows of a key head rounded up to 2, 4 or 8: leave the scores too
 };

@@ -12,7 +12,8 @@
 // A tile's chain is: K converted -> S -> softmax -> P V, and the next S directly behind P V. Barriers, each used once a tile:
 //   K   converters: K and the tile's record are there     S   S is complete (K is free)
 //   V   converters: V is there                            P   softmax: P is there         PV  P V is complete (V, P's columns and O are free)
-// Every wait is bounded. One that runs out is reported through status_mirror, and all roles end.
+// Every wait is bounded. One that runs out is reported through status_mirror, and all roles end. The converter warps meet at named barriers, which have no limit, to
+// exchange a tile's words: so they agree at the first of them whether all go on, and leave together.
 //
 // NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
 // token gets NaN there.
@@ -279,7 +280,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         // The next tile that some row sees, from `next` on. All four warps come to the same answer: the words are exchanged through the record that is to have them.
         auto find = [&](int slot) {
           ChunkRecord& rec = sh.record[slot];
-          while (next < page_end) {
+          for (bool first = true; next < page_end; first = false) {
             cur.j0 = next * KC_PAGE;
             cur.desc = ahead_desc;
 #pragma unroll
@@ -301,7 +302,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             }
             const uint32_t pre = __ballot_sync(0xffffffffu, (cur.desc & TD_PRE) != 0u), ins = __ballot_sync(0xffffffffu, (cur.desc & TD_INS) != 0u);
             peek();
-            named_bar_sync(1, 128);   // everyone has looked at the words of the tile before
+            if (!first) named_bar_sync(1, 128);   // everyone has looked at the words of the tile before, in this slot
             if (lane == 0) {
               rec.words[0][r >> 5] = pre;
               rec.words[1][r >> 5] = ctx;
@@ -329,12 +330,24 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             if (cur.page[x] >= 0 && (i >> 2) * 64 + col < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(base[x] + (i & 1) * 32 * D + (i >> 2) * 64));
           }
         };
+        // A wait of one warp can run out while another's is met: with metadata all hear of it at a barrier that every one of them comes to, before the next words are exchanged.
+        auto drop = [&](int which, int tile) {   // wait time-out test build: the first converter warp of CTA 0 takes the wait as one that has run out
+#ifdef KD_TEST_DROP_LOAD
+          if (shape.test_drop == which && blockIdx.x == 0 && warp == 4 && tile == 1) {
+            raise_abort(&sh.abort, CH_SITE | 1 << 4 | which);
+            return true;
+          }
+#endif
+          return false;
+        };
         int u = 0;   // tiles of this pass
         bool have = find(n_k % CH_RECORDS);
         if (have) fetch(c.k);
         for (;; ++u) {
           // (K's place and the record's slot are free when the scores of the tile before are complete; the slot of two tiles before by then, too)
-          if (u > 0 && !(ok = wait(CB_S, n_t + u - 1, 1))) break;
+          if (u > 0) ok = ok && !drop(7, u) && wait(CB_S, n_t + u - 1, 1);
+          if (metadata) ok = named_bar_all(1, 128, ok);
+          if (!ok) break;
           ChunkRecord& rec = sh.record[(n_k + u) % CH_RECORDS];
           if (r == 0) {
             rec.ks[0] = cur.ks[0];
@@ -358,7 +371,10 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (!have) break;
           fetch(c.v);
           have = find((n_k + u + 1) % CH_RECORDS);
-          if (u > 0 && !(ok = wait(CB_PV, n_t + u - 1, 1))) break;
+          if (u > 0 && (drop(8, u) || !(ok = wait(CB_PV, n_t + u - 1, 1)))) {
+            ok = false;
+            continue;   // (to the barrier)
+          }
           if (safe) store_tile<D, true>(sh.v, place, reg, sh.nan_bits + row0, col);
           else store_tile<D, false>(sh.v, place, reg, nullptr, col);
           fence_proxy_async_smem();

@@ -536,6 +536,12 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// the same, and whether every thread brought true
+__device__ __forceinline__ bool named_bar_all(uint32_t id, uint32_t nthreads, bool mine) {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %3, 0;\nbar.red.and.pred q, %1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"(id), "r"(nthreads), "r"(mine ? 1u : 0u) : "memory");
+  return r != 0u;
+}
 __device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

@@ -206,3 +206,18 @@ def test_wait_timeout_in_the_cache_attention_of_many_rows(D, drop):
     env.pop("KD_CHECK_STATUS", None)
     r = subprocess.run([sys.executable, "-c", CHILD_CACHE % {"root": ROOT, "D": D, "drop": drop}], env=env, capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "unwound and recovered" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+@pytest.mark.parametrize("meta", [True, False], ids=["metadata", "plain"])
+@pytest.mark.parametrize("drop", [7, 8], ids=["S", "PV"])
+def test_wait_of_one_converter_warp_runs_out_in_the_cache_attention_of_many_rows(drop, meta):
+    """One of the four warps takes a wait as run out that the others see met: none of them is left at a barrier that the others do not come to."""
+    from kerneldev_b200.build import build
+    lib = build(name="waittest", extra_flags=WAITTEST_FLAGS)
+    env = dict(os.environ, KD_LIB_PATH=str(lib))
+    env.pop("KD_CHECK_STATUS", None)
+    child = CHILD_CACHE % {"root": ROOT, "D": 64, "drop": drop}
+    if meta:
+        child = child.replace("KVCache.empty(12, 2, D, device=dev)", "KVCache.empty(12, 2, D, device=dev, metadata=True)")
+    r = subprocess.run([sys.executable, "-c", child], env=env, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "unwound and recovered" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
