@@ -304,7 +304,8 @@ typedef struct kd_cache_seqs {
 } kd_cache_seqs;
 
 /* New keys and values behind the lens[b] tokens that sequence b has. The caller adds n_new to lens. A block that holds tokens already keeps
- * its scale or gets a larger one; what it holds is then rounded again, which is exact but for subnormal numbers. */
+ * its scale or gets a larger one; what it holds is then rounded again, which is exact but for subnormal numbers. A sequence with lens[b] outside 0 .. 64 blocks or n_new[b]
+ * outside 0 .. T gets nothing; of tokens that the table has no pages for, those that fit are written. */
 typedef struct kd_cache_tokens {
   kd_tensor k, v;           /* (B, H, T, D); pointers and byte strides multiples of 16 */
   int32_t T, dtype;         /* KD_F16 / KD_BF16 / KD_F32 */

@@ -83,11 +83,15 @@ cache_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ 
   const int h = static_cast<int>(item % static_cast<uint32_t>(c.H));
   item /= static_cast<uint32_t>(c.H);
   const int w = static_cast<int>(item % static_cast<uint32_t>(W)), b = static_cast<int>(item / static_cast<uint32_t>(W));
-  const int len = sequence_length(c, s, b);
-  int n = t.n_new != nullptr ? checked_count(c, t.n_new[b], t.T) : t.T;
-  if (n > s.blocks * KC_PAGE - len) {
+  // A length or a number of tokens that cannot be says nothing of where to write: nothing is. (Clamped, as for reading, a negative length would open the first page anew.) What the
+  // table has no more pages for is left out.
+  const int len = s.lens[b], room = s.blocks * KC_PAGE;
+  int n = t.n_new != nullptr ? t.n_new[b] : t.T;
+  const bool valid = len >= 0 && len <= room && n >= 0 && n <= t.T;
+  if (!valid || n > room - len) {
     if (threadIdx.x == 0) cache_report(c, KC_BAD_LENGTH);
-    n = s.blocks * KC_PAGE - len;
+    if (!valid) return;
+    n = room - len;
   }
   const int block = len / KC_PAGE + w, base = block * KC_PAGE;
   if (base >= len + n || n == 0) return;

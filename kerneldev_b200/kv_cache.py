@@ -15,7 +15,7 @@ later keeps its scale or gets a larger one, and what it holds is rounded again: 
 Sequences. ``page_table`` int32 (batch, blocks) names the pages of every sequence in order, ``lens`` int32 (batch,) counts its tokens; both
 stay on the device, so that a step can be captured into a CUDA graph. Pages are the caller's to hand out. What the table holds behind a
 sequence's last block is not read. Sequences may share pages as long as none of them appends to one. A length that the table has no
-pages for, or a page that does not exist, is no fault: the excess is left out, and the next call with the cache raises ``ValueError``
+pages for, or a page that does not exist, is no fault: the excess is left out (``cache_append`` writes nothing to a sequence whose length or number of new tokens cannot be), and the next call with the cache raises ``ValueError``
 (with ``KD_CHECK_STATUS=1`` the same one, which then waits for the device).
 
 There is no backward: inputs that require gradients are refused unless gradients are off.

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import kv_cache_oracle as ko
-from tests.test_gpu_kv_cache import DEV, as_oracle, filled, i32, make_cache, rand_kv, tables
+from tests.test_gpu_kv_cache import DEV, as_oracle, assert_cache, check_attention, filled, i32, make_cache, rand_kv, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +157,82 @@ def test_values_far_apart(B, Hkv, G, T, kind, D):
     w = torch.zeros((B, Hkv, n), device=DEV)
     o, lse = cache_attention(q, c, i32(table), i32(lens), return_lse=True, weights=w)
     check_causal(c, q, table, lens, o, lse, w)
+
+
+# ---- lengths and pages that do not fit ----------------------------------------------------------------------------
+
+def appended(rng, c, T):
+    x = rand_kv(rng, (2, 3, 2, T, 64), torch.bfloat16).to(DEV)
+    m = rng.random((2, 3, T)) < 0.5
+    return x, dict(in_span=torch.tensor(m[0], device=DEV), is_prefix=torch.tensor(m[1], device=DEV))
+
+
+@pytest.mark.parametrize("lens,new", [([-1, 40, 0], None), ([-3, -2 ** 31, 2 ** 31 - 1], None), ([257, 256, 300], None), ([100, 64, 63], [-1, 5, -2 ** 31]), ([0, 0, 0], [71, 2 ** 31 - 1, 70]),
+                                      ([-70, 10, 10], [70, 70, 0]), ([230, 200, 255], None)])
+def test_append_of_lengths_that_cannot_be_changes_nothing(lens, new):
+    """A negative length, one beyond the table, a negative number of tokens, more than there are: bytes, scales and descriptors of that sequence stay, the other ones get their tokens. What
+    goes beyond the last page is cut."""
+    from kerneldev_b200 import cache_append
+    rng = np.random.default_rng(abs(lens[0]))
+    T = 70
+    c, table = filled(rng, 3, 2, 64, [256, 200, 100], torch.bfloat16, True)
+    want = as_oracle(c)
+    x, m = appended(rng, c, T)
+    n = [T] * 3 if new is None else new
+    valid = [0 <= a <= 256 and 0 <= b <= T for a, b in zip(lens, n)]
+    count = [min(b, 256 - a) if ok else 0 for a, b, ok in zip(lens, n, valid)]
+    with pytest.raises(ValueError, match="length"):
+        cache_append(c, x[0], x[1], i32(table), i32(lens), None if new is None else i32(new), **m)
+    d = ko.descriptors(m["in_span"].cpu().numpy(), np.zeros((3, T), int), m["is_prefix"].cpu().numpy())
+    ko.append(want, x[0].cpu().double().numpy(), x[1].cpu().double().numpy(), table, [a if ok else 0 for a, ok in zip(lens, valid)], count, d)
+    assert_cache(c, want)
+
+
+def test_calls_with_bad_lengths_and_pages_keep_what_is_valid(monkeypatch):
+    """Readers leave out what does not fit and nothing else; writers change no page but the ones that are named."""
+    from kerneldev_b200 import cache_append, cache_attention, cache_evict, cache_read
+    rng = np.random.default_rng(1)
+    c, table = filled(rng, 2, 2, 64, [250, 100], torch.bfloat16, False)
+    want = as_oracle(c)
+    q = rand_kv(rng, (2, 4, 1, 64), torch.bfloat16, False).to(DEV)
+    w = torch.tensor(rng.random((2, 2, 256)), dtype=torch.float32, device=DEV)
+    good, lens = i32(table), i32([250, 100])
+    free = [p for p in range(c.k.shape[0]) if p not in table]
+    index, kept_lens, kept = cache_evict(c, good, lens, w, i32([[free[0]], [free[1]]]), 64)
+    c.k.view(torch.uint8)[free] = 0x7F
+    c.v.view(torch.uint8)[free] = 0x7F
+    c.k_scale[free] = c.v_scale[free] = 2.0 ** 31
+    assert_cache(c, want)
+    k, v = cache_read(c, good, lens, 256)
+    monkeypatch.delenv("KD_CHECK_STATUS")
+
+    def reported(match):
+        torch.cuda.synchronize()
+        with pytest.raises(ValueError, match=match):
+            cache_read(c, good, lens, 1)
+        assert_cache(c, want)
+
+    wrong = table.copy()
+    wrong[0, 1], wrong[1, 0] = c.k.shape[0], -1
+    bk, bv = cache_read(c, i32(wrong), lens, 256)
+    reported("page number")
+    for got, full in ((bk, k), (bv, v)):
+        full = full.clone()
+        full[0, :, 64:128] = full[1, :, :64] = 0
+        assert torch.equal(got, full)
+    o, lse = cache_attention(q, c, i32(wrong), lens, return_lse=True)
+    reported("page number")
+    for b, pages, n in ((0, [table[0, i] for i in (0, 2, 3)], 186), (1, [table[1, 1]], 36)):   # the same tokens without the page: one query, which sees all
+        po, pl = cache_attention(q[b:b + 1], c, i32([pages]), i32([n]), return_lse=True)
+        assert torch.allclose(pl, lse[b:b + 1], atol=1e-5) and torch.allclose(po.float(), o[b:b + 1].float(), rtol=2.0 ** -7, atol=1e-3)
+    for bad, same in (([257, -1], [256, 0]), ([2 ** 31 - 1, 100], [256, 100])):
+        got = cache_attention(q, c, good, i32(bad), return_lse=True)
+        reported("length")
+        assert all(torch.equal(x, y) for x, y in zip(got, cache_attention(q, c, good, i32(same), return_lse=True)))
+    got = cache_evict(c, good, lens, w, i32([[-5], [2 ** 31 - 1]]), 64)
+    reported("page number")
+    assert all(torch.equal(x, y) for x, y in zip(got, (index, kept_lens, kept)))
+    x = rand_kv(rng, (2, 2, 2, 3, 64), torch.bfloat16).to(DEV)
+    cache_append(c, x[0], x[1], i32([[-1] * 4, [c.k.shape[0]] * 4]), lens)
+    reported("page number")
+    check_attention(c, q, table, [250, 100], [1, 1], cache_attention(q, c, good, lens, return_lse=True))
