@@ -311,7 +311,7 @@ typedef struct kd_cache_tokens {
   int32_t T, dtype;         /* KD_F16 / KD_BF16 / KD_F32 */
   const int32_t* n_new;     /* NULL: T, or (B) how many of the T are there */
   const uint8_t* in_span;   /* (B, T) as in kd_meta, for the T new tokens; NULL: none is. Read only with kd_cache.desc */
-  const int64_t* span_id;
+  const int64_t* span_id;   /* one that does not fit 24 signed bits is reported as KD_STATUS_SPAN_RANGE */
   const uint8_t* is_prefix;
   int64_t in_span_stride_b, span_id_stride_b, is_prefix_stride_b;
 } kd_cache_tokens;

@@ -1,7 +1,7 @@
 // Host path of the 8-bit key/value cache (part of host.cpp, which includes it): argument checks, allocations and calls.
 
-// A cache is the caller's tensors; its status word is a word of pinned memory that the kernels write when a length or a page number
-// does not fit, or a bounded wait gave up. The next call looks at it without a synchronisation.
+// A cache is the caller's tensors; its status word is a word of pinned memory that the kernels write when a length, a page number or
+// a span id does not fit, or a bounded wait gave up. The next call looks at it without a synchronisation.
 struct KVCache {
   Tensor k, v, k_scale, v_scale;
   OptTensor desc;
@@ -49,7 +49,7 @@ struct KVCache {
     const uint32_t s = *status;
     if (s == 0) return;
     *status = 0;
-    if ((s & kStatusTimeout) != 0) Plan::raise_status(s);
+    if ((s & (kStatusTimeout | kStatusSpanRange)) != 0) Plan::raise_status(s);
     KD_VALUE((s & 0xFu) != 1u, "an earlier call was given a sequence length, or a number of new tokens, outside what its page table holds");
     KD_VALUE(false, "an earlier call was given a page number outside the cache");
   }

@@ -148,6 +148,7 @@ cache_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ 
     const bool ins = t.in_span != nullptr && t.in_span[b * t.in_span_stride_b + i] != 0;
     const bool pre = t.is_prefix != nullptr && t.is_prefix[b * t.is_prefix_stride_b + i] != 0;
     const int64_t sid = t.span_id != nullptr ? t.span_id[b * t.span_id_stride_b + i] : 0;
+    if (span_id_out_of_range(sid)) cache_report(c, KD_STATUS_SPAN_RANGE);
     c.desc[at * KC_PAGE + threadIdx.x] = pack_token(ins, pre, sid, true);
   }
 }

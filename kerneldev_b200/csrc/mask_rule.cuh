@@ -32,6 +32,9 @@ __host__ __device__ __forceinline__ uint32_t sees_of_flags(uint32_t f) {
   return u;
 }
 
+// a span id that a descriptor cannot tell from another one
+__host__ __device__ __forceinline__ bool span_id_out_of_range(int64_t sid) { return sid >= (1 << 23) || sid < -(1 << 23); }
+
 __host__ __device__ __forceinline__ uint32_t pack_token(bool in_span, bool is_prefix, int64_t span_id,
                                                         bool alive) {
   if (!alive) return 0u;

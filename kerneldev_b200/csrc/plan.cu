@@ -10,7 +10,6 @@ namespace kd {
 // 1. pack: metadata -> descriptors + per-tile summaries
 // ---------------------------------------------------------------------------------------
 __device__ __forceinline__ int tokens_of(const kd_meta& m, int b) { return m.lens != nullptr ? min(m.lens[b], m.T) : m.T; }
-__device__ __forceinline__ bool out_of_range(int64_t sid) { return sid >= (1 << 23) || sid < -(1 << 23); }
 
 // descriptor of token t of a sequence of n_b tokens
 __device__ __forceinline__ uint32_t describe(const kd_meta& m, int b, int t, int n_b, bool& bad_id) {
@@ -20,7 +19,7 @@ __device__ __forceinline__ uint32_t describe(const kd_meta& m, int b, int t, int
   const bool ins = m.in_span ? (m.in_span[b * m.in_span_stride_b + t] != 0) : false;
   const bool pre = m.is_prefix ? (m.is_prefix[b * m.is_prefix_stride_b + t] != 0) : false;
   const int64_t sid = m.span_id ? m.span_id[b * m.span_id_stride_b + t] : 0;
-  bad_id = out_of_range(sid);
+  bad_id = span_id_out_of_range(sid);
   return pack_token(ins, pre, sid, true);
 }
 
@@ -274,7 +273,7 @@ __global__ void __launch_bounds__(PS_THREADS) plan_small_kernel(kd_meta m, PlanV
   bool any_bad = false;
   if (b == 0 && m.rules && m.span_id != nullptr)
     for (int s = 0; s < m.B; ++s)
-      for (int t = tid, n = tokens_of(m, s); t < n; t += PS_THREADS) any_bad |= out_of_range(m.span_id[s * m.span_id_stride_b + t]);
+      for (int t = tid, n = tokens_of(m, s); t < n; t += PS_THREADS) any_bad |= span_id_out_of_range(m.span_id[s * m.span_id_stride_b + t]);
   const bool bad = __syncthreads_or(any_bad) != 0;
   if (b == 0 && tid == 0) {
     *pv.status = 0u;

@@ -60,7 +60,7 @@ def cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, page_table: t
     k, v: (batch, cache heads, time, head_dim) float16, bfloat16 or float32, any strides. new_lens: int32 (batch,), how many of
     the ``time`` tokens a sequence really has (None: all); the rest, and every slot behind them in a block that held tokens, stays as
     it was. in_span / is_prefix bool and span_id int64 (batch, time): the new tokens' metadata as for ``flash_attention`` (a missing one
-    is all zeros), for a cache with ``desc``."""
+    is all zeros; a span_id beyond 24 signed bits is reported as a bad length is), for a cache with ``desc``."""
     _ext.cache_append(cache._core, k, v, page_table, lens, new_lens, in_span, span_id, is_prefix)
 
 

@@ -236,3 +236,20 @@ def test_calls_with_bad_lengths_and_pages_keep_what_is_valid(monkeypatch):
     cache_append(c, x[0], x[1], i32([[-1] * 4, [c.k.shape[0]] * 4]), lens)
     reported("page number")
     check_attention(c, q, table, [250, 100], [1, 1], cache_attention(q, c, good, lens, return_lse=True))
+
+
+@pytest.mark.parametrize("sid", [2 ** 23, -2 ** 23 - 1, 2 ** 24 + 1, -2 ** 63])
+def test_span_ids_that_a_descriptor_cannot_hold_are_reported(sid):
+    """Two ids that agree in their low 24 bits would see one another; the ones at the ends of the range are well, and so is a wrong one behind the new tokens."""
+    from kerneldev_b200 import KVCache, cache_append
+    c = KVCache.empty(3, 2, 64, device=DEV, metadata=True)
+    k = torch.zeros((2, 2, 70, 64), dtype=torch.bfloat16, device=DEV)
+    t, n = i32([[0, 1], [2, 2]]), i32([0, 0])
+    ins = torch.ones((2, 70), dtype=torch.bool, device=DEV)
+    ids = torch.full((2, 70), 2 ** 23 - 1, dtype=torch.int64, device=DEV)
+    ids[0, 3] = -2 ** 23
+    ids[1, 9] = sid
+    cache_append(c, k, k, t, n, i32([70, 9]), in_span=ins, span_id=ids)
+    with pytest.raises(ValueError, match="24 signed bits"):
+        cache_append(c, k, k, t, n, i32([70, 10]), in_span=ins, span_id=ids)
+    cache_append(c, k, k, t, n, i32([70, 9]), in_span=ins, span_id=ids)   # reported once
