@@ -289,7 +289,7 @@ int kd_cocktail_grad(const kd_cocktail* p, void* stream);
 typedef struct kd_cache {
   void *k, *v;              /* e4m3 (pages, H, KD_CACHE_PAGE, D) contiguous, 16-byte aligned */
   float *k_scale, *v_scale; /* (pages, H) contiguous */
-  uint32_t* desc;           /* NULL: no metadata, or (pages, H, KD_CACHE_PAGE) token descriptors: bit 0 prefix, 1 context, 2 in a span, 3 [MASKQ], 4 same-span
+  uint32_t* desc;           /* NULL: no metadata, or (pages, H, KD_CACHE_PAGE) token descriptors, contiguous, 16-byte aligned: bit 0 prefix, 1 context, 2 in a span, 3 [MASKQ], 4 same-span
                                rule armed, 5..7 the key classes (prefix, context, span) that the token sees as a query wherever they are, 8.. the span
                                id's low 24 bits */
   int32_t pages, H, D;      /* H key/value heads; D a multiple of 16 from 16 to 128 */

@@ -392,7 +392,8 @@ static int check_cache(const kd_cache* c, const kd_cache_seqs* s) {
   if (c->pages < 1 || c->H < 1) return set_error(KD_ERR_ARG, "bad cache shape pages=%d H=%d", c->pages, c->H);
   if (c->D < 16 || c->D > 128 || c->D % 16 != 0) return set_error(KD_ERR_ARG, "head dim %d not supported (a multiple of 16 from 16 to 128)", c->D);
   if (!c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(KD_ERR_ARG, "k / v / k_scale / v_scale is null");
-  if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) != 0) return set_error(KD_ERR_ALIGN, "k / v not 16-byte aligned");
+  if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->desc)) & 15u) != 0)
+    return set_error(KD_ERR_ALIGN, "k / v / desc not 16-byte aligned");   // (a null desc is)
   if (s->B < 0 || s->blocks < 0) return set_error(KD_ERR_ARG, "bad shape B=%d blocks=%d", s->B, s->blocks);
   if (s->blocks > (1 << 24)) return set_error(KD_ERR_LIMIT, "blocks=%d exceeds 2^24", s->blocks);
   if (s->B > 0 && !s->lens) return set_error(KD_ERR_ARG, "lens is null");

@@ -81,6 +81,21 @@ def test_entry_points_reject_bad_arguments_before_touching_cuda():
     assert lib.kd_cache_read(ref(c), ref(s), None, 1, m.KD_F16, None, None, None) == 0
 
 
+def test_entry_points_reject_descriptors_that_16_byte_copies_cannot_read():
+    m, lib, c, s = _cache()
+    ref = ctypes.byref
+    t, q, e, n = m.KdCacheTokens(), m.KdCacheQueries(), m.KdCacheEviction(), ctypes.c_size_t()
+    t.T, t.dtype = 0, m.KD_BF16
+    q.H, q.T, q.dtype, q.sm_scale = 2, 0, m.KD_F16, 1.0
+    e.keep = 1
+    s.B = 0   # nothing to do, were it not for desc
+    for offset, code in ((0, 0), (4, -2), (8, -2), (12, -2), (16, 0)):
+        c.desc = 0x10000 + offset
+        for rc in (lib.kd_cache_append(ref(c), ref(s), ref(t), None), lib.kd_cache_attention(ref(c), ref(s), ref(q), None), lib.kd_cache_evict(ref(c), ref(s), ref(e), None),
+                   lib.kd_cache_attention_workspace(ref(c), ref(s), ref(q), ref(n)), lib.kd_cache_read(ref(c), ref(s), None, 0, m.KD_F16, None, None, None)):
+            assert rc == code and (rc == 0 or b"desc" in lib.kd_last_error())
+
+
 def test_cache_has_no_cpu_path():
     from kerneldev_b200 import KVCache
     with pytest.raises(RuntimeError, match="no CPU path"):
