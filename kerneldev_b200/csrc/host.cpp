@@ -171,17 +171,19 @@ struct Capture {
   }
 };
 
+// A status word's copy in host memory, to which kernels write.
+struct StatusMirror {
+  StatusWords::Word word = status_words().take();
+  volatile uint32_t* const at = reinterpret_cast<volatile uint32_t*>(word.first.data_ptr<int32_t>() + word.second);
+  ~StatusMirror() { status_words().give_back(std::move(word)); }
+};
+
 struct Plan {
   int64_t B, T;
   at::Device device;
   kd_plan_layout layout;
   Tensor buf;
-  struct Mirror {                  // the status word's copy in host memory
-    StatusWords::Word word = status_words().take();
-    volatile uint32_t* const at = reinterpret_cast<volatile uint32_t*>(word.first.data_ptr<int32_t>() + word.second);
-    ~Mirror() { status_words().give_back(std::move(word)); }
-  };
-  std::shared_ptr<Mirror> mirror = std::make_shared<Mirror>();   // (the cache looks at those of plans that it has dropped)
+  std::shared_ptr<StatusMirror> mirror = std::make_shared<StatusMirror>();   // (the cache looks at those of plans that it has dropped)
   volatile uint32_t* host_word = mirror->at;
   // the status word and its mirror as tensors: views cost more than a launch, and only reports and tests want them
   Tensor status_dev() const { return buf.narrow(0, static_cast<int64_t>(layout.off_status), 4).view(at::kInt); }
@@ -302,26 +304,26 @@ struct Plan {
 };
 using PlanPtr = std::shared_ptr<Plan>;
 
-// Plans that graphs have let go of. The driver runs a graph's destructors on a thread of its own, where no CUDA call may be made, and a plan
-// that goes frees memory and an event: the next look-up of a plan does.
+// Plans and status words that graphs have let go of. The driver runs a graph's destructors on a thread of its own, where no CUDA call may be made, and a plan
+// that goes frees memory and an event: the next look-up of a plan, or call with a key/value cache, does.
 class LetGo {
  public:
-  void add(PlanPtr plan) {
+  void add(std::shared_ptr<void> held) {
     std::lock_guard<std::mutex> lock(m_);
-    plans_.push_back(std::move(plan));
+    held_.push_back(std::move(held));
     any_.store(true);
   }
   void clear() {
     if (!any_.load()) return;
-    std::vector<PlanPtr> gone;   // destroyed after the lock is released
+    std::vector<std::shared_ptr<void>> gone;   // destroyed after the lock is released
     std::lock_guard<std::mutex> lock(m_);
-    gone.swap(plans_);
+    gone.swap(held_);
     any_.store(false);
   }
 
  private:
   std::mutex m_;
-  std::vector<PlanPtr> plans_;
+  std::vector<std::shared_ptr<void>> held_;
   std::atomic<bool> any_{false};
 };
 LetGo& let_go() {
@@ -329,20 +331,21 @@ LetGo& let_go() {
   return *l;
 }
 
-// A captured launch has the plan's address and nothing else, and the cache may drop the plan: the graph keeps it, as do the graphs made from it.
-void hold_for_graph(const PlanPtr& plan, const Capture& capture) {
-  if (capture.graph == nullptr || plan->held_by.load() == capture.id) return;
-  auto held = std::make_unique<PlanPtr>(plan);
+// A captured launch has the address of a plan, or of a status word, and nothing else, and its owner may drop it: the graph keeps it, as do the graphs made from it.
+// held_by: the last capture whose graph has been given it.
+void hold_for_graph(std::shared_ptr<void> what, std::atomic<unsigned long long>& held_by, const Capture& capture) {
+  if (capture.graph == nullptr || held_by.load() == capture.id) return;
+  auto held = std::make_unique<std::shared_ptr<void>>(std::move(what));
   cudaUserObject_t object;
   C10_CUDA_CHECK(cudaUserObjectCreate(&object, held.get(), [](void* p) {
-    std::unique_ptr<PlanPtr> h(static_cast<PlanPtr*>(p));
+    std::unique_ptr<std::shared_ptr<void>> h(static_cast<std::shared_ptr<void>*>(p));
     let_go().add(std::move(*h));
   }, 1, cudaUserObjectNoDestructorSync));
   held.release();
   const cudaError_t e = cudaGraphRetainUserObject(capture.graph, object, 1, cudaGraphUserObjectMove);
   if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
   C10_CUDA_CHECK(e);
-  plan->held_by.store(capture.id);
+  held_by.store(capture.id);
 }
 
 // The cache key: identity, version and geometry of the metadata tensors (the plan keeps their memory alive, so an address
@@ -438,7 +441,7 @@ class PlanCache {
   std::mutex m_;
   size_t bytes_ = 0;   // of the plans in the cache
   Entries order_;   // least recently used first
-  std::deque<std::shared_ptr<Plan::Mirror>> dropped_;   // status words of the last kSize plans that left for others
+  std::deque<std::shared_ptr<StatusMirror>> dropped_;   // status words of the last kSize plans that left for others
   std::unordered_map<PlanKey, Entries::iterator, PlanKeyHash> map_;
 };
 PlanCache& cache() {
@@ -537,7 +540,7 @@ std::tuple<Tensor, Tensor> forward(const Tensor& q_, const Tensor& k_, const Ten
   c10::cuda::CUDAGuard guard(q.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture(stream);
-  hold_for_graph(plan, capture);
+  hold_for_graph(plan, plan->held_by, capture);
   p.plan_ready = plan->ready_on(stream, capture) ? 1 : 0;
   check(o32 != nullptr ? lib.attn_fwd_f32(&p, &f, stream) : lib.attn_fwd(&p, stream));
   plan->launched_on(stream, capture);
@@ -587,7 +590,7 @@ std::tuple<Tensor, Tensor, Tensor> backward(const Tensor& q_, const Tensor& k_, 
   c10::cuda::CUDAGuard guard(q.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture(stream);
-  hold_for_graph(plan, capture);
+  hold_for_graph(plan, plan->held_by, capture);
   p.plan_ready = plan->ready_on(stream, capture) ? 1 : 0;
   check(f32 ? lib.attn_bwd_f32(&p, &f, stream) : signs != nullptr ? lib.attn_bwd_hadamard(&p, signs, stream) : lib.attn_bwd(&p, stream));
   plan->after_launch();

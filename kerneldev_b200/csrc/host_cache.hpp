@@ -5,8 +5,8 @@
 struct KVCache {
   Tensor k, v, k_scale, v_scale;
   OptTensor desc;
-  StatusWords::Word word;
-  volatile uint32_t* status = nullptr;
+  std::shared_ptr<StatusMirror> mirror;
+  std::atomic<unsigned long long> held_by{0};   // the last capture whose graph has been given the mirror to hold
   kd_cache abi{};
 
   KVCache(const Tensor& k_, const Tensor& v_, const Tensor& ks, const Tensor& vs, const OptTensor& d) : k(k_), v(v_), k_scale(ks), v_scale(vs), desc(d) {
@@ -26,8 +26,7 @@ struct KVCache {
       KD_VALUE(t->device() == k.device(), "the tensors of a cache must be on one device");
       KD_VALUE(t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "the tensors of a cache must be contiguous and 16-byte aligned");
     }
-    word = status_words().take();
-    status = reinterpret_cast<volatile uint32_t*>(word.first.data_ptr<int32_t>() + word.second);
+    mirror = std::make_shared<StatusMirror>();
     abi.k = k.data_ptr();
     abi.v = v.data_ptr();
     abi.k_scale = k_scale.data_ptr<float>();
@@ -36,25 +35,31 @@ struct KVCache {
     abi.pages = static_cast<int32_t>(P);
     abi.H = static_cast<int32_t>(H);
     abi.D = static_cast<int32_t>(D);
-    abi.status_mirror = const_cast<uint32_t*>(status);
+    abi.status_mirror = const_cast<uint32_t*>(mirror->at);
   }
   KVCache(const KVCache&) = delete;
-  ~KVCache() { status_words().give_back(std::move(word)); }
 
   // before a call's launch: what earlier ones reported, and whether the addresses still are the tensors' (storages can be resized or replaced)
   void poll() {
     KD_VALUE(k.const_data_ptr() == abi.k && v.const_data_ptr() == abi.v && k_scale.const_data_ptr() == abi.k_scale && v_scale.const_data_ptr() == abi.v_scale &&
                  (abi.desc == nullptr || desc->const_data_ptr() == abi.desc),
              "the tensors of the cache have been given other memory: make a new KVCache of them");
-    const uint32_t s = *status;
+    const uint32_t s = *mirror->at;
     if (s == 0) return;
-    *status = 0;
+    *mirror->at = 0;
     if ((s & (kStatusTimeout | kStatusSpanRange)) != 0) Plan::raise_status(s);
     KD_VALUE((s & 0xFu) != 1u, "an earlier call was given a sequence length, or a number of new tokens, outside what its page table holds");
     KD_VALUE(false, "an earlier call was given a page number outside the cache");
   }
-  void after_launch(cudaStream_t stream) {
-    if (!check_every_launch() || Capture(stream).active) return;
+  // A captured launch writes to the status word at every replay, whatever has become of this handle.
+  Capture before_launch(cudaStream_t stream) {
+    const Capture capture(stream);
+    hold_for_graph(mirror, held_by, capture);
+    let_go().clear();
+    return capture;
+  }
+  void after_launch(cudaStream_t stream, const Capture& capture) {
+    if (!check_every_launch() || capture.active) return;
     C10_CUDA_CHECK(cudaStreamSynchronize(stream));
     poll();
   }
@@ -146,8 +151,9 @@ void cache_append(KVCache& c, const Tensor& k_, const Tensor& v_, const Tensor& 
   c.poll();
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const Capture capture = c.before_launch(stream);
   check(lib.cache_append(&c.abi, &s.abi, &t, stream));
-  c.after_launch(stream);
+  c.after_launch(stream, capture);
 }
 
 std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const Tensor& table, const Tensor& lens, const OptTensor& q_lens,
@@ -204,9 +210,10 @@ std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const T
   }
   c.poll();
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const Capture capture = c.before_launch(stream);
   check(lib.cache_attention(&c.abi, &s.abi, &p, stream));
   if (!out.is_same(o)) o.copy_(out);
-  c.after_launch(stream);
+  c.after_launch(stream, capture);
   return {o, return_lse ? lse : Tensor()};
 }
 
@@ -240,8 +247,9 @@ std::tuple<Tensor, Tensor, Tensor> cache_evict(KVCache& c, const Tensor& table, 
   c.poll();
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const Capture capture = c.before_launch(stream);
   check(lib.cache_evict(&c.abi, &s.abi, &e, stream));
-  c.after_launch(stream);
+  c.after_launch(stream, capture);
   return {index, out_lens, out_w};
 }
 
@@ -260,7 +268,8 @@ std::tuple<Tensor, Tensor> cache_read(KVCache& c, const Tensor& table, const Ten
   c.poll();
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const Capture capture = c.before_launch(stream);
   check(lib.cache_read(&c.abi, &s.abi, from, static_cast<int32_t>(count), dtype_code(type), &kt, &vt, stream));
-  c.after_launch(stream);
+  c.after_launch(stream, capture);
   return {k, v};
 }

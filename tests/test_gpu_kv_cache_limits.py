@@ -253,3 +253,36 @@ def test_span_ids_that_a_descriptor_cannot_hold_are_reported(sid):
     with pytest.raises(ValueError, match="24 signed bits"):
         cache_append(c, k, k, t, n, i32([70, 10]), in_span=ins, span_id=ids)
     cache_append(c, k, k, t, n, i32([70, 9]), in_span=ins, span_id=ids)   # reported once
+
+
+def test_a_graph_keeps_the_status_word_of_its_cache(monkeypatch):
+    """A replay reports into the word that the capture has seen. The cache is gone, and as many others have come as there are words: none of them, and no plan, hears of it."""
+    from kerneldev_b200 import KVCache, cache_append, cache_read
+    monkeypatch.delenv("KD_CHECK_STATUS", raising=False)
+    c = KVCache.empty(2, 1, 64, device=DEV)
+    tensors = (c.k, c.v, c.k_scale, c.v_scale)
+    x = torch.zeros((1, 1, 1, 64), dtype=torch.float16, device=DEV)
+    t, lens, outs = i32([[0]]), i32([3]), []
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):   # two captures in turn, and a call outside between them
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            cache_append(c, x, x, t, lens)
+            outs.append(cache_read(c, t, lens, 4))
+        graphs.append(g)
+        cache_append(c, x, x, t, lens)
+    del c
+    others = [KVCache(*tensors) for _ in range(2100)]
+    lens.fill_(-1)
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for o in others:
+        cache_read(o, t, lens, 0)   # looks at the word and launches nothing
+    del graphs, g
+    torch.cuda.synchronize()
+    lens.fill_(3)
+    others.append(KVCache(*tensors))
+    cache_append(others[-1], x, x, t, lens)
+    cache_read(others[0], t, lens, 1)
