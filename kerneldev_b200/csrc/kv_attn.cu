@@ -639,7 +639,7 @@ cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd
   __shared__ JoinShared sh;
   const int warp = threadIdx.x >> 5, per_head = (shape.rows + ROWS - 1) / ROWS;
   const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + warp / kGroups;
-  const int len = sequence_length(c, s, b), n = query_count(c, p, b);
+  const int len = sequence_length<true>(c, s, b), n = query_count<true>(c, p, b);
   const ItemParts parts = parts_of(c, s, p, shape, b, h, row_of_head / shape.item_rows, len, n);
   pdl_wait();
   pdl_launch_dependents();
@@ -657,7 +657,7 @@ cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_const
   __shared__ float2 s_stat[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, groups = (s.blocks * KC_PAGE + KS_TOKENS - 1) / KS_TOKENS;
   const int bh = blockIdx.x / groups, group = blockIdx.x - bh * groups, b = bh / c.H, h = bh - b * c.H;
-  const int len = sequence_length(c, s, b), n = query_count(c, p, b);
+  const int len = sequence_length<true>(c, s, b), n = query_count<true>(c, p, b);
   if (group * KS_TOKENS >= len && group > 0) return;
   ItemParts parts{0, 0, 0, 1};
   if (shape.ctas > 0) parts = parts_of(c, s, p, shape, b, h, 0, len, n);

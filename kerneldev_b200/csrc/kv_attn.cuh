@@ -66,8 +66,9 @@ struct Item {
   int b, h, tile, len;
 };
 
+template <bool kAhead = false>
 __device__ __forceinline__ int query_count(const kd_cache& c, const kd_cache_queries& p, int b) {
-  return p.q_lens != nullptr ? checked_count(c, p.q_lens[b], p.T) : p.T;
+  return p.q_lens != nullptr ? checked_count(c, length_word<kAhead>(p.q_lens + b), p.T) : p.T;
 }
 
 // one row's mask; r: row of the key head (query r / G of head r % G of the group)
@@ -105,16 +106,17 @@ struct FlatPlace {
   int b, ht, at, units, len, tiles;   // ht: head * tiles + tile; unit `at` of `units` of the item; len and tiles: of the sequence
 };
 __device__ __forceinline__ int pages_of_length(int len) { return (len + KC_PAGE - 1) / KC_PAGE; }
+template <bool kAhead = false>   // see length_word
 struct FlatOrder {
   int held, held_tiles;       // length and tiles of sequence `lane`
   uint32_t most;              // pages of a unit
   uint32_t total;             // even: pages ...
   uint32_t ctas, each, more;  // ... and the CTAs that have them: `each`, and one more for the first `more`
 
-  static __device__ __forceinline__ int length_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? sequence_length(c, s, b) : 0; }
+  static __device__ __forceinline__ int length_of(const kd_cache& c, const kd_cache_seqs& s, int b) { return b < s.B ? sequence_length<kAhead>(c, s, b) : 0; }
   static __device__ __forceinline__ int tiles_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b) {
     if (p.q_lens == nullptr) return shape.tiles;
-    return b < s.B ? (query_count(c, p, b) * shape.G + shape.item_rows - 1) / shape.item_rows : 0;
+    return b < s.B ? (query_count<kAhead>(c, p, b) * shape.G + shape.item_rows - 1) / shape.item_rows : 0;
   }
   __device__ __forceinline__ uint32_t units_of(int len) const { return (pages_of_length(len) + most - 1) / most; }
   __device__ __forceinline__ void look_up(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape) {
@@ -194,7 +196,7 @@ __device__ __forceinline__ ItemShare share_of_cta(const kd_cache& c, const kd_ca
     r.pages = r.here = p.q_lens != nullptr && r.it.tile * shape.item_rows >= query_count(c, p, b) * shape.G ? 0 : pages_of_length(r.it.len);   // (rows without a query: zeros)
     return r;
   }
-  FlatOrder order;
+  FlatOrder<> order;
   order.look_up(c, s, p, shape);
   uint32_t unit = blockIdx.x, left = 0;
   if (shape.even) {
@@ -223,14 +225,14 @@ __device__ __forceinline__ ItemShare share_of_cta(const kd_cache& c, const kd_ca
   return r;
 }
 
-// The parts of an item, `count` of them: `first`, then one every `step` from `next` on. One part alone is no part: its CTA has written the rows.
+// The parts of an item, for the kernels that join them, ahead of their wait for the kernel that makes them. `count` of them: `first`, then one every `step` from `next` on. One part alone is no part: its CTA has written the rows.
 struct ItemParts {
   uint32_t first, next, step;
   int count;
   __device__ __forceinline__ uint32_t at(int k) const { return k == 0 ? first : next + (k - 1) * step; }
 };
 __device__ __forceinline__ ItemParts parts_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& shape, int b, int h, int tile, int len, int n_queries) {
-  FlatOrder order;
+  FlatOrder<true> order;
   order.look_up(c, s, p, shape);
   const int tiles = (n_queries * shape.G + shape.item_rows - 1) / shape.item_rows;
   const uint32_t units = tile < tiles ? order.units_of(len) : 0, first = order.before(c, s, p, shape, b) + (h * tiles + tile) * units;

@@ -28,8 +28,12 @@ __device__ __forceinline__ int checked_count(const kd_cache& c, int n, int most)
   cache_report(c, KC_BAD_LENGTH);
   return n < 0 ? 0 : most;
 }
+// kAhead: ahead of the wait for the kernel before (see pdl_wait), past L1: the line may be there from before the length was written
+template <bool kAhead = false>
+__device__ __forceinline__ int length_word(const int32_t* p) { return kAhead ? __ldcg(p) : *p; }
+template <bool kAhead = false>
 __device__ __forceinline__ int sequence_length(const kd_cache& c, const kd_cache_seqs& s, int b) {
-  return checked_count(c, s.lens[b], s.blocks * KC_PAGE);
+  return checked_count(c, length_word<kAhead>(s.lens + b), s.blocks * KC_PAGE);
 }
 // the page of a sequence's block, -1 where the table names none that exists
 __device__ __forceinline__ int checked_page(const kd_cache& c, int page) {

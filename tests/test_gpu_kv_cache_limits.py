@@ -286,3 +286,31 @@ def test_a_graph_keeps_the_status_word_of_its_cache(monkeypatch):
     others.append(KVCache(*tensors))
     cache_append(others[-1], x, x, t, lens)
     cache_read(others[0], t, lens, 1)
+
+
+@pytest.mark.parametrize("T,G,weigh", [(1, 8, False), (1, 8, True), (40, 2, False)])
+def test_a_length_that_has_just_been_written(monkeypatch, T, G, weigh):
+    """The join looks the lengths up while the attention before it runs, on SMs of which many had the old length in their L1 from an append."""
+    from kerneldev_b200 import KVCache, cache_append, cache_attention
+    rng = np.random.default_rng(9)
+    c = KVCache.empty(64, 4, 64, device=DEV)
+    t, lens, back = i32([list(range(64))]), i32([600]), i32([600])
+    x = rand_kv(rng, (2, 1, 4, 2000, 64), torch.float16, False).to(DEV)
+    cache_append(c, x[0], x[1], t, i32([0]))
+    q = rand_kv(rng, (1, 4 * G, T, 64), torch.float16, False).to(DEV)
+    w = torch.zeros((1, 4, 4096), device=DEV) if weigh else None
+    lengths = rng.integers(600, 2000, 60)
+    want = []
+    for n in lengths:
+        want.append(cache_attention(q, c, t, i32([n]), return_lse=True))
+    torch.cuda.synchronize()
+    new = [i32([n]) for n in lengths]
+    got = []
+    monkeypatch.delenv("KD_CHECK_STATUS", raising=False)   # without a wait after each call
+    for n in new:
+        cache_append(c, x[0, :, :, 600:], x[1, :, :, 600:], t, lens.copy_(back))
+        lens.copy_(n)
+        got.append(cache_attention(q, c, t, lens, return_lse=True, weights=w))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
