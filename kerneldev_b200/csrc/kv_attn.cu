@@ -20,7 +20,7 @@
 // probabilities that is 2^-28 of the row's largest, or 2^-20 of the unit's.
 //
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
-// taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs.
+// taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs. So does one that has met scores beyond KA_FAR.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -239,15 +239,8 @@ struct QueryLoad {
     for (int i = 0; i < PER; ++i) {
       const int r = warp * PER + i;
       int e = 0;
-      if (bf16) {
-        auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
-        const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[i].x), size(v[i].x >> 16)), max(size(v[i].y), size(v[i].y >> 16))));
-        if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
-        const float f = exp2i(e);
-        const float2 a = unpack2<true>(v[i].x), b = unpack2<true>(v[i].y);
-        v[i] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
-      }
-      if (lane == 0) q.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+      if (bf16) e = row_to_halves(v[i]);
+      if (lane == 0) q.factor[r] = row_factor(p.sm_scale, e);
       if (d < D) q.frag[r / KA_TILE][S::k_word(d)][(r % KA_TILE) * 4 + S::k_lane(d)] = v[i];
     }
     __syncthreads();
@@ -279,6 +272,7 @@ template <int D, int NT>
 struct Walker {
   float o[NT][D / 16][4];
   float ref[NT][2], sum[NT][2];
+  bool met_far;   // some row was far at some time
 
   // starts the copies of a unit (nothing at or beyond `last`)
   static __device__ __forceinline__ void fetch(const kd_cache& c, const Lane<D>& place, int h, int unit, int last, int page, char* stage) {
@@ -309,9 +303,10 @@ struct Walker {
 
   // next_page: what begin returned
   // scores: of the item's first token, or null: they are not wanted
+  // far: a second pass over rows that are (see KA_FAR). Scores are rounded first, ref is the largest and no more, and V's scale goes into the units of O instead.
   template <bool kSafe>
   __device__ __forceinline__ void walk(const kd_cache& c, const kd_cache_seqs& s, const Lane<D>& place, const Item& it, const QueryTile<D, NT>& q, int first, int last, int next_page,
-                                       char* ring, float* all_scores, int score_rows) {
+                                       char* ring, float* all_scores, int score_rows, bool far) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -324,7 +319,9 @@ struct Walker {
     }
     const int32_t* table = s.table + it.b * s.table_stride;
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
-    int ev_top = KC_EXP_MIN;   // the largest so far
+    int ev_top = KC_EXP_MIN, o_unit = 0;
+    const float slack = kSafe && far ? 0.f : KA_SLACK;
+    met_far = false;
     char* stage = ring;
     for (int unit = first; unit < last; unit += KA_WARPS) {
       cp_async_wait<0>();
@@ -338,8 +335,18 @@ struct Walker {
       const uint32_t* desc = c.desc != nullptr ? reinterpret_cast<const uint32_t*>(stage + Stage<D>::DESC_AT) : nullptr;
       const int page = reinterpret_cast<const int*>(scale)[2], j0 = unit * KA_UNIT;
       const float ks = scale[0];
-      const int ev = scale_exponent(scale[1]);
+      const int ev_page = scale_exponent(scale[1]), ev = kSafe && far ? 0 : ev_page;   // (of far rows: nothing of it in the exponent)
       const bool apart = scales_apart(ev, ev, ev_top);
+      if (kSafe && far && ev_page != o_unit) {
+        const float to = exp2i(o_unit - ev_page);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[n][m][x] *= to;
+        o_unit = ev_page;
+      }
       float sc[NT][2][4];
       scores<D, NT>(at, place, q, sc);
       uint32_t p[2][NT][2], vis[2][NT][2];
@@ -349,7 +356,7 @@ struct Walker {
         float k[2], add[2], high[2], old[2];
         bool moves = false;
         if (NT == 1 && all_scores != nullptr && 2 * t < score_rows) {
-          const float k0 = fmaxf(ks * q.factor[2 * t], KA_TINY), k1 = fmaxf(ks * q.factor[2 * t + 1], KA_TINY);
+          const float k0 = score_factor(ks, q.factor[2 * t]), k1 = score_factor(ks, q.factor[2 * t + 1]);
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             *reinterpret_cast<float2*>(all_scores + static_cast<size_t>(j0 + 8 * y + g) * score_rows + 2 * t) = make_float2(sc[n][y >> 1][2 * (y & 1)] * k0, sc[n][y >> 1][2 * (y & 1) + 1] * k1);
@@ -357,7 +364,7 @@ struct Walker {
         auto set_add = [&](int x) { add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x]; };
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          k[x] = fmaxf(ks * q.factor[n * KA_TILE + 2 * t + x], KA_TINY);
+          k[x] = score_factor(ks, q.factor[n * KA_TILE + 2 * t + x]);
           // the row's maximum, over the lanes of its tokens
           float top = fmaxf(fmaxf(sc[n][0][x], sc[n][0][2 + x]), fmaxf(sc[n][1][x], sc[n][1][2 + x]));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
@@ -365,7 +372,7 @@ struct Walker {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           high[x] = fmaf(top, k[x], static_cast<float>(ev));
           old[x] = ref[n][x];
-          const bool up = above_reference(high[x], old[x]);
+          const bool up = high[x] > old[x] + slack;
           moves = moves || up;
           ref[n][x] = up ? rintf(high[x]) : old[x];   // (ahead of the vote: the exponentials wait for it)
           set_add(x);
@@ -375,15 +382,18 @@ struct Walker {
           float shrink[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float total = sum[n][x];
+            if (apart) {
+              float total = sum[n][x];
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            if (apart && below_reference(high[x], old[x])) {
-              ref[n][x] = reference_below(high[x], old[x], total);
-              set_add(x);
+              for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+              if (below_reference(high[x], old[x])) {
+                ref[n][x] = reference_below(high[x], old[x], total);
+                set_add(x);
+              }
             }
             shrink[x] = exp2_whole(old[x] - ref[n][x]);
             sum[n][x] *= shrink[x];
+            met_far = met_far || is_far(ref[n][x]);
           }
 #pragma unroll
           for (int m = 0; m < D / 16; ++m)
@@ -397,6 +407,17 @@ struct Walker {
             for (int y = 0; y < 2; ++y)
               vis[i][n][y] = transpose8x8((sc[n][i][2 * y] == -INFINITY ? 0u : 0x3C00u) | (sc[n][i][2 * y + 1] == -INFINITY ? 0u : 0x3C000000u));
         }
+        if (kSafe && far)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              float& v = sc[n][y >> 1][2 * (y & 1) + x];
+              v = __fsub_rn(__fmul_rn(v, k[x]), ref[n][x] == -INFINITY ? 0.f : ref[n][x]);
+            }
+            k[x] = 1.f;
+            add[x] = KA_OFFSET;
+          }
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -421,6 +442,15 @@ struct Walker {
     }
     cp_async_wait<0>();
     __syncwarp();
+    if (kSafe && far) {
+      const float to = exp2i(o_unit);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[n][m][x] *= to;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -490,10 +520,11 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
     }
     Walker<D, NT> w;
     float* scores = shape.score_rows > 0 ? ws.scores + (static_cast<size_t>(it.b) * c.H + it.h) * s.blocks * KC_PAGE * shape.score_rows : nullptr;
-    w.template walk<false>(c, s, place, it, sh.q, first, last, next_page, ring, scores, shape.score_rows);
-    if (w.any_nan()) {
+    w.template walk<false>(c, s, place, it, sh.q, first, last, next_page, ring, scores, shape.score_rows, false);
+    const bool far = __any_sync(0xffffffffu, w.met_far);
+    if (w.any_nan() || far) {
       next_page = Walker<D, NT>::begin(c, s, place, it, first, last, ring);
-      w.template walk<true>(c, s, place, it, sh.q, first, last, next_page, ring, nullptr, 0);
+      w.template walk<true>(c, s, place, it, sh.q, first, last, next_page, ring, nullptr, 0, far);
     }
     if (g == 0)
 #pragma unroll
@@ -705,11 +736,18 @@ cache_join_weights_kernel(const __grid_constant__ kd_cache c, const __grid_const
       for (int y = 0; y < 2; ++y) {
         const float score = y == 0 ? v.x : v.y;
         const float2 st = r + y < shape.rows ? s_stat[r + y] : make_float2(0.f, 0.f);
-        if (st.y != 0.f && score != -INFINITY) add += fast_exp2(score + (KA_OFFSET - st.x)) * st.y;   // rows that exist, tokens that they see
+        if (st.y != 0.f && score != -INFINITY) add += fast_exp2((score - st.x) + KA_OFFSET) * st.y;   // rows that exist, tokens that they see
       }
     }
     weights[j] += add;
   }
+}
+
+// no more than 1 (the statistics of many rows are from scores that were added up in another order: in far rows that can be many powers of two), and NaN stays NaN
+__device__ __forceinline__ float at_most_one(float x) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(1.f));
+  return y;
 }
 
 // weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
@@ -785,10 +823,10 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
         for (int x = 0; x < 2; ++x) {
           const int r = n * KA_TILE + 2 * t + x;
           const float2 st = s_stat[r];
-          const float f = fmaxf(q.factor[r] * ks[i], KA_TINY);
+          const float f = score_factor(ks[i], q.factor[r]);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float v = sc[n][y >> 1][2 * (y & 1) + x], pr = fast_exp2(fmaf(v, f, KA_OFFSET - st.x)) * st.y;
+          for (int y = 0; y < 4; ++y) {   // (from rounded scores, as the statistics of far rows are)
+            const float v = sc[n][y >> 1][2 * (y & 1) + x], pr = at_most_one(fast_exp2(__fsub_rn(__fmul_rn(v, f), st.x) + KA_OFFSET) * st.y);
             if (st.y != 0.f && v != -INFINITY) sums[i][y] += pr;   // rows that exist, tokens that they see
           }
         }

@@ -10,7 +10,15 @@ namespace kd {
 
 constexpr float KA_OFFSET = 8.f, KA_SLACK = 6.f, KA_DEPTH = 12.f, KA_LOG2E = 1.4426950408889634f;
 constexpr int KA_APART = 4;   // exponents of V scales that share a reference
-constexpr float KA_TINY = 1e-37f;   // in place of factors that a float flushes to 0 (every score is as good as 0 then): masked scores stay -inf, and not 0 * inf
+// What products of halves are multiplied with to be scores: the K scale, up to 2^31, and the query row's factor. Not infinite, so that zeros stay 0 (a row's factor ends at 2^96: with
+// sm_scale 1 that of numbers of 2^110), and not 0, so that masked scores stay -inf (where a float flushes it, every score is as good as 0).
+__device__ __forceinline__ float row_factor(float sm_scale, int e) { return fminf(sm_scale * KA_LOG2E * exp2i(-e), 7.9e28f); }
+__device__ __forceinline__ float score_factor(float k_scale, float row) { return fmaxf(k_scale * row, 1e-37f); }
+// s - ref comes from one fused product, with the steps of the exact product, where a rounded score has steps of 2^-24 of its size: from 2^24 on (in powers of two) the largest
+// probability could be any power of two, and the weights, which are from rounded scores, leave those of the statistics before. Rows that come across scores
+// from here on are done once more from rounded scores (the second passes).
+constexpr float KA_FAR = 65536.f;
+__device__ __forceinline__ bool is_far(float ref) { return fabsf(ref) >= KA_FAR && fabsf(ref) != INFINITY; }
 
 // What the mask needs of a query row. A row that does not exist, or sees nothing, has limit 0, sees 0 and a key that no descriptor matches.
 struct RowMask {
@@ -52,7 +60,6 @@ __device__ __forceinline__ bool scales_apart(int ev_low, int ev_high, int& ev_to
   ev_top = max(ev_top, ev_high);
   return ev_top - ev_low > KA_APART;
 }
-__device__ __forceinline__ bool above_reference(float high, float ref) { return high > ref + KA_SLACK; }
 __device__ __forceinline__ bool below_reference(float high, float ref) { return high < ref - KA_DEPTH && high != -INFINITY; }
 // Downwards no further than lets the row's sum reach 2^64: O is below 2^40 times that.
 __device__ __forceinline__ float reference_below(float high, float ref, float sum) {
@@ -61,6 +68,17 @@ __device__ __forceinline__ float reference_below(float high, float ref, float su
 }
 // 2^x of a whole number or an infinity; 0 below 2^-126
 __device__ __forceinline__ float exp2_whole(float x) { return __uint_as_float(static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x))) + 127) << 23); }
+
+// four numbers of a bfloat16 row, a lane each, to halves: times the power of two that brings the row's largest finite magnitude to 2^14; returns its exponent
+__device__ __forceinline__ int row_to_halves(uint2& v) {
+  auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v.x), size(v.x >> 16)), max(size(v.y), size(v.y >> 16))));
+  const int e = top != 0u ? min(112, 14 - (static_cast<int>(top >> 7) - 127)) : 0;   // -113 .. 112: a float, as its inverse
+  const float f = exp2i(e);
+  const float2 a = unpack2<true>(v.x), b = unpack2<true>(v.y);
+  v = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
+  return e;
+}
 
 struct Item {
   int b, h, tile, len;

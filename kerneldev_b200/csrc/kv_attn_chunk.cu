@@ -16,7 +16,7 @@
 // exchange a tile's words: so they agree at the first of them whether all go on, and leave together.
 //
 // NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
-// token gets NaN there.
+// token gets NaN there. So is one that has met scores beyond KA_FAR, from rounded scores, with V's scale in the units of O.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -59,7 +59,7 @@ struct ChunkShared {
   ChunkRows rows;
   ItemShare item;                    // in shared memory: the roles need their registers (with 30 of them taken, the converters' loads were spilled, which waits for them)
   uint64_t bar[5];
-  uint32_t tmem, any_nan;
+  uint32_t tmem, redo;               // redo: a pass has met NaN (1), far rows (2: see KA_FAR)
   int tiles;                         // of the pass
   AbortFlag abort;
 };
@@ -168,7 +168,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
     // ---- Q as halves (bfloat16 times a power of two, see kv_attn.cu), masks and what the rows see together ----
     if (tid == 0) {
       sh.rows = ChunkRows{0u, 0u, 0, 0};
-      sh.any_nan = 0u;
+      sh.redo = 0u;
     }
     all_sync();
     constexpr int BATCH = 8, WARPS = CH_THREADS / 32;   // rows that a warp has on their way at once
@@ -189,15 +189,8 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
       for (int x = 0; x < BATCH; ++x) {
         const int r = r0 + x * WARPS;
         int e = 0;
-        if (p.dtype == KD_BF16) {
-          auto size = [](uint32_t u) { return (u & 0x7FFFu) < 0x7F80u ? u & 0x7FFFu : 0u; };
-          const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(size(v[x].x), size(v[x].x >> 16)), max(size(v[x].y), size(v[x].y >> 16))));
-          if (top != 0u) e = max(-60, min(60, 14 - (static_cast<int>(top >> 7) - 127)));
-          const float f = exp2i(e);
-          const float2 a = unpack2<true>(v[x].x), b = unpack2<true>(v[x].y);
-          v[x] = make_uint2(pack2<false>(a.x * f, a.y * f), pack2<false>(b.x * f, b.y * f));
-        }
-        if (lane == 0) sh.factor[r] = p.sm_scale * KA_LOG2E * exp2i(-e);
+        if (p.dtype == KD_BF16) e = row_to_halves(v[x]);
+        if (lane == 0) sh.factor[r] = row_factor(p.sm_scale, e);
         if (d < D) *reinterpret_cast<uint2*>(sh.q + chunk_place(r, d)) = v[x];
       }
     }
@@ -224,7 +217,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
     const int tiles = sh.tiles;
     n_k += tiles + 1;
     n_t += tiles;
-    const bool more = pass == 0 && sh.any_nan != 0u && sh.abort.v == 0u;   // NaN: once more, with care
+    const bool more = pass == 0 && sh.redo != 0u && sh.abort.v == 0u;   // once more, with care
     if (!more) done += max(sh.item.here, 1);
     all_sync();
     return more;
@@ -236,6 +229,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
       int pass = 0;
       do {
         const bool safe = pass == 1;
+        const int most_apart = safe && (sh.redo & 2u) != 0u ? 0 : KA_APART;
         // ---------------------------------------- converters ----------------------------------------
         const int r = tid - 128;   // this thread's token of the tile for the descriptors
         const ChunkRows rows = sh.rows;
@@ -272,7 +266,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (next - batch > 30) open_batch(next, next - batch == 32 ? raw_ahead : ask(next));
           const int p0 = __shfl_sync(0xffffffffu, batch_page, next - batch), p1 = __shfl_sync(0xffffffffu, batch_page, next - batch + 1), page = r < KC_PAGE ? p0 : p1;
           const int apart = __shfl_sync(0xffffffffu, batch_ev, next - batch) - __shfl_sync(0xffffffffu, batch_ev, next - batch + 1);
-          step = p0 >= 0 && p1 >= 0 && (apart < -KA_APART || apart > KA_APART) ? 1 : 2;
+          step = p0 >= 0 && p1 >= 0 && (apart < -most_apart || apart > most_apart) ? 1 : 2;
           const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0 && r < KC_PAGE * step;
           ahead_desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
         };
@@ -395,7 +389,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
       const Item it = sh.item.it;
       int pass = 0;
       do {
-        const bool safe = pass == 1;
+        const bool safe = pass == 1, far = safe && (sh.redo & 2u) != 0u;
         // ---------------------------------------- softmax ----------------------------------------
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16, mS = tS + lanes, mO = tO + lanes;
         const RowMask mask = sh.mask[tid];
@@ -417,7 +411,9 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           commit_uniform(bar(CB_PV));
         };
         float ref = -INFINITY, sum = 0.f;
-        int ev_top = KC_EXP_MIN;
+        int ev_top = KC_EXP_MIN, o_unit = 0;
+        bool met_far = false;
+        const float slack = far ? 0.f : KA_SLACK, offset = far ? 0.f : KA_OFFSET;   // (far: 8 - ref would round)
         uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
         bool ok = true;
         int u = 0;
@@ -428,8 +424,9 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (warp == 0) issue_scores();
           uint32_t w[4];
           row_words(mask, rec, metadata, lane, w);
-          const float kf[2] = {fmaxf(rec.ks[0] * factor, KA_TINY), fmaxf(rec.ks[1] * factor, KA_TINY)};
-          const int ev[2] = {rec.ev[0], rec.ev[1]};
+          float kf[2] = {score_factor(rec.ks[0], factor), score_factor(rec.ks[1], factor)};
+          // (far: both pages of a tile have one V scale, and it goes into the units of O)
+          const int ev_tile = rec.ev[0], ev[2] = {far ? 0 : ev_tile, far ? 0 : rec.ev[1]};
           if (safe) {
             if (!(ok = wait(CB_V, n_t + u, 0))) break;
             for (int j = 0; j < CH_TOKENS; ++j) {
@@ -446,6 +443,19 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           // Scores of 64 tokens (a page) in registers at a time: page 0's for its maximum alone, then page 1's, which stay there; after the exponentials of a half page its
           // registers take page 0's scores again.
           uint32_t x[2][32];
+          if (far) {   // rounded scores in the place of the products
+#pragma unroll 1
+            for (int i = 0; i < CH_TOKENS; i += 16) {
+              uint32_t y[16];
+              tmem_ld16(mS + i, y);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__fmul_rn(__uint_as_float(y[j]), i < KC_PAGE ? kf[0] : kf[1]));
+              tmem_st16(mS + i, y);
+            }
+            tmem_wait_st();
+            kf[0] = kf[1] = 1.f;
+          }
           auto masked = [&](uint32_t (&y)[32], uint32_t bits) {
             if (__all_sync(0xffffffffu, bits == 0xFFFFFFFFu)) return;
 #pragma unroll
@@ -473,24 +483,27 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             top[page] = fmaxf(highest(x[0]), highest(x[1]));
           }
           const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
-          const bool up = above_reference(high, ref), down = scales_apart(min(ev[0], ev[1]), max(ev[0], ev[1]), ev_top) && below_reference(high, ref);
-          if (__any_sync(0xffffffffu, up || down)) {
-            const float to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref, shrink = exp2_whole(ref - to);
-            if (u > 0 && __any_sync(0xffffffffu, to != ref && ref != -INFINITY)) {   // O is complete: its last product came before these scores
+          const bool up = high > ref + slack, down = scales_apart(min(ev[0], ev[1]), max(ev[0], ev[1]), ev_top) && below_reference(high, ref);
+          const bool units = far && ev_tile != o_unit;   // the whole CTA
+          if (__any_sync(0xffffffffu, up || down || units)) {
+            const float to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref, shrink_o = exp2_whole(ref - to) * (units ? exp2i(o_unit - ev_tile) : 1.f), shrink = exp2_whole(ref - to);
+            met_far = met_far || is_far(to);
+            if (units) o_unit = ev_tile;
+            if (u > 0 && __any_sync(0xffffffffu, units || (to != ref && ref != -INFINITY))) {   // O is complete: its last product came before these scores
 #pragma unroll 1
               for (int i = 0; i < D; i += 16) {
                 uint32_t y[16];
                 tmem_ld16(mO + i, y);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink);
+                for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
                 tmem_st16(mO + i, y);
               }
             }
             sum *= shrink;
             ref = to;
           }
-          const float base = ref == -INFINITY ? 0.f : KA_OFFSET - ref;
+          const float base = ref == -INFINITY ? 0.f : offset - ref;
 #pragma unroll
           for (int half = 0; half < 4; ++half) {   // page 1's halves, then page 0's; P of a page over its first 32 columns
             const int page = half < 2 ? 1 : 0, part = half & 1;
@@ -525,12 +538,16 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         }
         if (ok && u > 0) ok = wait(CB_PV, n_t + u - 1, 0);
         tc_fence_after_sync();
+        if (far) {   // as with the offset
+          sum *= 256.f;
+          o_unit += 8;
+        }
         // ---- this row's output ----
         const int row = it.tile * KC_ROWS + tid;
         const bool live = mask.limit > 0, exists = row < shape.rows, whole = sh.item.here == sh.item.pages;
         const size_t part = sh.item.part;
         const int i = row / shape.G, hq = it.h * shape.G + row - i * shape.G;
-        const float inv = !whole ? 1.f : live && sum != 0.f ? 1.f / sum : 0.f;
+        const float inv = (!whole ? 1.f : live && sum != 0.f ? 1.f / sum : 0.f) * exp2i(o_unit);   // (of far rows: O's units)
         bool bad = false;
         if (ok) {
           if (exists && whole) write_stats(p, ws, shape.stats, (static_cast<size_t>(it.b) * p.H + hq) * p.T + i, live, ref, sum);
@@ -560,7 +577,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           tc_fence_before_sync();
         }
-        if (bad) sh.any_nan = 1u;
+        if (bad || met_far) atomicOr(&sh.redo, (bad ? 1u : 0u) | (met_far ? 2u : 0u));
         if (tid == 0) sh.tiles = u;   // (the converters' count is the same)
         if (!ok && warp == 0) {   // what has been issued ends before TMEM is given back
           if (u > 0) drain_wait(bar(CB_PV), (n_t + u - 1) & 1);

@@ -314,3 +314,92 @@ def test_a_length_that_has_just_been_written(monkeypatch, T, G, weigh):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ---- scores and queries at the ends of their range ----------------------------------------------------------------
+
+@pytest.mark.parametrize("B,Hkv,G,T", [(1, 1, 2, 1), *SHARED])
+@pytest.mark.parametrize("power,kind", [(10, "bf16"), (17, "bf16"), (20, "negative"), (21, "nan"), (45, "bf16"), (80, "bf16"), (100, "negative"), (110, "nan"), (30, "f16"), (-90, "bf16"), (-120, "bf16")])
+def test_scores_far_from_zero(B, Hkv, G, T, power, kind):
+    """Every second head's queries are whole numbers times 2**power (or, with f16, all keys are), the others' are whole numbers. All products and sums are exact, so that scores that are
+    equal are equal in any order of summation, and the others are at least 2**power log2(e) / 8 apart in powers of two: from 2**9 on a row's weight belongs to its largest scores, evenly. (Their
+    error in powers of two, on which the tolerance of the other rows rests, does not matter.) nan: a value that the last query alone sees."""
+    from kerneldev_b200 import cache_append, cache_attention
+    rng = np.random.default_rng(abs(power) + T)
+    D, n = 64, 1300 if B > 1 else 400
+    dtype = torch.float16 if kind == "f16" else torch.bfloat16
+    lens = rng.integers(n - 200, n, B)
+    pages = B * (-(-n // 64))
+    c = make_cache(pages, Hkv, D)
+    table = tables(rng, B, pages // B, pages)
+    k = rng.integers(1, 4, (B, Hkv, n, D)) if kind == "negative" else rng.integers(-3, 4, (B, Hkv, n, D))
+    v = rand_kv(rng, (B, Hkv, n, D), torch.float32, False).numpy()
+    v[:, :, 192:256] *= 2.0 ** 20 if kind != "f16" else 2.0 ** 7
+    q = rng.integers(-2, 0, (B, Hkv * G, T, D)) if kind == "negative" else rng.integers(-2, 3, (B, Hkv * G, T, D))
+    k, q = k.astype(np.float64), q.astype(np.float64)
+    large = (np.arange(Hkv * G) % 2 == 0) if kind != "f16" else np.ones(Hkv * G, bool)
+    if kind == "f16":
+        k *= 2.0 ** power
+    else:
+        q[:, large] *= 2.0 ** power
+    if kind == "nan" and T > 1:
+        for b in range(B):
+            v[b, :, lens[b] - 1] = np.nan
+    cache_append(c, torch.tensor(k, dtype=torch.float32, device=DEV), torch.tensor(v, device=DEV), i32(table), i32(np.zeros(B)), i32(lens))
+    w = torch.zeros((B, Hkv, n), device=DEV)
+    o, lse = cache_attention(torch.tensor(q).to(dtype).to(DEV), c, i32(table), i32(lens), return_lse=True, weights=w)
+    o, lse, w = (t.double().cpu().numpy() for t in (o, lse, w))
+    want = as_oracle(c)
+    eps = torch.finfo(dtype).eps
+    for b in range(B):
+        for h in range(Hkv):
+            keys, vals = ko.values(want, table[b], int(lens[b]), h, "k"), ko.values(want, table[b], int(lens[b]), h, "v")
+            assert np.array_equal(keys, k[b, h, :lens[b]])
+            total, slack = np.zeros(lens[b]), np.zeros(lens[b])
+            for g in range(G):
+                hq = h * G + g
+                rows = T - 1 if kind == "nan" and T > 1 else T
+                if rows < T:
+                    assert np.isnan(o[b, hq, rows]).all()
+                see = np.arange(lens[b])[None] <= (lens[b] - T + np.arange(T))[:, None]
+                s = np.where(see, q[b, hq] @ keys.T / 8, -np.inf)
+                top = s.max(1, keepdims=True)
+                p = np.exp(s - top)
+                l = p.sum(1, keepdims=True)
+                p /= l
+                clean = np.nan_to_num(vals)
+                ref, a = p @ clean, p @ np.abs(clean)
+                mag = np.where(see, np.abs(q[b, hq]) @ np.abs(keys).T, 0).max(1) / 8
+                delta = (np.full(T, 2.0 ** -20) if large[hq] and power >= 9 else 2.0 ** -21 * (mag * 1.5 + 2)) + lens[b] * 2.0 ** -24
+                floor = 2.0 ** -28 * (see @ np.abs(clean)) * p.max(1, keepdims=True) * (1 - (large[hq] and power >= 9))   # see cache_attention on weights
+                tol = eps / 2 * (np.abs(ref) + 0.01 * a) + a * (2.0 ** -11 + 2 * delta[:, None]) + floor + 2.0 ** -25
+                err = np.abs(o[b, hq] - ref)[:rows]
+                assert (err <= tol[:rows]).all(), f"O: {(err / tol[:rows]).max()} of the tolerance at {b, hq, np.unravel_index((err / tol[:rows]).argmax(), err.shape)}"
+                rl = (top / np.log(2.0) + np.log2(l))[:, 0]
+                assert (np.abs(lse[b, hq] - rl) <= 2 * delta + 2.0 ** -21 * np.abs(rl)).all(), "LSE"
+                total += p.sum(0)
+                # below 2**16 a row's sum is of exact products and the weights are of scores rounded to 2**-24 of them: their ratio is off by that times log(2), in the scores' units
+                steps = np.where(np.abs(top) < 2.0 ** 16, 2.0 ** -23 * np.abs(top), 0)
+                slack += (p * (3 * delta[:, None] + steps + G * T * 2.0 ** -24)).sum(0)
+            assert (np.abs(w[b, h, :lens[b]] - total) <= slack + total * G * T * 2.0 ** -24 + 1e-30).all(), "weights"
+
+
+def test_a_query_of_large_numbers_over_keys_of_small_ones():
+    """The products are ordinary numbers, whatever their factors are: queries of 2**100 over keys of 2**-32 * 448 and less, and the other way round."""
+    from kerneldev_b200 import cache_append, cache_attention
+    rng = np.random.default_rng(3)
+    for T in (1, 40):
+        for power in (-34, 30):
+            c = make_cache(20, 1, 64)
+            table = tables(rng, 1, 20, 20)
+            x = rand_kv(rng, (2, 1, 1, 1200, 64), torch.float32, False)
+            x[0] *= 2.0 ** power
+            cache_append(c, x[0].to(DEV), x[1].to(DEV), i32(table), i32([0]))
+            q = (rand_kv(rng, (1, 2, T, 64), torch.float32, False) * 2.0 ** (100 if power < 0 else -100)).to(torch.bfloat16).to(DEV)
+            scale = 2.0 ** (-100 - power if power < 0 else 100 - power) / 8
+            if scale >= 1e30:
+                continue
+            o, lse = cache_attention(q, c, i32(table), i32([1200]), return_lse=True, sm_scale=scale)
+            got = cache_attention((q.float() * 2.0 ** (-100 if power < 0 else 100)).to(torch.bfloat16), c, i32(table), i32([1200]), return_lse=True, sm_scale=2.0 ** -power / 8)
+            assert torch.equal(o, got[0]) and torch.equal(lse, got[1])
+            check_attention(c, (q.float() * 2.0 ** (-100 if power < 0 else 100)).to(torch.bfloat16), table, [1200], [T], got, scale=2.0 ** -power / 8)
