@@ -852,6 +852,13 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
 constexpr int CHUNK_FROM = 32;
 static int rows_of_item(int rows) { return rows > CHUNK_FROM ? KC_ROWS : rows <= KA_TILE ? KA_TILE : rows <= 2 * KA_TILE ? 2 * KA_TILE : 4 * KA_TILE; }
 
+// The scores that few rows leave for the weights: 4 bytes for each row and token of the page table (by its width, for the lengths are on the device), 4.3 GB for 128 sequences of 8 heads, 8 rows and
+// tables for 131,072 tokens. Beyond 256 MB, and an eighth of what the cache itself takes, K is read and multiplied again instead (cache_weights_kernel): 32 sequences of 8192 tokens, 8 heads of 128, 8 rows
+// 137 us with the scores and 179 without; 64 sequences 276 and 350; 1 of 131,072 70 and 99; 8 of 4096, 4 rows, 21 and 34.
+constexpr size_t KA_SCORES_LIMIT = size_t(256) << 20;
+static size_t scores_bytes(const kd_cache& c, const kd_cache_seqs& s, const AttnShape& a) { return static_cast<size_t>(s.B) * c.H * s.blocks * KC_PAGE * a.score_rows * sizeof(float); }
+static size_t scores_limit(const kd_cache& c) { return std::max(KA_SCORES_LIMIT, static_cast<size_t>(c.pages) * c.H * KC_PAGE * 2 * c.D / 8); }
+
 static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p) {
   AttnShape a;
   a.G = p.H / c.H;
@@ -864,6 +871,7 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   a.tiles = (a.rows + rows - 1) / rows;
   a.stats = p.weights != nullptr;
   a.score_rows = !a.stats || a.rows > KA_TILE ? 0 : a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : 8;
+  if (scores_bytes(c, s, a) > scores_limit(c)) a.score_rows = 0;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles, pages = items * s.blocks;
   // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
   const int slots = 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
@@ -882,7 +890,7 @@ static size_t workspace_of(const kd_cache& c, const kd_cache_seqs& s, const kd_c
     return at;
   };
   const size_t part_rows = (a.even ? size_t(2) : size_t(1)) * a.ctas * rows_of_item(a.rows);
-  ws->scores = reinterpret_cast<float*>(take(static_cast<size_t>(s.B) * c.H * s.blocks * KC_PAGE * a.score_rows * sizeof(float)));
+  ws->scores = reinterpret_cast<float*>(take(scores_bytes(c, s, a)));
   ws->stats = reinterpret_cast<float2*>(take(a.stats ? static_cast<size_t>(s.B) * p.H * p.T * sizeof(float2) : 0));
   ws->part_o = reinterpret_cast<float*>(take(part_rows * c.D * sizeof(float)));
   ws->part_ml = reinterpret_cast<float2*>(take(part_rows * sizeof(float2)));
@@ -958,7 +966,7 @@ static int launch_dim(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_
     e = few ? launch(cache_join_kernel<KJ_WARPS>, static_cast<unsigned>(heads * a.rows), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
             : launch(cache_join_kernel<1>, static_cast<unsigned>(heads * ((a.rows + KJ_WARPS - 1) / KJ_WARPS)), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
   }
-  if (e == cudaSuccess) e = rows == 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);   // (one tile of rows: above)
+  if (e == cudaSuccess) e = rows <= 2 * KA_TILE ? launch_weights<D, 2>(c, s, p, a, ws, stream) : launch_weights<D, 4>(c, s, p, a, ws, stream);   // (one tile of rows: above, but beyond scores_limit)
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));
   return 0;
 }

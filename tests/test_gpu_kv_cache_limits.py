@@ -403,3 +403,22 @@ def test_a_query_of_large_numbers_over_keys_of_small_ones():
             got = cache_attention((q.float() * 2.0 ** (-100 if power < 0 else 100)).to(torch.bfloat16), c, i32(table), i32([1200]), return_lse=True, sm_scale=2.0 ** -power / 8)
             assert torch.equal(o, got[0]) and torch.equal(lse, got[1])
             check_attention(c, (q.float() * 2.0 ** (-100 if power < 0 else 100)).to(torch.bfloat16), table, [1200], [T], got, scale=2.0 ** -power / 8)
+
+
+def test_weights_of_few_rows_over_page_tables_that_are_wide():
+    """Tables for more tokens than there is room for scores: the weights come from K once more."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(70)
+    B, Hkv, G = 6, 4, 8
+    lens = rng.integers(1, 700, B)
+    c, table = filled(rng, B, Hkv, 64, lens, torch.bfloat16, False)
+    q = rand_kv(rng, (B, Hkv * G, 1, 64), torch.bfloat16, False).to(DEV)
+    for width in (1 << 14, 1 << 10):   # 768 MB of scores, 48 MB
+        wide = torch.zeros((B, width), dtype=torch.int32, device=DEV)
+        wide[:, :table.shape[1]] = i32(table)
+        w = torch.zeros((B, Hkv, 700), device=DEV)
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        o, lse = cache_attention(q, c, wide, i32(lens), return_lse=True, weights=w)
+        assert torch.cuda.max_memory_allocated() - held < (64 << 20)
+        check_causal(c, q, table, lens, o, lse, w)

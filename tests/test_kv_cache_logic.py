@@ -96,6 +96,25 @@ def test_entry_points_reject_descriptors_that_16_byte_copies_cannot_read():
             assert rc == code and (rc == 0 or b"desc" in lib.kd_last_error())
 
 
+def test_workspace_of_weights_is_bounded_by_the_cache():
+    """However wide the page tables are: 256 MB, or an eighth of the cache's own bytes, and the parts and statistics besides. What is below that keeps its place for the scores."""
+    m, lib, c, s = _cache()
+    q, n = m.KdCacheQueries(), ctypes.c_size_t()
+    q.T, q.dtype, q.sm_scale, q.weights = 1, m.KD_F16, 1.0, 0x10000
+    for B, H, rows, blocks, pages, D in ((128, 8, 8, 2048, 4000, 128), (1, 1, 1, 1 << 24, 10, 16), (64, 8, 5, 1 << 16, 100000, 64), (16, 4, 8, 64, 1024, 128), (128, 8, 8, 2048, 128 * 2048, 128)):
+        s.B, s.blocks, s.table_stride, c.H, c.D, c.pages, q.H = B, blocks, blocks, H, D, pages, H * rows
+        bytes_ = []
+        for q.weights in (None, 0x10000):
+            assert lib.kd_cache_attention_workspace(ctypes.byref(c), ctypes.byref(s), ctypes.byref(q), ctypes.byref(n)) == 0
+            bytes_.append(n.value)
+        limit = max(256 << 20, pages * H * 64 * 2 * D // 8)
+        scores = B * H * blocks * 64 * {1: 2, 5: 8, 8: 8}[rows] * 4
+        stats = B * H * rows * 8
+        extra = bytes_[1] - bytes_[0]
+        assert extra <= limit + stats + 1024
+        assert extra >= scores if scores <= limit else extra <= stats + 1024
+
+
 def test_cache_has_no_cpu_path():
     from kerneldev_b200 import KVCache
     with pytest.raises(RuntimeError, match="no CPU path"):
