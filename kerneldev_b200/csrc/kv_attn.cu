@@ -847,8 +847,9 @@ cache_weights_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
-// Rows of an item: as many tiles of eight as the rows fill, up to four; beyond CHUNK_FROM rows the items are those of the kernel for many rows
-// (8 x 4096 tokens of 8 heads of 128: 32 rows take 35 us here and 71 there, 36 rows 45 there; here they would be two items that read the cache twice).
+// Rows of an item: as many tiles of eight as the rows fill, up to four; beyond CHUNK_FROM rows the items are those of the kernel for many rows, which fills its 128 rows up, but would be two or
+// more items here, that read the cache as often. us here and there: 8 x 4096 tokens of 8 heads of 128, 20 rows 33 and 42, 32 rows 34 and 40, 36 rows 52 and 41, 64 rows 53 and 42; 32 x 4096, 32 rows
+// 98 and 143, 36 rows 168 and 145. (2 x 1300 tokens of 4 heads of 64 would be faster here further on: 36 rows 14 and 21, 64 rows 17 and 22.)
 constexpr int CHUNK_FROM = 32;
 static int rows_of_item(int rows) { return rows > CHUNK_FROM ? KC_ROWS : rows <= KA_TILE ? KA_TILE : rows <= 2 * KA_TILE ? 2 * KA_TILE : 4 * KA_TILE; }
 
@@ -873,7 +874,10 @@ static AttnShape shape_of(const kd_cache& c, const kd_cache_seqs& s, const kd_ca
   a.score_rows = !a.stats || a.rows > KA_TILE ? 0 : a.rows <= 2 ? 2 : a.rows <= 4 ? 4 : 8;
   if (scores_bytes(c, s, a) > scores_limit(c)) a.score_rows = 0;
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles, pages = items * s.blocks;
-  // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits.
+  // Up to eight pages a head, or with many heads for each SM, a CTA takes whole heads and nothing is joined; so it is where the flat order would need more than 32 bits. us with whole heads and with
+  // pages shared, from 16 heads for each SM on: 300 x 2000 tokens of 8 heads of 128, 4 rows, 190 and 230; 128 x 4096 of 32 heads, a row each, 600 and 650; 1000 x 700 of 4 heads of 64 87 and 316; 5000 x 600 of one
+  // head 95 and 1600 (every CTA goes through all lengths). Where one sequence is far longer than all others its heads are what a call waits for: 300 x 500 tokens of 8 heads with one of 10,000 122 and 127, with one of
+  // 100,000 690 and 176. The lengths are on the device, and the table's width alone does not tell such a batch from one whose tables have room to grow.
   const int slots = 148 * (rows == KC_ROWS ? KC_CTAS : ctas_of(rows / KA_TILE));
   a.ctas = s.blocks <= 8 || items > 148 * 16 || pages >= (1 << 30) ? 0 : slots;
   a.even = a.ctas > 0 && items > slots / 2;   // see FlatOrder
