@@ -17,6 +17,8 @@
 //
 // NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
 // token gets NaN there. So is one that has met scores beyond KA_FAR, from rounded scores, with V's scale in the units of O.
+#include <stddef.h>
+
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -53,7 +55,7 @@ struct ChunkShared {
   static constexpr int BLOCKS = D > 64 ? 2 : 1, BLOCK = 128 * 128, TILE = BLOCKS * BLOCK;   // blocks of 64 head dims of 128 rows (16 KB: see koff_kmajor and desc_lo_mnmajor)
   uint8_t q[TILE], k[TILE], v[TILE];
   ChunkRecord record[CH_RECORDS];
-  uint16_t nan_bits[CH_TOKENS][8];   // second pass alone: which of a token's head dims are NaN, 16 to a word
+  alignas(16) uint16_t nan_bits[CH_TOKENS][8];   // second pass alone: which of a token's head dims are NaN, 16 to a word; read 16 bytes at a time
   float factor[KC_ROWS];
   RowMask mask[KC_ROWS];
   ChunkRows rows;
@@ -63,6 +65,7 @@ struct ChunkShared {
   int tiles;                         // of the pass
   AbortFlag abort;
 };
+static_assert(offsetof(ChunkShared<64>, nan_bits) % 16 == 0 && offsetof(ChunkShared<128>, nan_bits) % 16 == 0, "nan_bits are read 16 bytes at a time");
 enum { CB_K, CB_S, CB_V, CB_P, CB_PV };
 
 // byte of element (row, d) in a tile: 64 head dims of a row are 128 bytes, swizzled

@@ -69,6 +69,30 @@ def test_share_whose_visible_keys_are_all_nan(B, Hkv, G, T, weigh):
             assert torch.isnan(w[b, Hkv - 1, :int(lens[b]) - T + 1]).all() and torch.isfinite(w[b, :Hkv - 1]).all() and torch.isfinite(w[:b]).all()
 
 
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 112, 128])
+@pytest.mark.parametrize("G,T", [(3, 1), (2, 40)])
+def test_nan_of_single_values_at_every_head_dim(D, G, T):
+    """Values that are NaN in one column each, in tokens that some rows see and others do not: the column is NaN in the rows that see it, all else is as without them."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(D + T)
+    B, n = 2, 900
+    c, table = filled(rng, B, 1, D, [n, n], torch.bfloat16, False)
+    q = rand_kv(rng, (B, G, T, D), torch.bfloat16, False).to(DEV)
+    clean = cache_attention(q, c, i32(table), i32([n, n]), return_lse=True)
+    v = c.v.view(torch.uint8)
+    nan = torch.zeros((B, T, D), dtype=torch.bool, device=DEV)
+    for b in range(B):
+        for d in range(b, D, 3):
+            at = n - 1 - int(rng.integers(T)) if d % 2 else int(rng.integers(n))
+            v[table[b, at // 64], 0, at % 64, d] = 0x7F if d % 4 else 0xFF
+            nan[b, max(at - (n - T), 0):, d] = True
+    o, lse = cache_attention(q, c, i32(table), i32([n, n]), return_lse=True)
+    nan = nan[:, None].expand(B, G, T, D)
+    assert torch.isnan(o[nan]).all() and torch.isfinite(o[~nan]).all() and torch.equal(lse, clean[1])
+    change = (o - clean[0]).float().abs()[~nan]   # a column's NaN took the place of a number: the others are sums of the same products
+    assert not change.any()
+
+
 def values_of(rng, B, Hkv, n, D, kind):
     """Keys and values of which a page holds numbers of 2**38 and the next one of 2**-20; the large ones are few, so that in their page all other channels become zeros."""
     x = rand_kv(rng, (2, B, Hkv, n, D), torch.float32, False)
