@@ -16,7 +16,7 @@
 // O = sum p' v / sum p' 2^-ev. A half has 30 exponents for p', the scales of two pages may lie 63 apart, and what a page of small values brings must not
 // get lost beside a page that has one large number: its other channels may be all zeros. So ref follows the maximum of s + ev, in steps of 6 or more; the offset of 8 keeps
 // probabilities down to 2^-22 of the largest out of the half's subnormals, so that long tails keep their weight. And where a unit's scale is more than 2^4 below one that came before it, ref follows
-// the unit's own maximum down (below_reference): its largest p' is 2^-4 at least. What has been added up is rescaled by powers of two, exactly. A half is off by 2^-25 at most below 2^-14: in
+// the unit's own maximum down (below_reference): its largest p' is 2^-4 at least. A half is off by 2^-25 at most below 2^-14: in
 // probabilities that is 2^-28 of the row's largest, or 2^-20 of the unit's.
 //
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
@@ -319,7 +319,8 @@ struct Walker {
     }
     const int32_t* table = s.table + it.b * s.table_stride;
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
-    int ev_top = KC_EXP_MIN, o_unit = 0;
+    Scales scales;
+    int o_unit = 0;
     const float slack = kSafe && far ? 0.f : KA_SLACK;
     met_far = false;
     char* stage = ring;
@@ -336,7 +337,7 @@ struct Walker {
       const int page = reinterpret_cast<const int*>(scale)[2], j0 = unit * KA_UNIT;
       const float ks = scale[0];
       const int ev_page = scale_exponent(scale[1]), ev = kSafe && far ? 0 : ev_page;   // (of far rows: nothing of it in the exponent)
-      const bool apart = scales_apart(ev, ev, ev_top);
+      scales.see(ev, ev);
       if (kSafe && far && ev_page != o_unit) {
         const float to = exp2i(o_unit - ev_page);
 #pragma unroll
@@ -374,15 +375,19 @@ struct Walker {
           old[x] = ref[n][x];
           const bool up = high[x] > old[x] + slack;
           moves = moves || up;
-          ref[n][x] = up ? rintf(high[x]) : old[x];   // (ahead of the vote: the exponentials wait for it)
+          ref[n][x] = up ? high[x] : old[x];   // (ahead of the vote: the exponentials wait for it)
           set_add(x);
         }
-        if (apart) moves = moves || below_reference(high[0], old[0]) || below_reference(high[1], old[1]);
+        if (scales.apart) moves = moves || below_reference(high[0], old[0]) || below_reference(high[1], old[1]);
         if (__any_sync(0xffffffffu, moves)) {
           float shrink[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (apart) {
+            if (scales.ever && ref[n][x] != old[x]) {
+              ref[n][x] = rintf(high[x]);
+              set_add(x);
+            }
+            if (scales.apart) {
               float total = sum[n][x];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -391,7 +396,7 @@ struct Walker {
                 set_add(x);
               }
             }
-            shrink[x] = exp2_whole(old[x] - ref[n][x]);
+            shrink[x] = rescale(old[x], ref[n][x]);
             sum[n][x] *= shrink[x];
             met_far = met_far || is_far(ref[n][x]);
           }

@@ -52,22 +52,30 @@ struct AttnWorkspace {
 
 __device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) > 0x7F800000u; }
 
-// The reference of a row's exponents (see the head of kv_attn.cu), a whole number: what has been added up is rescaled by powers of two, without a rounding however often
-// it moves. high: the largest s + ev of the tokens in hand, -inf where the row sees none, NaN where it has no number: neither moves it. Down only where the scale of the tokens
-// in hand is the cause (scales_apart). (With the limit for all tokens, 2 x 512 queries at 8192 took 200 us in place of 190: most rows of a hierarchical mask have tiles of which they see
-// a few unlikely tokens.)
-__device__ __forceinline__ bool scales_apart(int ev_low, int ev_high, int& ev_top) {   // ev_top: the largest so far
-  ev_top = max(ev_top, ev_high);
-  return ev_top - ev_low > KA_APART;
-}
+// The reference of a row's exponents (see the head of kv_attn.cu). high: the largest s + ev of the tokens in hand, -inf where the row sees none, NaN where it has no number: neither moves it. Up it
+// goes to the largest number itself, whose probability is then rounded without an error: the weight of one token is often most of a row's. Down only where the scale of the tokens
+// in hand is the cause (apart). (With the limit for all tokens, 2 x 512 queries at 8192 took 200 us in place of 190: most rows of a hierarchical mask have tiles of which they see
+// a few unlikely tokens.) From the first such tokens on it stays whole, so that it may move with every page and what has been added up is not rounded.
+struct Scales {
+  int top = KC_EXP_MIN;         // the largest exponent so far
+  bool apart, ever = false;     // the ones in hand are far below it; some were
+  __device__ __forceinline__ void see(int low, int high) {
+    top = max(top, high);
+    apart = top - low > KA_APART;
+    ever = ever || apart;
+  }
+};
 __device__ __forceinline__ bool below_reference(float high, float ref) { return high < ref - KA_DEPTH && high != -INFINITY; }
 // Downwards no further than lets the row's sum reach 2^64: O is below 2^40 times that.
 __device__ __forceinline__ float reference_below(float high, float ref, float sum) {
   const int room = max(64 - (static_cast<int>(__float_as_uint(sum) >> 23) - 127), 0);
   return fmaxf(rintf(high), ref - static_cast<float>(room));
 }
-// 2^x of a whole number or an infinity; 0 below 2^-126
-__device__ __forceinline__ float exp2_whole(float x) { return __uint_as_float(static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x))) + 127) << 23); }
+// what was added up with reference `from` is worth with `to`: 2^(from - to), of whole numbers exactly, and 1 where nothing moves (-inf, too)
+__device__ __forceinline__ float rescale(float from, float to) {
+  const float x = from - to, y = fast_exp2(x), whole = __uint_as_float(static_cast<uint32_t>(max(-127, min(127, __float2int_rn(x))) + 127) << 23);
+  return from == to ? 1.f : x == rintf(x) ? whole : y;
+}
 
 // four numbers of a bfloat16 row, a lane each, to halves: times the power of two that brings the row's largest finite magnitude to 2^14; returns its exponent
 __device__ __forceinline__ int row_to_halves(uint2& v) {

@@ -414,7 +414,8 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           commit_uniform(bar(CB_PV));
         };
         float ref = -INFINITY, sum = 0.f;
-        int ev_top = KC_EXP_MIN, o_unit = 0;
+        Scales scales;
+        int o_unit = 0;
         bool met_far = false;
         const float slack = far ? 0.f : KA_SLACK, offset = far ? 0.f : KA_OFFSET;   // (far: 8 - ref would round)
         uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
@@ -486,10 +487,11 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             top[page] = fmaxf(highest(x[0]), highest(x[1]));
           }
           const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
-          const bool up = high > ref + slack, down = scales_apart(min(ev[0], ev[1]), max(ev[0], ev[1]), ev_top) && below_reference(high, ref);
+          scales.see(min(ev[0], ev[1]), max(ev[0], ev[1]));
+          const bool up = high > ref + slack, down = scales.apart && below_reference(high, ref);
           const bool units = far && ev_tile != o_unit;   // the whole CTA
           if (__any_sync(0xffffffffu, up || down || units)) {
-            const float to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref, shrink_o = exp2_whole(ref - to) * (units ? exp2i(o_unit - ev_tile) : 1.f), shrink = exp2_whole(ref - to);
+            const float to = up ? (scales.ever ? rintf(high) : high) : down ? reference_below(high, ref, sum) : ref, shrink = rescale(ref, to), shrink_o = units ? shrink * exp2i(o_unit - ev_tile) : shrink;
             met_far = met_far || is_far(to);
             if (units) o_unit = ev_tile;
             if (u > 0 && __any_sync(0xffffffffu, units || (to != ref && ref != -INFINITY))) {   // O is complete: its last product came before these scores

@@ -114,7 +114,7 @@ def values_of(rng, B, Hkv, n, D, kind):
 def check_causal(c, q, table, lens, o, lse, weights):
     """Against the definition in 64 bits, without metadata. Tolerances as derived in test_gpu_kv_cache.py, and one term more: probabilities are rounded to halves, whose steps end at
     2**-24. With M the row's largest p 2**ev (ev: the exponent of the page's V scale), P its largest p and m the largest p 2**ev of a page, the kernels bring a token's p 2**ev to a half after a
-    factor of at least 2**8 / (sqrt(2) M), and of 2**8 / (sqrt(2) 2**4 P 2**ev) or 2**-4 / (sqrt(2) m) (their reference is a whole number, hence the root): it is off by 2**-25 / factor, which is
+    factor of at least 2**8 / (sqrt(2) M), and of 2**8 / (sqrt(2) 2**4 P 2**ev) or 2**-4 / (sqrt(2) m) (their reference may be the whole number next to the largest, hence the root): it is off by 2**-25 / factor, which is
     sqrt(2) 2**-33 min(M, max(2**4 P 2**ev, 2**12 m)), times the stored number. A tile of many rows has two pages whose exponents are at most 4 apart: m of a page and its neighbours. Taken as 2**-32."""
     want = as_oracle(c)
     B, H, T, D = q.shape
@@ -446,3 +446,23 @@ def test_weights_of_few_rows_over_page_tables_that_are_wide():
         o, lse = cache_attention(q, c, wide, i32(lens), return_lse=True, weights=w)
         assert torch.cuda.max_memory_allocated() - held < (64 << 20)
         check_causal(c, q, table, lens, o, lse, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("G,T", [(1, 1), (12, 1), (2, 16), (1, 40), (4, 40)])
+def test_a_token_that_has_all_the_weight_gives_its_value(dtype, G, T):
+    """The first query of a sequence sees its own token alone, another one a key that makes 60 bits of difference: their outputs are the cached numbers, which both types hold."""
+    from kerneldev_b200 import cache_append, cache_attention, cache_read
+    rng = np.random.default_rng(G + T)
+    D, lens = 64, [T, 1, 1300]
+    c = make_cache(70, 1, D)
+    table = tables(rng, 3, 21, 70)
+    x = rand_kv(rng, (2, 3, 1, 1300, D), torch.float32, False)
+    x[0, 2, 0, 700] = 40.0
+    cache_append(c, x[0].to(DEV), x[1].to(DEV), i32(table), i32([0, 0, 0]), i32(lens))
+    q = rand_kv(rng, (3, G, T, D), torch.float32, False)
+    q[2] = 1.0 + 0.1 * torch.tensor(rng.random((G, T, D)))
+    o = cache_attention(q.to(dtype).to(DEV), c, i32(table), i32(lens), i32([T, 1, T]))
+    v = cache_read(c, i32(table), i32(lens), 1300, dtype=dtype)[1]
+    assert torch.equal(o[0, :, 0], v[0, 0, :1].expand(G, D)) and torch.equal(o[1, :, 0], v[1, 0, :1].expand(G, D))
+    assert torch.equal(o[2], v[2, 0, 700].expand(G, T, D))
