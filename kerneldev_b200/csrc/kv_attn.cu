@@ -272,7 +272,7 @@ template <int D, int NT>
 struct Walker {
   float o[NT][D / 16][4];
   float ref[NT][2], sum[NT][2];
-  bool met_far;   // some row was far at some time
+  Scales scales;
 
   // starts the copies of a unit (nothing at or beyond `last`)
   static __device__ __forceinline__ void fetch(const kd_cache& c, const Lane<D>& place, int h, int unit, int last, int page, char* stage) {
@@ -319,10 +319,9 @@ struct Walker {
     }
     const int32_t* table = s.table + it.b * s.table_stride;
     const int free_end = c.desc != nullptr ? 0 : q.min_limit;   // units below it need no mask
-    Scales scales;
+    scales = Scales{};
     int o_unit = 0;
     const float slack = kSafe && far ? 0.f : KA_SLACK;
-    met_far = false;
     char* stage = ring;
     for (int unit = first; unit < last; unit += KA_WARPS) {
       cp_async_wait<0>();
@@ -374,31 +373,29 @@ struct Walker {
           high[x] = fmaf(top, k[x], static_cast<float>(ev));
           old[x] = ref[n][x];
           const bool up = high[x] > old[x] + slack;
-          moves = moves || up;
+          moves = moves | up | (scales.apart & (high[x] < old[x] - KA_DEPTH));   // (no branch here: it costs 4 % of the time with 32 rows; -inf is seen to below)
           ref[n][x] = up ? high[x] : old[x];   // (ahead of the vote: the exponentials wait for it)
           set_add(x);
         }
-        if (scales.apart) moves = moves || below_reference(high[0], old[0]) || below_reference(high[1], old[1]);
         if (__any_sync(0xffffffffu, moves)) {
           float shrink[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (scales.ever && ref[n][x] != old[x]) {
-              ref[n][x] = rintf(high[x]);
-              set_add(x);
-            }
-            if (scales.apart) {
+          for (int x = 0; x < 2; ++x) shrink[x] = ref[n][x] == old[x] ? 1.f : fast_exp2(old[x] - ref[n][x]);
+          if (scales.ever())
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
               float total = sum[n][x];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-              if (below_reference(high[x], old[x])) {
-                ref[n][x] = reference_below(high[x], old[x], total);
-                set_add(x);
-              }
+              if (ref[n][x] != old[x]) ref[n][x] = rintf(high[x]);
+              else if (scales.apart && below_reference(high[x], old[x])) ref[n][x] = reference_below(high[x], old[x], total);
+              set_add(x);
+              shrink[x] = rescale(old[x], ref[n][x]);
             }
-            shrink[x] = rescale(old[x], ref[n][x]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
             sum[n][x] *= shrink[x];
-            met_far = met_far || is_far(ref[n][x]);
+            scales.look(ref[n][x]);
           }
 #pragma unroll
           for (int m = 0; m < D / 16; ++m)
@@ -526,7 +523,7 @@ cache_attention_kernel(const __grid_constant__ kd_cache c, const __grid_constant
     Walker<D, NT> w;
     float* scores = shape.score_rows > 0 ? ws.scores + (static_cast<size_t>(it.b) * c.H + it.h) * s.blocks * KC_PAGE * shape.score_rows : nullptr;
     w.template walk<false>(c, s, place, it, sh.q, first, last, next_page, ring, scores, shape.score_rows, false);
-    const bool far = __any_sync(0xffffffffu, w.met_far);
+    const bool far = __any_sync(0xffffffffu, w.scales.met_far());
     if (w.any_nan() || far) {
       next_page = Walker<D, NT>::begin(c, s, place, it, first, last, ring);
       w.template walk<true>(c, s, place, it, sh.q, first, last, next_page, ring, nullptr, 0, far);

@@ -57,13 +57,16 @@ __device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0
 // in hand is the cause (apart). (With the limit for all tokens, 2 x 512 queries at 8192 took 200 us in place of 190: most rows of a hierarchical mask have tiles of which they see
 // a few unlikely tokens.) From the first such tokens on it stays whole, so that it may move with every page and what has been added up is not rounded.
 struct Scales {
-  int top = KC_EXP_MIN;         // the largest exponent so far
-  bool apart, ever = false;     // the ones in hand are far below it; some were
+  uint32_t seen = 64 + KC_EXP_MIN;   // the largest exponent so far + 64 (8 bits); 256: some were far below it; 512: a row was far (see KA_FAR). One register
+  bool apart;                        // the ones in hand are far below it
   __device__ __forceinline__ void see(int low, int high) {
-    top = max(top, high);
-    apart = top - low > KA_APART;
-    ever = ever || apart;
+    const int top = max(static_cast<int>(seen & 255u), high + 64);
+    apart = top - (low + 64) > KA_APART;
+    seen = (seen & ~255u) | static_cast<uint32_t>(top) | (apart ? 256u : 0u);
   }
+  __device__ __forceinline__ bool ever() const { return (seen & 256u) != 0u; }
+  __device__ __forceinline__ void look(float ref) { seen |= is_far(ref) ? 512u : 0u; }
+  __device__ __forceinline__ bool met_far() const { return (seen & 512u) != 0u; }
 };
 __device__ __forceinline__ bool below_reference(float high, float ref) { return high < ref - KA_DEPTH && high != -INFINITY; }
 // Downwards no further than lets the row's sum reach 2^64: O is below 2^40 times that.

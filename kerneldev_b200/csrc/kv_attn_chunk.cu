@@ -250,8 +250,9 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         // chain of loads (page, scale) stood between two tiles.
         const int32_t* table = s.table + it.b * s.table_stride;
         const int page0 = sh.item.page0, page_end = page0 + sh.item.here;
-        int next = page0, step = 2, batch = page0, batch_page, raw_ahead = 0, batch_ev;
+        int next = page0, batch = page0, batch_page, raw_ahead = 0, batch_ev;
         float batch_ks;
+        uint32_t alone;   // bit l: the V scales of page l of the batch and the next one are too far apart for one reference of the exponents
         auto ask = [&](int from) { return from + lane < page_end ? table[from + lane] : -1; };
         auto open_batch = [&](int from, int raw) {
           batch = from;
@@ -260,17 +261,17 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           batch_ks = batch_page >= 0 ? c.k_scale[place] : 1.f;
           batch_ev = batch_page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
           raw_ahead = ask(from + 32);
+          const int apart = batch_ev - __shfl_down_sync(0xffffffffu, batch_ev, 1), page_behind = __shfl_down_sync(0xffffffffu, batch_page, 1);
+          alone = __ballot_sync(0xffffffffu, batch_page >= 0 && page_behind >= 0 && (apart < -most_apart || apart > most_apart));
         };
         open_batch(page0, ask(page0));
-        // The descriptor of this thread's token of the tile at `next`, asked for when the tile before it was found, and the tile's pages: two, or one where the V scales of
-        // two are too far apart for one reference of the exponents.
+        auto is_alone = [&]() { return (alone >> (next - batch) & 1u) != 0u; };
+        // The descriptor of this thread's token of the tile at `next`, asked for when the tile before it was found, and the tile's pages: two, or one that is alone.
         uint32_t ahead_desc = 0u;
         auto peek = [&]() {
           if (next - batch > 30) open_batch(next, next - batch == 32 ? raw_ahead : ask(next));
           const int p0 = __shfl_sync(0xffffffffu, batch_page, next - batch), p1 = __shfl_sync(0xffffffffu, batch_page, next - batch + 1), page = r < KC_PAGE ? p0 : p1;
-          const int apart = __shfl_sync(0xffffffffu, batch_ev, next - batch) - __shfl_sync(0xffffffffu, batch_ev, next - batch + 1);
-          step = p0 >= 0 && p1 >= 0 && (apart < -most_apart || apart > most_apart) ? 1 : 2;
-          const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0 && r < KC_PAGE * step;
+          const bool alive = next < page_end && next * KC_PAGE + r < it.len && page >= 0 && (r < KC_PAGE || !is_alone());
           ahead_desc = !alive ? 0u : metadata ? c.desc[block_index(c, page, it.h) * KC_PAGE + (r & (KC_PAGE - 1))] : TD_CTX;
         };
         peek();
@@ -286,11 +287,12 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
               cur.ks[x] = __shfl_sync(0xffffffffu, batch_ks, next - batch + x);
               cur.ev[x] = __shfl_sync(0xffffffffu, batch_ev, next - batch + x);
             }
-            if (step == 1) cur.page[1] = -1;
+            const bool single = is_alone();
+            if (single) cur.page[1] = -1;
             if (cur.page[1] < 0) cur.ev[1] = cur.ev[0];   // (a page that is not there says nothing about scales)
             if (cur.page[0] < 0) cur.ev[0] = cur.ev[1];
             const uint32_t ctx = __ballot_sync(0xffffffffu, (cur.desc & TD_CTX) != 0u);
-            next += step;
+            next += single ? 1 : 2;
             if (!metadata) {
               if (cur.j0 >= rows.max_limit) return false;   // (the limits are no more than the length)
               peek();
@@ -416,7 +418,6 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         float ref = -INFINITY, sum = 0.f;
         Scales scales;
         int o_unit = 0;
-        bool met_far = false;
         const float slack = far ? 0.f : KA_SLACK, offset = far ? 0.f : KA_OFFSET;   // (far: 8 - ref would round)
         uint32_t nan_cols[4] = {0u, 0u, 0u, 0u};
         bool ok = true;
@@ -491,8 +492,13 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           const bool up = high > ref + slack, down = scales.apart && below_reference(high, ref);
           const bool units = far && ev_tile != o_unit;   // the whole CTA
           if (__any_sync(0xffffffffu, up || down || units)) {
-            const float to = up ? (scales.ever ? rintf(high) : high) : down ? reference_below(high, ref, sum) : ref, shrink = rescale(ref, to), shrink_o = units ? shrink * exp2i(o_unit - ev_tile) : shrink;
-            met_far = met_far || is_far(to);
+            float to = up ? high : ref, shrink = up ? fast_exp2(ref - to) : 1.f;
+            if (scales.ever()) {
+              to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref;
+              shrink = rescale(ref, to);
+            }
+            const float shrink_o = units ? shrink * exp2i(o_unit - ev_tile) : shrink;
+            scales.look(to);
             if (units) o_unit = ev_tile;
             if (u > 0 && __any_sync(0xffffffffu, units || (to != ref && ref != -INFINITY))) {   // O is complete: its last product came before these scores
 #pragma unroll 1
@@ -582,7 +588,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           }
           tc_fence_before_sync();
         }
-        if (bad || met_far) atomicOr(&sh.redo, (bad ? 1u : 0u) | (met_far ? 2u : 0u));
+        if (bad || scales.met_far()) atomicOr(&sh.redo, (bad ? 1u : 0u) | (scales.met_far() ? 2u : 0u));
         if (tid == 0) sh.tiles = u;   // (the converters' count is the same)
         if (!ok && warp == 0) {   // what has been issued ends before TMEM is given back
           if (u > 0) drain_wait(bar(CB_PV), (n_t + u - 1) & 1);
