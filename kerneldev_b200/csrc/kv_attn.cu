@@ -754,7 +754,7 @@ __device__ __forceinline__ float at_most_one(float x) {
 
 // weights[j] += sum over the query rows of the head of softmax_j, from the rows' maxima and sums. A warp has a unit of tokens for all
 // rows, so that nothing is added twice and the order is fixed; a CTA kPages pages of one head: 8, and 2 where those would be CTAs for less than half
-// of the SMs (8 x 2000 tokens of one head, 1024 rows: 203 us with 2, 301 with 8; 2 x 8192 tokens of 8 heads, 512 rows: 284 and 223: each CTA goes through all query rows). The queries of the next tile of rows are asked for before the tile in hand is worked on.
+// of the SMs (8 x 2000 tokens of one head, 1024 rows: 203 us with 2, 301 with 8; 2 x 8192 tokens of 8 heads, 512 rows: 284 and 223; now 206 and 231: each CTA goes through all query rows). The queries of the next tile of rows are asked for before the tile in hand is worked on.
 template <int D>
 constexpr int KW_STAGE = Stage<D>::V_AT + KA_UNIT * 4;   // K and descriptors
 template <int D, int NT, int kPages>
