@@ -78,8 +78,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, l
     its head; tokens beyond its last dimension are left out. sm_scale: head_dim ** -0.5 by default. out_layout: "contiguous", or "input" for O in
     the memory layout of q.
 
-    A weight enters the product with v with 11 bits, and with an error of no more than 2**-28 of the row's largest weight, or, where the value scales of pages
-    are more than 2**4 apart, 2**-20 of its page's largest.
+    A weight enters the product with v with 11 bits, and with an error of no more than 2**-28 of the row's largest weight (2**-25 in rows with scores
+    beyond 2**16, in powers of two), or, where the value scales of pages are more than 2**4 apart, 2**-20 of its page's largest.
 
     Returns O in the type of q, or (O, LSE) with ``return_lse`` (float32 (batch, heads, time), base 2)."""
     if out_layout not in ("contiguous", "input"):
