@@ -36,7 +36,7 @@ extern "C" {
 
 #define KD_F16 0
 #define KD_BF16 1
-#define KD_F32 2   /* kd_span_mean and kd_cocktail only */
+#define KD_F32 2   /* where an entry point says so */
 
 #define KD_TILE 128 /* mask classification and kernel tile edge (tokens) */
 
@@ -273,6 +273,36 @@ int kd_cocktail_index(const int64_t* tokens, int64_t stride_b, int32_t B, int32_
                       int32_t* first_mask, int32_t* counts_host, void* stream);
 int kd_cocktail_scores(const kd_cocktail* p, void* stream);
 int kd_cocktail_grad(const kd_cocktail* p, void* stream);
+
+/* ---- rotation of the heads of q and k by position, with their norms -------------------------------------------------
+ * No counterpart in the reference, whose GPTModel adds learned positions to the embeddings (model.py:127-160). Stands ahead of kd_attn_fwd and
+ * kd_cache_append.
+ *
+ * Row x of D numbers (one head of one token): y = weight * x / sqrt(mean(x^2) + eps) where there is a weight, else y = x. Pair i of R / 2, elements i and
+ * i + R / 2 or, interleaved, 2 i and 2 i + 1: (a, b) -> (a cos - b sin, b cos + a sin) with the angle position * steps[i] / 2^64 turns. Elements from R on are y.
+ * All in 32 bits and rounded once. kd_rotate writes q_out and k_out; kd_rotate_grad reads their gradients from q_out and k_out and writes dq and dk (q and k are read
+ * for those that have a weight) and, where they are not NULL, dq_weight and dk_weight, summed over all rows in a fixed order. */
+typedef struct kd_rotation {
+  kd_tensor q, k;           /* (B, Hq, T, D) and (B, Hk, T, D); pointers and byte strides multiples of 16 */
+  kd_tensor q_out, k_out;
+  kd_tensor dq, dk;         /* kd_rotate_grad */
+  const void *q_weight, *k_weight;   /* NULL: no norm, or D numbers */
+  void *dq_weight, *dk_weight;       /* kd_rotate_grad: NULL, or D numbers; need the weight and workspace */
+  const uint64_t* steps;    /* (R / 2) turns of a pair for a step of its position, as fractions of 2^64; 8-byte aligned */
+  const void* positions;    /* (axes, B, T) of int32, or int64 with pos_is_64; NULL: 0 .. T - 1 */
+  const int32_t* offsets;   /* NULL, or (B), added to the positions of the first axis; with positions NULL to those of all pairs */
+  int64_t pos_stride_a, pos_stride_b, pos_stride_t;   /* elements; any, 0 among them */
+  int32_t B, Hq, Hk, T, D, R;   /* Hk may be 0. D and R multiples of 16, R <= D <= 128 */
+  int32_t dtype, w_dtype;   /* KD_F16 / KD_BF16 / KD_F32, of all tensors; of the weights */
+  int32_t interleaved, pos_is_64;
+  int32_t axes;             /* 1 to 3: pairs below ends[0] turn by the first axis, below ends[1] by the second, others by the third */
+  int32_t ends[2];
+  float eps;
+  void* workspace;          /* kd_rotate_grad with dq_weight or dk_weight: kd_rotate_grad_workspace bytes, 16-byte aligned */
+} kd_rotation;
+int kd_rotate(const kd_rotation* p, void* stream);
+int kd_rotate_grad(const kd_rotation* p, void* stream);
+int kd_rotate_grad_workspace(const kd_rotation* p, size_t* bytes);
 
 /* ---- key/value cache in 8 bits: attention over it, appending, reading, eviction -------------------------------------
  * No counterpart in the reference, whose GPTModel.generate (model.py:316-355) runs the whole sequence again for every token.

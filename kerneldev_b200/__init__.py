@@ -6,6 +6,7 @@ Public surface (mirrors the reference's ``original_kernel`` module for the atten
   metadata_from_tokens                                          -- in_span / span_id / is_prefix from token ids
   span_index, span_means, cocktail_scores                       -- the span-mean head of model.py:258-296
   KVCache, cache_append, cache_attention, cache_evict, cache_read -- generating with a key/value cache in 8 bits
+  Rotation, rotate_heads                                        -- norms of queries and keys, rotation by positions
 
 Names are resolved on first use, so that ``python -m kerneldev_b200.build`` can (re)build the
 shared library before anything tries to load it. The first use of the operator loads
@@ -17,6 +18,7 @@ _EXPORTS = {
     "clear_plan_cache": "plan", "metadata_from_tokens": "metadata",
     "span_means": "cocktail", "cocktail_scores": "cocktail", "span_index": "cocktail",
     "KVCache": "kv_cache", "cache_append": "kv_cache", "cache_attention": "kv_cache", "cache_evict": "kv_cache", "cache_read": "kv_cache",
+    "Rotation": "rotate", "rotate_heads": "rotate",
 }
 
 __all__ = sorted(_EXPORTS)

@@ -29,6 +29,7 @@ EXPORTS = (
     "kd_cocktail_index", "kd_cocktail_scores", "kd_cocktail_grad",
     "kd_cast",
     "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read",
+    "kd_rotate", "kd_rotate_grad", "kd_rotate_grad_workspace",
 )
 
 
@@ -101,6 +102,18 @@ class KdCacheEviction(Structure):
     ]
 
 
+class KdRotation(Structure):
+    _fields_ = [
+        ("q", KdTensor), ("k", KdTensor), ("q_out", KdTensor), ("k_out", KdTensor), ("dq", KdTensor), ("dk", KdTensor),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("dq_weight", c_void_p), ("dk_weight", c_void_p),
+        ("steps", c_void_p), ("positions", c_void_p), ("offsets", c_void_p),
+        ("pos_stride_a", c_int64), ("pos_stride_b", c_int64), ("pos_stride_t", c_int64),
+        ("B", c_int32), ("Hq", c_int32), ("Hk", c_int32), ("T", c_int32), ("D", c_int32), ("R", c_int32),
+        ("dtype", c_int32), ("w_dtype", c_int32), ("interleaved", c_int32), ("pos_is_64", c_int32), ("axes", c_int32), ("ends", c_int32 * 2),
+        ("eps", c_float), ("workspace", c_void_p),
+    ]
+
+
 class KdError(RuntimeError):
     """A libkd_attention.so entry point rejected its arguments or a CUDA call failed."""
 
@@ -145,9 +158,12 @@ def load() -> ctypes.CDLL:
     lib.kd_cache_attention_workspace.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheQueries), POINTER(c_size_t)]
     lib.kd_cache_evict.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheEviction), c_void_p]
     lib.kd_cache_read.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), c_void_p, c_int32, c_int32, POINTER(KdTensor), POINTER(KdTensor), c_void_p]
+    lib.kd_rotate.argtypes = lib.kd_rotate_grad.argtypes = [POINTER(KdRotation), c_void_p]
+    lib.kd_rotate_grad_workspace.argtypes = [POINTER(KdRotation), POINTER(c_size_t)]
     for name in ("kd_plan_layout_get", "kd_classify", "kd_mask_dense", "kd_attn_fwd", "kd_attn_bwd", "kd_attn_bwd_hadamard", "kd_attn_bwd_static",
                  "kd_workspace_bytes", "kd_workspace_bytes_fused", "kd_hadamard", "kd_metadata_from_tokens", "kd_span_index", "kd_span_mean",
-                 "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read"):
+                 "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read",
+                 "kd_rotate", "kd_rotate_grad", "kd_rotate_grad_workspace"):
         getattr(lib, name).restype = c_int32
     _lib = lib
     return lib

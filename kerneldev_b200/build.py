@@ -21,7 +21,7 @@ HOST_SOURCE = CSRC / "host.cpp"
 INCLUDE_DIR = PKG_DIR.parent / "include"
 
 SOURCES = ["capi.cu", "plan.cu", "attn_fwd.cu", "attn_fwd_wide.cu", "attn_bwd.cu", "attn_bwd_fused.cu", "hadamard.cu", "metadata.cu", "cocktail.cu", "cast.cu",
-           "kv_cache.cu", "kv_attn.cu", "kv_attn_chunk.cu"]
+           "kv_cache.cu", "kv_attn.cu", "kv_attn_chunk.cu", "rotate.cu"]
 HEADERS = sorted(p.name for p in (Path(__file__).resolve().parent / "csrc").glob("*.cuh"))
 
 NVCC_FLAGS = [
@@ -49,7 +49,7 @@ def _stale() -> bool:
 
 def build_host(force: bool = False) -> Path:
     """Compiles the host extension (csrc/host.cpp) against the installed torch."""
-    deps = [HOST_SOURCE, CSRC / "host_cache.hpp", INCLUDE_DIR / "kd_attention.h"]
+    deps = [HOST_SOURCE, CSRC / "host_cache.hpp", CSRC / "host_rotate.hpp", INCLUDE_DIR / "kd_attention.h"]
     if not force and HOST_PATH.exists() and all(d.stat().st_mtime <= HOST_PATH.stat().st_mtime for d in deps):
         return HOST_PATH
     import sysconfig

@@ -379,6 +379,71 @@ int kd_span_mean(int32_t backward, const void* a, int64_t a_sb, int64_t a_st, vo
                           static_cast<cudaStream_t>(stream));
 }
 
+// ---- rotation of heads ----
+
+static int check_rotation(const kd_rotation* p) {
+  if (!p) return set_error(KD_ERR_ARG, "rotation is null");
+  if (p->B < 0 || p->T < 0 || p->Hq < 1 || p->Hk < 0) return set_error(KD_ERR_ARG, "bad shape B=%d Hq=%d Hk=%d T=%d", p->B, p->Hq, p->Hk, p->T);
+  if (p->D < 16 || p->D > 128 || p->D % 16 != 0) return set_error(KD_ERR_ARG, "head dim %d not supported (a multiple of 16 from 16 to 128)", p->D);
+  if (p->R < 16 || p->R > p->D || p->R % 16 != 0) return set_error(KD_ERR_ARG, "%d rotated elements not supported (a multiple of 16 from 16 to the head dim)", p->R);
+  for (int t : {p->dtype, p->w_dtype})
+    if (t != KD_F16 && t != KD_BF16 && t != KD_F32) return set_error(KD_ERR_ARG, "dtype %d not supported", t);
+  if (p->axes < 1 || p->axes > 3) return set_error(KD_ERR_ARG, "%d axes not supported (1 to 3)", p->axes);
+  if (p->axes > 1 && !p->positions) return set_error(KD_ERR_ARG, "several axes need positions");
+  if (p->axes < 3 && p->positions && p->ends[p->axes - 1] < p->R / 2) return set_error(KD_ERR_ARG, "pairs from %d on have no axis", p->ends[p->axes - 1]);
+  if (!(p->eps >= 0.f) || !(p->eps < 1e30f)) return set_error(KD_ERR_ARG, "eps must not be negative, and finite");
+  if (!p->steps) return set_error(KD_ERR_ARG, "steps is null");
+  if ((reinterpret_cast<uintptr_t>(p->steps) & 7u) != 0) return set_error(KD_ERR_ALIGN, "steps not 8-byte aligned");
+  if (static_cast<int64_t>(p->B) * p->T > INT32_MAX - 256) return set_error(KD_ERR_LIMIT, "%d x %d tokens are too many for one call", p->B, p->T);
+  return 0;
+}
+
+static int check_rotated(const kd_rotation* p, bool grad) {
+  const int es = p->dtype == KD_F32 ? 4 : 2;
+  for (int i = 0; i < (p->Hk > 0 ? 2 : 1); ++i) {
+    const kd_tensor &x = i == 0 ? p->q : p->k, &y = i == 0 ? p->q_out : p->k_out, &dx = i == 0 ? p->dq : p->dk;
+    const bool read = !grad || (i == 0 ? p->q_weight : p->k_weight) != nullptr;
+    const char* name = i == 0 ? "q" : "k";
+    if ((read && !x.ptr) || !y.ptr || (grad && !dx.ptr)) return set_error(KD_ERR_ARG, "%s, its output or its gradient is null", name);
+    if ((read && !aligned16(x, es)) || !aligned16(y, es) || (grad && !aligned16(dx, es)))
+      return set_error(KD_ERR_ALIGN, "%s, its output or its gradient: pointers and byte strides must be multiples of 16", name);
+  }
+  return 0;
+}
+
+int kd_rotate(const kd_rotation* p, void* stream) {
+  int rc = check_rotation(p);
+  if (rc) return rc;
+  if (p->B == 0 || p->T == 0) return 0;
+  if ((rc = check_rotated(p, false)) != 0 || (rc = check_device()) != 0) return rc;
+  return launch_rotate(*p, false, static_cast<cudaStream_t>(stream));
+}
+
+int kd_rotate_grad_workspace(const kd_rotation* p, size_t* bytes) {
+  const int rc = check_rotation(p);
+  if (rc) return rc;
+  if (!bytes) return set_error(KD_ERR_ARG, "bytes is null");
+  *bytes = p->B == 0 || p->T == 0 ? 0 : rotate_grad_workspace(*p);
+  return 0;
+}
+
+int kd_rotate_grad(const kd_rotation* p, void* stream) {
+  int rc = check_rotation(p);
+  if (rc) return rc;
+  if ((p->dq_weight && !p->q_weight) || (p->dk_weight && (!p->k_weight || p->Hk == 0))) return set_error(KD_ERR_ARG, "the gradient of a weight that is not there");
+  if (p->B == 0 || p->T == 0) {
+    if (p->dq_weight || p->dk_weight) return set_error(KD_ERR_ARG, "the gradient of a weight of no rows is not written");
+    return 0;
+  }
+  if ((rc = check_rotated(p, true)) != 0) return rc;
+  if (p->dq_weight || p->dk_weight) {
+    if (!p->workspace) return set_error(KD_ERR_ARG, "workspace is null");
+    if ((reinterpret_cast<uintptr_t>(p->workspace) & 15u) != 0) return set_error(KD_ERR_ALIGN, "workspace not 16-byte aligned");
+  }
+  if ((rc = check_device()) != 0) return rc;
+  return launch_rotate(*p, true, static_cast<cudaStream_t>(stream));
+}
+
 // ---- the 8-bit cache ----
 
 static int check_cache_strides(const kd_tensor& t, int es, const char* name) {

@@ -130,4 +130,7 @@ int launch_span_mean(bool backward, const void* a, int64_t a_sb, int64_t a_st, v
                      int T, int C, int S, int dtype, const int32_t* starts, const int32_t* ends, const int32_t* n_starts,
                      const int32_t* n_ends, cudaStream_t stream);
 
+int launch_rotate(const kd_rotation& p, bool grad, cudaStream_t stream);
+size_t rotate_grad_workspace(const kd_rotation& p);
+
 }  // namespace kd

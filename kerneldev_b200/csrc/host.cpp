@@ -16,7 +16,9 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <atomic>
@@ -76,6 +78,9 @@ struct Library {
   decltype(&kd_cache_attention_workspace) cache_attention_workspace = nullptr;
   decltype(&kd_cache_evict) cache_evict = nullptr;
   decltype(&kd_cache_read) cache_read = nullptr;
+  decltype(&kd_rotate) rotate = nullptr;
+  decltype(&kd_rotate_grad) rotate_grad = nullptr;
+  decltype(&kd_rotate_grad_workspace) rotate_grad_workspace = nullptr;
   decltype(&kd_last_error) last_error = nullptr;
 };
 Library lib;
@@ -104,6 +109,9 @@ void bind(const py::dict& a) {
   take(lib.cache_attention_workspace, a, "kd_cache_attention_workspace");
   take(lib.cache_evict, a, "kd_cache_evict");
   take(lib.cache_read, a, "kd_cache_read");
+  take(lib.rotate, a, "kd_rotate");
+  take(lib.rotate_grad, a, "kd_rotate_grad");
+  take(lib.rotate_grad_workspace, a, "kd_rotate_grad_workspace");
   take(lib.last_error, a, "kd_last_error");
 }
 
@@ -979,6 +987,10 @@ Tensor cocktail_scores(const Tensor& x_, const Tensor& tokens_, int64_t tok_span
 
 #include "host_cache.hpp"
 
+// ---- rotation of heads -----------------------------------------------------------------------------------------
+
+#include "host_rotate.hpp"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1024,6 +1036,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cocktail_scores", &cocktail_scores, NoGil());
   py::class_<KVCache, KVCachePtr>(m, "KVCache")
       .def(py::init<const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&>(), NoGil());
+  py::class_<Rotation, RotationPtr>(m, "Rotation").def(py::init<const Tensor&, int64_t, bool, const std::vector<int64_t>&>(), NoGil());
+  m.def("rotate_heads", &rotate_heads, NoGil());
   m.def("cache_append", &cache_append, NoGil());
   m.def("cache_attention", &cache_attention, NoGil());
   m.def("cache_evict", &cache_evict, NoGil());
