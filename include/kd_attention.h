@@ -386,6 +386,25 @@ int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_evi
 int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k,
                   const kd_tensor* v, void* stream);
 
+/* ---- the same cache in 4 bits -----------------------------------------------------------------------------------------
+ * Numbers are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even element in the low half, and stand for their value times the scale of their group: 16 numbers of a
+ * row side by side. A scale is a byte, bits 14 .. 7 of an IEEE half (5 bits of exponent, 3 of mantissa, no sign, subnormals among them): the nearest to a sixth of the group's largest magnitude, 10240
+ * (byte 226) at most. Numbers are the nearest to what they are divided by it; ties go to even; larger ones saturate. Byte 255 stands for 16 NaN: of a group that has an infinity or NaN
+ * in it. Bytes 227 .. 254 are never written. An append does not touch what is there, and eviction moves bytes as they are. All else is as above. */
+typedef struct kd_cache4 {
+  void *k, *v;              /* e2m1 (pages, H, KD_CACHE_PAGE, D / 2 bytes) contiguous, 16-byte aligned */
+  uint8_t *k_scale, *v_scale; /* (pages, H, KD_CACHE_PAGE, D / 16) contiguous, 16-byte aligned */
+  uint32_t* desc;           /* as in kd_cache */
+  int32_t pages, H, D;
+  uint32_t* status_mirror;
+} kd_cache4;
+int kd_cache4_append(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream);
+int kd_cache4_attention(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream);
+int kd_cache4_attention_workspace(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes);
+int kd_cache4_evict(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream);
+int kd_cache4_read(const kd_cache4* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k,
+                   const kd_tensor* v, void* stream);
+
 /* Message for the last negative return value on this host thread. */
 const char* kd_last_error(void);
 

@@ -29,6 +29,7 @@ EXPORTS = (
     "kd_cocktail_index", "kd_cocktail_scores", "kd_cocktail_grad",
     "kd_cast",
     "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read",
+    "kd_cache4_append", "kd_cache4_attention", "kd_cache4_attention_workspace", "kd_cache4_evict", "kd_cache4_read",
     "kd_rotate", "kd_rotate_grad", "kd_rotate_grad_workspace",
 )
 
@@ -72,6 +73,10 @@ class KdCache(Structure):
         ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("desc", c_void_p),
         ("pages", c_int32), ("H", c_int32), ("D", c_int32), ("status_mirror", c_void_p),
     ]
+
+
+class KdCache4(Structure):
+    _fields_ = list(KdCache._fields_)   # (its scales are bytes)
 
 
 class KdCacheSeqs(Structure):
@@ -158,11 +163,14 @@ def load() -> ctypes.CDLL:
     lib.kd_cache_attention_workspace.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheQueries), POINTER(c_size_t)]
     lib.kd_cache_evict.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), POINTER(KdCacheEviction), c_void_p]
     lib.kd_cache_read.argtypes = [POINTER(KdCache), POINTER(KdCacheSeqs), c_void_p, c_int32, c_int32, POINTER(KdTensor), POINTER(KdTensor), c_void_p]
+    for name in ("append", "attention", "attention_workspace", "evict", "read"):   # the 8-bit cache's, with the other structure
+        getattr(lib, f"kd_cache4_{name}").argtypes = [POINTER(KdCache4), *getattr(lib, f"kd_cache_{name}").argtypes[1:]]
     lib.kd_rotate.argtypes = lib.kd_rotate_grad.argtypes = [POINTER(KdRotation), c_void_p]
     lib.kd_rotate_grad_workspace.argtypes = [POINTER(KdRotation), POINTER(c_size_t)]
     for name in ("kd_plan_layout_get", "kd_classify", "kd_mask_dense", "kd_attn_fwd", "kd_attn_bwd", "kd_attn_bwd_hadamard", "kd_attn_bwd_static",
                  "kd_workspace_bytes", "kd_workspace_bytes_fused", "kd_hadamard", "kd_metadata_from_tokens", "kd_span_index", "kd_span_mean",
                  "kd_cache_append", "kd_cache_attention", "kd_cache_attention_workspace", "kd_cache_evict", "kd_cache_read",
+                 "kd_cache4_append", "kd_cache4_attention", "kd_cache4_attention_workspace", "kd_cache4_evict", "kd_cache4_read",
                  "kd_rotate", "kd_rotate_grad", "kd_rotate_grad_workspace"):
         getattr(lib, name).restype = c_int32
     _lib = lib

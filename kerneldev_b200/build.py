@@ -21,7 +21,7 @@ HOST_SOURCE = CSRC / "host.cpp"
 INCLUDE_DIR = PKG_DIR.parent / "include"
 
 SOURCES = ["capi.cu", "plan.cu", "attn_fwd.cu", "attn_fwd_wide.cu", "attn_bwd.cu", "attn_bwd_fused.cu", "hadamard.cu", "metadata.cu", "cocktail.cu", "cast.cu",
-           "kv_cache.cu", "kv_attn.cu", "kv_attn_chunk.cu", "rotate.cu"]
+           "kv_cache.cu", "kv_cache4.cu", "kv_attn.cu", "kv_attn_rows8.cu", "kv_attn_rows4.cu", "kv_attn_chunk8.cu", "kv_attn_chunk4.cu", "rotate.cu"]
 HEADERS = sorted(p.name for p in (Path(__file__).resolve().parent / "csrc").glob("*.cuh"))
 
 NVCC_FLAGS = [

@@ -1,6 +1,7 @@
 // extern "C" surface of libkd_attention.so: argument validation, tensor-map encoding,
 // error strings. Declarations and the reference interfaces they replace: include/kd_attention.h.
 #include <stdarg.h>
+#include <stddef.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -444,7 +445,24 @@ int kd_rotate_grad(const kd_rotation* p, void* stream) {
   return launch_rotate(*p, true, static_cast<cudaStream_t>(stream));
 }
 
-// ---- the 8-bit cache ----
+// ---- the caches in 8 and 4 bits ----
+
+// The kernels take a 4-bit cache as a kd_cache whose scales are bytes: the structures have the same fields in the same places.
+static_assert(sizeof(kd_cache) == sizeof(kd_cache4) && offsetof(kd_cache, k_scale) == offsetof(kd_cache4, k_scale) && offsetof(kd_cache, desc) == offsetof(kd_cache4, desc) &&
+                  offsetof(kd_cache, pages) == offsetof(kd_cache4, pages) && offsetof(kd_cache, status_mirror) == offsetof(kd_cache4, status_mirror),
+              "kd_cache4 is laid out as kd_cache");
+struct AnyCache {
+  kd_cache c;
+  int bits;
+  bool null;
+  explicit AnyCache(const kd_cache* p) : c{}, bits(8), null(p == nullptr) {
+    if (p) c = *p;
+  }
+  explicit AnyCache(const kd_cache4* p) : c{}, bits(4), null(p == nullptr) {
+    if (p) memcpy(&c, p, sizeof c);
+  }
+};
+
 
 static int check_cache_strides(const kd_tensor& t, int es, const char* name) {
   if (!t.ptr) return set_error(KD_ERR_ARG, "%s is null", name);
@@ -452,13 +470,15 @@ static int check_cache_strides(const kd_tensor& t, int es, const char* name) {
   return 0;
 }
 
-static int check_cache(const kd_cache* c, const kd_cache_seqs* s) {
-  if (!c || !s) return set_error(KD_ERR_ARG, "cache / sequences is null");
+static int check_cache(const AnyCache& any, const kd_cache_seqs* s) {
+  if (any.null || !s) return set_error(KD_ERR_ARG, "cache / sequences is null");
+  const kd_cache* c = &any.c;
   if (c->pages < 1 || c->H < 1) return set_error(KD_ERR_ARG, "bad cache shape pages=%d H=%d", c->pages, c->H);
   if (c->D < 16 || c->D > 128 || c->D % 16 != 0) return set_error(KD_ERR_ARG, "head dim %d not supported (a multiple of 16 from 16 to 128)", c->D);
   if (!c->k || !c->v || !c->k_scale || !c->v_scale) return set_error(KD_ERR_ARG, "k / v / k_scale / v_scale is null");
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->desc)) & 15u) != 0)
     return set_error(KD_ERR_ALIGN, "k / v / desc not 16-byte aligned");   // (a null desc is)
+  if (any.bits == 4 && ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15u) != 0) return set_error(KD_ERR_ALIGN, "k_scale / v_scale not 16-byte aligned");
   if (s->B < 0 || s->blocks < 0) return set_error(KD_ERR_ARG, "bad shape B=%d blocks=%d", s->B, s->blocks);
   if (s->blocks > (1 << 24)) return set_error(KD_ERR_LIMIT, "blocks=%d exceeds 2^24", s->blocks);
   if (s->B > 0 && !s->lens) return set_error(KD_ERR_ARG, "lens is null");
@@ -467,7 +487,7 @@ static int check_cache(const kd_cache* c, const kd_cache_seqs* s) {
   return 0;
 }
 
-int kd_cache_append(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream) {
+static int cache_append(const AnyCache& c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream) {
   int rc = check_cache(c, s);
   if (rc) return rc;
   if (!t) return set_error(KD_ERR_ARG, "tokens is null");
@@ -477,11 +497,10 @@ int kd_cache_append(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_to
   const int es = t->dtype == KD_F32 ? 4 : 2;
   if ((rc = check_cache_strides(t->k, es, "k")) != 0 || (rc = check_cache_strides(t->v, es, "v")) != 0) return rc;
   if ((rc = check_device()) != 0) return rc;
-  return launch_cache_append(*c, *s, *t, static_cast<cudaStream_t>(stream));
+  return (c.bits == 8 ? launch_cache_append : launch_cache4_append)(c.c, *s, *t, static_cast<cudaStream_t>(stream));
 }
 
-int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k,
-                  const kd_tensor* v, void* stream) {
+static int cache_read(const AnyCache& c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k, const kd_tensor* v, void* stream) {
   int rc = check_cache(c, s);
   if (rc) return rc;
   if (count < 0) return set_error(KD_ERR_ARG, "bad token count %d", count);
@@ -491,10 +510,10 @@ int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* star
   const int es = dtype == KD_F32 ? 4 : 2;
   if ((rc = check_cache_strides(*k, es, "k")) != 0 || (rc = check_cache_strides(*v, es, "v")) != 0) return rc;
   if ((rc = check_device()) != 0) return rc;
-  return launch_cache_read(*c, *s, start, count, dtype, *k, *v, static_cast<cudaStream_t>(stream));
+  return (c.bits == 8 ? launch_cache_read : launch_cache4_read)(c.c, *s, start, count, dtype, *k, *v, static_cast<cudaStream_t>(stream));
 }
 
-int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream) {
+static int cache_evict(const AnyCache& c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream) {
   int rc = check_cache(c, s);
   if (rc) return rc;
   if (!e) return set_error(KD_ERR_ARG, "eviction is null");
@@ -505,39 +524,50 @@ int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_evi
   if ((e->w_len > 0 && !e->weights) || !e->out_table || !e->index || !e->out_weights || !e->out_lens)
     return set_error(KD_ERR_ARG, "weights / out_table / index / out_weights / out_lens is null");
   if ((rc = check_device()) != 0) return rc;
-  return launch_cache_evict(*c, *s, *e, static_cast<cudaStream_t>(stream));
+  return launch_cache_evict(c.c, *s, *e, c.bits, static_cast<cudaStream_t>(stream));
 }
 
-static int check_queries(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q) {
+static int check_queries(const AnyCache& c, const kd_cache_seqs* s, const kd_cache_queries* q) {
   int rc = check_cache(c, s);
   if (rc) return rc;
   if (!q) return set_error(KD_ERR_ARG, "queries is null");
-  if (q->T < 0 || q->H < 1 || q->H % c->H != 0) return set_error(KD_ERR_ARG, "bad queries: T=%d, H=%d for %d heads of keys", q->T, q->H, c->H);
+  if (q->T < 0 || q->H < 1 || q->H % c.c.H != 0) return set_error(KD_ERR_ARG, "bad queries: T=%d, H=%d for %d heads of keys", q->T, q->H, c.c.H);
   if (q->dtype != KD_F16 && q->dtype != KD_BF16) return set_error(KD_ERR_ARG, "dtype %d not supported (fp16 / bf16)", q->dtype);
   if (static_cast<int64_t>(s->B) * q->H > INT32_MAX / (q->T > 0 ? q->T : 1))
     return set_error(KD_ERR_LIMIT, "%d x %d x %d query rows are too many", s->B, q->H, q->T);
   return 0;
 }
 
-int kd_cache_attention_workspace(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes) {
+static int cache_workspace(const AnyCache& c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes) {
   const int rc = check_queries(c, s, q);
   if (rc) return rc;
   if (!bytes) return set_error(KD_ERR_ARG, "bytes is null");
-  *bytes = s->B == 0 || q->T == 0 ? 0 : cache_attention_workspace(*c, *s, *q);
+  *bytes = s->B == 0 || q->T == 0 ? 0 : cache_attention_workspace(c.c, *s, *q, c.bits);
   return 0;
 }
 
-int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) {
+static int cache_attention(const AnyCache& c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) {
   int rc = check_queries(c, s, q);
   if (rc) return rc;
   if (!(q->sm_scale > 0.f) || !(q->sm_scale < 1e30f)) return set_error(KD_ERR_ARG, "sm_scale must be positive and finite");
   if (s->B == 0 || q->T == 0) return 0;
   if ((rc = check_cache_strides(q->q, 2, "q")) != 0 || (rc = check_cache_strides(q->o, 2, "o")) != 0) return rc;
   if (q->weights && q->w_len < 0) return set_error(KD_ERR_ARG, "w_len is negative");
-  if (!q->workspace && cache_attention_workspace(*c, *s, *q) > 0) return set_error(KD_ERR_ARG, "workspace is null");
+  if (!q->workspace && cache_attention_workspace(c.c, *s, *q, c.bits) > 0) return set_error(KD_ERR_ARG, "workspace is null");
   if ((reinterpret_cast<uintptr_t>(q->workspace) & 15u) != 0) return set_error(KD_ERR_ALIGN, "workspace not 16-byte aligned");
   if ((rc = check_device()) != 0) return rc;
-  return launch_cache_attention(*c, *s, *q, static_cast<cudaStream_t>(stream));
+  return launch_cache_attention(c.c, *s, *q, c.bits, static_cast<cudaStream_t>(stream));
 }
+
+int kd_cache_append(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream) { return cache_append(AnyCache(c), s, t, stream); }
+int kd_cache4_append(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_tokens* t, void* stream) { return cache_append(AnyCache(c), s, t, stream); }
+int kd_cache_attention(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) { return cache_attention(AnyCache(c), s, q, stream); }
+int kd_cache4_attention(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_queries* q, void* stream) { return cache_attention(AnyCache(c), s, q, stream); }
+int kd_cache_attention_workspace(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes) { return cache_workspace(AnyCache(c), s, q, bytes); }
+int kd_cache4_attention_workspace(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_queries* q, size_t* bytes) { return cache_workspace(AnyCache(c), s, q, bytes); }
+int kd_cache_evict(const kd_cache* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream) { return cache_evict(AnyCache(c), s, e, stream); }
+int kd_cache4_evict(const kd_cache4* c, const kd_cache_seqs* s, const kd_cache_eviction* e, void* stream) { return cache_evict(AnyCache(c), s, e, stream); }
+int kd_cache_read(const kd_cache* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k, const kd_tensor* v, void* stream) { return cache_read(AnyCache(c), s, start, count, dtype, k, v, stream); }
+int kd_cache4_read(const kd_cache4* c, const kd_cache_seqs* s, const int32_t* start, int32_t count, int32_t dtype, const kd_tensor* k, const kd_tensor* v, void* stream) { return cache_read(AnyCache(c), s, start, count, dtype, k, v, stream); }
 
 }  // extern "C"

@@ -78,6 +78,11 @@ struct Library {
   decltype(&kd_cache_attention_workspace) cache_attention_workspace = nullptr;
   decltype(&kd_cache_evict) cache_evict = nullptr;
   decltype(&kd_cache_read) cache_read = nullptr;
+  decltype(&kd_cache4_append) cache4_append = nullptr;
+  decltype(&kd_cache4_attention) cache4_attention = nullptr;
+  decltype(&kd_cache4_attention_workspace) cache4_attention_workspace = nullptr;
+  decltype(&kd_cache4_evict) cache4_evict = nullptr;
+  decltype(&kd_cache4_read) cache4_read = nullptr;
   decltype(&kd_rotate) rotate = nullptr;
   decltype(&kd_rotate_grad) rotate_grad = nullptr;
   decltype(&kd_rotate_grad_workspace) rotate_grad_workspace = nullptr;
@@ -109,6 +114,11 @@ void bind(const py::dict& a) {
   take(lib.cache_attention_workspace, a, "kd_cache_attention_workspace");
   take(lib.cache_evict, a, "kd_cache_evict");
   take(lib.cache_read, a, "kd_cache_read");
+  take(lib.cache4_append, a, "kd_cache4_append");
+  take(lib.cache4_attention, a, "kd_cache4_attention");
+  take(lib.cache4_attention_workspace, a, "kd_cache4_attention_workspace");
+  take(lib.cache4_evict, a, "kd_cache4_evict");
+  take(lib.cache4_read, a, "kd_cache4_read");
   take(lib.rotate, a, "kd_rotate");
   take(lib.rotate_grad, a, "kd_rotate_grad");
   take(lib.rotate_grad_workspace, a, "kd_rotate_grad_workspace");
@@ -983,7 +993,7 @@ Tensor cocktail_scores(const Tensor& x_, const Tensor& tokens_, int64_t tok_span
   return scores;
 }
 
-// ---- 8-bit key/value cache -------------------------------------------------------------------------------------
+// ---- key/value cache -------------------------------------------------------------------------------------------
 
 #include "host_cache.hpp"
 

@@ -1,4 +1,4 @@
-// Host path of the 8-bit key/value cache (part of host.cpp, which includes it): argument checks, allocations and calls.
+// Host path of the key/value caches in 8 and 4 bits (part of host.cpp, which includes it): argument checks, allocations and calls.
 
 // A cache is the caller's tensors; its status word is a word of pinned memory that the kernels write when a length, a page number or
 // a span id does not fit, or a bounded wait gave up. The next call looks at it without a synchronisation.
@@ -8,16 +8,33 @@ struct KVCache {
   std::shared_ptr<StatusMirror> mirror;
   std::atomic<unsigned long long> held_by{0};   // the last capture whose graph has been given the mirror to hold
   kd_cache abi{};
+  int bits;   // 4: the scales are bytes
+
+  // A call of the library with this cache.
+  template <typename F8, typename F4, typename... A>
+  int call(F8* eight, F4* four, A... args) const {
+    if (bits == 8) return eight(&abi, args...);
+    kd_cache4 c{abi.k, abi.v, reinterpret_cast<uint8_t*>(abi.k_scale), reinterpret_cast<uint8_t*>(abi.v_scale), abi.desc, abi.pages, abi.H, abi.D, abi.status_mirror};
+    return four(&c, args...);
+  }
 
   KVCache(const Tensor& k_, const Tensor& v_, const Tensor& ks, const Tensor& vs, const OptTensor& d) : k(k_), v(v_), k_scale(ks), v_scale(vs), desc(d) {
     KD_VALUE(k.dim() == 4 && k.size(2) == KD_CACHE_PAGE, "k must be (pages, heads, ", KD_CACHE_PAGE, ", head_dim), got ", k.sizes());
     KD_VALUE(v.sizes() == k.sizes(), "k and v must have the same shape, got ", k.sizes(), ", ", v.sizes());
-    KD_VALUE(k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn, "k and v must be float8_e4m3fn");
-    const int64_t P = k.size(0), H = k.size(1), D = k.size(3);
+    bits = k.scalar_type() == at::kByte ? 4 : 8;
+    const auto type = bits == 4 ? at::kByte : at::kFloat8_e4m3fn;
+    KD_VALUE(k.scalar_type() == type && v.scalar_type() == type, "k and v must be float8_e4m3fn, or uint8 for numbers of 4 bits");
+    const int64_t P = k.size(0), H = k.size(1), D = bits == 4 ? 2 * k.size(3) : k.size(3);
     KD_VALUE(D % 16 == 0 && D >= 16 && D <= 128, "head_dim ", D, " is not supported (a multiple of 16 from 16 to 128)");
     KD_VALUE(P >= 1 && P <= INT32_MAX && H >= 1 && H <= INT32_MAX, "a cache has at least one page and one head, got ", k.sizes());
-    for (const Tensor* s : {&k_scale, &v_scale})
-      KD_VALUE(s->dim() == 2 && s->size(0) == P && s->size(1) == H && s->scalar_type() == at::kFloat, "scales must be float32 (pages, heads) = (", P, ", ", H, ")");
+    for (const Tensor* s : {&k_scale, &v_scale}) {
+      if (bits == 4) {
+        KD_VALUE(s->dim() == 4 && s->size(0) == P && s->size(1) == H && s->size(2) == KD_CACHE_PAGE && s->size(3) == D / 16 && s->scalar_type() == at::kByte,
+                 "scales of numbers of 4 bits must be uint8 (pages, heads, ", KD_CACHE_PAGE, ", head_dim / 16) = (", P, ", ", H, ", ", KD_CACHE_PAGE, ", ", D / 16, ")");
+      } else {
+        KD_VALUE(s->dim() == 2 && s->size(0) == P && s->size(1) == H && s->scalar_type() == at::kFloat, "scales must be float32 (pages, heads) = (", P, ", ", H, ")");
+      }
+    }
     if (desc.has_value())
       KD_VALUE(desc->dim() == 3 && desc->size(0) == P && desc->size(1) == H && desc->size(2) == KD_CACHE_PAGE && desc->scalar_type() == at::kInt,
                "desc must be int32 (pages, heads, ", KD_CACHE_PAGE, ")");
@@ -29,8 +46,8 @@ struct KVCache {
     mirror = std::make_shared<StatusMirror>();
     abi.k = k.data_ptr();
     abi.v = v.data_ptr();
-    abi.k_scale = k_scale.data_ptr<float>();
-    abi.v_scale = v_scale.data_ptr<float>();
+    abi.k_scale = static_cast<float*>(k_scale.data_ptr());
+    abi.v_scale = static_cast<float*>(v_scale.data_ptr());
     abi.desc = desc.has_value() ? reinterpret_cast<uint32_t*>(desc->data_ptr<int32_t>()) : nullptr;
     abi.pages = static_cast<int32_t>(P);
     abi.H = static_cast<int32_t>(H);
@@ -110,7 +127,7 @@ void check_heads(const KVCache& c, const Tensor& t, const char* name, int64_t he
   KD_VALUE(t.dim() == 4, name, " must be (batch, heads, time, head_dim)");
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor; there is no CPU path");
   KD_VALUE(t.device() == c.k.device(), name, " must live on ", c.k.device());
-  KD_VALUE(t.size(3) == c.k.size(3), name, " has head_dim ", t.size(3), ", the cache ", c.k.size(3));
+  KD_VALUE(t.size(3) == c.abi.D, name, " has head_dim ", t.size(3), ", the cache ", c.abi.D);
   KD_VALUE(heads == 0 || t.size(1) == heads, name, " has ", t.size(1), " heads, the cache ", heads);
   KD_VALUE(t.size(2) <= (1 << 30), name, " has too many tokens");
 }
@@ -152,7 +169,7 @@ void cache_append(KVCache& c, const Tensor& k_, const Tensor& v_, const Tensor& 
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture = c.before_launch(stream);
-  check(lib.cache_append(&c.abi, &s.abi, &t, stream));
+  check(c.call(lib.cache_append, lib.cache4_append, &s.abi, &t, stream));
   c.after_launch(stream, capture);
 }
 
@@ -203,7 +220,7 @@ std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const T
   }
   c10::cuda::CUDAGuard guard(c.k.device());
   size_t bytes = 0;
-  check(lib.cache_attention_workspace(&c.abi, &s.abi, &p, &bytes));
+  check(c.call(lib.cache_attention_workspace, lib.cache4_attention_workspace, &s.abi, &p, &bytes));
   if (bytes > 0) {
     workspace = empty_on({static_cast<int64_t>(bytes)}, at::kByte, q.device());
     p.workspace = workspace.data_ptr();
@@ -211,7 +228,7 @@ std::tuple<Tensor, Tensor> cache_attention(KVCache& c, const Tensor& q_, const T
   c.poll();
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture = c.before_launch(stream);
-  check(lib.cache_attention(&c.abi, &s.abi, &p, stream));
+  check(c.call(lib.cache_attention, lib.cache4_attention, &s.abi, &p, stream));
   if (!out.is_same(o)) o.copy_(out);
   c.after_launch(stream, capture);
   return {o, return_lse ? lse : Tensor()};
@@ -248,7 +265,7 @@ std::tuple<Tensor, Tensor, Tensor> cache_evict(KVCache& c, const Tensor& table, 
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture = c.before_launch(stream);
-  check(lib.cache_evict(&c.abi, &s.abi, &e, stream));
+  check(c.call(lib.cache_evict, lib.cache4_evict, &s.abi, &e, stream));
   c.after_launch(stream, capture);
   return {index, out_lens, out_w};
 }
@@ -269,7 +286,7 @@ std::tuple<Tensor, Tensor> cache_read(KVCache& c, const Tensor& table, const Ten
   c10::cuda::CUDAGuard guard(c.k.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const Capture capture = c.before_launch(stream);
-  check(lib.cache_read(&c.abi, &s.abi, from, static_cast<int32_t>(count), dtype_code(type), &kt, &vt, stream));
+  check(c.call(lib.cache_read, lib.cache4_read, &s.abi, from, static_cast<int32_t>(count), dtype_code(type), &kt, &vt, stream));
   c.after_launch(stream, capture);
   return {k, v};
 }

@@ -1,7 +1,8 @@
-// What the two kernels of the cache's attention share (kv_attn.cu: few query rows, kv_attn_chunk.cu: many): rows and their masks, how the pages
+// What the two kernels of the cache's attention share (kv_attn_rows.cuh: few query rows, kv_attn_chunk.cuh: many): rows and their masks, how the pages
 // are shared out, the parts that a join puts together.
 #pragma once
 #include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "kv_cache.cuh"
@@ -52,7 +53,7 @@ struct AttnWorkspace {
 
 __device__ __forceinline__ bool is_nan(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) > 0x7F800000u; }
 
-// The reference of a row's exponents (see the head of kv_attn.cu). high: the largest s + ev of the tokens in hand, -inf where the row sees none, NaN where it has no number: neither moves it. Up it
+// The reference of a row's exponents (see the head of kv_attn_rows.cuh). high: the largest s + ev of the tokens in hand, -inf where the row sees none, NaN where it has no number: neither moves it. Up it
 // goes to the largest number itself, whose probability is then rounded without an error: the weight of one token is often most of a row's. Down only where the scale of the tokens
 // in hand is the cause (apart). (With the limit for all tokens, 2 x 512 queries at 8192 took 200 us in place of 190: most rows of a hierarchical mask have tiles of which they see
 // a few unlikely tokens.) From the first such tokens on it stays whole, so that it may move with every page and what has been added up is not rounded.
@@ -318,8 +319,33 @@ inline cudaError_t launch_shares(bool even, void (*kernel)(P...), unsigned grid,
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-// kv_attn_chunk.cu
+// call: a generic lambda that takes the head dim as a type
+template <typename F>
+static cudaError_t by_head_dim(int D, F call) {
+  switch (D) {
+    case 16: return call(std::integral_constant<int, 16>{});
+    case 32: return call(std::integral_constant<int, 32>{});
+    case 48: return call(std::integral_constant<int, 48>{});
+    case 64: return call(std::integral_constant<int, 64>{});
+    case 80: return call(std::integral_constant<int, 80>{});
+    case 96: return call(std::integral_constant<int, 96>{});
+    case 112: return call(std::integral_constant<int, 112>{});
+    default: return call(std::integral_constant<int, 128>{});
+  }
+}
+
+// kv_attn_rows.cuh: warps of a CTA, rows of a tile, tokens of a unit
+constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32, KA_TILE = 8, KA_UNIT = 32;
+// CTAs of an SM, by tiles of query rows: what registers and shared memory allow
+__host__ __device__ constexpr int ctas_of(int nt) { return nt <= 2 ? 3 : 2; }
+// kv_attn_chunk.cuh
 constexpr int KC_ROWS = 128, KC_CTAS = 2;   // query rows of an item, CTAs of an SM
-int launch_attention_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+// for each number format: attention of few rows, the weights from the rows' statistics, attention of many rows
+cudaError_t launch_attention_rows8(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+cudaError_t launch_attention_rows4(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+cudaError_t launch_attention_weights8(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+cudaError_t launch_attention_weights4(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+cudaError_t launch_attention_chunk8(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
+cudaError_t launch_attention_chunk4(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream);
 
 }  // namespace kd

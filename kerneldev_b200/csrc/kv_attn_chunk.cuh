@@ -1,13 +1,13 @@
-// Attention over the 8-bit cache for many query rows of a key head (a chunk of a prompt): 128 rows of a CTA on tcgen05, two CTAs an SM.
+// Attention over the cache for many query rows of a key head (a chunk of a prompt), for both number formats (kBits): 128 rows of a CTA on tcgen05, two CTAs an SM.
 //
-// The products are GEMMs here, so the cache's tiles are converted once for 128 rows: e4m3 to halves (exact) into swizzled shared memory, and both
+// The products are GEMMs here, so the cache's tiles are converted once for 128 rows: to halves (exact; numbers of 4 bits with their scales) into swizzled shared memory, and both
 // products run on halves with S, P and O in TMEM. Roles (256 threads, so that each has 128 registers):
 //   warps 0-3  softmax, a thread to a row: masks, running maximum, P over the scores it was made from. Warp 0 issues the products: P V when all four
 //              warps' P is there, directly behind it the next scores
 //   warps 4-7  converters: 128 tokens (two pages) at a time from global memory through registers, one tile ahead. They decide which tiles are worked on:
 //              one that no row of the CTA sees is left out (spans of a hierarchical mask, tokens behind the chunk)
 // Q, one K tile and one V tile are 96 KB at head dim 128 and S and O 256 columns, so that two CTAs share an SM: the exponentials of one run under
-// the products of the other. Scales, the offset of the probabilities and the slack of the maximum are as in kv_attn.cu.
+// the products of the other. Scales, the offset of the probabilities and the slack of the maximum are as in kv_attn_rows.cuh.
 //
 // A tile's chain is: K converted -> S -> softmax -> P V, and the next S directly behind P V. Barriers, each used once a tile:
 //   K   converters: K and the tile's record are there     S   S is complete (K is free)
@@ -17,6 +17,7 @@
 //
 // NaN: an item whose output has any is done once more with NaN values as zeros and a bit for each (token, dim) that was one; a row that sees the
 // token gets NaN there. So is one that has met scores beyond KA_FAR, from rounded scores, with V's scale in the units of O.
+#pragma once
 #include <stddef.h>
 
 #include <algorithm>
@@ -96,13 +97,26 @@ __device__ __forceinline__ void row_words(const RowMask& m, const ChunkRecord& r
   }
 }
 
+// 16 numbers of a token as they are stored
+template <int kBits>
+struct Piece16;
+template <>
+struct Piece16<8> {
+  uint4 v;
+};
+template <>
+struct Piece16<4> {
+  uint2 v;
+  uint32_t scale;   // the byte
+};
+
 // A converter thread's bytes of a tile as halves: rounds of 32 tokens and a block of 64 head dims, at fixed distances from the first one's two places.
 // kWithoutNan: NaN as zeros, and a bit for each in nan_bits (of the first round's token and head dims).
 template <int D, bool kWithoutNan>
-__device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[2], const uint4 (&reg)[4 * ChunkShared<D>::BLOCKS], uint16_t (*nan_bits)[8], int col) {
+__device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[2], const Piece16<8> (&reg)[4 * ChunkShared<D>::BLOCKS], uint16_t (*nan_bits)[8], int col) {
 #pragma unroll
   for (int i = 0; i < 4 * ChunkShared<D>::BLOCKS; ++i) {
-    uint32_t w[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+    uint32_t w[4] = {reg[i].v.x, reg[i].v.y, reg[i].v.z, reg[i].v.w};
     if constexpr (kWithoutNan) {
       uint32_t bits = 0;
 #pragma unroll
@@ -121,7 +135,28 @@ __device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[
   }
 }
 
-template <int D>
+// ... of 4 bits: a group's numbers times its scale
+template <int D, bool kWithoutNan>
+__device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[2], const Piece16<4> (&reg)[4 * ChunkShared<D>::BLOCKS], uint16_t (*nan_bits)[8], int col) {
+#pragma unroll
+  for (int i = 0; i < 4 * ChunkShared<D>::BLOCKS; ++i) {
+    uint32_t s = both_halves(reg[i].scale);
+    if constexpr (kWithoutNan) {
+      const uint32_t gone = nan_scales(s);
+      s &= ~gone;
+      const int d = (i >> 2) * 64 + col;
+      if (d < D) nan_bits[32 * (i & 3)][d / 16] = static_cast<uint16_t>(gone);
+    }
+    uint32_t h[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) h[x] = times(e2m1x2_to_f16x2(x < 4 ? reg[i].v.x : reg[i].v.y, x & 3), s);
+    uint8_t* at = to + (i & 3) * 4096 + (i >> 2) * ChunkShared<D>::BLOCK;
+    *reinterpret_cast<uint4*>(at + place[0]) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(at + place[1]) = make_uint4(h[4], h[5], h[6], h[7]);
+  }
+}
+
+template <int kBits, int D>
 __global__ void __launch_bounds__(CH_THREADS, KC_CTAS)
 cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                              const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
@@ -168,7 +203,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
     if (sh.item.here < 0) return false;
     const Item it = sh.item.it;
 
-    // ---- Q as halves (bfloat16 times a power of two, see kv_attn.cu), masks and what the rows see together ----
+    // ---- Q as halves (bfloat16 times a power of two, see kv_attn_rows.cuh), masks and what the rows see together ----
     if (tid == 0) {
       sh.rows = ChunkRows{0u, 0u, 0, 0};
       sh.redo = 0u;
@@ -244,7 +279,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           float ks[2];
           uint32_t desc;
         } cur;
-        uint4 reg[ROUNDS];   // K of a tile, then its V: each is asked for when the other has been stored, and awaited when its place is free
+        Piece16<kBits> reg[ROUNDS];   // K of a tile, then its V: each is asked for when the other has been stored, and awaited when its place is free
         bool ok = true;
         // Page numbers and scales of 32 blocks in the lanes of each warp, the page numbers of the 32 behind them already asked for: with a look-up for each tile, its
         // chain of loads (page, scale) stood between two tiles.
@@ -258,9 +293,13 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           batch = from;
           batch_page = from + lane < page_end ? checked_page(c, raw) : -1;
           const size_t place = block_index(c, max(batch_page, 0), it.h);
-          batch_ks = batch_page >= 0 ? c.k_scale[place] : 1.f;
-          batch_ev = batch_page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
+          batch_ks = kBits == 8 && batch_page >= 0 ? c.k_scale[place] : 1.f;
+          batch_ev = kBits == 8 && batch_page >= 0 ? scale_exponent(c.v_scale[place]) : 0;
           raw_ahead = ask(from + 32);
+          if constexpr (kBits == 4) {
+            alone = 0u;
+            return;
+          }
           const int apart = batch_ev - __shfl_down_sync(0xffffffffu, batch_ev, 1), page_behind = __shfl_down_sync(0xffffffffu, batch_page, 1);
           alone = __ballot_sync(0xffffffffu, batch_page >= 0 && page_behind >= 0 && (apart < -most_apart || apart > most_apart));
         };
@@ -318,15 +357,29 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           return false;
         };
         const uint32_t place[2] = {chunk_place(row0, col), chunk_place(row0, col + 8)};   // of later rounds at fixed distances: 32 tokens 4 KB, a block 16 KB
-        auto fetch = [&](const void* from) {
-          const uint8_t* base[2];
+        auto fetch = [&](const void* from, const float* scales) {
+          const uint8_t *base[2], *scale[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) base[x] = static_cast<const uint8_t*>(from) + (block_index(c, max(cur.page[x], 0), it.h) * KC_PAGE + row0) * D + col;
+          for (int x = 0; x < 2; ++x) {
+            const size_t row = block_index(c, max(cur.page[x], 0), it.h) * KC_PAGE + row0;
+            base[x] = static_cast<const uint8_t*>(from) + (kBits == 8 ? row * D + col : row * (D / 2) + col / 2);
+            scale[x] = kBits == 4 ? scales4(scales) + row * (D / K4_GROUP) + col / K4_GROUP : nullptr;
+          }
 #pragma unroll
           for (int i = 0; i < ROUNDS; ++i) {   // tokens 32 (i & 3) + row0, head dims 64 (i >> 2) + col
             const int x = (i & 3) >> 1;
-            reg[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (cur.page[x] >= 0 && (i >> 2) * 64 + col < D) reg[i] = __ldg(reinterpret_cast<const uint4*>(base[x] + (i & 1) * 32 * D + (i >> 2) * 64));
+            const bool there = cur.page[x] >= 0 && (i >> 2) * 64 + col < D;
+            if constexpr (kBits == 8) {
+              reg[i].v = make_uint4(0u, 0u, 0u, 0u);
+              if (there) reg[i].v = __ldg(reinterpret_cast<const uint4*>(base[x] + (i & 1) * 32 * D + (i >> 2) * 64));
+            } else {
+              reg[i].v = make_uint2(0u, 0u);
+              reg[i].scale = 0u;
+              if (there) {
+                reg[i].v = __ldg(reinterpret_cast<const uint2*>(base[x] + (i & 1) * 32 * (D / 2) + (i >> 2) * 32));
+                reg[i].scale = __ldg(scale[x] + (i & 1) * 32 * (D / K4_GROUP) + (i >> 2) * 4);
+              }
+            }
           }
         };
         // A wait of one warp can run out while another's is met: with metadata all hear of it at a barrier that every one of them comes to, before the next words are exchanged.
@@ -341,7 +394,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
         };
         int u = 0;   // tiles of this pass
         bool have = find(n_k % CH_RECORDS);
-        if (have) fetch(c.k);
+        if (have) fetch(c.k, c.k_scale);
         for (;; ++u) {
           // (K's place and the record's slot are free when the scores of the tile before are complete; the slot of two tiles before by then, too)
           if (u > 0) ok = ok && !drop(7, u) && wait(CB_S, n_t + u - 1, 1);
@@ -368,7 +421,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
 #endif
           if (lane == 0) mbar_arrive(bar(CB_K));
           if (!have) break;
-          fetch(c.v);
+          fetch(c.v, c.v_scale);
           have = find((n_k + u + 1) % CH_RECORDS);
           if (u > 0 && (drop(8, u) || !(ok = wait(CB_PV, n_t + u - 1, 1)))) {
             ok = false;
@@ -383,7 +436,7 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           } else
 #endif
           if (lane == 0) mbar_arrive(bar(CB_V));
-          if (have) fetch(c.k);
+          if (have) fetch(c.k, c.k_scale);
         }
       } while (again(pass++));
       if (sh.abort.v != 0u || !shape.even) break;
@@ -429,9 +482,9 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
           if (warp == 0) issue_scores();
           uint32_t w[4];
           row_words(mask, rec, metadata, lane, w);
-          float kf[2] = {score_factor(rec.ks[0], factor), score_factor(rec.ks[1], factor)};
+          float kf[2] = {score_factor(kBits == 8 ? rec.ks[0] : 1.f, factor), score_factor(kBits == 8 ? rec.ks[1] : 1.f, factor)};
           // (far: both pages of a tile have one V scale, and it goes into the units of O)
-          const int ev_tile = rec.ev[0], ev[2] = {far ? 0 : ev_tile, far ? 0 : rec.ev[1]};
+          const int ev_tile = kBits == 8 ? rec.ev[0] : 0, ev[2] = {far ? 0 : ev_tile, far || kBits == 4 ? 0 : rec.ev[1]};
           if (safe) {
             if (!(ok = wait(CB_V, n_t + u, 0))) break;
             for (int j = 0; j < CH_TOKENS; ++j) {
@@ -488,12 +541,13 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
             top[page] = fmaxf(highest(x[0]), highest(x[1]));
           }
           const float high = fmaxf(fmaf(top[0], kf[0], static_cast<float>(ev[0])), fmaf(top[1], kf[1], static_cast<float>(ev[1])));
-          scales.see(min(ev[0], ev[1]), max(ev[0], ev[1]));
+          if (kBits == 8) scales.see(min(ev[0], ev[1]), max(ev[0], ev[1]));
+          else scales.apart = false;
           const bool up = high > ref + slack, down = scales.apart && below_reference(high, ref);
           const bool units = far && ev_tile != o_unit;   // the whole CTA
           if (__any_sync(0xffffffffu, up || down || units)) {
             float to = up ? high : ref, shrink = up ? fast_exp2(ref - to) : 1.f;
-            if (scales.ever()) {
+            if (kBits == 8 && scales.ever()) {
               to = up ? rintf(high) : down ? reference_below(high, ref, sum) : ref;
               shrink = rescale(ref, to);
             }
@@ -605,32 +659,16 @@ cache_attention_chunk_kernel(const __grid_constant__ kd_cache c, const __grid_co
   if (warp == 4) tmem_dealloc(tS, 256);
 }
 
-template <int D>
+template <int kBits, int D>
 static cudaError_t launch_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
   constexpr size_t kShared = sizeof(ChunkShared<D>);
   static_assert(kShared <= 113 * 1024, "two CTAs share an SM");
   static SmemOptIn opt_in;
   static SharedFirst shared_first;
-  cudaError_t e = opt_in(cache_attention_chunk_kernel<D>, kShared);
-  if (e == cudaSuccess) e = shared_first(cache_attention_chunk_kernel<D>);
+  cudaError_t e = opt_in(cache_attention_chunk_kernel<kBits, D>, kShared);
+  if (e == cudaSuccess) e = shared_first(cache_attention_chunk_kernel<kBits, D>);
   const int64_t items = static_cast<int64_t>(s.B) * c.H * a.tiles;
-  return e != cudaSuccess ? e : launch_shares(a.ctas > 0 && a.even, cache_attention_chunk_kernel<D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), CH_THREADS, kShared, stream, c, s, p, a, ws);
-}
-
-int launch_attention_chunk(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_queries& p, const AttnShape& a, const AttnWorkspace& ws, cudaStream_t stream) {
-  cudaError_t e;
-  switch (c.D) {
-    case 16: e = launch_chunk<16>(c, s, p, a, ws, stream); break;
-    case 32: e = launch_chunk<32>(c, s, p, a, ws, stream); break;
-    case 48: e = launch_chunk<48>(c, s, p, a, ws, stream); break;
-    case 64: e = launch_chunk<64>(c, s, p, a, ws, stream); break;
-    case 80: e = launch_chunk<80>(c, s, p, a, ws, stream); break;
-    case 96: e = launch_chunk<96>(c, s, p, a, ws, stream); break;
-    case 112: e = launch_chunk<112>(c, s, p, a, ws, stream); break;
-    default: e = launch_chunk<128>(c, s, p, a, ws, stream);
-  }
-  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention_chunk launch: %s", cudaGetErrorString(e));
-  return 0;
+  return e != cudaSuccess ? e : launch_shares(a.ctas > 0 && a.even, cache_attention_chunk_kernel<kBits, D>, static_cast<unsigned>(a.ctas > 0 ? a.ctas : items), CH_THREADS, kShared, stream, c, s, p, a, ws);
 }
 
 }  // namespace kd

@@ -1,12 +1,10 @@
-// The 8-bit key/value cache without its attention: appending, reading, eviction. See kd_attention.h for the format.
+// The 8-bit key/value cache without its attention: appending, reading, eviction (whose search serves the 4-bit cache as well). See kd_attention.h for the format.
 // All are bound by memory traffic, for a handful of tokens by launches.
 #include <algorithm>
 
 #include "kv_cache.cuh"
 
 namespace kd {
-
-constexpr int KC_THREADS = 256, KC_CHUNKS = KC_PAGE * 128 / 16 / KC_THREADS;   // 16-byte chunks of a block that a thread holds, at most
 
 // max over the block's threads; scratch: a word for each warp
 __device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t* scratch) {
@@ -16,59 +14,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t* scratch) {
   m = scratch[threadIdx.x & (KC_THREADS / 32 - 1)];
   return __reduce_max_sync(0xffffffffu, m);
 }
-
-// 16 numbers of a row as they came: two 16-byte words of a 16-bit type, four of float
-template <int kType>
-struct Raw16 {
-  static constexpr int WORDS = kType == KD_F32 ? 4 : 2;
-  uint4 v[WORDS];
-  __device__ __forceinline__ void load(const void* p) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) v[i] = __ldg(static_cast<const uint4*>(p) + i);
-  }
-  // The largest finite magnitude as the bits of a float, and whether there is a number that is not finite. 16-bit types two at a time: magnitudes
-  // are ordered as their bits are.
-  __device__ __forceinline__ uint32_t amax(bool& special) const {
-    uint32_t top = 0, out = 0;
-    constexpr uint32_t kInf = kType == KD_F32 ? 0x7F800000u : kType == KD_BF16 ? 0x7F807F80u : 0x7C007C00u;
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kType == KD_F32) {
-          const uint32_t u = w[j] & 0x7FFFFFFFu;
-          out |= u >= kInf ? 1u : 0u;
-          top = max(top, u >= kInf ? 0u : u);
-        } else {
-          const uint32_t u = w[j] & 0x7FFF7FFFu, beyond = __vcmpgeu2(u, kInf);
-          out |= beyond;
-          top = __vmaxu2(top, u & ~beyond);
-        }
-      }
-    }
-    special = special || out != 0u;
-    if constexpr (kType == KD_F32) return top;
-    const uint32_t one = max(top & 0xFFFFu, top >> 16);
-    return kType == KD_BF16 ? one << 16 : __float_as_uint(unpack2<false>(one).x);
-  }
-  __device__ __forceinline__ void floats(float (&f)[16]) const {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kType == KD_F32) {
-          f[4 * i + j] = __uint_as_float(w[j]);
-        } else {
-          const float2 x = unpack2<kType == KD_BF16>(w[j]);
-          f[8 * i + 2 * j] = x.x;
-          f[8 * i + 2 * j + 1] = x.y;
-        }
-      }
-    }
-  }
-};
 
 // One block of one head of a sequence, K or V: reads the tokens that are new in it once, keeps them in registers as they came while the CTA
 // agrees on the scale, and writes them as bytes. (Kept as floats they took twice the registers, and half as many CTAs had loads on their way.)
@@ -542,7 +487,7 @@ static cudaError_t launch_cluster(void (*kernel)(P...), unsigned cluster, dim3 g
   return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
-int launch_cache_evict(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_eviction& e, cudaStream_t stream) {
+int launch_cache_evict(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_eviction& e, int bits, cudaStream_t stream) {
   const int W = (e.keep + KC_PAGE - 1) / KC_PAGE;
   const int64_t items = static_cast<int64_t>(s.B) * c.H, grid = items * W;
   // As many CTAs, and threads of them, as hold the longest sequence's keys in registers: 256 threads for up to 4096 tokens, whose barriers are
@@ -553,7 +498,8 @@ int launch_cache_evict(const kd_cache& c, const kd_cache_seqs& s, const kd_cache
   while (threads < KE_MAX_THREADS && static_cast<int64_t>(threads) * cluster * KE_KEYS < tokens) threads *= 2;
   if (grid > INT32_MAX || items * cluster > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d sequences that keep %d tokens of %d heads are too many for one call", s.B, e.keep, c.H);
   cudaError_t r = launch_cluster(cache_select_kernel, cluster, static_cast<unsigned>(items * cluster), threads, stream, c, s, e, cluster);
-  if (r == cudaSuccess) r = launch(cache_gather_kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, e, W);
+  if (r == cudaSuccess)
+    r = bits == 8 ? launch(cache_gather_kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, e, W) : launch_cache4_gather(c, s, e, static_cast<unsigned>(grid), W, stream);
   if (r != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_evict launch: %s", cudaGetErrorString(r));
   return 0;
 }

@@ -1,0 +1,212 @@
+// The 4-bit key/value cache without its attention: appending, reading, and moving what eviction keeps. See kd_attention.h for the format.
+// All are bound by memory traffic, for a handful of tokens by launches. A group of 16 numbers has a scale of its own, so a thread has a group, nothing is agreed on among
+// threads, and what a page holds already is never touched.
+#include "kv_cache.cuh"
+
+namespace kd {
+
+constexpr int C4_CHUNKS = 2 * KC_CHUNKS;   // groups of K and V that a thread holds, at most
+
+struct Group4 {
+  uint2 v;
+  uint32_t scale;
+};
+// A group as it is stored. The scale is the nearest to a sixth of the largest magnitude, and the numbers the nearest to what they are in its units; ties go to even. A
+// quotient by 6 in 32 bits is never rounded onto the middle of two scales: a float next to six times a number of 5 bits is 2^-24 of it away, and a quotient's rounding moves it less. 16-bit
+// numbers are multiplied with the rounded 1 / scale, and the product is brought to a grid of 2^-13 (by the sum with 1536, of which one step is that much): that puts it on the middle of two levels exactly where the
+// quotient is, since numbers of 11 bits and scales of 4 have no other quotient within 2^-14 of a middle (tests/test_kv_cache4_logic.py goes through all of them; without the grid, 7 eighths of 13 fail). Floats are divided.
+template <int kType>
+__device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
+  bool special = false;
+  const float sixth = __fdiv_rn(__uint_as_float(raw.amax(special)), 6.f);
+  const uint32_t u = __float_as_uint(sixth);
+  uint32_t byte = sixth < 0x1p-14f ? static_cast<uint32_t>(__float2int_rn(sixth * 0x1p17f)) : min(K4_TOP, ((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - 896u);
+  const float scale = unpack2<false>(byte << 7).x, inverse = byte != 0u ? __frcp_rn(scale) : 0.f;
+  float f[16];
+  raw.floats(f);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (kType == KD_F32) f[i] = byte != 0u ? __fdiv_rn(f[i], scale) : 0.f;
+    else f[i] = __fsub_rn(__fmaf_rn(f[i], inverse, 1536.f), 1536.f);
+  }
+  if (special) return Group4{make_uint2(0u, 0u), K4_NAN};
+  return Group4{make_uint2(f32x8_to_e2m1x8(f), f32x8_to_e2m1x8(f + 8)), byte};
+}
+
+// One block of one head of a sequence, K and V.
+template <int kType>
+__global__ void __launch_bounds__(KC_THREADS)
+cache4_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_tokens t, int W) {
+  pdl_wait();
+  pdl_launch_dependents();
+  uint32_t item = blockIdx.x;
+  const int h = static_cast<int>(item % static_cast<uint32_t>(c.H));
+  item /= static_cast<uint32_t>(c.H);
+  const int w = static_cast<int>(item % static_cast<uint32_t>(W)), b = static_cast<int>(item / static_cast<uint32_t>(W));
+  // (as for the 8-bit cache: a length or a number of tokens that cannot be says nothing of where to write, and what the table has no more pages for is left out)
+  const int len = s.lens[b], room = s.blocks * KC_PAGE;
+  int n = t.n_new != nullptr ? t.n_new[b] : t.T;
+  const bool valid = len >= 0 && len <= room && n >= 0 && n <= t.T;
+  if (!valid || n > room - len) {
+    if (threadIdx.x == 0) cache_report(c, KC_BAD_LENGTH);
+    if (!valid) return;
+    n = room - len;
+  }
+  const int block = len / KC_PAGE + w, base = block * KC_PAGE;
+  if (base >= len + n || n == 0) return;
+  const int raw_page = s.table[b * s.table_stride + block];
+  const int lo = max(len - base, 0), hi = min(len + n - base, KC_PAGE);   // slots lo .. hi - 1 are new
+  const int per_row = c.D / K4_GROUP, chunks = KC_PAGE * per_row;
+  constexpr int kSize = kType == KD_F32 ? 4 : 2;
+  Raw16<kType> raw[C4_CHUNKS];
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
+    const kd_tensor& x = both >= chunks ? t.v : t.k;
+    if (both < 2 * chunks && slot >= lo && slot < hi)
+      raw[i].load(static_cast<const char*>(x.ptr) + (b * x.stride_b + h * x.stride_h + static_cast<int64_t>(base + slot - len) * x.stride_t + col * K4_GROUP) * kSize);
+  }
+  const int page = checked_page(c, raw_page);
+  if (page < 0) return;
+  const size_t at = block_index(c, page, h);
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row;
+    if (both >= 2 * chunks || slot < lo || (slot >= hi && lo > 0)) continue;
+    Group4 g{make_uint2(0u, 0u), 0u};   // a page that is opened holds nothing of its earlier use
+    if (slot < hi) g = quantise_group(raw[i]);
+    const size_t place = at * chunks + chunk;
+    reinterpret_cast<uint2*>(both >= chunks ? c.v : c.k)[place] = g.v;
+    reinterpret_cast<uint8_t*>(both >= chunks ? c.v_scale : c.k_scale)[place] = static_cast<uint8_t>(g.scale);
+  }
+  if (c.desc != nullptr && static_cast<int>(threadIdx.x) >= lo && static_cast<int>(threadIdx.x) < hi) {
+    const int64_t i = base + static_cast<int>(threadIdx.x) - len;
+    const bool ins = t.in_span != nullptr && t.in_span[b * t.in_span_stride_b + i] != 0;
+    const bool pre = t.is_prefix != nullptr && t.is_prefix[b * t.is_prefix_stride_b + i] != 0;
+    const int64_t sid = t.span_id != nullptr ? t.span_id[b * t.span_id_stride_b + i] : 0;
+    if (span_id_out_of_range(sid)) cache_report(c, KD_STATUS_SPAN_RANGE);
+    c.desc[at * KC_PAGE + threadIdx.x] = pack_token(ins, pre, sid, true);
+  }
+}
+
+int launch_cache4_append(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_tokens& t, cudaStream_t stream) {
+  const int W = (t.T + KC_PAGE - 2) / KC_PAGE + 1;   // blocks that T tokens can touch
+  const int64_t grid = static_cast<int64_t>(s.B) * W * c.H;
+  if (grid > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d sequences of %d new tokens and %d heads are too many for one call", s.B, t.T, c.H);
+  auto* kernel = t.dtype == KD_F16 ? cache4_append_kernel<KD_F16> : t.dtype == KD_BF16 ? cache4_append_kernel<KD_BF16> : cache4_append_kernel<KD_F32>;
+  const cudaError_t e = launch(kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, t, W);
+  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache4_append_kernel launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+// ---- reading ------------------------------------------------------------------------------------------------------
+
+// 64 tokens of one head, K and V: the loads of both are on their way together
+template <int kType>
+__global__ void __launch_bounds__(KC_THREADS)
+cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const int32_t* __restrict__ start, int count, int groups,
+                   const __grid_constant__ kd_tensor k, const __grid_constant__ kd_tensor v) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t item = blockIdx.x / static_cast<uint32_t>(groups);
+  const int r0 = static_cast<int>(blockIdx.x - item * groups) * KC_PAGE;
+  const int b = static_cast<int>(item / static_cast<uint32_t>(c.H)), h = static_cast<int>(item - static_cast<uint32_t>(b) * c.H);
+  const int len = sequence_length(c, s, b), per_row = c.D / K4_GROUP, chunks = KC_PAGE * per_row;
+  const int64_t from = start != nullptr ? start[b] : 0;
+  Group4 g[C4_CHUNKS];
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
+    const int64_t j = from + r0 + slot;
+    g[i] = Group4{make_uint2(0u, 0u), 0u};
+    if (both < 2 * chunks && r0 + slot < count && j >= 0 && j < len) {
+      const int page = page_of(c, s, b, static_cast<int>(j / KC_PAGE));
+      if (page >= 0) {
+        const size_t place = (block_index(c, page, h) * KC_PAGE + j % KC_PAGE) * per_row + col;
+        g[i].v = reinterpret_cast<const uint2*>(both >= chunks ? c.v : c.k)[place];
+        g[i].scale = scales4(both >= chunks ? c.v_scale : c.k_scale)[place];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
+    if (both >= 2 * chunks || r0 + slot >= count) continue;
+    constexpr int kSize = kType == KD_F32 ? 4 : 2;
+    const kd_tensor& out = both >= chunks ? v : k;
+    const uint32_t scale = both_halves(g[i].scale);
+    float f[16];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float2 two = unpack2<false>(times(e2m1x2_to_f16x2(x < 4 ? g[i].v.x : g[i].v.y, x & 3), scale));
+      f[2 * x] = two.x;
+      f[2 * x + 1] = two.y;
+    }
+    store16<kType>(static_cast<char*>(out.ptr) + (b * out.stride_b + h * out.stride_h + static_cast<int64_t>(r0 + slot) * out.stride_t + col * K4_GROUP) * kSize, f);
+  }
+}
+
+int launch_cache4_read(const kd_cache& c, const kd_cache_seqs& s, const int32_t* start, int count, int dtype, const kd_tensor& k, const kd_tensor& v, cudaStream_t stream) {
+  const int groups = (count + KC_PAGE - 1) / KC_PAGE;
+  const int64_t grid = static_cast<int64_t>(s.B) * c.H * groups;
+  if (grid > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d sequences of %d tokens and %d heads are too many for one call", s.B, count, c.H);
+  auto* kernel = dtype == KD_F16 ? cache4_read_kernel<KD_F16> : dtype == KD_BF16 ? cache4_read_kernel<KD_BF16> : cache4_read_kernel<KD_F32>;
+  const cudaError_t e = launch(kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, start, count, groups, k, v);
+  if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache4_read_kernel launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+// ---- eviction -----------------------------------------------------------------------------------------------------
+
+// One block of what a head keeps, K and V: the tokens' bytes as they are (see cache_select_kernel for which).
+__global__ void __launch_bounds__(KC_THREADS)
+cache4_gather_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_eviction e, int W) {
+  pdl_wait();
+  pdl_launch_dependents();
+  __shared__ size_t s_row[KC_PAGE];
+  const uint32_t item = blockIdx.x / static_cast<uint32_t>(W);
+  const int w = static_cast<int>(blockIdx.x - item * W), b = static_cast<int>(item / static_cast<uint32_t>(c.H)), h = static_cast<int>(item - static_cast<uint32_t>(b) * c.H);
+  const int n = sequence_length(c, s, b), m = min(n, e.keep), base = w * KC_PAGE;
+  if (base >= m) return;
+  const int page = checked_page(c, e.out_table[b * e.out_table_stride + w]);
+  if (page < 0) return;
+  const size_t to = block_index(c, page, h);
+  if (threadIdx.x < KC_PAGE) {
+    const int slot = threadIdx.x;
+    size_t row = SIZE_MAX;   // there is no such token
+    if (base + slot < m) {
+      const int j = e.index[static_cast<size_t>(item) * e.keep + base + slot], source = page_of(c, s, b, j / KC_PAGE);
+      if (source >= 0) row = block_index(c, source, h) * KC_PAGE + j % KC_PAGE;
+      if (c.desc != nullptr) c.desc[to * KC_PAGE + slot] = source >= 0 ? c.desc[row] : 0u;
+    }
+    s_row[slot] = row;
+  }
+  __syncthreads();
+  const int per_row = c.D / K4_GROUP, chunks = KC_PAGE * per_row;
+  Group4 g[C4_CHUNKS];
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row;
+    g[i] = Group4{make_uint2(0u, 0u), 0u};
+    const size_t row = both < 2 * chunks ? s_row[slot] : SIZE_MAX;
+    if (row != SIZE_MAX) {
+      const size_t place = row * per_row + (chunk - slot * per_row);
+      g[i].v = reinterpret_cast<const uint2*>(both >= chunks ? c.v : c.k)[place];
+      g[i].scale = scales4(both >= chunks ? c.v_scale : c.k_scale)[place];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C4_CHUNKS; ++i) {
+    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both;
+    if (both >= 2 * chunks) break;
+    const size_t place = to * chunks + chunk;
+    reinterpret_cast<uint2*>(both >= chunks ? c.v : c.k)[place] = g[i].v;
+    reinterpret_cast<uint8_t*>(both >= chunks ? c.v_scale : c.k_scale)[place] = static_cast<uint8_t>(g[i].scale);
+  }
+}
+
+cudaError_t launch_cache4_gather(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_eviction& e, unsigned grid, int W, cudaStream_t stream) {
+  return launch(cache4_gather_kernel, grid, KC_THREADS, 0, stream, c, s, e, W);
+}
+
+}  // namespace kd

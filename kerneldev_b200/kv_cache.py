@@ -1,4 +1,4 @@
-"""Generating with a key/value cache in 8 bits.
+"""Generating with a key/value cache in 8 bits, or in 4.
 
 ``GPTModel.generate`` (model.py:316-355) runs the whole sequence through every layer again for each new token. With a cache
 a layer appends the new tokens' keys and values (``cache_append``) and attends from the new tokens alone (``cache_attention``),
@@ -9,6 +9,12 @@ Format. Pages of 64 tokens: ``k`` and ``v`` float8_e4m3fn (pages, heads, 64, hea
 A stored number stands for its value times the scale of its page and head: 2**e with -32 <= e <= 31, the smallest e that lets the block's
 largest finite magnitude be at most 448 * 2**e. Larger numbers saturate; infinities and NaN are stored as NaN. A block that receives tokens
 later keeps its scale or gets a larger one, and what it holds is rounded again: exactly, but for numbers that become subnormal.
+
+In 4 bits (``KVCache.empty(..., bits=4)``), 9/16 of that memory: ``k`` and ``v`` uint8 (pages, heads, 64, head_dim / 2), two e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) in a byte, the even
+element in the low half; ``k_scale`` and ``v_scale`` uint8 (pages, heads, 64, head_dim / 16), one scale for 16 elements side by side: bits 14 to 7 of a float16. It is the one nearest to a sixth of their largest
+magnitude, 10240 at most, and a number is the nearest to what it is divided by the scale; ties go to even, larger numbers saturate. 16 elements with an infinity or NaN among them
+are stored as NaN, all 16 (byte 255; bytes 227 to 254 must not occur). An append never changes what is there. Every function below takes either cache.
+
 ``desc`` (optional) holds the mask descriptor of every token: int32, bit 0 prefix, 1 context, 2 in a span, 3 [MASKQ], 4 same-span rule armed,
 5 to 7 the classes of keys that the token sees wherever they are, from 8 the span id.
 
@@ -44,11 +50,18 @@ class KVCache:
         self.k, self.v, self.k_scale, self.v_scale, self.desc = k, v, k_scale, v_scale, desc
 
     @classmethod
-    def empty(cls, pages: int, heads: int, head_dim: int, device="cuda", metadata: bool = False) -> "KVCache":
-        """A new pool; ``metadata``: with room for the mask descriptors."""
+    def empty(cls, pages: int, heads: int, head_dim: int, device="cuda", metadata: bool = False, bits: int = 8) -> "KVCache":
+        """A new pool; ``metadata``: with room for the mask descriptors; ``bits``: 8 or 4."""
+        if bits not in (4, 8):
+            raise ValueError(f"a cache has 8 or 4 bits, not {bits}")
+        desc = torch.zeros((pages, heads, PAGE), dtype=torch.int32, device=device) if metadata else None
+        if bits == 4:
+            if head_dim % 16:
+                raise ValueError(f"head_dim {head_dim} is not supported (a multiple of 16 from 16 to 128)")
+            k, v, k_scale, v_scale = (torch.zeros((pages, heads, PAGE, n), dtype=torch.uint8, device=device) for n in (head_dim // 2, head_dim // 2, head_dim // 16, head_dim // 16))
+            return cls(k, v, k_scale, v_scale, desc)
         k, v = (torch.zeros((pages, heads, PAGE, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
         scales = torch.ones((2, pages, heads), dtype=torch.float32, device=device)
-        desc = torch.zeros((pages, heads, PAGE), dtype=torch.int32, device=device) if metadata else None
         return cls(k, v, scales[0].clone(), scales[1].clone(), desc)
 
 
@@ -79,7 +92,7 @@ def cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, l
     the memory layout of q.
 
     A weight enters the product with v with 11 bits, and with an error of no more than 2**-28 of the row's largest weight (2**-25 in rows with scores
-    beyond 2**16, in powers of two), or, where the value scales of pages are more than 2**4 apart, 2**-20 of its page's largest.
+    beyond 2**16, in powers of two), or, where the value scales of an 8-bit cache's pages are more than 2**4 apart, 2**-20 of its page's largest.
 
     Returns O in the type of q, or (O, LSE) with ``return_lse`` (float32 (batch, heads, time), base 2)."""
     if out_layout not in ("contiguous", "input"):
