@@ -5,54 +5,27 @@
 // dw = the sum of g x r over all rows. All in 32 bits, rounded once.
 //
 // Angles. A step is kept as a 64-bit fraction of a turn, so that position * step modulo 2^64 is the fraction of a turn that is left, exact to position / 2^64 turns
-// whatever the position: its upper 32 bits are the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21, beside 2^-9 or 2^-12 of the output), for float sincospif's.
+// whatever the position: its upper 32 bits are the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21, beside 2^-9 or 2^-12 of the output), for float polynomials.
 //
-// Bound by memory: each number is read and written once. A row has a group of L lanes, 16 numbers to each: the pairs of a lane are its own, and a lane keeps its
-// sines and cosines for all heads of its token.
+// Bound by memory: each number is read and written once. A row has a group of D / 16 lanes, 16 numbers to each: the pairs of a lane are its own, and a lane keeps its
+// sines and cosines for all heads of a run. Rows are asked for ahead by asynchronous copies into shared memory, so that what is in flight takes no registers: with loads into registers a backward of
+// 16 x 4096 tokens of 32 heads of 64 (bf16) took 235 us, so 155 (805 MB, 5.2 TB/s; the forward 95 us, 5.6 TB/s, 106 before). A lane's pieces lie a part of the row apart, so that a copy of all lanes takes whole
+// sectors: with 32 bytes side by side to a lane, interleaved pairs of 16384 tokens of 40 heads of 128 took 79 us, so 58.
 #include <algorithm>
+#include <numeric>
 
+#include "attn_common.cuh"
 #include "common.cuh"
 #include "sm100_prims.cuh"
 
 namespace kd {
 
-constexpr int RT_THREADS = 256, RT_GRAD_BLOCKS = 148 * 2;
-
-// eight numbers of a row as they came
-template <int kType>
-struct Chunk8 {
-  static constexpr int WORDS = kType == KD_F32 ? 2 : 1;
-  uint4 v[WORDS];
-  __device__ __forceinline__ void load(const char* p) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void floats(float* f) const {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (kType == KD_F32) {
-          f[4 * i + j] = __uint_as_float(w[j]);
-        } else {
-          const float2 x = unpack2<kType == KD_BF16>(w[j]);
-          f[2 * j] = x.x;
-          f[2 * j + 1] = x.y;
-        }
-      }
-    }
-  }
-  static __device__ __forceinline__ void store(char* p, const float* f) {
-    if constexpr (kType == KD_F32) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-    } else {
-      constexpr bool kBf16 = kType == KD_BF16;
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<kBf16>(f[0], f[1]), pack2<kBf16>(f[2], f[3]), pack2<kBf16>(f[4], f[5]), pack2<kBf16>(f[6], f[7]));
-    }
-  }
-};
+// CTAs of an SM (registers allow two of the backward's; three of the forward's were 3 to 8 % slower), and bytes that a thread has in its ring: rows in flight are what reaches the memory's rate. 128 bytes
+// for the forward cost 16 x 4096 tokens of 32 heads of 64 nothing and 2 x 2945 of 16 of 80 (float) 14 %, 384 gained nothing.
+constexpr int RT_THREADS = 256, RT_WARPS = RT_THREADS / 32, RT_CTAS = 2, RT_RING = 256;
+// Lanes of a row, 16 numbers to each, and rows of a warp (whose last two or four lanes may be idle).
+constexpr __host__ __device__ int lanes_of(int D) { return D / 16; }
+constexpr __host__ __device__ int tokens_of(int D) { return RT_WARPS * (32 / lanes_of(D)); }
 
 __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
   if (dtype == KD_F32) return static_cast<const float*>(w)[i];
@@ -64,17 +37,16 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
 template <int kType>
 __device__ __forceinline__ void turn(int32_t fraction, float& c, float& s) {
   if constexpr (kType == KD_F32) {
-    // the nearest quarter first, in whole numbers: what is left is a float that is off by 2^-27
+    // The nearest quarter first, in whole numbers; of the rest, an angle t of pi / 4 at most, the Taylor polynomials of sine and cosine to t^9 and t^10 (the next terms are below 2^-29). sincospif took
+    // three times the instructions, which with few heads to a token was half of the time.
     const int32_t quarter = static_cast<int32_t>(static_cast<uint32_t>(fraction) + (1u << 29)) >> 30;   // -2 .. 1, modulo a turn
     const int32_t rest = static_cast<int32_t>(static_cast<uint32_t>(fraction) - (static_cast<uint32_t>(quarter) << 30));
-    float x, y;
-    sincospif(static_cast<float>(rest) * 0x1p-31f, &y, &x);
-    c = (quarter & 1) != 0 ? -y : x;
-    s = (quarter & 1) != 0 ? x : y;
-    if ((quarter & 2) != 0) {
-      c = -c;
-      s = -s;
-    }
+    const float a = static_cast<float>(rest) * (6.28318530717958648f * 0x1p-32f), q = a * a;
+    const float x = fmaf(q, fmaf(q, fmaf(q, fmaf(q, fmaf(q, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+    const float y = fmaf(a * q, fmaf(q, fmaf(q, fmaf(q, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), a);
+    const float even = (quarter & 1) != 0 ? -y : x, odd = (quarter & 1) != 0 ? x : y;
+    c = (quarter & 2) != 0 ? -even : even;
+    s = (quarter & 2) != 0 ? -odd : odd;
   } else {
     const float angle = static_cast<float>(fraction) * (3.14159265358979f * 0x1p-31f);
     c = __cosf(angle);
@@ -82,7 +54,7 @@ __device__ __forceinline__ void turn(int32_t fraction, float& c, float& s) {
   }
 }
 
-// 16 numbers of a lane; kBack: by the negative angles
+// 16 numbers of a lane, eight pairs; kBack: by the negative angles
 template <bool kBack>
 __device__ __forceinline__ void rotate16(float (&f)[16], const float (&c)[8], const float (&s)[8], bool interleaved) {
   if (interleaved) {
@@ -102,165 +74,232 @@ __device__ __forceinline__ void rotate16(float (&f)[16], const float (&c)[8], co
   }
 }
 
-// sum over a row's lanes
+// Sum over the L lanes of a row that begins at lane `base`; i: this lane's number in it. All lanes of the warp call it.
 template <int L>
-__device__ __forceinline__ float row_sum(float x) {
+__device__ __forceinline__ float row_sum(float x, int base, int i) {
+  if constexpr ((L & (L - 1)) == 0) {
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+    for (int o = 1; o < L; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  } else {   // pairs first where L is even, then the sums in a ring
+    constexpr int RING = L % 2 == 0 ? L / 2 : L;
+    if (L % 2 == 0) x += __shfl_sync(0xffffffffu, x, base + (i + L / 2) % L);
+    float sum = x;
+#pragma unroll
+    for (int o = 1; o < RING; ++o) sum += __shfl_sync(0xffffffffu, x, base + (i + o) % L);
+    return sum;
+  }
 }
 
-// How the work is cut: blockIdx.y a run of heads of q (the first splits_q) or k, blockIdx.x tiles of 256 / L tokens.
+// How the work is cut: `heads` heads of q (the first runs_q runs) or k, and tiles of tokens, which `ctas` CTAs share.
 struct RotateShape {
-  int splits_q, heads, tiles;
-  float* partial;   // backward with weights: (gridDim.y, gridDim.x, D) sums of a CTA
+  int runs_q, heads, tiles, ctas;
+  float* partial;   // backward with weights: (runs, ctas, D) sums of a CTA
 };
 
-template <int kType, int L, bool kGrad>
-__global__ void __launch_bounds__(RT_THREADS) rotate_kernel(const __grid_constant__ kd_rotation p, const __grid_constant__ RotateShape shape) {
-  constexpr int GROUPS = RT_THREADS / L, kSize = kType == KD_F32 ? 4 : 2;
-  constexpr int BATCH = (kGrad ? 2 : 4) / (kType == KD_F32 ? 2 : 1);   // heads that a lane has on their way
+// A lane's 16 numbers of one tensor's row, in pieces of 16 bytes: piece i of a row's lanes lies side by side, so that a load takes whole sectors. A run of elements (those that turn, or those that do
+// not) is cut into as many parts as a lane has pieces; with that, both elements of a pair are the same lane's in either order of pairs.
+template <int kType>
+struct Lane16 {
+  static constexpr int SIZE = kType == KD_F32 ? 4 : 2, PIECES = SIZE, EACH = 16 / SIZE;   // numbers of a piece
+  int start, part;   // the first piece's first element; elements of a part
+  __device__ __forceinline__ Lane16(int u, int R, int D) : start(16 * u < R ? EACH * u : R + EACH * (u - R / 16)), part((16 * u < R ? R : D - R) / PIECES) {}
+  __device__ __forceinline__ int element(int j) const { return start + j / EACH * part + j % EACH; }   // of number j
+  static __device__ __forceinline__ void floats(const uint4& v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kType == KD_F32) {
+        f[j] = __uint_as_float(w[j]);
+      } else {
+        const float2 x = unpack2<kType == KD_BF16>(w[j]);
+        f[2 * j] = x.x;
+        f[2 * j + 1] = x.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* row, const float (&f)[16]) const {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      uint4 v;
+      if constexpr (kType == KD_F32) {
+        v = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+      } else {
+        constexpr bool kBf16 = kType == KD_BF16;
+        v = make_uint4(pack2<kBf16>(f[8 * i], f[8 * i + 1]), pack2<kBf16>(f[8 * i + 2], f[8 * i + 3]), pack2<kBf16>(f[8 * i + 4], f[8 * i + 5]), pack2<kBf16>(f[8 * i + 6], f[8 * i + 7]));
+      }
+      *reinterpret_cast<uint4*>(row + element(i * EACH) * SIZE) = v;
+    }
+  }
+};
+
+// The rows on their way: a ring of each thread's own, in shared memory. Nobody else reads its places, so that no barrier is needed; what is in flight costs no registers.
+template <int kType, bool kGrad>
+struct RotateRing {
+  static constexpr int PIECES = Lane16<kType>::PIECES * (kGrad ? 2 : 1);   // of a row: x, then the gradient
+  static constexpr int STAGES = RT_RING / (16 * PIECES), BYTES = STAGES * PIECES * 16 * RT_THREADS;
+  static __device__ __forceinline__ uint32_t place(uint32_t ring, int stage, int piece) { return ring + ((stage * PIECES + piece) * RT_THREADS + threadIdx.x) * 16; }
+};
+
+template <int N>
+__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
+template <int kType, int D, bool kGrad>
+__global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __grid_constant__ kd_rotation p, const __grid_constant__ RotateShape shape) {
+  using Row = Lane16<kType>;
+  using Ring = RotateRing<kType, kGrad>;
+  constexpr int L = lanes_of(D), ROWS = 32 / L, kSize = Row::SIZE;
+  extern __shared__ __align__(16) char smem[];
   pdl_wait();
   pdl_launch_dependents();
-  const int u = threadIdx.x & (L - 1), group = threadIdx.x / L;
-  const bool is_k = static_cast<int>(blockIdx.y) >= shape.splits_q, mine = u < p.D / 16, turns = 16 * u < p.R;
-  const int split = blockIdx.y - (is_k ? shape.splits_q : 0), h0 = split * shape.heads, h1 = min(h0 + shape.heads, is_k ? p.Hk : p.Hq);
+  const uint32_t ring = smem_u32(smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / L, u = lane - group * L, base = group * L;
+  const int run = blockIdx.x / shape.ctas, cta = blockIdx.x - run * shape.ctas;
+  const bool is_k = run >= shape.runs_q, mine = group < ROWS, turns = 16 * u < p.R;
+  const int h0 = (run - (is_k ? shape.runs_q : 0)) * shape.heads, h1 = h0 + shape.heads;
   const kd_tensor& x = is_k ? p.k : p.q;
   const kd_tensor& y = is_k ? p.k_out : p.q_out;
   const kd_tensor& dx = is_k ? p.dk : p.dq;
   const void* weight = is_k ? p.k_weight : p.q_weight;
-  // the lane's two pieces of eight
-  const int first = p.interleaved != 0 || !turns ? 16 * u : 8 * u, second = p.interleaved != 0 || !turns ? first + 8 : p.R / 2 + first;
-  float w[16], dw[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    w[i] = mine && weight != nullptr ? weight_at(weight, p.w_dtype, (i < 8 ? first : second - 8) + i) : 1.f;
-    dw[i] = 0.f;
-  }
-  const float inv_d = 1.f / static_cast<float>(p.D);
+  const bool reads_x = !kGrad || weight != nullptr;
+  const Row mine16(u, p.R, D);
   const int tokens = p.B * p.T;
-#pragma unroll 1
-  for (int tile = blockIdx.x; tile < shape.tiles; tile += gridDim.x) {
-    const int token = tile * GROUPS + group;
-    const bool live = token < tokens && mine;
-    const int b = min(token, tokens - 1) / p.T, t = min(token, tokens - 1) - b * p.T;
-    float c[8], s[8];
-    if (turns && mine) {
-      int64_t at[3];
+  struct Place {
+    int b, t;
+    bool live;
+  };
+  auto place_of = [&](int tile) {
+    const int token = tile * tokens_of(D) + warp * ROWS + group, at = min(token, tokens - 1), b = at / p.T;
+    return Place{b, at - b * p.T, token < tokens && mine};
+  };
+  auto row_of = [&](const kd_tensor& z, const Place& at, int h) { return static_cast<char*>(z.ptr) + (at.b * z.stride_b + h * z.stride_h + at.t * z.stride_t) * kSize; };
+
+  // the next row to ask for
+  int ask_tile = cta, ask_h = h0, ask_stage = 0;
+  Place ask_at = place_of(ask_tile);
+  auto ask = [&]() {
+    if (ask_tile < shape.tiles) {
+      if (ask_at.live) {
+        if (reads_x) {
+          const char* row = row_of(x, ask_at, ask_h);
 #pragma unroll
-      for (int a = 0; a < 3; ++a) {
-        at[a] = t;
-        if (a < p.axes && p.positions != nullptr) {
-          const int64_t i = a * p.pos_stride_a + b * p.pos_stride_b + t * p.pos_stride_t;
-          at[a] = p.pos_is_64 != 0 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
-        }
-      }
-      if (p.offsets != nullptr) at[0] += p.offsets[b];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int pair = 8 * u + i;
-        const int64_t n = p.positions == nullptr || pair < p.ends[0] ? at[0] : pair < p.ends[1] ? at[1] : at[2];
-        turn<kType>(static_cast<int32_t>((static_cast<uint64_t>(n) * p.steps[pair]) >> 32), c[i], s[i]);
-      }
-    }
-    const int64_t from = b * x.stride_b + t * x.stride_t, to_y = b * y.stride_b + t * y.stride_t, to_dx = kGrad ? b * dx.stride_b + t * dx.stride_t : 0;
-#pragma unroll 1
-    for (int h = h0; h < h1; h += BATCH) {
-      Chunk8<kType> rx[BATCH][2], rg[kGrad ? BATCH : 1][2];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        if (!live || h + i >= h1) continue;
-        if (!kGrad || weight != nullptr) {
-          const char* row = static_cast<const char*>(x.ptr) + (from + (h + i) * x.stride_h) * kSize;
-          rx[i][0].load(row + first * kSize);
-          rx[i][1].load(row + second * kSize);
+          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, i), row + mine16.element(i * Row::EACH) * kSize);
         }
         if constexpr (kGrad) {
-          const char* row = static_cast<const char*>(y.ptr) + (to_y + (h + i) * y.stride_h) * kSize;
-          rg[i][0].load(row + first * kSize);
-          rg[i][1].load(row + second * kSize);
+          const char* row = row_of(y, ask_at, ask_h);
+#pragma unroll
+          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, Row::PIECES + i), row + mine16.element(i * Row::EACH) * kSize);
         }
       }
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const bool here = live && h + i < h1;
-        float f[16];
-        if constexpr (!kGrad) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) f[j] = 0.f;
-          if (here) {
-            rx[i][0].floats(f);
-            rx[i][1].floats(f + 8);
-          }
-          if (weight != nullptr) {
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum = fmaf(f[j], f[j], sum);
-            const float r = __frsqrt_rn(fmaf(row_sum<L>(sum), inv_d, p.eps));
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = f[j] * r * w[j];
-          }
-          if (turns) rotate16<false>(f, c, s, p.interleaved != 0);
-          if (here) {
-            char* row = static_cast<char*>(y.ptr) + (to_y + (h + i) * y.stride_h) * kSize;
-            Chunk8<kType>::store(row + first * kSize, f);
-            Chunk8<kType>::store(row + second * kSize, f + 8);
-          }
-        } else {
-          float g[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) f[j] = g[j] = 0.f;
-          if (here) {
-            rg[i][0].floats(g);
-            rg[i][1].floats(g + 8);
-          }
-          if (turns) rotate16<true>(g, c, s, p.interleaved != 0);
-          if (weight != nullptr) {
-            if (here) {
-              rx[i][0].floats(f);
-              rx[i][1].floats(f + 8);
-            }
-            float sum = 0.f, dot = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              sum = fmaf(f[j], f[j], sum);
-              dot = fmaf(g[j] * w[j], f[j], dot);
-            }
-            const float r = __frsqrt_rn(fmaf(row_sum<L>(sum), inv_d, p.eps)), back = row_sum<L>(dot) * inv_d * r * r;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              dw[j] = fmaf(g[j], f[j] * r, dw[j]);
-              g[j] = r * fmaf(-f[j], back, g[j] * w[j]);
-            }
-          }
-          if (here) {
-            char* row = static_cast<char*>(dx.ptr) + (to_dx + (h + i) * dx.stride_h) * kSize;
-            Chunk8<kType>::store(row + first * kSize, g);
-            Chunk8<kType>::store(row + second * kSize, g + 8);
-          }
-        }
+      if (++ask_h == h1) {
+        ask_h = h0;
+        ask_tile += shape.ctas;
+        ask_at = place_of(ask_tile);
       }
     }
+    ask_stage = ask_stage + 1 == Ring::STAGES ? 0 : ask_stage + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < Ring::STAGES - 1; ++i) ask();
+
+  float w[16], dw[kGrad ? 16 : 1];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    w[i] = mine && weight != nullptr ? weight_at(weight, p.w_dtype, mine16.element(i)) : 1.f;
+    if (kGrad) dw[i] = 0.f;
   }
+  int stage = 0;
+#pragma unroll 1
+  for (int tile = cta; tile < shape.tiles; tile += shape.ctas) {
+    const Place at = place_of(tile);
+    float c[8], s[8];
+    if (turns && mine) {
+      int64_t n[3];
+#pragma unroll
+      for (int a = 0; a < 3; ++a) {
+        n[a] = at.t;
+        if (a < p.axes && p.positions != nullptr) {
+          const int64_t i = a * p.pos_stride_a + at.b * p.pos_stride_b + at.t * p.pos_stride_t;
+          n[a] = p.pos_is_64 != 0 ? static_cast<const int64_t*>(p.positions)[i] : static_cast<const int32_t*>(p.positions)[i];
+        }
+      }
+      if (p.offsets != nullptr) n[0] += p.offsets[at.b];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int pair = p.interleaved != 0 ? mine16.element(2 * i) / 2 : mine16.element(i);
+        const int64_t here = p.positions == nullptr || pair < p.ends[0] ? n[0] : pair < p.ends[1] ? n[1] : n[2];
+        turn<kType>(static_cast<int32_t>((static_cast<uint64_t>(here) * p.steps[pair]) >> 32), c[i], s[i]);
+      }
+    }
+#pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+      await_copies<Ring::STAGES - 2>();
+      float f[16];
+      auto take = [&](int from, float (&to)[16], bool there) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i] = 0.f;
+        if (there)
+#pragma unroll
+          for (int i = 0; i < Row::PIECES; ++i) Row::floats(lds16(Ring::place(ring, stage, from + i)), to + i * Row::EACH);
+      };
+      if constexpr (!kGrad) {
+        take(0, f, at.live);
+        if (weight != nullptr) {
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum = fmaf(f[j], f[j], sum);
+          const float r = __frsqrt_rn(fmaf(row_sum<L>(sum, base, u), 1.f / D, p.eps));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) f[j] = f[j] * r * w[j];
+        }
+        if (turns) rotate16<false>(f, c, s, p.interleaved != 0);
+        if (at.live) mine16.store(row_of(y, at, h), f);
+      } else {
+        float g[16];
+        take(Row::PIECES, g, at.live);
+        if (turns) rotate16<true>(g, c, s, p.interleaved != 0);
+        if (weight != nullptr) {
+          take(0, f, at.live);
+          float sum = 0.f, dot = 0.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            sum = fmaf(f[j], f[j], sum);
+            dot = fmaf(g[j] * w[j], f[j], dot);
+          }
+          const float r = __frsqrt_rn(fmaf(row_sum<L>(sum, base, u), 1.f / D, p.eps)), back = row_sum<L>(dot, base, u) * (1.f / D) * r * r;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            dw[j] = fmaf(g[j], f[j] * r, dw[j]);
+            g[j] = r * fmaf(-f[j], back, g[j] * w[j]);
+          }
+        }
+        if (at.live) mine16.store(row_of(dx, at, h), g);
+      }
+      ask();   // (into the place of the row before: its numbers have been used)
+      stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
+    }
+  }
+  await_copies<0>();
   if constexpr (kGrad) {
     if (weight == nullptr || shape.partial == nullptr) return;
-    // the CTA's sums, in a fixed order: over the groups of a warp, then over the warps
-    __shared__ float sums[RT_THREADS / 32][16 * L];
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-#pragma unroll
-      for (int o = L; o < 32; o <<= 1) dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], o);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane < L && mine)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sums[warp][(j < 8 ? first : second - 8) + j] = dw[j];
+    // the CTA's sums, in a fixed order: over the rows of its warps
     __syncthreads();
-    float* out = shape.partial + (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * p.D;
-    for (int d = threadIdx.x; d < p.D; d += RT_THREADS) {
-      float total = 0.f;
+    float* sums = reinterpret_cast<float*>(smem);
+    if (mine)
 #pragma unroll
-      for (int i = 0; i < RT_THREADS / 32; ++i) total += sums[i][d];
-      out[d] = total;
+      for (int j = 0; j < 16; ++j) sums[(warp * ROWS + group) * D + mine16.element(j)] = dw[j];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float total = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < RT_WARPS * ROWS; ++i) total += sums[i * D + threadIdx.x];
+      shape.partial[static_cast<size_t>(blockIdx.x) * D + threadIdx.x] = total;
     }
   }
 }
@@ -292,58 +331,72 @@ __global__ void __launch_bounds__(RT_THREADS) rotate_weight_kernel(const __grid_
 }
 
 struct RotateGrid {
-  int lanes, blocks, splits_q, splits_k, heads, tiles;
+  int runs_q, runs_k, heads, tiles, ctas;
 };
-// Heads are cut until there are CTAs for all SMs; a lane's sines and cosines are for all heads of a run.
-static RotateGrid grid_of(const kd_rotation& p, bool grad) {
-  RotateGrid g;
-  const int units = p.D / 16;
-  g.lanes = units > 4 ? 8 : units > 2 ? 4 : units;
-  const int64_t tokens = static_cast<int64_t>(p.B) * p.T, groups = RT_THREADS / g.lanes;
-  g.tiles = static_cast<int>((tokens + groups - 1) / groups);
-  const int wanted = grad ? RT_GRAD_BLOCKS : 148 * 8, most = std::max(p.Hq, p.Hk);
-  const int64_t cuts = std::max<int64_t>(1, (wanted + 2 * static_cast<int64_t>(g.tiles) - 1) / (2 * static_cast<int64_t>(g.tiles)));
-  g.heads = static_cast<int>(std::max<int64_t>(1, most / std::min<int64_t>(cuts, most)));
-  g.splits_q = (p.Hq + g.heads - 1) / g.heads;
-  g.splits_k = (p.Hk + g.heads - 1) / g.heads;
-  g.blocks = grad ? std::min(g.tiles, std::max(1, RT_GRAD_BLOCKS / (g.splits_q + g.splits_k))) : g.tiles;
-  return g;
+// Runs of as many heads as q and k have equal ones of, so that all CTAs of one wave have the same; the run that has the least to do, by heads and by what the sines and cosines of a tile cost beside a head.
+static RotateGrid grid_of(const kd_rotation& p) {
+  const int64_t tokens = static_cast<int64_t>(p.B) * p.T, tile = tokens_of(p.D), tiles = (tokens + tile - 1) / tile, room = 148 * RT_CTAS;
+  const int both = p.Hk > 0 ? std::gcd(p.Hq, p.Hk) : p.Hq;
+  const float angles = p.dtype == KD_F32 ? 1.5f : 0.7f;
+  RotateGrid best{};
+  float least = 0.f;
+  for (int heads = 1; heads <= std::min(both, 64); ++heads) {
+    if (both % heads != 0) continue;
+    const int64_t runs = (p.Hq + p.Hk) / heads, each = (tiles * runs + room - 1) / room;
+    const float cost = static_cast<float>(each) * (static_cast<float>(heads) + angles);
+    if (best.heads != 0 && cost > least) continue;
+    least = cost;
+    best = RotateGrid{p.Hq / heads, p.Hk / heads, heads, static_cast<int>(tiles), static_cast<int>((tiles + each - 1) / each)};
+  }
+  return best;
 }
 
 size_t rotate_grad_workspace(const kd_rotation& p) {
   if (p.dq_weight == nullptr && p.dk_weight == nullptr) return 0;
-  const RotateGrid g = grid_of(p, true);
-  return static_cast<size_t>(g.splits_q + g.splits_k) * g.blocks * p.D * sizeof(float);
+  const RotateGrid g = grid_of(p);
+  return static_cast<size_t>(g.runs_q + g.runs_k) * g.ctas * p.D * sizeof(float);
+}
+
+template <int kType, int D, bool kGrad>
+static cudaError_t launch_of(const kd_rotation& p, const RotateGrid& g, const RotateShape& s, cudaStream_t stream) {
+  constexpr int kShared = RotateRing<kType, kGrad>::BYTES;
+  static_assert(!kGrad || kShared >= tokens_of(D) * D * 4, "the weights' sums take the ring's place");
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(rotate_kernel<kType, D, kGrad>, kShared);
+  return e != cudaSuccess ? e : launch(rotate_kernel<kType, D, kGrad>, static_cast<unsigned>((g.runs_q + g.runs_k) * g.ctas), RT_THREADS, kShared, stream, p, s);
 }
 
 template <int kType, bool kGrad>
-static cudaError_t launch_lanes(const kd_rotation& p, const RotateGrid& g, const RotateShape& s, cudaStream_t stream) {
-  const dim3 grid(g.blocks, g.splits_q + g.splits_k);
-  switch (g.lanes) {
-    case 1: return launch(rotate_kernel<kType, 1, kGrad>, grid, RT_THREADS, 0, stream, p, s);
-    case 2: return launch(rotate_kernel<kType, 2, kGrad>, grid, RT_THREADS, 0, stream, p, s);
-    case 4: return launch(rotate_kernel<kType, 4, kGrad>, grid, RT_THREADS, 0, stream, p, s);
-    default: return launch(rotate_kernel<kType, 8, kGrad>, grid, RT_THREADS, 0, stream, p, s);
+static cudaError_t launch_dim(const kd_rotation& p, const RotateGrid& g, const RotateShape& s, cudaStream_t stream) {
+  switch (p.D) {
+    case 16: return launch_of<kType, 16, kGrad>(p, g, s, stream);
+    case 32: return launch_of<kType, 32, kGrad>(p, g, s, stream);
+    case 48: return launch_of<kType, 48, kGrad>(p, g, s, stream);
+    case 64: return launch_of<kType, 64, kGrad>(p, g, s, stream);
+    case 80: return launch_of<kType, 80, kGrad>(p, g, s, stream);
+    case 96: return launch_of<kType, 96, kGrad>(p, g, s, stream);
+    case 112: return launch_of<kType, 112, kGrad>(p, g, s, stream);
+    default: return launch_of<kType, 128, kGrad>(p, g, s, stream);
   }
 }
 
 template <bool kGrad>
 static cudaError_t launch_type(const kd_rotation& p, const RotateGrid& g, const RotateShape& s, cudaStream_t stream) {
   switch (p.dtype) {
-    case KD_F16: return launch_lanes<KD_F16, kGrad>(p, g, s, stream);
-    case KD_BF16: return launch_lanes<KD_BF16, kGrad>(p, g, s, stream);
-    default: return launch_lanes<KD_F32, kGrad>(p, g, s, stream);
+    case KD_F16: return launch_dim<KD_F16, kGrad>(p, g, s, stream);
+    case KD_BF16: return launch_dim<KD_BF16, kGrad>(p, g, s, stream);
+    default: return launch_dim<KD_F32, kGrad>(p, g, s, stream);
   }
 }
 
 int launch_rotate(const kd_rotation& p, bool grad, cudaStream_t stream) {
-  const RotateGrid g = grid_of(p, grad);
+  const RotateGrid g = grid_of(p);
   const bool weights = grad && (p.dq_weight != nullptr || p.dk_weight != nullptr);
-  if (g.splits_q + g.splits_k > 65535) return set_error(KD_ERR_LIMIT, "%d and %d heads are too many for one call", p.Hq, p.Hk);
-  const RotateShape s{g.splits_q, g.heads, g.tiles, weights ? static_cast<float*>(p.workspace) : nullptr};
+  if (static_cast<int64_t>(g.runs_q + g.runs_k) * g.ctas > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d and %d heads are too many for one call", p.Hq, p.Hk);
+  const RotateShape s{g.runs_q, g.heads, g.tiles, g.ctas, weights ? static_cast<float*>(p.workspace) : nullptr};
   cudaError_t e = grad ? launch_type<true>(p, g, s, stream) : launch_type<false>(p, g, s, stream);
   if (e == cudaSuccess && weights)
-    e = launch(rotate_weight_kernel, 2 * (p.D / RW_COLS), RT_THREADS, 0, stream, p, static_cast<const float*>(p.workspace), g.splits_q * g.blocks, g.splits_k * g.blocks);
+    e = launch(rotate_weight_kernel, 2 * (p.D / RW_COLS), RT_THREADS, 0, stream, p, static_cast<const float*>(p.workspace), g.runs_q * g.ctas, g.runs_k * g.ctas);
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "rotate_kernel launch: %s", cudaGetErrorString(e));
   return 0;
 }
