@@ -1,6 +1,8 @@
 // The 4-bit key/value cache without its attention: appending, reading, and moving what eviction keeps. See kd_attention.h for the format.
 // All are bound by memory traffic, for a handful of tokens by launches. A group of 16 numbers has a scale of its own, so a thread has a group, nothing is agreed on among
 // threads, and what a page holds already is never touched.
+#include <type_traits>
+
 #include "kv_cache.cuh"
 
 namespace kd {
@@ -11,17 +13,25 @@ struct Group4 {
   uint2 v;
   uint32_t scale;
 };
-// A group as it is stored. The scale is the nearest to a sixth of the largest magnitude, and the numbers the nearest to what they are in its units; ties go to even. A
-// quotient by 6 in 32 bits is never rounded onto the middle of two scales: a float next to six times a number of 5 bits is 2^-24 of it away, and a quotient's rounding moves it less. 16-bit
-// numbers are multiplied with the rounded 1 / scale, and the product is brought to a grid of 2^-13 (by the sum with 1536, of which one step is that much): that puts it on the middle of two levels exactly where the
-// quotient is, since numbers of 11 bits and scales of 4 have no other quotient within 2^-14 of a middle (tests/test_kv_cache4_logic.py goes through all of them; without the grid, 7 eighths of 13 fail). Floats are divided.
+__device__ __forceinline__ float inverse_of(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// A group as it is stored. The scale is the nearest to a sixth of the largest magnitude, and the numbers the nearest to what they are in its units; ties go to even.
+// Floats are divided; a quotient is never rounded onto the middle of two steps: a float next to a middle times 6 or times a scale of 4 bits is 2^-24 of it away, and a quotient's rounding moves it
+// less. 16-bit numbers are multiplied with a rounded inverse, and the product brought to a coarser grid (2^-16 of itself; 2^-13 by the fused sum with 1536, of which one step is that much), which puts it on a middle
+// exactly where the quotient is: numbers of 11 bits have no other quotient that near to one (tests/test_kv_cache4_logic.py goes through all of them). That takes a third of the instructions of divisions.
 template <int kType>
 __device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
   bool special = false;
-  const float sixth = __fdiv_rn(__uint_as_float(raw.amax(special)), 6.f);
-  const uint32_t u = __float_as_uint(sixth);
-  uint32_t byte = sixth < 0x1p-14f ? static_cast<uint32_t>(__float2int_rn(sixth * 0x1p17f)) : min(K4_TOP, ((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - 896u);
-  const float scale = unpack2<false>(byte << 7).x, inverse = byte != 0u ? __frcp_rn(scale) : 0.f;
+  const float top = __uint_as_float(raw.amax(special));
+  uint32_t u;
+  if constexpr (kType == KD_F32) u = __float_as_uint(__fdiv_rn(top, 6.f));
+  else u = (__float_as_uint(top * (1.f / 6.f)) + 0x40u) & ~0x7Fu;
+  const float sixth = __uint_as_float(u);
+  const uint32_t byte = sixth < 0x1p-14f ? static_cast<uint32_t>(__float2int_rn(sixth * 0x1p17f)) : min(K4_TOP, ((u + 0x7FFFFu + (u >> 20 & 1u)) >> 20) - 896u);
+  const float scale = unpack2<false>(byte << 7).x, inverse = byte != 0u ? inverse_of(scale) : 0.f;
   float f[16];
   raw.floats(f);
 #pragma unroll
@@ -34,7 +44,7 @@ __device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
 }
 
 // One block of one head of a sequence, K and V.
-template <int kType>
+template <int kType, int D>
 __global__ void __launch_bounds__(KC_THREADS)
 cache4_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_tokens t, int W) {
   pdl_wait();
@@ -56,29 +66,33 @@ cache4_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
   if (base >= len + n || n == 0) return;
   const int raw_page = s.table[b * s.table_stride + block];
   const int lo = max(len - base, 0), hi = min(len + n - base, KC_PAGE);   // slots lo .. hi - 1 are new
-  const int per_row = c.D / K4_GROUP, chunks = KC_PAGE * per_row;
-  constexpr int kSize = kType == KD_F32 ? 4 : 2;
-  Raw16<kType> raw[C4_CHUNKS];
+  constexpr int GROUPS = D / K4_GROUP, CHUNKS = KC_PAGE * GROUPS, EACH = (CHUNKS + KC_THREADS - 1) / KC_THREADS, kSize = kType == KD_F32 ? 4 : 2;
+  Raw16<kType> raw[2][EACH];
 #pragma unroll
-  for (int i = 0; i < C4_CHUNKS; ++i) {
-    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
-    const kd_tensor& x = both >= chunks ? t.v : t.k;
-    if (both < 2 * chunks && slot >= lo && slot < hi)
-      raw[i].load(static_cast<const char*>(x.ptr) + (b * x.stride_b + h * x.stride_h + static_cast<int64_t>(base + slot - len) * x.stride_t + col * K4_GROUP) * kSize);
+  for (int y = 0; y < 2; ++y) {
+    const kd_tensor& x = y == 0 ? t.k : t.v;
+    const char* rows = static_cast<const char*>(x.ptr) + (b * x.stride_b + h * x.stride_h + (base - len) * x.stride_t) * kSize;   // of the block's first slot
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int chunk = i * KC_THREADS + threadIdx.x, slot = chunk / GROUPS, col = chunk % GROUPS;
+      if (slot >= lo && slot < hi) raw[y][i].load(rows + (slot * x.stride_t + col * K4_GROUP) * kSize);
+    }
   }
   const int page = checked_page(c, raw_page);
   if (page < 0) return;
   const size_t at = block_index(c, page, h);
 #pragma unroll
-  for (int i = 0; i < C4_CHUNKS; ++i) {
-    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row;
-    if (both >= 2 * chunks || slot < lo || (slot >= hi && lo > 0)) continue;
-    Group4 g{make_uint2(0u, 0u), 0u};   // a page that is opened holds nothing of its earlier use
-    if (slot < hi) g = quantise_group(raw[i]);
-    const size_t place = at * chunks + chunk;
-    reinterpret_cast<uint2*>(both >= chunks ? c.v : c.k)[place] = g.v;
-    reinterpret_cast<uint8_t*>(both >= chunks ? c.v_scale : c.k_scale)[place] = static_cast<uint8_t>(g.scale);
-  }
+  for (int y = 0; y < 2; ++y)
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int chunk = i * KC_THREADS + threadIdx.x, slot = chunk / GROUPS;
+      if (slot >= KC_PAGE || slot < lo || (slot >= hi && lo > 0)) continue;
+      Group4 g{make_uint2(0u, 0u), 0u};   // a page that is opened holds nothing of its earlier use
+      if (slot < hi) g = quantise_group(raw[y][i]);
+      const size_t place = at * CHUNKS + chunk;
+      reinterpret_cast<uint2*>(y == 0 ? c.k : c.v)[place] = g.v;
+      reinterpret_cast<uint8_t*>(y == 0 ? c.k_scale : c.v_scale)[place] = static_cast<uint8_t>(g.scale);
+    }
   if (c.desc != nullptr && static_cast<int>(threadIdx.x) >= lo && static_cast<int>(threadIdx.x) < hi) {
     const int64_t i = base + static_cast<int>(threadIdx.x) - len;
     const bool ins = t.in_span != nullptr && t.in_span[b * t.in_span_stride_b + i] != 0;
@@ -89,60 +103,104 @@ cache4_append_kernel(const __grid_constant__ kd_cache c, const __grid_constant__
   }
 }
 
+// call: a generic lambda that takes the type and the head dim as types
+template <typename F>
+static cudaError_t by_type_and_dim(int dtype, int D, F call) {
+  auto dims = [&](auto type) {
+    switch (D) {
+      case 16: return call(type, std::integral_constant<int, 16>{});
+      case 32: return call(type, std::integral_constant<int, 32>{});
+      case 48: return call(type, std::integral_constant<int, 48>{});
+      case 64: return call(type, std::integral_constant<int, 64>{});
+      case 80: return call(type, std::integral_constant<int, 80>{});
+      case 96: return call(type, std::integral_constant<int, 96>{});
+      case 112: return call(type, std::integral_constant<int, 112>{});
+      default: return call(type, std::integral_constant<int, 128>{});
+    }
+  };
+  return dtype == KD_F16 ? dims(std::integral_constant<int, KD_F16>{}) : dtype == KD_BF16 ? dims(std::integral_constant<int, KD_BF16>{}) : dims(std::integral_constant<int, KD_F32>{});
+}
+
 int launch_cache4_append(const kd_cache& c, const kd_cache_seqs& s, const kd_cache_tokens& t, cudaStream_t stream) {
   const int W = (t.T + KC_PAGE - 2) / KC_PAGE + 1;   // blocks that T tokens can touch
   const int64_t grid = static_cast<int64_t>(s.B) * W * c.H;
   if (grid > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d sequences of %d new tokens and %d heads are too many for one call", s.B, t.T, c.H);
-  auto* kernel = t.dtype == KD_F16 ? cache4_append_kernel<KD_F16> : t.dtype == KD_BF16 ? cache4_append_kernel<KD_BF16> : cache4_append_kernel<KD_F32>;
-  const cudaError_t e = launch(kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, t, W);
+  const cudaError_t e = by_type_and_dim(t.dtype, c.D, [&](auto type, auto dim) {
+    return launch(cache4_append_kernel<decltype(type)::value, decltype(dim)::value>, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, t, W);
+  });
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache4_append_kernel launch: %s", cudaGetErrorString(e));
   return 0;
 }
 
 // ---- reading ------------------------------------------------------------------------------------------------------
 
-// 64 tokens of one head, K and V: the loads of both are on their way together
-template <int kType>
+// 64 tokens of one head, K and V, which lie in two pages at most: the loads of all are on their way together. A thread makes 16 bytes at a time, so that stores take whole sectors.
+template <int kType, int D>
 __global__ void __launch_bounds__(KC_THREADS)
 cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const int32_t* __restrict__ start, int count, int groups,
                    const __grid_constant__ kd_tensor k, const __grid_constant__ kd_tensor v) {
   pdl_wait();
   pdl_launch_dependents();
+  constexpr int kSize = kType == KD_F32 ? 4 : 2, N = 16 / kSize, ROW = D / N, ITEMS = KC_PAGE * ROW, EACH = (ITEMS + KC_THREADS - 1) / KC_THREADS;   // N numbers of a thread
   const uint32_t item = blockIdx.x / static_cast<uint32_t>(groups);
   const int r0 = static_cast<int>(blockIdx.x - item * groups) * KC_PAGE;
   const int b = static_cast<int>(item / static_cast<uint32_t>(c.H)), h = static_cast<int>(item - static_cast<uint32_t>(b) * c.H);
-  const int len = sequence_length(c, s, b), per_row = c.D / K4_GROUP, chunks = KC_PAGE * per_row;
-  const int64_t from = start != nullptr ? start[b] : 0;
-  Group4 g[C4_CHUNKS];
+  const int len = sequence_length(c, s, b);
+  const int64_t from = (start != nullptr ? start[b] : 0) + static_cast<int64_t>(r0);
+  const int64_t block = from >= 0 ? from / KC_PAGE : -((KC_PAGE - 1 - from) / KC_PAGE);   // of the first token
+  size_t rows[2];   // the pages' first token
+  bool there[2];
 #pragma unroll
-  for (int i = 0; i < C4_CHUNKS; ++i) {
-    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
-    const int64_t j = from + r0 + slot;
-    g[i] = Group4{make_uint2(0u, 0u), 0u};
-    if (both < 2 * chunks && r0 + slot < count && j >= 0 && j < len) {
-      const int page = page_of(c, s, b, static_cast<int>(j / KC_PAGE));
-      if (page >= 0) {
-        const size_t place = (block_index(c, page, h) * KC_PAGE + j % KC_PAGE) * per_row + col;
-        g[i].v = reinterpret_cast<const uint2*>(both >= chunks ? c.v : c.k)[place];
-        g[i].scale = scales4(both >= chunks ? c.v_scale : c.k_scale)[place];
-      }
+  for (int x = 0; x < 2; ++x) {
+    const int page = block + x >= 0 && (block + x) * KC_PAGE < len && (x == 0 || from > block * KC_PAGE) ? page_of(c, s, b, static_cast<int>(block + x)) : -1;
+    there[x] = page >= 0;
+    rows[x] = block_index(c, max(page, 0), h) * KC_PAGE;
+  }
+  uint32_t codes[2][EACH], scale[2][EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int x = i * KC_THREADS + threadIdx.x, slot = x / ROW, d = x % ROW * N;
+    const int64_t j = from + slot;
+    const int in = static_cast<int>(j - block * KC_PAGE), second = in >= KC_PAGE ? 1 : 0;
+    const size_t row = rows[second] + (in - second * KC_PAGE);
+    const bool live = slot < KC_PAGE && r0 + slot < count && j >= 0 && j < len && there[second];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      codes[y][i] = scale[y][i] = 0u;
+      if (!live) continue;
+      const uint8_t* at = static_cast<const uint8_t*>(y == 0 ? c.k : c.v) + (row * D + d) / 2;
+      codes[y][i] = N == 8 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
+      scale[y][i] = scales4(y == 0 ? c.k_scale : c.v_scale)[row * (D / K4_GROUP) + d / K4_GROUP];
     }
   }
 #pragma unroll
-  for (int i = 0; i < C4_CHUNKS; ++i) {
-    const int both = i * KC_THREADS + threadIdx.x, chunk = both >= chunks ? both - chunks : both, slot = chunk / per_row, col = chunk - slot * per_row;
-    if (both >= 2 * chunks || r0 + slot >= count) continue;
-    constexpr int kSize = kType == KD_F32 ? 4 : 2;
-    const kd_tensor& out = both >= chunks ? v : k;
-    const uint32_t scale = both_halves(g[i].scale);
-    float f[16];
+  for (int i = 0; i < EACH; ++i) {
+    const int x = i * KC_THREADS + threadIdx.x, slot = x / ROW, d = x % ROW * N;
+    if (slot >= KC_PAGE || r0 + slot >= count) continue;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const float2 two = unpack2<false>(times(e2m1x2_to_f16x2(x < 4 ? g[i].v.x : g[i].v.y, x & 3), scale));
-      f[2 * x] = two.x;
-      f[2 * x + 1] = two.y;
+    for (int y = 0; y < 2; ++y) {
+      const kd_tensor& out = y == 0 ? k : v;
+      const uint32_t s2 = both_halves(scale[y][i]);
+      uint32_t w[4];
+      if constexpr (N == 4) {   // (both bytes of a word of 32 bits: see the keys in kv_attn_rows.cuh)
+        const uint32_t word = codes[y][i] | codes[y][i] << 16;
+        const float2 lo = unpack2<false>(times(e2m1x2_to_f16x2(word, 0), s2)), hi = unpack2<false>(times(e2m1x2_to_f16x2(word, 1), s2));
+        w[0] = __float_as_uint(lo.x);
+        w[1] = __float_as_uint(lo.y);
+        w[2] = __float_as_uint(hi.x);
+        w[3] = __float_as_uint(hi.y);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          w[m] = times(e2m1x2_to_f16x2(codes[y][i], m), s2);
+          if (kType == KD_BF16) {
+            const float2 two = unpack2<false>(w[m]);
+            w[m] = pack2<true>(two.x, two.y);
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<char*>(out.ptr) + (b * out.stride_b + h * out.stride_h + static_cast<int64_t>(r0 + slot) * out.stride_t + d) * kSize) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    store16<kType>(static_cast<char*>(out.ptr) + (b * out.stride_b + h * out.stride_h + static_cast<int64_t>(r0 + slot) * out.stride_t + col * K4_GROUP) * kSize, f);
   }
 }
 
@@ -150,8 +208,9 @@ int launch_cache4_read(const kd_cache& c, const kd_cache_seqs& s, const int32_t*
   const int groups = (count + KC_PAGE - 1) / KC_PAGE;
   const int64_t grid = static_cast<int64_t>(s.B) * c.H * groups;
   if (grid > INT32_MAX) return set_error(KD_ERR_LIMIT, "%d sequences of %d tokens and %d heads are too many for one call", s.B, count, c.H);
-  auto* kernel = dtype == KD_F16 ? cache4_read_kernel<KD_F16> : dtype == KD_BF16 ? cache4_read_kernel<KD_BF16> : cache4_read_kernel<KD_F32>;
-  const cudaError_t e = launch(kernel, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, start, count, groups, k, v);
+  const cudaError_t e = by_type_and_dim(dtype, c.D, [&](auto type, auto dim) {
+    return launch(cache4_read_kernel<decltype(type)::value, decltype(dim)::value>, static_cast<unsigned>(grid), KC_THREADS, 0, stream, c, s, start, count, groups, k, v);
+  });
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache4_read_kernel launch: %s", cudaGetErrorString(e));
   return 0;
 }

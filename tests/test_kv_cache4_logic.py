@@ -40,22 +40,35 @@ def test_oracle_takes_the_nearest():
     assert k4.quantise(np.full((1, 16), 6 * 17 / 16))[1] == 120 and k4.quantise(np.full((1, 16), 6 * 19 / 16))[1] == 122   # scales of 1 and 1.25: 1.0625 is between 1 and 1.125
 
 
-def test_product_with_the_rounded_inverse_decides_as_the_quotient_does():
-    """What the kernels do with 16-bit numbers: x times the float nearest to 1 / scale, brought to a grid of 2**-13 by a fused sum with 1536, decides on the same side of each middle of two levels as
+def test_product_with_a_rounded_inverse_decides_as_the_quotient_does():
+    """What the kernels do with 16-bit numbers: x times a float within 2**-22 of 1 / scale, brought to a grid of 2**-13 by a fused sum with 1536, decides on the same side of each middle of two levels as
     x / scale, for every x of 11 bits (halves, and bfloat16 of 8 bits among them) and every scale of 4 bits. Powers of two apart, that is all of them: quotients are 6.4 at most."""
     x = np.arange(1024, 2048, dtype=np.float64)
     plain = 0
     for m in range(8, 16):
-        inverse = (np.float32(1) / np.float32(m)).astype(np.float64)   # nearest: numpy divides as IEEE says
-        for e in range(-30, -4):
-            v = x * 2.0 ** e
-            v = v[v <= 6.5 * m]
-            q = (v * inverse + 1536.0).astype(np.float32) - np.float32(1536)   # (the sum has 48 bits: exact in 64, rounded once)
-            for middle in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0):
-                exact = np.sign(v - middle * m)
-                assert np.array_equal(np.sign(q.astype(np.float64) - middle), exact)
-                plain += (np.sign((v * inverse).astype(np.float32).astype(np.float64) - middle) != exact).sum()
+        nearest = np.float32(1) / np.float32(m)   # numpy divides as IEEE says
+        for inverse in (nearest, np.nextafter(nearest, np.float32(0)), np.nextafter(nearest, np.float32(1))):   # the hardware's is off by one step at most
+            inverse = np.float64(inverse)
+            for e in range(-30, -4):
+                v = x * 2.0 ** e
+                v = v[v <= 6.5 * m]
+                q = (v * inverse + 1536.0).astype(np.float32) - np.float32(1536)   # (the sum has 48 bits: exact in 64, rounded once)
+                for middle in (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0):
+                    exact = np.sign(v - middle * m)
+                    assert np.array_equal(np.sign(q.astype(np.float64) - middle), exact)
+                    plain += (np.sign((v * inverse).astype(np.float32).astype(np.float64) - middle) != exact).sum()
     assert plain > 0   # the grid is needed
+
+
+def test_product_with_a_sixth_decides_as_the_quotient_does():
+    """What the kernels do with the largest of a group of 16-bit numbers: times the float nearest to 1 / 6, rounded to 17 bits, then to the nearest scale."""
+    x = (np.arange(1024, 2048, dtype=np.float64)[:, None] * 2.0 ** np.arange(-40.0, 7.0)).ravel()
+    x = x[x <= 65504]
+    u = (x.astype(np.float32) * (np.float32(1) / np.float32(6))).view(np.uint32)
+    u = (u + np.uint32(0x40)) & ~np.uint32(0x7F)
+    sixth = u.view(np.float32)
+    byte = np.where(sixth < 2.0 ** -14, np.rint(sixth * np.float32(2.0 ** 17)).astype(np.int64), np.minimum(k4.TOP, ((u + np.uint32(0x7FFFF) + (u >> 20 & 1)) >> 20).astype(np.int64) - 896))
+    assert np.array_equal(byte, k4._nearest(x, 6.0 * k4.SCALES))
 
 
 def test_quotient_by_six_is_not_rounded_onto_the_middle_of_two_scales():
