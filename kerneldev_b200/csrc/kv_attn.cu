@@ -71,21 +71,25 @@ __device__ __forceinline__ void join_row(const kd_cache& c, const kd_cache_queri
 
 // The rows of all items: eight warps for a row where there are few rows (a long context has dozens of parts), one where there are many. Rows without a query, and those of
 // sequences without a token, get their zeros here. What it needs to know of the lengths was there before the kernel ahead of it, so it is looked up while that one runs.
-template <int kGroups>
+// kRows: rows of a warp, of one item: what it has to know of the lengths is then looked up once for all of them (512 queries each of 2 x 8192 tokens of 8 heads, 4 rows a query: 30,000 warps went through
+// all lengths and divisions for a row each, and the join took 35 us, so 27).
+template <int kGroups, int kRows>
 __global__ void __launch_bounds__(KJ_WARPS * 32)
 cache_join_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ kd_cache_seqs s, const __grid_constant__ kd_cache_queries p,
                   const __grid_constant__ AttnShape shape, const __grid_constant__ AttnWorkspace ws) {
-  constexpr int ROWS = KJ_WARPS / kGroups;
+  constexpr int ROWS = KJ_WARPS / kGroups * kRows;
   static_assert(kGroups == 1 || ROWS == 1, "join_row's barriers are the whole CTA's");
   __shared__ JoinShared sh;
   const int warp = threadIdx.x >> 5, per_head = (shape.rows + ROWS - 1) / ROWS;
-  const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, row_of_head = (blockIdx.x - bh * per_head) * ROWS + warp / kGroups;
+  const int bh = blockIdx.x / per_head, b = bh / c.H, h = bh - b * c.H, first_row = (blockIdx.x - bh * per_head) * ROWS;
   const int len = sequence_length<true>(c, s, b), n = query_count<true>(c, p, b);
-  const ItemParts parts = parts_of(c, s, p, shape, b, h, row_of_head / shape.item_rows, len, n);
+  const ItemParts parts = parts_of(c, s, p, shape, b, h, first_row / shape.item_rows, len, n);
   pdl_wait();
   pdl_launch_dependents();
-  if (parts.count == 1 || row_of_head >= shape.rows) return;   // the one CTA has written the row
-  join_row<kGroups>(c, p, shape, ws, parts, b, h, row_of_head, len, n, warp % kGroups, &sh);
+  if (parts.count == 1) return;   // the one CTA has written the rows
+#pragma unroll 1
+  for (int row = first_row + warp / kGroups; row < min(first_row + ROWS, shape.rows); row += KJ_WARPS / kGroups)
+    join_row<kGroups>(c, p, shape, ws, parts, b, h, row, len, n, warp % kGroups, &sh);
 }
 
 // The weights of few rows, from the scores that the kernel ahead has left, and the join: a CTA has KS_TOKENS tokens of a head, the first ones of a head its rows too. (One launch
@@ -234,12 +238,14 @@ int launch_cache_attention(const kd_cache& c, const kd_cache_seqs& s, const kd_c
   }
   if (e == cudaSuccess && a.ctas > 0) {
     // (1024 CTAs for as many rows of two or three parts were two waves)
-    const bool few = heads * a.rows <= 148 * 2;
-    static SharedFirst first_few, first_many;
-    e = few ? first_few(cache_join_kernel<KJ_WARPS>) : first_many(cache_join_kernel<1>);
+    const bool few = heads * a.rows <= 148 * 2, many = a.item_rows >= 4 * KJ_WARPS && heads * a.rows >= 148 * 2 * 4 * KJ_WARPS;
+    static SharedFirst first_few, first_some, first_many;
+    e = few ? first_few(cache_join_kernel<KJ_WARPS, 1>) : many ? first_many(cache_join_kernel<1, 4>) : first_some(cache_join_kernel<1, 1>);
     if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_join_kernel attribute: %s", cudaGetErrorString(e));
-    e = few ? launch(cache_join_kernel<KJ_WARPS>, static_cast<unsigned>(heads * a.rows), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
-            : launch(cache_join_kernel<1>, static_cast<unsigned>(heads * ((a.rows + KJ_WARPS - 1) / KJ_WARPS)), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
+    auto ctas = [&](int rows) { return static_cast<unsigned>(heads * ((a.rows + rows - 1) / rows)); };
+    e = few    ? launch(cache_join_kernel<KJ_WARPS, 1>, ctas(1), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
+        : many ? launch(cache_join_kernel<1, 4>, ctas(4 * KJ_WARPS), KJ_WARPS * 32, 0, stream, c, s, p, a, ws)
+               : launch(cache_join_kernel<1, 1>, ctas(KJ_WARPS), KJ_WARPS * 32, 0, stream, c, s, p, a, ws);
   }
   if (e == cudaSuccess) e = bits == 8 ? launch_attention_weights8(c, s, p, a, ws, stream) : launch_attention_weights4(c, s, p, a, ws, stream);
   if (e != cudaSuccess) return set_error(KD_ERR_DEVICE, "cache_attention launch: %s", cudaGetErrorString(e));

@@ -181,9 +181,9 @@ struct QueryTile {
 };
 
 // S^T of a unit: c[n][i][x] of lane (g, t): token 16 i + g + 8 (x >> 1), row 2 t + (x & 1) of tile n
-template <int kBits, int D, int NT>
-__device__ __forceinline__ void scores(uint32_t stage, const Lane<kBits, D>& at, const QueryTile<D, NT>& q, float (&c)[NT][2][4]) {
-  const int lane = threadIdx.x & 31;
+// ... query(n, s): the operands of step s of tile n
+template <int kBits, int D, int NT, typename F>
+__device__ __forceinline__ void scores_of(uint32_t stage, const Lane<kBits, D>& at, F query, float (&c)[NT][2][4]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     using S = Spread<kBits, D>;
@@ -212,12 +212,17 @@ __device__ __forceinline__ void scores(uint32_t stage, const Lane<kBits, D>& at,
       const uint4 a = make_uint4(lo.lo, hi.lo, lo.hi, hi.hi);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint2 b = q.frag[n][s][lane];
+        const uint2 b = query(n, s);
         if (s == 0) mma_f16_first(c[n][i], a, b.x, b.y);
         else mma_f16(c[n][i], a, b.x, b.y);
       }
     }
   }
+}
+template <int kBits, int D, int NT>
+__device__ __forceinline__ void scores(uint32_t stage, const Lane<kBits, D>& at, const QueryTile<D, NT>& q, float (&c)[NT][2][4]) {
+  const int lane = threadIdx.x & 31;
+  scores_of<kBits, D, NT>(stage, at, [&](int n, int s) { return q.frag[n][s][lane]; }, c);
 }
 
 // bytes 0 and 1 (2 and 3) of two words in turn: for two tokens' values of two head dims
@@ -429,6 +434,16 @@ struct Walker {
     int o_unit = 0;
     const float slack = kSafe && far ? 0.f : KA_SLACK;
     char* stage = ring;
+    // One tile of rows over numbers of 4 bits: instructions are what bounds it, and what does not change from unit to unit stays in registers.
+    constexpr bool kHold = kBits == 4 && NT == 1;
+    [[maybe_unused]] uint2 held[kHold ? D / 16 : 1];
+    [[maybe_unused]] float held_factor[2], held_add[2] = {0.f, 0.f};
+    if constexpr (kHold) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) held[i] = q.frag[0][i][lane];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) held_factor[x] = score_factor(1.f, q.factor[2 * t + x]);
+    }
     for (int unit = first; unit < last; unit += KA_WARPS) {
       cp_async_wait<0>();
       __syncwarp();   // everyone's copies of this unit are there, and everyone is done with the one before it, whose place the next one takes
@@ -455,59 +470,94 @@ struct Walker {
         o_unit = ev_page;
       }
       float sc[NT][2][4];
-      scores<kBits, D, NT>(at, place, q, sc);
+      if constexpr (kHold) scores_of<kBits, D, NT>(at, place, [&](int, int i) { return held[i]; }, sc);
+      else scores<kBits, D, NT>(at, place, q, sc);
       uint32_t p[2][NT][2], vis[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (page < 0 || j0 + KA_UNIT > free_end) mask_scores(sc[n], desc, j0, g, t, page < 0 ? 0 : it.len, &q.mask[n * KA_TILE]);
-        float k[2], add[2], high[2], old[2];
-        bool moves = false;
+        float k[2], add[2];
         if (NT == 1 && all_scores != nullptr && 2 * t < score_rows) {
           const float k0 = score_factor(ks, q.factor[2 * t]), k1 = score_factor(ks, q.factor[2 * t + 1]);
 #pragma unroll
           for (int y = 0; y < 4; ++y)
             *reinterpret_cast<float2*>(all_scores + static_cast<size_t>(j0 + 8 * y + g) * score_rows + 2 * t) = make_float2(sc[n][y >> 1][2 * (y & 1)] * k0, sc[n][y >> 1][2 * (y & 1) + 1] * k1);
         }
-        auto set_add = [&](int x) { add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x]; };
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          k[x] = score_factor(ks, q.factor[n * KA_TILE + 2 * t + x]);
-          // the row's maximum, over the lanes of its tokens
-          float top = fmaxf(fmaxf(sc[n][0][x], sc[n][0][2 + x]), fmaxf(sc[n][1][x], sc[n][1][2 + x]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          high[x] = fmaf(top, k[x], static_cast<float>(ev));
-          old[x] = ref[n][x];
-          const bool up = high[x] > old[x] + slack;
-          moves = moves | up | (scales.apart & (high[x] < old[x] - KA_DEPTH));   // (no branch here: it costs 4 % of the time with 32 rows; -inf is seen to below)
-          ref[n][x] = up ? high[x] : old[x];   // (ahead of the vote: the exponentials wait for it)
-          set_add(x);
-        }
-        if (__any_sync(0xffffffffu, moves)) {
-          float shrink[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) shrink[x] = ref[n][x] == old[x] ? 1.f : fast_exp2(old[x] - ref[n][x]);
-          if (kBits == 8 && scales.ever())
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              float total = sum[n][x];
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-              if (ref[n][x] != old[x]) ref[n][x] = rintf(high[x]);
-              else if (scales.apart && below_reference(high[x], old[x])) ref[n][x] = reference_below(high[x], old[x], total);
-              set_add(x);
-              shrink[x] = rescale(old[x], ref[n][x]);
-            }
+        if constexpr (kHold) {
+          // A row's reference stays while no lane has a score beyond it: the maximum over the lanes is formed only then.
+          float top[2];
+          bool moves = false;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            sum[n][x] *= shrink[x];
-            scales.look(ref[n][x]);
+            k[x] = held_factor[x];
+            top[x] = fmaxf(fmaxf(sc[n][0][x], sc[n][0][2 + x]), fmaxf(sc[n][1][x], sc[n][1][2 + x])) * k[x];
+            moves = moves | (top[x] > ref[n][x] + slack);
           }
+          if (__any_sync(0xffffffffu, moves)) {
+            float shrink[2];
 #pragma unroll
-          for (int m = 0; m < D / 16; ++m)
+            for (int x = 0; x < 2; ++x) {
+              top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+              top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+              top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+              const float to = top[x] > ref[n][x] + slack ? top[x] : ref[n][x];
+              shrink[x] = to == ref[n][x] ? 1.f : fast_exp2(ref[n][x] - to);
+              ref[n][x] = to;
+              held_add[x] = to == -INFINITY ? 0.f : KA_OFFSET - to;
+              sum[n][x] *= shrink[x];
+              scales.look(to);
+            }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[n][m][x] *= shrink[x & 1];
+            for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[n][m][x] *= shrink[x & 1];
+          }
+          add[0] = held_add[0];
+          add[1] = held_add[1];
+        } else {
+          float high[2], old[2];
+          bool moves = false;
+          auto set_add = [&](int x) { add[x] = ref[n][x] == -INFINITY ? 0.f : static_cast<float>(ev) + KA_OFFSET - ref[n][x]; };
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            k[x] = score_factor(ks, q.factor[n * KA_TILE + 2 * t + x]);
+            // the row's maximum, over the lanes of its tokens
+            float top = fmaxf(fmaxf(sc[n][0][x], sc[n][0][2 + x]), fmaxf(sc[n][1][x], sc[n][1][2 + x]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            high[x] = fmaf(top, k[x], static_cast<float>(ev));
+            old[x] = ref[n][x];
+            const bool up = high[x] > old[x] + slack;
+            moves = moves | up | (scales.apart & (high[x] < old[x] - KA_DEPTH));   // (no branch here: it costs 4 % of the time with 32 rows; -inf is seen to below)
+            ref[n][x] = up ? high[x] : old[x];   // (ahead of the vote: the exponentials wait for it)
+            set_add(x);
+          }
+          if (__any_sync(0xffffffffu, moves)) {
+            float shrink[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) shrink[x] = ref[n][x] == old[x] ? 1.f : fast_exp2(old[x] - ref[n][x]);
+            if (kBits == 8 && scales.ever())
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                float total = sum[n][x];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                if (ref[n][x] != old[x]) ref[n][x] = rintf(high[x]);
+                else if (scales.apart && below_reference(high[x], old[x])) ref[n][x] = reference_below(high[x], old[x], total);
+                set_add(x);
+                shrink[x] = rescale(old[x], ref[n][x]);
+              }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              sum[n][x] *= shrink[x];
+              scales.look(ref[n][x]);
+            }
+#pragma unroll
+            for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[n][m][x] *= shrink[x & 1];
+          }
         }
         if constexpr (kSafe) {
 #pragma unroll
