@@ -149,7 +149,7 @@ struct RotateBackward : torch::autograd::Node {
       if (!g.defined()) return like.zeros();
       KD_VALUE(g.sizes() == at::IntArrayRef(like.sizes) && g.device() == *like.device, "the gradient of an output of shape ", like.sizes, " on ", *like.device, " has shape ", g.sizes(),
                " on ", g.device());
-      return rows16(g.to(like.type));
+      return rows16(g.scalar_type() == like.type ? g : g.to(like.type));
     };
     // (saved tensors may have been moved and brought back with other strides)
     if (tq.defined()) tq = rows16(tq);
