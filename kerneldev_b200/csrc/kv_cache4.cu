@@ -18,14 +18,33 @@ __device__ __forceinline__ float inverse_of(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// The largest magnitude of 16 numbers as the bits of a float, which are those of an infinity or NaN where one of the numbers is.
+template <int kType>
+__device__ __forceinline__ uint32_t group_max(const Raw16<kType>& raw) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < Raw16<kType>::WORDS; ++i) {
+    const uint32_t w[4] = {raw.v[i].x, raw.v[i].y, raw.v[i].z, raw.v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kType == KD_F32) top = max(top, w[j] & 0x7FFFFFFFu);
+      else if constexpr (kType == KD_BF16) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w[j] & 0x7FFF7FFFu));
+      else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w[j] & 0x7FFF7FFFu));
+    }
+  }
+  if constexpr (kType == KD_F32) return top;
+  const float2 two = unpack2<kType == KD_BF16>(top);
+  return max(__float_as_uint(two.x), __float_as_uint(two.y)) & 0x7FFFFFFFu;
+}
 // A group as it is stored. The scale is the nearest to a sixth of the largest magnitude, and the numbers the nearest to what they are in its units; ties go to even.
 // Floats are divided; a quotient is never rounded onto the middle of two steps: a float next to a middle times 6 or times a scale of 4 bits is 2^-24 of it away, and a quotient's rounding moves it
 // less. 16-bit numbers are multiplied with a rounded inverse, and the product brought to a coarser grid (2^-16 of itself; 2^-13 by the fused sum with 1536, of which one step is that much), which puts it on a middle
 // exactly where the quotient is: numbers of 11 bits have no other quotient that near to one (tests/test_kv_cache4_logic.py goes through all of them). That takes a third of the instructions of divisions.
 template <int kType>
 __device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
-  bool special = false;
-  const float top = __uint_as_float(raw.amax(special));
+  const uint32_t top_bits = group_max(raw);
+  if (top_bits >= 0x7F800000u) return Group4{make_uint2(0u, 0u), K4_NAN};
+  const float top = __uint_as_float(top_bits);
   uint32_t u;
   if constexpr (kType == KD_F32) u = __float_as_uint(__fdiv_rn(top, 6.f));
   else u = (__float_as_uint(top * (1.f / 6.f)) + 0x40u) & ~0x7Fu;
@@ -39,7 +58,6 @@ __device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
     if constexpr (kType == KD_F32) f[i] = byte != 0u ? __fdiv_rn(f[i], scale) : 0.f;
     else f[i] = __fsub_rn(__fmaf_rn(f[i], inverse, 1536.f), 1536.f);
   }
-  if (special) return Group4{make_uint2(0u, 0u), K4_NAN};
   return Group4{make_uint2(f32x8_to_e2m1x8(f), f32x8_to_e2m1x8(f + 8)), byte};
 }
 
@@ -141,45 +159,45 @@ cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ k
                    const __grid_constant__ kd_tensor k, const __grid_constant__ kd_tensor v) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int kSize = kType == KD_F32 ? 4 : 2, N = 16 / kSize, ROW = D / N, ITEMS = KC_PAGE * ROW, EACH = (ITEMS + KC_THREADS - 1) / KC_THREADS;   // N numbers of a thread
+  constexpr int kSize = kType == KD_F32 ? 4 : 2, N = 16 / kSize, ROW = D / N, SLOTS = KC_THREADS / ROW, EACH = (KC_PAGE + SLOTS - 1) / SLOTS;   // N numbers of a thread, SLOTS tokens at a time
   const uint32_t item = blockIdx.x / static_cast<uint32_t>(groups);
   const int r0 = static_cast<int>(blockIdx.x - item * groups) * KC_PAGE;
   const int b = static_cast<int>(item / static_cast<uint32_t>(c.H)), h = static_cast<int>(item - static_cast<uint32_t>(b) * c.H);
-  const int len = sequence_length(c, s, b);
+  const int len = sequence_length(c, s, b), first = threadIdx.x / ROW, d = threadIdx.x % ROW * N, here = min(KC_PAGE, count - r0);
+  if (first >= SLOTS) return;
   const int64_t from = (start != nullptr ? start[b] : 0) + static_cast<int64_t>(r0);
   const int64_t block = from >= 0 ? from / KC_PAGE : -((KC_PAGE - 1 - from) / KC_PAGE);   // of the first token
-  size_t rows[2];   // the pages' first token
-  bool there[2];
+  const int in = static_cast<int>(from - block * KC_PAGE);                                // its place there
+  // tokens live .. end - 1 exist
+  const int live = static_cast<int>(max(int64_t(0), min(int64_t(KC_PAGE), -from))), end = static_cast<int>(max(int64_t(0), min(int64_t(here), len - from)));
+  int64_t rows[2];   // of token 0, if it were in this page; negative: there is none
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const int page = block + x >= 0 && (block + x) * KC_PAGE < len && (x == 0 || from > block * KC_PAGE) ? page_of(c, s, b, static_cast<int>(block + x)) : -1;
-    there[x] = page >= 0;
-    rows[x] = block_index(c, max(page, 0), h) * KC_PAGE;
+    const int page = live < end && block + x >= 0 && (block + x) * KC_PAGE < len && (x == 0 || in > 0) ? page_of(c, s, b, static_cast<int>(block + x)) : -1;
+    rows[x] = page >= 0 ? static_cast<int64_t>(block_index(c, page, h)) * KC_PAGE + in - x * KC_PAGE : INT64_MIN / 2;
   }
   uint32_t codes[2][EACH], scale[2][EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int x = i * KC_THREADS + threadIdx.x, slot = x / ROW, d = x % ROW * N;
-    const int64_t j = from + slot;
-    const int in = static_cast<int>(j - block * KC_PAGE), second = in >= KC_PAGE ? 1 : 0;
-    const size_t row = rows[second] + (in - second * KC_PAGE);
-    const bool live = slot < KC_PAGE && r0 + slot < count && j >= 0 && j < len && there[second];
+    const int slot = first + i * SLOTS;
+    const int64_t row = rows[in + slot >= KC_PAGE ? 1 : 0] + slot;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       codes[y][i] = scale[y][i] = 0u;
-      if (!live) continue;
-      const uint8_t* at = static_cast<const uint8_t*>(y == 0 ? c.k : c.v) + (row * D + d) / 2;
+      if (slot < live || slot >= end || row < 0) continue;
+      const uint8_t* at = static_cast<const uint8_t*>(y == 0 ? c.k : c.v) + (row * (D / 2) + d / 2);
       codes[y][i] = N == 8 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
       scale[y][i] = scales4(y == 0 ? c.k_scale : c.v_scale)[row * (D / K4_GROUP) + d / K4_GROUP];
     }
   }
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const int x = i * KC_THREADS + threadIdx.x, slot = x / ROW, d = x % ROW * N;
-    if (slot >= KC_PAGE || r0 + slot >= count) continue;
+  for (int y = 0; y < 2; ++y) {
+    const kd_tensor& out = y == 0 ? k : v;
+    char* to = static_cast<char*>(out.ptr) + (b * out.stride_b + h * out.stride_h + static_cast<int64_t>(r0 + first) * out.stride_t + d) * kSize;
+    const int64_t step = SLOTS * out.stride_t * kSize;
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const kd_tensor& out = y == 0 ? k : v;
+    for (int i = 0; i < EACH; ++i, to += step) {
+      if (first + i * SLOTS >= here) continue;
       const uint32_t s2 = both_halves(scale[y][i]);
       uint32_t w[4];
       if constexpr (N == 4) {   // (both bytes of a word of 32 bits: see the keys in kv_attn_rows.cuh)
@@ -199,7 +217,7 @@ cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ k
           }
         }
       }
-      *reinterpret_cast<uint4*>(static_cast<char*>(out.ptr) + (b * out.stride_b + h * out.stride_h + static_cast<int64_t>(r0 + slot) * out.stride_t + d) * kSize) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
