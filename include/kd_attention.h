@@ -275,7 +275,7 @@ int kd_cocktail_scores(const kd_cocktail* p, void* stream);
 int kd_cocktail_grad(const kd_cocktail* p, void* stream);
 
 /* ---- rotation of the heads of q and k by position, with their norms -------------------------------------------------
- * No counterpart in the reference, whose GPTModel adds learned positions to the embeddings (model.py:127-160). Stands ahead of kd_attn_fwd and
+ * No counterpart in the reference, whose GPTModel adds learned positions to the embeddings (model.py:152, :188-191). Stands ahead of kd_attn_fwd and
  * kd_cache_append.
  *
  * Row x of D numbers (one head of one token): y = weight * x / sqrt(mean(x^2) + eps) where there is a weight, else y = x. Pair i of R / 2, elements i and

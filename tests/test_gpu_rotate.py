@@ -357,3 +357,64 @@ def test_rotation_then_attention_trains_as_the_definition_says():
         err = (x.double().cpu() - y).abs()
         assert bool((err <= 2e-2 * (300 if name == "w" else 1) + 1e-2 * y.abs()).all()), name
         assert float(err.norm() / y.norm()) < 1e-2, name
+
+
+def test_offsets_beyond_32_bits():
+    """Heads 2**32 elements apart."""
+    from kerneldev_b200 import Rotation, rotate_heads
+    free, _ = torch.cuda.mem_get_info()
+    if free < 2 ** 34 + 2 ** 30:
+        pytest.skip("needs 17 GB")
+    memory = torch.empty(2 ** 32 + 4096, dtype=torch.bfloat16, device=DEV)
+    x, grad = [memory.as_strided((1, 2, 3, 64), (2 ** 32, 2 ** 32, 64, 1), at).normal_() for at in (0, 2048)]
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    rotation = Rotation(64, device=DEV)
+    y, _ = rotate_heads(x, None, rotation, q_weight=w)
+    z, _ = rotate_heads(x.contiguous(), None, rotation, q_weight=w)
+    assert torch.equal(y, z)
+    assert torch.equal(torch.autograd.grad(y, w, grad)[0], torch.autograd.grad(z, w, grad.contiguous())[0])
+
+
+def test_two_calls_at_once_on_two_threads():
+    """Each with a stream and leaves of its own."""
+    import threading
+    from kerneldev_b200 import Rotation, rotate_heads
+    rotation = Rotation(64, device=DEV)
+    work, errors = [], []
+    for i in range(2):
+        q = torch.randn((2, 4, 300 + i, 64), device=DEV).bfloat16().requires_grad_()
+        w = torch.randn(64, device=DEV, requires_grad=True)
+        y, _ = rotate_heads(q, None, rotation, q_weight=w)
+        work.append((q, w, y.detach(), torch.autograd.grad(y, (q, w), y.detach())))
+    torch.cuda.synchronize()
+
+    def go(q, w, y, grads):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    z, _ = rotate_heads(q, None, rotation, q_weight=w)
+                    got = torch.autograd.grad(z, (q, w), y)
+                torch.cuda.current_stream().synchronize()
+                assert torch.equal(z, y) and all(torch.equal(a, b) for a, b in zip(got, grads))
+        except BaseException as e:   # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=go, args=x) for x in work]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+
+
+def test_second_derivatives_have_no_history():
+    """As those of flash_attention: with create_graph the gradients are plain tensors."""
+    from kerneldev_b200 import Rotation, rotate_heads
+    q = torch.randn((1, 1, 3, 16), device=DEV, requires_grad=True)
+    y, _ = rotate_heads(q, None, Rotation(16, device=DEV))
+    g, = torch.autograd.grad(y.square().sum(), q, create_graph=True)
+    assert not g.requires_grad
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):   # what a backward reads again may not change
+        w = torch.ones(16, device=DEV, requires_grad=True)
+        pos = torch.zeros((1, 3), dtype=torch.int32, device=DEV)
+        y, _ = rotate_heads(q, None, Rotation(16, device=DEV), pos, q_weight=w)
+        pos += 1
+        torch.autograd.grad(y.sum(), q)
