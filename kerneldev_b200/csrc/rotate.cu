@@ -9,8 +9,9 @@
 //
 // Bound by memory: each number is read and written once. A row has a group of D / 16 lanes, 16 numbers to each: the pairs of a lane are its own, and a lane keeps its
 // sines and cosines for all heads of a run. Rows are asked for ahead by asynchronous copies into shared memory, so that what is in flight takes no registers: with loads into registers a backward of
-// 16 x 4096 tokens of 32 heads of 64 (bf16) took 235 us, so 155 (805 MB, 5.2 TB/s; the forward 95 us, 5.6 TB/s, 106 before). A lane's pieces lie a part of the row apart, so that a copy of all lanes takes whole
-// sectors: with 32 bytes side by side to a lane, interleaved pairs of 16384 tokens of 40 heads of 128 took 79 us, so 58.
+// 16 x 4096 tokens of 32 heads of 64 (bf16) took 235 us, so 133 (805 MB, 6.0 TB/s; the forward 87 us, 6.1 TB/s, 106 before); instructions come next, of which addresses formed anew and zeros for rows that
+// are not there cost 22 us. A lane's pieces lie a part of the row apart, so that a copy of all lanes takes whole
+// sectors: with 32 bytes side by side to a lane, interleaved pairs of 16384 tokens of 40 heads of 128 took 79 us, so 57.
 #include <algorithm>
 #include <numeric>
 
@@ -118,6 +119,7 @@ struct Lane16 {
       }
     }
   }
+  // row: of the first piece
   __device__ __forceinline__ void store(char* row, const float (&f)[16]) const {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -128,7 +130,7 @@ struct Lane16 {
         constexpr bool kBf16 = kType == KD_BF16;
         v = make_uint4(pack2<kBf16>(f[8 * i], f[8 * i + 1]), pack2<kBf16>(f[8 * i + 2], f[8 * i + 3]), pack2<kBf16>(f[8 * i + 4], f[8 * i + 5]), pack2<kBf16>(f[8 * i + 6], f[8 * i + 7]));
       }
-      *reinterpret_cast<uint4*>(row + element(i * EACH) * SIZE) = v;
+      *reinterpret_cast<uint4*>(row + i * part * SIZE) = v;
     }
   }
 };
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / L, u = lane - group * L, base = group * L;
   const int run = blockIdx.x / shape.ctas, cta = blockIdx.x - run * shape.ctas;
   const bool is_k = run >= shape.runs_q, mine = group < ROWS, turns = 16 * u < p.R;
-  const int h0 = (run - (is_k ? shape.runs_q : 0)) * shape.heads, h1 = h0 + shape.heads;
+  const int h0 = (run - (is_k ? shape.runs_q : 0)) * shape.heads;
   const kd_tensor& x = is_k ? p.k : p.q;
   const kd_tensor& y = is_k ? p.k_out : p.q_out;
   const kd_tensor& dx = is_k ? p.dk : p.dq;
@@ -177,29 +179,40 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
     const int token = tile * tokens_of(D) + warp * ROWS + group, at = min(token, tokens - 1), b = at / p.T;
     return Place{b, at - b * p.T, token < tokens && mine};
   };
-  auto row_of = [&](const kd_tensor& z, const Place& at, int h) { return static_cast<char*>(z.ptr) + (at.b * z.stride_b + h * z.stride_h + at.t * z.stride_t) * kSize; };
+  // the lane's first piece in the first head of the run; further heads are a step apart
+  auto row_of = [&](const kd_tensor& z, const Place& at) { return static_cast<char*>(z.ptr) + (at.b * z.stride_b + h0 * z.stride_h + at.t * z.stride_t + mine16.start) * kSize; };
 
   // the next row to ask for
-  int ask_tile = cta, ask_h = h0, ask_stage = 0;
-  Place ask_at = place_of(ask_tile);
+  int ask_tile = cta, ask_h = 0, ask_stage = 0;   // ask_h: of the run
+  bool ask_live;
+  const char *ask_x, *ask_y = nullptr;
+  auto open = [&]() {
+    const Place at = place_of(ask_tile);
+    ask_live = at.live;
+    ask_x = row_of(x, at);
+    if (kGrad) ask_y = row_of(y, at);
+  };
+  open();
+  // (Pointers that move on from head to head in the backward; in the forward, where they were 3 to 4 % slower, products with the head.)
   auto ask = [&]() {
     if (ask_tile < shape.tiles) {
-      if (ask_at.live) {
-        if (reads_x) {
-          const char* row = row_of(x, ask_at, ask_h);
+      const char* row = kGrad ? ask_x : ask_x + ask_h * x.stride_h * kSize;
+      if (ask_live) {
+        if (reads_x)
 #pragma unroll
-          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, i), row + mine16.element(i * Row::EACH) * kSize);
-        }
-        if constexpr (kGrad) {
-          const char* row = row_of(y, ask_at, ask_h);
+          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, i), row + i * mine16.part * kSize);
+        if constexpr (kGrad)
 #pragma unroll
-          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, Row::PIECES + i), row + mine16.element(i * Row::EACH) * kSize);
-        }
+          for (int i = 0; i < Row::PIECES; ++i) cp_async16(Ring::place(ring, ask_stage, Row::PIECES + i), ask_y + i * mine16.part * kSize);
       }
-      if (++ask_h == h1) {
-        ask_h = h0;
+      if (kGrad) {
+        ask_x += x.stride_h * kSize;
+        ask_y += y.stride_h * kSize;
+      }
+      if (++ask_h == shape.heads) {
+        ask_h = 0;
         ask_tile += shape.ctas;
-        ask_at = place_of(ask_tile);
+        open();
       }
     }
     ask_stage = ask_stage + 1 == Ring::STAGES ? 0 : ask_stage + 1;
@@ -237,19 +250,20 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
         turn<kType>(static_cast<int32_t>((static_cast<uint64_t>(here) * p.steps[pair]) >> 32), c[i], s[i]);
       }
     }
+    char* to = row_of(kGrad ? dx : y, at);
+    const int64_t to_step = (kGrad ? dx : y).stride_h * kSize;
 #pragma unroll 1
-    for (int h = h0; h < h1; ++h) {
+    for (int h = 0; h < shape.heads; ++h) {
       await_copies<Ring::STAGES - 2>();
       float f[16];
-      auto take = [&](int from, float (&to)[16], bool there) {
+      auto take = [&](int from, float (&into)[16]) {   // (a row that is not there is whatever its place holds, and stays in its lanes)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) to[i] = 0.f;
-        if (there)
-#pragma unroll
-          for (int i = 0; i < Row::PIECES; ++i) Row::floats(lds16(Ring::place(ring, stage, from + i)), to + i * Row::EACH);
+        for (int i = 0; i < Row::PIECES; ++i) Row::floats(lds16(Ring::place(ring, stage, from + i)), into + i * Row::EACH);
       };
       if constexpr (!kGrad) {
-        take(0, f, at.live);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = 0.f;   // (without these, and loads for dead rows too, the forward is 5 % slower)
+        if (at.live) take(0, f);
         if (weight != nullptr) {
           float sum = 0.f;
 #pragma unroll
@@ -259,13 +273,13 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
           for (int j = 0; j < 16; ++j) f[j] = f[j] * r * w[j];
         }
         if (turns) rotate16<false>(f, c, s, p.interleaved != 0);
-        if (at.live) mine16.store(row_of(y, at, h), f);
+        if (at.live) mine16.store(to + h * to_step, f);
       } else {
         float g[16];
-        take(Row::PIECES, g, at.live);
+        take(Row::PIECES, g);
         if (turns) rotate16<true>(g, c, s, p.interleaved != 0);
         if (weight != nullptr) {
-          take(0, f, at.live);
+          take(0, f);
           float sum = 0.f, dot = 0.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
@@ -275,11 +289,11 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
           const float r = __frsqrt_rn(fmaf(row_sum<L>(sum, base, u), 1.f / D, p.eps)), back = row_sum<L>(dot, base, u) * (1.f / D) * r * r;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            dw[j] = fmaf(g[j], f[j] * r, dw[j]);
+            if (at.live) dw[j] = fmaf(g[j], f[j] * r, dw[j]);
             g[j] = r * fmaf(-f[j], back, g[j] * w[j]);
           }
         }
-        if (at.live) mine16.store(row_of(dx, at, h), g);
+        if (at.live) mine16.store(to + h * to_step, g);
       }
       ask();   // (into the place of the row before: its numbers have been used)
       stage = stage + 1 == Ring::STAGES ? 0 : stage + 1;
