@@ -653,3 +653,51 @@ def test_wait_timeout_in_the_attention_of_many_rows(drop):
     assert "bits=4" in child
     r = subprocess.run([sys.executable, "-c", child], env=env, capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "unwound and recovered" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
+
+
+@pytest.mark.parametrize("B,Hkv,G,T", [(2, 2, 3, 1), (2, 1, 8, 3), (40, 8, 1, 1), (2, 2, 2, 40), (40, 4, 1, 40)])
+@pytest.mark.parametrize("weigh", [False, True], ids=["plain", "weigh"])
+def test_share_whose_visible_keys_are_all_nan(B, Hkv, G, T, weigh):
+    """All keys of a run of pages are NaN: no row that sees them has a number, whichever CTA's share they are."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(B + T)
+    lens = rng.integers(1200, 1900, B)
+    c, table = filled(rng, B, Hkv, 64, lens, torch.bfloat16, False)
+    q = rand_kv(rng, (B, Hkv * G, T, 64), torch.bfloat16, False).to(DEV)
+    clean = cache_attention(q, c, i32(table), i32(lens), return_lse=True)
+    b, blocks = B - 1, -(-int(lens[B - 1]) // 64)
+    for first in (0, blocks // 2, blocks - 8):
+        pages = table[b, first:first + 7]
+        old = c.k_scale[pages, Hkv - 1].clone()
+        c.k_scale[pages, Hkv - 1] = 0xFF
+        w = torch.zeros((B, Hkv, 1900), device=DEV) if weigh else None
+        o, lse = cache_attention(q, c, i32(table), i32(lens), return_lse=True, weights=w)
+        c.k_scale[pages, Hkv - 1] = old
+        hit = torch.zeros(lse.shape, dtype=torch.bool, device=DEV)
+        hit[b, (Hkv - 1) * G:] = True
+        assert torch.isnan(o[hit]).all() and torch.isnan(lse[hit]).all()
+        assert torch.equal(o[~hit], clean[0][~hit]) and torch.equal(lse[~hit], clean[1][~hit])
+        if weigh:
+            assert torch.isnan(w[b, Hkv - 1, :int(lens[b]) - T + 1]).all() and torch.isfinite(w[b, :Hkv - 1]).all() and torch.isfinite(w[:b]).all()
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("G,T", [(3, 1), (4, 3), (2, 40)])
+def test_nan_of_single_groups_at_every_head_dim(D, G, T):
+    """Groups of values that are NaN, in tokens that some rows see and others do not: their columns are NaN in the rows that see them, all else is as without them."""
+    from kerneldev_b200 import cache_attention
+    rng = np.random.default_rng(D + T)
+    B, n = 2, 900
+    c, table = filled(rng, B, 1, D, [n, n], torch.bfloat16, False)
+    q = rand_kv(rng, (B, G, T, D), torch.bfloat16, False).to(DEV)
+    clean = cache_attention(q, c, i32(table), i32([n, n]), return_lse=True)
+    nan = torch.zeros((B, T, D), dtype=torch.bool, device=DEV)
+    for b in range(B):
+        for g in range(b, D // 16, 2):
+            at = n - 1 - int(rng.integers(T)) if g % 2 else int(rng.integers(n))
+            c.v_scale[table[b, at // 64], 0, at % 64, g] = 0xFF
+            nan[b, max(at - (n - T), 0):, 16 * g:16 * g + 16] = True
+    o, lse = cache_attention(q, c, i32(table), i32([n, n]), return_lse=True)
+    nan = nan[:, None].expand(B, G, T, D)
+    assert torch.isnan(o[nan]).all() and torch.isfinite(o[~nan]).all() and torch.equal(lse, clean[1])
+    assert torch.equal(o[~nan], clean[0][~nan])   # a column's NaN took the place of a number: the others are sums of the same products
