@@ -119,9 +119,13 @@ struct RotateBackward : torch::autograd::Node {
     const auto current = at::cuda::getCurrentCUDAStream();
     if (!Capture(current.stream()).active) return;
     const auto* asked = torch::autograd::get_current_graph_task_exec_info();
-    if (asked != nullptr && !asked->empty()) return;   // torch.autograd.grad: nothing is added to leaves
+    const bool all = asked == nullptr || asked->empty();   // else only those asked for by name: torch.autograd.grad hands their gradients out, backward(inputs=...) adds them
     for (const auto& edge : next_edges())
       if (auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) {
+        if (!all) {
+          const auto named = asked->find(leaf);
+          if (named == asked->end() || !named->second.needed_) continue;
+        }
         const auto stream = leaf->stream();
         TORCH_CHECK(!stream.has_value() || *stream == current.unwrap(),
                     "a backward pass of rotate_heads cannot be captured while an earlier graph of the same leaves lives: its gradients are added on that graph's stream. "

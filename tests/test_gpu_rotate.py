@@ -325,6 +325,38 @@ print("alive:", torch.isfinite(q.grad).all().item())
     assert r.returncode == 0 and "refused: True" in r.stdout and "alive: True" in r.stdout, r.stdout + r.stderr
 
 
+def test_captured_backward_for_named_leaves_beside_an_eager_graph_is_refused():
+    """backward(inputs=...) adds to the leaves that it names: refused too, where one of those belongs to the eager graph, and captured where none does. (In a process of its own, as above.)"""
+    code = """
+import torch
+from kerneldev_b200 import Rotation, rotate_heads
+rotation = Rotation(32, device="cuda")
+q, w = torch.randn((1, 2, 4, 32), device="cuda", requires_grad=True), torch.ones(32, device="cuda", requires_grad=True)
+fresh = torch.ones(32, device="cuda", requires_grad=True)
+eager, _ = rotate_heads(q, None, rotation, q_weight=w)
+g = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(g):
+        y, _ = rotate_heads(q, None, rotation, q_weight=fresh)
+        y.sum().backward(inputs=[q])
+except RuntimeError as e:
+    print("refused:", "cannot be captured" in str(e))
+torch.cuda.synchronize()
+fresh = torch.ones(32, device="cuda", requires_grad=True)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y, _ = rotate_heads(q, None, rotation, q_weight=fresh)
+    y.sum().backward(inputs=[fresh])
+g.replay()
+torch.cuda.synchronize()
+eager.sum().backward()
+print("alive:", torch.equal(fresh.grad, w.grad) and torch.isfinite(q.grad).all().item())
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "refused: True" in r.stdout and "alive: True" in r.stdout, r.stdout + r.stderr
+
+
 def test_rotation_then_attention_trains_as_the_definition_says():
     """rotate_heads and flash_attention together: causal attention of turned and normalised heads, and the gradients of everything ahead of it."""
     from kerneldev_b200 import Rotation, flash_attention, rotate_heads
