@@ -93,7 +93,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, l
 
     For more than eight query rows of a key head, and where the scores of fewer would take more than 256 MB and an eighth of the cache, ``weights`` comes
     from scores that are added up a second time, in float32 and in another order: a row's weights are then off by a factor that grows with its
-    scores, about 2**-21 of them as an exponent of two. Where scores lie beyond 2**16 that is a few per cent and more, beyond 2**21 they say nothing.
+    scores (in powers of two, or with the sum of the sizes of their products where those cancel), at most about 2**-21 of them: a few per cent at 2**16 (0.1 % was measured), and
+    beyond 2**21 they say nothing.
 
     A weight enters the product with v with 11 bits, and with an error of no more than 2**-28 of the row's largest weight (2**-25 in rows with scores
     beyond 2**16, in powers of two), or, where the value scales of an 8-bit cache's pages are more than 2**4 apart, 2**-20 of its page's largest.
