@@ -112,6 +112,21 @@ struct RotateBackward : torch::autograd::Node {
   RotateArgs args;
   Geometry q_like, k_like;
   bool has_k, has_qw, has_kw;
+  bool history_lost = false;   // (under mutex_)
+
+  // Gradients have no history of their own. Where they are to have one (create_graph) and depend on what is differentiated, that is said. A loss with such gradients in it and other terms
+  // comes through this node again, and would lack their part: that is refused.
+  void refuse_lost_history(const torch::autograd::variable_list& grads) {
+    TORCH_CHECK(!history_lost,
+                "rotate_heads is differentiable once: an earlier backward pass through this call, with create_graph=True, gave gradients without a history, and what depends on them would be missing "
+                "from this one. Use retain_graph=True where no second derivative is wanted");
+    if (!at::GradMode::is_enabled()) return;
+    for (int i = 0; i < (has_k ? 2 : 1); ++i) {
+      const bool row = next_edge(i).is_valid(), weight = next_edge(i + 2).is_valid(), norm = i == 0 ? has_qw : has_kw;
+      history_lost = history_lost || ((row || weight) && grads[i].defined() && grads[i].requires_grad()) || (row && norm);
+    }
+    if (history_lost) TORCH_WARN("rotate_heads is differentiable once: with create_graph=True its gradients have no history, and second derivatives through them will be missing");
+  }
 
   // A gradient that is added to a leaf in a captured backward pass is added on the stream that the leaf's first graph was made on, while that lives: where that is not the capturing
   // one, torch's engine ends the process. So this is refused before it comes to that.
@@ -138,6 +153,7 @@ struct RotateBackward : torch::autograd::Node {
     Tensor tq, tk, tqw, tkw, tp, to;
     {
       std::lock_guard<std::mutex> lock(mutex_);
+      refuse_lost_history(grads);
       tq = q.unpack();
       tk = k.unpack();
       tqw = q_weight.unpack();

@@ -92,7 +92,8 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, rotation: Rotation, po
     q_weight, k_weight: (head_dim,) in any of the three types. With one, a row x becomes weight * x / sqrt(mean(x**2) + eps) before it is turned; the mean is taken in 32 bits
     (squares beyond its range make the row zeros). Everything is computed in 32 bits and rounded once.
 
-    Differentiable, once, in q, k and the weights; sums over rows are taken in a fixed order. A backward pass that adds to leaves cannot be captured while an
+    Differentiable, once, in q, k and the weights; sums over rows are taken in a fixed order. With ``create_graph`` the gradients are plain tensors all the same: where a second derivative would go through
+    them a warning says so, and a later backward pass through the same call, as that of a loss with these gradients and other terms, is refused. A backward pass that adds to leaves cannot be captured while an
     earlier graph of the same leaves lives (it is refused). out_layout: "contiguous", or "input" for the outputs and gradients in the memory layouts of q and k."""
     if out_layout not in ("contiguous", "input"):
         raise ValueError("out_layout must be 'contiguous' or 'input'")
