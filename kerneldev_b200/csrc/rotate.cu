@@ -4,8 +4,8 @@
 // position * step[p]: (a, b) -> (a cos - b sin, b cos + a sin). Backward, with g the gradient turned back: dx = g, or r (g w - x r^2 mean(g w x)), and
 // dw = the sum of g x r over all rows. All in 32 bits, rounded once.
 //
-// Angles. A step is kept as a 64-bit fraction of a turn, so that position * step modulo 2^64 is the fraction of a turn that is left, exact to position / 2^64 turns
-// whatever the position: its upper 32 bits are the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21, beside 2^-9 or 2^-12 of the output), for float polynomials.
+// Angles. A step is kept as a 64-bit fraction of a turn, so that position * step modulo 2^64 is the fraction of a turn that is left, exact to position / 2^65 turns
+// whatever the position: rounded to 32 bits it is the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21, beside 2^-9 or 2^-12 of the output), for float polynomials.
 //
 // Bound by memory: each number is read and written once. A row has a group of D / 16 lanes, 16 numbers to each: the pairs of a lane are its own, and a lane keeps its
 // sines and cosines for all heads of a run. Rows are asked for ahead by asynchronous copies into shared memory, so that what is in flight takes no registers: with loads into registers a backward of
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_CTAS) rotate_kernel(const __gri
       for (int i = 0; i < 8; ++i) {
         const int pair = p.interleaved != 0 ? mine16.element(2 * i) / 2 : mine16.element(i);
         const int64_t here = p.positions == nullptr || pair < p.ends[0] ? n[0] : pair < p.ends[1] ? n[1] : n[2];
-        turn<kType>(static_cast<int32_t>((static_cast<uint64_t>(here) * p.steps[pair]) >> 32), c[i], s[i]);
+        turn<kType>(static_cast<int32_t>((static_cast<uint64_t>(here) * p.steps[pair] + (1ull << 31)) >> 32), c[i], s[i]);
       }
     }
     char* to = row_of(kGrad ? dx : y, at);
