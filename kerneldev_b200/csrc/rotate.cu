@@ -5,7 +5,8 @@
 // dw = the sum of g x r over all rows. All in 32 bits, rounded once.
 //
 // Angles. A step is kept as a 64-bit fraction of a turn, so that position * step modulo 2^64 is the fraction of a turn that is left, exact to position / 2^65 turns
-// whatever the position: rounded to 32 bits it is the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21, beside 2^-9 or 2^-12 of the output), for float polynomials.
+// whatever the position: rounded to 32 bits it is the angle. For 16-bit types sine and cosine are the hardware's (off by 2^-21.4 and 2^-21.2 for what it is given, an angle that is off by 2^-21.7 as a float: 2^-20 together,
+// beside 2^-9 or 2^-12 of the output), for float polynomials (2^-23.2).
 //
 // Bound by memory: each number is read and written once. A row has a group of D / 16 lanes, 16 numbers to each: the pairs of a lane are its own, and a lane keeps its
 // sines and cosines for all heads of a run. Rows are asked for ahead by asynchronous copies into shared memory, so that what is in flight takes no registers: with loads into registers a backward of

@@ -50,7 +50,7 @@ class Rotation:
     (scaled ones of a longer context, or those of several axes), by default base ** (-2 i / rotary_dim). sections: how many pairs turn by the first, second and third axis of the
     positions (time, height and width of a video's patches), rotary_dim / 2 together; None: there is one axis.
 
-    Angles are exact to 2**-32 of a turn at any 32-bit position; sines and cosines to 2**-23 for float32 heads, 2**-21 for those of 16 bits."""
+    Angles are exact to 2**-32 of a turn at any 32-bit position; sines and cosines to 2**-23 for float32 heads, 2**-20 for those of 16 bits."""
 
     __slots__ = ("head_dim", "rotary_dim", "interleaved", "sections", "steps", "_core")
 
