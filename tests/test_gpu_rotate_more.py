@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import rotate_oracle as ro
-from tests.test_gpu_rotate import wide
+from tests.test_gpu_rotate import DT, HALF, assert_within, make, wide
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -76,3 +76,48 @@ def test_no_word_where_nothing_is_lost():
         y, _ = rotate_heads(x, None, rotation, q_weight=w)
         for _ in range(2):
             torch.autograd.grad(y, w, dy, create_graph=True)
+
+
+# D, R, Hq, Hk, B, T, type, weights' type, layout, sections, interleaved, which weights
+LARGE = [
+    (64, 64, 4, 4, 3, 6007, "bf16", "bf16", "bthd", None, False, "qk"),
+    (128, 64, 6, 3, 2, 6151, "f16", "f32", "bhtd", None, True, "qk"),
+    (80, 80, 4, 2, 2, 8009, "f32", "f32", "bthd", (8, 16, 16), False, "qk"),
+    (64, 64, 4, 4, 1, 16411, "f32", "f32", "bhtd", None, False, ""),
+    (48, 32, 3, 3, 2, 12011, "bf16", "f32", "bthd", (5, 11), True, "k"),
+    (128, 128, 8, 8, 1, 4099, "f32", "bf16", "bthd", None, False, "q"),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"d{c[0]}r{c[1]}-{c[6]}-{c[2]}+{c[3]}")
+def test_calls_of_several_heads_and_tiles_of_a_cta(case):
+    """What large calls do: a thread has five rows and more, of several heads and several tiles of tokens, which go round its ring. Tolerances as in tests/test_gpu_rotate.py; chains of the weights' sums are
+    at most 12 rows of a thread, 256 threads of a column, 10 CTAs of a lane and 32 lanes: 310 additions. Rows of float32 without a norm: the pair's length times 2**-22.5 for sine and cosine together, 2**-24 for
+    the product that is rounded before the sum, 2**-30 for the angle: below 2**-22."""
+    import ctypes
+
+    from kerneldev_b200 import Rotation, _capi, rotate_heads
+    D, R, Hq, Hk, B, T, dtype, wtype, layout, sections, interleaved, which = case
+    p, n = _capi.KdRotation(), ctypes.c_size_t()
+    p.B, p.T, p.Hq, p.Hk, p.D, p.R, p.dtype, p.w_dtype, p.axes, p.eps, p.steps = B, T, Hq, Hk, D, R, {"f16": _capi.KD_F16, "bf16": _capi.KD_BF16, "f32": 2}[dtype], 2, 1, 1e-6, 0x10000
+    p.dq_weight = 0x10000
+    assert _capi.load().kd_rotate_grad_workspace(ctypes.byref(p), ctypes.byref(n)) == 0
+    ctas, rows = n.value // (4 * D), (Hq + Hk) * B * T // (8 * (32 // (D // 16)))   # rows: of all threads' groups, in tiles
+    assert ctas <= 296 and rows >= 5 * ctas
+
+    q, k, w, pos = make(case, seed=7)
+    rotation, rot = Rotation(D, R, sections=sections, interleaved=interleaved, device=DEV), ro.rotation(D, R, sections=sections, interleaved=interleaved)
+    leaves = [t.requires_grad_() for t in (q, k, w["q"], w["k"]) if t is not None]
+    positions = torch.tensor(pos, device=DEV, dtype=torch.int32)
+    out = rotate_heads(q, k, rotation, positions if sections else positions[0], q_weight=w["q"], k_weight=w["k"], out_layout="input")
+    g = [torch.randn(y.shape, device=DEV).to(DT[dtype]) for y in out]
+    got = dict(zip((id(t) for t in leaves), torch.autograd.grad(out, leaves, g)))
+    for name, x, y, dy in zip("qk", (q, k), out, g):
+        weight = None if w[name] is None else wide(w[name])
+        exact = dtype == "f32" and weight is None
+        want, size = ro.forward(rot, wide(x), pos, weight)
+        assert_within(y, want, size * 2.0 ** (-22 if exact else -19) + np.abs(want) * HALF[dtype] + 1e-7 * (dtype == "f16"), name)
+        dx, dw, big, sums = ro.backward(rot, wide(x), wide(dy), pos, weight)
+        assert_within(got[id(x)], dx, big * 2.0 ** (-22 if exact else -18) + np.abs(dx) * HALF[dtype] + 1e-7 * (dtype == "f16"), "d" + name)
+        if dw is not None:
+            assert_within(got[id(w[name])], dw, sums * 2.0 ** -14 + np.abs(dw) * HALF[wtype] + 1e-7 * (wtype == "f16"), "d" + name + "_weight")
