@@ -149,7 +149,7 @@ __device__ __forceinline__ void store_tile(uint8_t* to, const uint32_t (&place)[
     }
     uint32_t h[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) h[x] = times(e2m1x2_to_f16x2(x < 4 ? reg[i].v.x : reg[i].v.y, x & 3), s);
+    for (int x = 0; x < 8; ++x) h[x] = times(e2m1x2_to_f16x2<true>(x < 4 ? reg[i].v.x : reg[i].v.y, x & 3), s);
     uint8_t* at = to + (i & 3) * 4096 + (i >> 2) * ChunkShared<D>::BLOCK;
     *reinterpret_cast<uint4*>(at + place[0]) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(at + place[1]) = make_uint4(h[4], h[5], h[6], h[7]);

@@ -205,10 +205,8 @@ __device__ __forceinline__ void scores_of(uint32_t stage, const Lane<kBits, D>& 
       if constexpr (kBits == 4) {
         constexpr int PIECE = S::KN / 4, WORDS = S::KU > 4 ? S::KU / 4 : 1;   // steps and words of a piece
         const int word = s / PIECE * WORDS + s % PIECE / 2, half = s % PIECE & 1;
-        // (Words of two bytes side by side: bytes of one that was loaded as 16 bits came out of the conversion as zeros.)
-        const uint32_t both = S::KU == 2 ? k[0][word] | k[1][word] << 16 : 0u;
-        lo = e2m1x4_to_f16x4(S::KU == 2 ? both : k[0][word], half, scale[0][s / Scales4<D>::STEPS]);
-        hi = e2m1x4_to_f16x4(S::KU == 2 ? both : k[1][word], S::KU == 2 ? 1 : half, scale[1][s / Scales4<D>::STEPS]);
+        lo = e2m1x4_to_f16x4<(S::KU > 2)>(k[0][word], half, scale[0][s / Scales4<D>::STEPS]);
+        hi = e2m1x4_to_f16x4<(S::KU > 2)>(k[1][word], half, scale[1][s / Scales4<D>::STEPS]);
       } else {
         lo = e4m3x4_to_f16x4(k[0][s]);
         hi = e4m3x4_to_f16x4(k[1][s]);
@@ -305,7 +303,8 @@ __device__ __forceinline__ void add_values4(float (&o)[NT][D / 16][4], const uin
             if (hit[j] > 0.f) o[n][m][j] = __uint_as_float(0x7FC00000u);
         }
       }
-      const uint4 a = make_uint4(times(e2m1x2_to_f16x2(b[0][0], i), s0), times(e2m1x2_to_f16x2(b[0][1], i), s0), times(e2m1x2_to_f16x2(b[1][0], i), s1), times(e2m1x2_to_f16x2(b[1][1], i), s1));
+      auto numbers = [&](int x, int y, uint32_t by) { return times(e2m1x2_to_f16x2<BYTES == 4>(b[x][y], i), by); };
+      const uint4 a = make_uint4(numbers(0, 0, s0), numbers(0, 1, s0), numbers(1, 0, s1), numbers(1, 1, s1));
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16(o[n][m], a, p[n][0], p[n][1]);
     }

@@ -99,13 +99,22 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// byte i of a word: two numbers as halves, the one in the low bits first
+// Byte i of a word: two numbers as halves, the one in the low bits first. kWhole: the caller converts all four bytes of the word. Of a word that is unpacked into four bytes at once the compiler (CUDA 12.9) converts zeros where
+// only one half of it is used, and of one that is unpacked by halves in place of the third byte; the third and fourth byte by a shift ahead of the halves are right, and all four at once are
+// (tests/e2m1_words_check.cu goes through sets of bytes and ways to load them). The shift everywhere would cost 128 x 8192 tokens of 8 heads of 128 220 us in place of 183.
+template <bool kWhole>
 __device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t w, int i) {
   uint32_t r;
-  if (i == 0) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, a;\n}\n" : "=r"(r) : "r"(w));
-  else if (i == 1) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(r) : "r"(w));
-  else if (i == 2) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, c;\n}\n" : "=r"(r) : "r"(w));
-  else asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, d;\n}\n" : "=r"(r) : "r"(w));
+  if constexpr (kWhole) {
+    if (i == 0) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, a;\n}\n" : "=r"(r) : "r"(w));
+    else if (i == 1) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(r) : "r"(w));
+    else if (i == 2) asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, c;\n}\n" : "=r"(r) : "r"(w));
+    else asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %1;\ncvt.rn.f16x2.e2m1x2 %0, d;\n}\n" : "=r"(r) : "r"(w));
+  } else {
+    if (i >= 2) w >>= 16;
+    if (i % 2 == 0) asm("{\n.reg .b16 l, h;\n.reg .b8 a, b;\nmov.b32 {l, h}, %1;\nmov.b16 {a, b}, l;\ncvt.rn.f16x2.e2m1x2 %0, a;\n}\n" : "=r"(r) : "r"(w));
+    else asm("{\n.reg .b16 l, h;\n.reg .b8 a, b;\nmov.b32 {l, h}, %1;\nmov.b16 {a, b}, l;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}\n" : "=r"(r) : "r"(w));
+  }
   return r;
 }
 // eight numbers, nearest, ties to even, 6 at most, as a word
@@ -117,7 +126,10 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1x8(const float* f) {
   return r;
 }
 // half `half` of a word: four numbers times their scale (twice in a word)
-__device__ __forceinline__ HalfPairs e2m1x4_to_f16x4(uint32_t w, int half, uint32_t scale) { return HalfPairs{times(e2m1x2_to_f16x2(w, 2 * half), scale), times(e2m1x2_to_f16x2(w, 2 * half + 1), scale)}; }
+template <bool kWhole>
+__device__ __forceinline__ HalfPairs e2m1x4_to_f16x4(uint32_t w, int half, uint32_t scale) {
+  return HalfPairs{times(e2m1x2_to_f16x2<kWhole>(w, 2 * half), scale), times(e2m1x2_to_f16x2<kWhole>(w, 2 * half + 1), scale)};
+}
 
 // 16 numbers of a row, 32 bytes of a 16-bit type, 64 of float
 template <int kType>

@@ -201,9 +201,9 @@ cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ k
       if (first + i * SLOTS >= here) continue;
       const uint32_t s2 = both_halves(scale[y][i]);
       uint32_t w[4];
-      if constexpr (N == 4) {   // (both bytes of a word of 32 bits: see the keys in kv_attn_rows.cuh)
-        const uint32_t word = codes[y][i] | codes[y][i] << 16;
-        const float2 lo = unpack2<false>(times(e2m1x2_to_f16x2(word, 0), s2)), hi = unpack2<false>(times(e2m1x2_to_f16x2(word, 1), s2));
+      if constexpr (N == 4) {
+        const HalfPairs four = e2m1x4_to_f16x4<false>(codes[y][i], 0, s2);
+        const float2 lo = unpack2<false>(four.lo), hi = unpack2<false>(four.hi);
         w[0] = __float_as_uint(lo.x);
         w[1] = __float_as_uint(lo.y);
         w[2] = __float_as_uint(hi.x);
@@ -211,7 +211,7 @@ cache4_read_kernel(const __grid_constant__ kd_cache c, const __grid_constant__ k
       } else {
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          w[m] = times(e2m1x2_to_f16x2(codes[y][i], m), s2);
+          w[m] = times(e2m1x2_to_f16x2<true>(codes[y][i], m), s2);
           if (kType == KD_BF16) {
             const float2 two = unpack2<false>(w[m]);
             w[m] = pack2<true>(two.x, two.y);
