@@ -20,8 +20,9 @@
 // probabilities that is 2^-28 of the row's largest, or 2^-20 of the unit's.
 //
 // Numbers of 4 bits have a scale for each 16 of a row: K = e2m1 times scale in one multiplication of two halves behind the conversion of two numbers, exact, V too; nothing of it is in the exponents, whose reference goes
-// up only. A unit is 4.6 KB and 560 to 640 instructions, which is what bounds it: 128 x 8192 tokens of 8 heads of 128 take 183 us (907 MB, 5.0 TB/s), 164 without the multiplications, 158 without the conversions too, and
-// no less with 16 warps an SM in place of 12, or with the input in L2.
+// up only. A unit is 4.6 KB and 560 to 640 instructions, and what bounds it is that they wait for one another: at 32 x 4096 tokens of 8 heads of 128 an instruction is 5.0 cycles in its warp's hands (1.1 of them for a result
+// at a fixed distance, 0.7 for the other warps, 0.5 for a pipe, 0.4 at barriers, 0.2 for memory), and 2.8 warps a scheduler cover 56 % of the issue slots. So each instruction counts, though slots are free: 128 x 8192 tokens
+// take 183 us (907 MB, 5.0 TB/s), 164 without the multiplications, 158 without the conversions too, 220 with a shift for each word, and no less with the input in L2.
 //
 // NaN. A masked token has p' = 0, and 0 * NaN of a masked value would be NaN. A warp that ends with a NaN walks its units once more, with NaN values
 // taken as zeros and, beside the product, one of indicators (row sees token, value is NaN) that puts NaN where it belongs. So does one that has met scores beyond KA_FAR.
