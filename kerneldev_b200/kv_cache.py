@@ -91,8 +91,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache, page_table: torch.Tensor, l
     its head; tokens beyond its last dimension are left out. sm_scale: head_dim ** -0.5 by default. out_layout: "contiguous", or "input" for O in
     the memory layout of q.
 
-    For more than eight query rows of a key head, and where the scores of fewer would take more than 256 MB and an eighth of the cache, ``weights`` comes
-    from scores that are added up a second time, in float32 and in another order: a row's weights are then off by a factor that grows with its
+    ``weights`` comes from scores in float32: those that O is made of, rounded once more, for up to eight query rows of a key head, and for more (and where the scores of
+    fewer would take more than 256 MB and an eighth of the cache) scores that are added up a second time in another order. Either way a row's weights are off by a factor that grows with its
     scores (in powers of two, or with the sum of the sizes of their products where those cancel), at most about 2**-21 of them: a few per cent at 2**16 (0.1 % was measured), and
     beyond 2**21 they say nothing.
 
