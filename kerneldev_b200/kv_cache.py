@@ -13,7 +13,8 @@ later keeps its scale or gets a larger one, and what it holds is rounded again: 
 In 4 bits (``KVCache.empty(..., bits=4)``), 9/16 of that memory: ``k`` and ``v`` uint8 (pages, heads, 64, head_dim / 2), two e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) in a byte, the even
 element in the low half; ``k_scale`` and ``v_scale`` uint8 (pages, heads, 64, head_dim / 16), one scale for 16 elements side by side: bits 14 to 7 of a float16. It is the one nearest to a sixth of their largest
 magnitude, 10240 at most, and a number is the nearest to what it is divided by the scale; ties go to even, larger numbers saturate. 16 elements with an infinity or NaN among them
-are stored as NaN, all 16 (byte 255; bytes 227 to 254 must not occur). An append never changes what is there. Every function below takes either cache.
+are stored as NaN, all 16 (byte 255; bytes 227 to 254 must not occur). An append never changes what is there. Every function below takes either cache. (Scales of this kind are this package's own: no matrix
+instruction and no other program's cache has them.)
 
 ``desc`` (optional) holds the mask descriptor of every token: int32, bit 0 prefix, 1 context, 2 in a span, 3 [MASKQ], 4 same-span rule armed,
 5 to 7 the classes of keys that the token sees wherever they are, from 8 the span id.

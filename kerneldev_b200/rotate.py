@@ -90,7 +90,7 @@ def rotate_heads(q: torch.Tensor, k: torch.Tensor | None, rotation: Rotation, po
     sequence's tokens are offsets[b], offsets[b] + 1, ... Neither: 0, 1, ... Both stay on the device, so that a step can be captured.
 
     q_weight, k_weight: (head_dim,) in any of the three types. With one, a row x becomes weight * x / sqrt(mean(x**2) + eps) before it is turned; the mean is taken in 32 bits
-    (squares beyond its range make the row zeros). Everything is computed in 32 bits and rounded once.
+    (squares beyond its range make the row zeros; with an eps of 0 a row whose squares are all below it, or zero, becomes infinities and NaN). Everything is computed in 32 bits and rounded once.
 
     Differentiable, once, in q, k and the weights; sums over rows are taken in a fixed order. With ``create_graph`` the gradients are plain tensors all the same: where a second derivative would go through
     them a warning says so, and a later backward pass through the same call, as that of a loss with these gradients and other terms, is refused. A backward pass that adds to leaves cannot be captured while an
