@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t group_max(const Raw16<kType>& raw) {
 // A group as it is stored. The scale is the nearest to a sixth of the largest magnitude, and the numbers the nearest to what they are in its units; ties go to even.
 // Floats are divided; a quotient is never rounded onto the middle of two steps: a float next to a middle times 6 or times a scale of 4 bits is 2^-24 of it away, and a quotient's rounding moves it
 // less. 16-bit numbers are multiplied with a rounded inverse, and the product brought to a coarser grid (2^-16 of itself; 2^-13 by the fused sum with 1536, of which one step is that much), which puts it on a middle
-// exactly where the quotient is: numbers of 11 bits have no other quotient that near to one (tests/test_kv_cache4_logic.py goes through all of them). That takes a third of the instructions of divisions.
+// exactly where the quotient is: numbers of 11 bits have no other quotient that near to one (tests/test_kv_cache4_rounding.py goes through all of them). That takes a third of the instructions of divisions.
 template <int kType>
 __device__ __forceinline__ Group4 quantise_group(const Raw16<kType>& raw) {
   const uint32_t top_bits = group_max(raw);
